@@ -40,7 +40,9 @@ def lib():
                      "gs_coo_sum_workspace_bytes", "gs_coo_pick_rows_workspace_bytes",
                      "gs_coo_block_values_workspace_bytes", "gs_random_walk_workspace_bytes",
                      "gs_metapath_walk_workspace_bytes",
-                     "gs_induced_slice_workspace_bytes", "gs_induced_slice_notify_workspace_bytes"):
+                     "gs_induced_slice_workspace_bytes", "gs_induced_slice_notify_workspace_bytes",
+                     "gs_embedding_grad_workspace_bytes", "gs_embedding_sparse_grad_workspace_bytes",
+                     "gs_expert_sort_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_size_t
         _lib.gs_sorted_union_max.restype = ctypes.c_int64
@@ -1307,3 +1309,134 @@ def coo2csc(key, value, num_keys, is_sorted, num_values=None):
                 _ptr(out_value), _ptr(perm), _ptr(ws), ctypes.c_size_t(ws.numel()), _stream(dev)),
            "gs_coo2csc")
     return indptr, (value if is_sorted else out_value), perm
+
+
+# ------------------------------------------------------ rows moved by ids ----
+_VALUE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _rows(t, name):
+    """(pointer, values between rows, width, value type) of a 2-D tensor whose rows are contiguous."""
+    if not t.is_cuda:
+        raise GsError("%s must be a GPU tensor (no CPU path in this library)" % name)
+    if t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1):
+        raise GsError("%s must be 2-D with contiguous rows" % name)
+    if t.dtype not in _VALUE_TYPES:
+        raise GsError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    return _ptr(t), _i64(t.stride(0)), _i64(t.size(1)), _VALUE_TYPES[t.dtype]
+
+
+def embedding_lookup(table, ids, scale=1.0):
+    idb = _ids(ids, "ids")
+    out = torch.empty(tuple(ids.shape) + (table.size(1),), dtype=table.dtype, device=table.device)
+    ptr, stride, dim, kind = _rows(table, "table")
+    _check(lib().gs_embedding_lookup(ptr, _i64(table.size(0)), stride, dim, kind, _ptr(ids), idb, _i64(ids.numel()),
+                                     ctypes.c_float(scale), _ptr(out), _stream(table.device)),
+           "gs_embedding_lookup")
+    return out
+
+
+def embedding_grad(grad, ids, num_rows, scale=1.0):
+    idb = _ids(ids, "ids")
+    ptr, stride, dim, kind = _rows(grad, "grad")
+    if grad.size(0) != ids.numel():
+        raise GsError("a gradient of %d rows for %d ids" % (grad.size(0), ids.numel()))
+    out = torch.empty(num_rows, grad.size(1), dtype=grad.dtype, device=grad.device)
+    ws = workspace(lib().gs_embedding_grad_workspace_bytes(_i64(ids.numel()), dim, kind), grad.device)
+    _check(lib().gs_embedding_grad(ptr, stride, dim, kind, _ptr(ids), idb, _i64(ids.numel()), _i64(num_rows),
+                                   ctypes.c_float(scale), _ptr(out), _ptr(ws), ctypes.c_size_t(ws.numel()),
+                                   _stream(grad.device)), "gs_embedding_grad")
+    return out
+
+
+def embedding_sparse_grad(grad, ids, num_rows, scale=1.0):
+    """(ids met, ascending; a row of sums each); synchronises the stream for how many there are."""
+    idb = _ids(ids, "ids")
+    ptr, stride, dim, kind = _rows(grad, "grad")
+    n, dev = ids.numel(), grad.device
+    if grad.size(0) != n:
+        raise GsError("a gradient of %d rows for %d ids" % (grad.size(0), n))
+    if n == 0:
+        return (torch.empty(0, dtype=torch.int64, device=dev),
+                torch.empty(0, grad.size(1), dtype=grad.dtype, device=dev))
+    ws = workspace(lib().gs_embedding_sparse_grad_workspace_bytes(_i64(n), dim, kind), dev)
+    box = torch.zeros(2, dtype=torch.int64, pin_memory=True)
+    st = _stream(dev)
+    _check(lib().gs_embedding_sparse_grad_count(_ptr(ids), idb, _i64(n), _i64(num_rows), dim, kind, _ptr(box), _i64(1),
+                                                _ptr(ws), ctypes.c_size_t(ws.numel()), st),
+           "gs_embedding_sparse_grad_count")
+    torch.cuda.current_stream(dev).synchronize()
+    met = torch.empty(int(box[0]), dtype=torch.int64, device=dev)
+    values = torch.empty(int(box[0]), grad.size(1), dtype=grad.dtype, device=dev)
+    if met.numel():
+        _check(lib().gs_embedding_sparse_grad_fill(ptr, stride, dim, kind, _i64(n), _i64(num_rows),
+                                                   ctypes.c_float(scale), _ptr(met), _ptr(values), _ptr(ws),
+                                                   ctypes.c_size_t(ws.numel()), st), "gs_embedding_sparse_grad_fill")
+    return met, values
+
+
+def expert_sort(experts, num_experts):
+    """(order, place, offsets) of experts [tokens] or [tokens, choices]."""
+    idb = _ids(experts, "experts")
+    n, dev = experts.numel(), experts.device
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    place = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
+    ws = workspace(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
+    _check(lib().gs_expert_sort(_ptr(experts), idb, _i64(n), _i64(num_experts), _ptr(order), _ptr(place), _ptr(offsets),
+                                _ptr(ws), ctypes.c_size_t(ws.numel()), _stream(dev)), "gs_expert_sort")
+    return order, place, offsets
+
+
+def _choices(place, rows, num_rows, name):
+    """(tokens, choices) of int32 places for a tensor of num_rows(tokens, choices) rows."""
+    _need(place, torch.int32, "place")
+    tokens, choices = place.size(0), place.size(1) if place.dim() == 2 else 1
+    if rows.size(0) != num_rows(tokens, choices):
+        raise GsError("%s has %d rows for places of %s" % (name, rows.size(0), tuple(place.shape)))
+    return tokens, choices
+
+
+def expert_gather(x, place, offsets):
+    ptr, stride, dim, kind = _rows(x, "x")
+    tokens, choices = _choices(place, x, lambda t, k: t, "x")
+    _need(offsets, torch.int64, "offsets")
+    rows = torch.empty(tokens * choices, x.size(1), dtype=x.dtype, device=x.device)
+    _check(lib().gs_expert_gather(ptr, stride, dim, kind, _ptr(place), _i64(tokens), _i64(choices), _ptr(offsets[-1:]),
+                                  _ptr(rows), _stream(x.device)), "gs_expert_gather")
+    return rows
+
+
+def _weights(weights, place):
+    if weights is None:
+        return _ptr(None), 0
+    if weights.dtype not in _VALUE_TYPES or weights.shape != place.shape or not weights.is_contiguous():
+        raise GsError("weights must be contiguous, of a value type and of the shape of place")
+    return _ptr(weights), _VALUE_TYPES[weights.dtype]
+
+
+def expert_combine(y, place, weights=None):
+    ptr, stride, dim, kind = _rows(y, "y")
+    tokens, choices = _choices(place, y, lambda t, k: t * k, "y")
+    out = torch.empty(tokens, y.size(1), dtype=y.dtype, device=y.device)
+    w, wkind = _weights(weights, place)
+    _check(lib().gs_expert_combine(ptr, stride, dim, kind, _ptr(place), _i64(tokens), _i64(choices), w, wkind, _ptr(out),
+                                   _stream(y.device)), "gs_expert_combine")
+    return out
+
+
+def expert_combine_grad(dout, y, place, offsets, weights=None):
+    """(gradient of y, gradient of the weights or None)."""
+    dptr, dstride, dim, kind = _rows(dout, "dout")
+    yptr, ystride, ydim, ykind = _rows(y, "y")
+    tokens, choices = _choices(place, y, lambda t, k: t * k, "y")
+    if dout.size(0) != tokens or ydim.value != dim.value or ykind != kind:
+        raise GsError("dout and y do not belong together")
+    _need(offsets, torch.int64, "offsets")
+    w, wkind = _weights(weights, place)
+    dy = torch.empty(tokens * choices, dout.size(1), dtype=dout.dtype, device=dout.device)
+    dw = torch.empty_like(weights) if weights is not None else None
+    _check(lib().gs_expert_combine_grad(dptr, dstride, yptr, ystride, dim, kind, _ptr(place), _i64(tokens), _i64(choices),
+                                        _ptr(offsets[-1:]), w, wkind, _ptr(dy), _ptr(dw), _stream(dout.device)),
+           "gs_expert_combine_grad")
+    return dy, dw

@@ -1,0 +1,511 @@
+// Embedding lookup with scaling, and its gradient by sorted ids, on gfx950.
+//
+//   lookup    out[n, :]  = scale * table[ids[n], :]
+//   gradient  grad[v, :] = scale * sum of dout[n, :] over the n with ids[n] = v
+//
+// No counterpart in the reference, whose examples index feature matrices with torch.  An id outside
+// the table stands for no row: zeros come out, nothing goes into the gradient, nothing is read.
+// Values are fp32, fp16 or bf16; products and sums are fp32, rounded once on the way out.
+//
+// The gradient adds in an order that follows from the ids alone, without atomics: the positions are
+// sorted by id (gs_key_sort.hpp), a group of lanes adds up a tile of consecutive sorted positions run
+// by run, and writes a row when the run lies inside its tile.  Runs that cross tiles leave partial
+// sums, at most two a tile, which are themselves a sorted list: the next launch adds them up in the
+// same way, and so on until one tile holds all.  So a row that half of the ids name costs no more
+// than any other, and sums of many addends are sums of sums, which keeps fp32 exact enough.
+#include "gs_key_sort.hpp"
+#include "gs_rows.hpp"
+
+namespace gs {
+namespace {
+
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------------ lookup ----
+// A chunk a lane (ITEMS of them, asked for together); a row's id is read by all its lanes, which is one
+// request.  What bounds it is the rows' bytes: random rows in, consecutive rows out.
+template <typename T, typename IdT, int ITEMS>
+__global__ void __launch_bounds__(kThreads)
+lookup_kernel(const T* __restrict__ table, int64_t num_rows, int64_t stride, int64_t dim, Divider chunks,
+              const IdT* __restrict__ ids, int64_t total, float scale, T* __restrict__ out) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * ITEMS);
+  const RowRange range(chunks, first);
+  int64_t id[ITEMS], to[ITEMS], at[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t j = k * kThreads + threadIdx.x;
+    const bool in = first + j < total;
+    uint32_t c;
+    const int64_t row = range.row(in ? j : 0, &c);
+    at[k] = chunk_start<T>(dim, c);
+    to[k] = in ? row * dim + at[k] : -1;
+    id[k] = ids[row];
+  }
+  Values<T> v[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    v[k] = Values<T>{};
+    if (id[k] >= 0 && id[k] < num_rows) v[k] = load_chunk(table + id[k] * stride + at[k], dim);
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    // (a scale of one leaves the bits as they are)
+    const Values<T> w = scale == 1.0f ? v[k] : narrow<T>(widen<T>(v[k]) * scale);
+    // (0 * inf where there is no row would be NaN)
+    const bool there = id[k] >= 0 && id[k] < num_rows;
+    if (to[k] >= 0) store_chunk(out + to[k], there ? w : Values<T>{}, dim);
+  }
+}
+
+// ---------------------------------------------------------------- gradient ----
+// Zeros everywhere, before the rows that are met are written.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) zero_kernel(T* __restrict__ out, int64_t n) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t whole = n / Chunk<T>::kVec, i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  for (int64_t i = i0; i < whole; i += stride) store_chunk(out + i * Chunk<T>::kVec, Values<T>{}, Chunk<T>::kVec);
+  if (i0 < n - whole * Chunk<T>::kVec) out[whole * Chunk<T>::kVec + i0] = T(0);
+}
+
+// What a tile leaves for the next launch: which output row, and whether a partial sum goes with it.
+struct Entry {
+  uint32_t row;
+  uint32_t state;
+};
+constexpr uint32_t kNone = 0, kSum = 1, kThrough = 2;  // (through: the run goes on, its sum is in the entry before)
+
+struct RunsOut {
+  float scale;
+  int64_t dim;
+  int64_t chunks;        // of a row
+  int slices;            // groups side by side over a row
+  int64_t* met;          // sparse: ids of the rows by their rank (null: dense)
+  const int64_t* rank;   // sparse: met rows before a sorted position
+  Entry* entries;        // 2 a tile (null where there is one tile)
+  float* sums;           // [2 * tiles, chunks * kVec]
+};
+
+// where a group's lane works: G lanes a group, 64 / G groups a wave
+struct GroupPlace {
+  int64_t tile;
+  int64_t chunk;  // of this lane; may lie behind the row's last
+  bool in;
+  template <int G>
+  static __device__ __forceinline__ GroupPlace of(int64_t tiles, int slices, int64_t chunks) {
+    const int64_t g = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+    GroupPlace p;
+    p.tile = g / slices;
+    p.chunk = (g - p.tile * slices) * G + (threadIdx.x & (G - 1));
+    p.in = p.tile < tiles && p.chunk < chunks;
+    if (p.tile >= tiles) p.tile = tiles - 1;  // (works along, writes nothing)
+    if (p.chunk >= chunks) p.chunk = 0;
+    return p;
+  }
+};
+
+// A run that ends: its row when it is whole, a partial sum when it crosses a tile's edge.
+template <typename T>
+struct RunWriter {
+  const RunsOut& o;
+  T* out;
+  const GroupPlace& p;
+  Entry first{0, kNone}, last{0, kNone};
+
+  __device__ __forceinline__ void finish(uint32_t row, const Wide<T>& sum, bool left, bool right) {
+    if (!left && !right) {
+      const int64_t at = chunk_start<T>(o.dim, p.chunk);
+      if (p.in) store_chunk(out + static_cast<int64_t>(row) * o.dim + at, narrow<T>(sum * o.scale), o.dim);
+      return;
+    }
+    const int slot = left ? 0 : 1;
+    float* to = o.sums + ((2 * p.tile + slot) * o.chunks + p.chunk) * Chunk<T>::kVec;
+    if (p.in) __builtin_memcpy(to, &sum, sizeof(sum));
+    if (left) {
+      first = Entry{row, kSum};
+      if (right) last = Entry{row, kThrough};
+    } else {
+      last = Entry{row, kSum};
+    }
+  }
+  __device__ __forceinline__ void entries() {
+    if (o.entries && p.in && p.chunk == 0) {
+      o.entries[2 * p.tile] = first;
+      o.entries[2 * p.tile + 1] = last;
+    }
+  }
+};
+
+constexpr int kBatch = 8;  // rows a group asks for together
+
+// Tiles of `size` sorted positions.
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads)
+sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t num_rows, const T* __restrict__ grad,
+                int64_t stride, int size, int64_t tiles, RunsOut o, T* __restrict__ out) {
+  const GroupPlace p = GroupPlace::of<G>(tiles, o.slices, o.chunks);
+  const int64_t base = p.tile * size;
+  const int count = n - base < size ? static_cast<int>(n - base) : size;
+  const int64_t at = chunk_start<T>(o.dim, p.chunk);
+  RunWriter<T> writer{o, out, p};
+  uint32_t key = key_sort::key_of(words[base]);
+  bool left = base > 0 && key_sort::key_of(words[base > 0 ? base - 1 : 0]) == key;
+  const uint32_t behind = base + count < n ? key_sort::key_of(words[base + count]) : num_rows;
+  int64_t row = key;
+  if (o.rank) row = o.rank[base] - (left ? 1 : 0);
+  if (o.met && !left && key < num_rows && p.in && p.chunk == 0) o.met[row] = key;
+  Wide<T> sum = {};
+  for (int j0 = 0; j0 < count; j0 += kBatch) {
+    key_sort::Word w[kBatch];
+    Values<T> v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) w[k] = words[base + (j0 + k < count ? j0 + k : count - 1)];
+    if (key_sort::key_of(w[0]) >= num_rows) {  // no rows from here on
+      if (j0 > 0 && key < num_rows) writer.finish(static_cast<uint32_t>(row), sum, left, false);
+      key = num_rows;
+      break;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) v[k] = load_chunk(grad + key_sort::position_of(w[k]) * stride + at, o.dim);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (j0 + k >= count) break;
+      const uint32_t next = key_sort::key_of(w[k]);
+      if (next != key) {
+        writer.finish(static_cast<uint32_t>(row), sum, left, false);
+        left = false;
+        key = next;
+        row = o.rank ? row + 1 : static_cast<int64_t>(key);
+        if (o.met && key < num_rows && p.in && p.chunk == 0) o.met[row] = key;
+        sum = Wide<T>{};
+        if (key >= num_rows) break;
+      }
+      sum += widen<T>(v[k]);
+    }
+    if (key >= num_rows) break;
+  }
+  if (key < num_rows) writer.finish(static_cast<uint32_t>(row), sum, left, behind == key);
+  writer.entries();
+}
+
+// Tiles of `size` entries that an earlier launch left, m of them; sums_in as RunsOut::sums.
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads)
+join_runs_kernel(const Entry* __restrict__ in, int64_t m, const float* __restrict__ sums_in, int size, int64_t tiles,
+                 RunsOut o, T* __restrict__ out) {
+  const GroupPlace p = GroupPlace::of<G>(tiles, o.slices, o.chunks);
+  const int64_t base = p.tile * size;
+  const int count = m - base < size ? static_cast<int>(m - base) : size;
+  RunWriter<T> writer{o, out, p};
+  const Entry before = base > 0 ? in[base - 1] : Entry{0, kNone};
+  const Entry behind = base + count < m ? in[base + count] : Entry{0, kNone};
+  bool open = false, left = false;
+  uint32_t row = 0;
+  Wide<T> sum = {};
+  for (int j0 = 0; j0 < count; j0 += kBatch) {
+    Entry e[kBatch];
+    Wide<T> v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) e[k] = in[base + (j0 + k < count ? j0 + k : count - 1)];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (j0 + k >= count) e[k].state = kNone;
+      v[k] = Wide<T>{};
+      if (e[k].state == kSum)
+        __builtin_memcpy(&v[k], sums_in + ((base + j0 + k) * o.chunks + p.chunk) * Chunk<T>::kVec, sizeof(v[k]));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (e[k].state == kNone) continue;  // (never inside a run)
+      if (!open || e[k].row != row) {
+        if (open) writer.finish(row, sum, left, false);
+        open = true;
+        row = e[k].row;
+        left = j0 + k == 0 && before.state != kNone && before.row == row;
+        sum = Wide<T>{};
+      }
+      sum += v[k];
+    }
+  }
+  if (open) writer.finish(row, sum, left, behind.state != kNone && behind.row == row);
+  writer.entries();
+}
+
+// ------------------------------------------------------------------- plans ----
+// The tiles of every launch: a function of the sizes alone.
+constexpr int kJoinSize = 64;
+constexpr int kMaxLevels = 8;
+
+struct SumPlan {
+  int64_t n, chunks;
+  int group, slices;  // lanes a group, groups over a row
+  int size;           // positions a tile of the first launch
+  int levels;
+  int64_t tiles[kMaxLevels];
+
+  SumPlan(int64_t n_, int64_t dim, int type) : n(n_) {
+    chunks = type == GS_F32 ? chunks_of<float>(dim) : chunks_of<_Float16>(dim);
+    group = 1;
+    while (group < kWave && group < chunks) group *= 2;
+    slices = static_cast<int>((chunks + group - 1) / group);
+    // as long as there are waves enough for the chip, longer tiles leave fewer partial sums
+    size = 32;
+    while (size > 8 && (n / size) * slices * group < int64_t(256) * 16 * kWave) size /= 2;
+    levels = 0;
+    int64_t t = (n + size - 1) / size;
+    tiles[levels++] = t;
+    while (t > 1) {
+      t = (2 * t + kJoinSize - 1) / kJoinSize;
+      tiles[levels++] = t;
+    }
+  }
+  int vec(int type) const { return 16 / value_bytes(type); }
+  size_t sums_bytes(int level, int type) const {
+    return static_cast<size_t>(2 * tiles[level]) * chunks * vec(type) * sizeof(float);
+  }
+};
+
+struct GradSpace {
+  key_sort::Space sort;
+  key_sort::Word* sorted;
+  int64_t* rank;        // sparse
+  int64_t* scan_tiles;  // sparse
+  Entry* entries[2];
+  float* sums[2];
+};
+
+// even levels write buffer 0, odd ones buffer 1, each sized for the first of them
+size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
+  size_t bytes = key_sort::space_bytes(p.n, 2);
+  if (sparse) bytes += padded(static_cast<size_t>(p.n + 1) * 8) + scan_workspace_bytes(p.n);
+  for (int l = 0; l < 2 && l + 1 < p.levels; ++l)
+    bytes += padded(static_cast<size_t>(2 * p.tiles[l]) * sizeof(Entry)) + padded(p.sums_bytes(l, type));
+  return bytes;
+}
+
+bool carve_grad(Carver& ws, const SumPlan& p, int type, uint32_t num_rows, bool sparse, GradSpace* s) {
+  key_sort::carve(ws, p.n, 2, &s->sort);
+  s->sorted = s->sort.word[(key_sort::passes_for(num_rows) - 1) & 1];
+  s->rank = sparse ? ws.take<int64_t>(static_cast<size_t>(p.n + 1)) : nullptr;
+  s->scan_tiles = sparse ? ws.take<int64_t>(scan_workspace_bytes(p.n) / 8) : nullptr;
+  for (int l = 0; l < 2; ++l) {
+    s->entries[l] = nullptr;
+    s->sums[l] = nullptr;
+    if (l + 1 < p.levels) {
+      s->entries[l] = ws.take<Entry>(static_cast<size_t>(2 * p.tiles[l]));
+      s->sums[l] = ws.take<float>(p.sums_bytes(l, type) / sizeof(float));
+    }
+  }
+  return ws.ok;
+}
+
+template <typename F>
+void with_group(int group, F&& f) {
+  switch (group) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 8: f(std::integral_constant<int, 8>()); break;
+    case 16: f(std::integral_constant<int, 16>()); break;
+    case 32: f(std::integral_constant<int, 32>()); break;
+    default: f(std::integral_constant<int, 64>()); break;
+  }
+}
+
+template <typename T>
+void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const T* grad, int64_t stride, int64_t dim,
+                 float scale, int64_t* met, T* out, hipStream_t st) {
+  with_group(p.group, [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    for (int l = 0; l < p.levels; ++l) {
+      const bool last = l == p.levels - 1;
+      const RunsOut o{scale, dim, p.chunks, p.slices, l == 0 ? met : nullptr, s.rank,
+                      last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
+      const dim3 grid(static_cast<unsigned>((p.tiles[l] * p.slices + kThreads / G - 1) / (kThreads / G)));
+      if (l == 0)
+        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(kThreads), 0, st, s.sorted, p.n, num_rows, grad, stride,
+                           p.size, p.tiles[0], o, out);
+      else
+        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(kThreads), 0, st, s.entries[(l - 1) & 1],
+                           2 * p.tiles[l - 1], s.sums[(l - 1) & 1], kJoinSize, p.tiles[l], o, out);
+    }
+  });
+}
+
+// heads of the sorted runs of rows that are there
+struct RunHeads {
+  const key_sort::Word* word;
+  uint32_t num_rows;
+  __device__ __forceinline__ int64_t operator()(int64_t i) const {
+    const uint32_t key = key_sort::key_of(word[i]);
+    const uint32_t before = key_sort::key_of(word[i > 0 ? i - 1 : 0]);
+    return key < num_rows && (i == 0 || before != key);
+  }
+};
+
+template <typename IdT>
+void sort_ids(const IdT* ids, int64_t n, uint32_t num_rows, const GradSpace& s, hipStream_t st) {
+  key_sort::sort(key_sort::IdWords<IdT>{ids, num_rows}, n, num_rows, s.sort, key_sort::WordsOut{s.sorted}, st);
+}
+
+int check_rows(const char* what, const void* rows, int64_t stride, int64_t dim, int type, int64_t n, int64_t num_rows) {
+  GS_REQUIRE(type == GS_F32 || type == GS_F16 || type == GS_BF16, "%s: value type %d is none of GS_F32, GS_F16, GS_BF16",
+             what, type);
+  GS_REQUIRE(n >= 0 && n < (int64_t(1) << 31), "%s: %lld ids, at most 2^31 - 1 are taken", what, static_cast<long long>(n));
+  GS_REQUIRE(num_rows >= 0 && num_rows < (int64_t(1) << 32) - 1, "%s: %lld rows, at most 2^32 - 2 are taken", what,
+             static_cast<long long>(num_rows));
+  GS_REQUIRE(dim >= 0 && dim < (int64_t(1) << 24), "%s: rows of %lld values, at most 2^24 - 1 are taken", what,
+             static_cast<long long>(dim));
+  GS_REQUIRE(stride >= 0, "%s: negative stride", what);
+  GS_REQUIRE(aligned_to(rows, value_bytes(type)), "%s: rows not aligned to their type", what);
+  return GS_OK;
+}
+int check_ids(const char* what, const void* ids, int id_bytes, int64_t n) {
+  GS_REQUIRE(valid_id_bytes(id_bytes), "%s: id_bytes must be 4 or 8, got %d", what, id_bytes);
+  GS_REQUIRE(n == 0 || ids, "%s: ids is null", what);
+  GS_REQUIRE(aligned_to(ids, id_bytes), "%s: ids not aligned to their type", what);
+  return GS_OK;
+}
+// whether every launch of the sums has a grid that can be launched
+int check_plan(const char* what, const SumPlan& p) {
+  if (p.tiles[0] * p.slices < (int64_t(1) << 31)) return GS_OK;
+  set_error_text("%s: %lld rows of %lld chunks are more than one launch takes", what, static_cast<long long>(p.n),
+                 static_cast<long long>(p.chunks));
+  return GS_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" {
+
+int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride, int64_t dim, int type,
+                        const void* ids, int id_bytes, int64_t n, float scale, void* out, void* stream) {
+  GS_RETURN_IF_ERROR(check_rows("gs_embedding_lookup", table, row_stride, dim, type, n, num_rows));
+  GS_RETURN_IF_ERROR(check_ids("gs_embedding_lookup", ids, id_bytes, n));
+  if (n == 0 || dim == 0) return GS_OK;
+  GS_REQUIRE(out && (table || num_rows == 0), "gs_embedding_lookup: null array");
+  GS_REQUIRE(aligned_to(out, value_bytes(type)), "gs_embedding_lookup: out not aligned to its type");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return with_value_type(type, "gs_embedding_lookup", [&](auto zero) {
+    using T = decltype(zero);
+    const int64_t chunks = chunks_of<T>(dim), total = n * chunks;
+    // four chunks a lane where that still leaves a workgroup for every compute unit
+    constexpr int kMany = 4;
+    const bool many = total >= int64_t(256) * kThreads * kMany;
+    const int64_t blocks = (total + kThreads * (many ? kMany : 1) - 1) / (kThreads * (many ? kMany : 1));
+    if (blocks >= (int64_t(1) << 31)) {
+      set_error_text("gs_embedding_lookup: %lld rows of %lld values are more than one launch takes",
+                     static_cast<long long>(n), static_cast<long long>(dim));
+      return static_cast<int>(GS_ERR_UNSUPPORTED);
+    }
+    const Divider by(static_cast<uint32_t>(chunks));
+    return with_id_type(id_bytes, [&](auto id) {
+      using IdT = decltype(id);
+      auto* kernel = many ? lookup_kernel<T, IdT, kMany> : lookup_kernel<T, IdT, 1>;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st,
+                         static_cast<const T*>(table), num_rows, row_stride, dim, by, static_cast<const IdT*>(ids), total,
+                         scale, static_cast<T*>(out));
+      return check_launch("embedding_lookup");
+    });
+  });
+}
+
+size_t gs_embedding_grad_workspace_bytes(int64_t n, int64_t dim, int type) {
+  if (n <= 0 || dim <= 0) return 256;
+  return grad_bytes(SumPlan(n, dim, type), type, false);
+}
+
+int gs_embedding_grad(const void* grad, int64_t grad_stride, int64_t dim, int type, const void* ids, int id_bytes,
+                      int64_t n, int64_t num_rows, float scale, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  GS_RETURN_IF_ERROR(check_rows("gs_embedding_grad", grad, grad_stride, dim, type, n, num_rows));
+  GS_RETURN_IF_ERROR(check_ids("gs_embedding_grad", ids, id_bytes, n));
+  if (num_rows == 0 || dim == 0) return GS_OK;
+  GS_REQUIRE(out && (grad || n == 0), "gs_embedding_grad: null array");
+  GS_REQUIRE(aligned_to(out, value_bytes(type)), "gs_embedding_grad: out not aligned to its type");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const SumPlan plan(n > 0 ? n : 1, dim, type);
+  GS_RETURN_IF_ERROR(check_plan("gs_embedding_grad", plan));
+  GradSpace space;
+  if (n > 0) {
+    Carver ws(workspace, workspace_bytes);
+    if (!carve_grad(ws, plan, type, static_cast<uint32_t>(num_rows), false, &space)) {
+      set_error_text("gs_embedding_grad: workspace needs %zu bytes, 256-byte aligned",
+                     gs_embedding_grad_workspace_bytes(n, dim, type));
+      return GS_ERR_WORKSPACE;
+    }
+  }
+  return with_value_type(type, "gs_embedding_grad", [&](auto zero) {
+    using T = decltype(zero);
+    const int64_t values = num_rows * dim;
+    hipLaunchKernelGGL(zero_kernel<T>, dim3(values < (int64_t(1) << 22) ? 256 : 2048), dim3(kThreads), 0, st,
+                       static_cast<T*>(out), values);
+    if (n > 0) {
+      with_id_type(id_bytes, [&](auto id) {
+        using IdT = decltype(id);
+        sort_ids(static_cast<const IdT*>(ids), n, static_cast<uint32_t>(num_rows), space, st);
+        return 0;
+      });
+      launch_sums(plan, space, static_cast<uint32_t>(num_rows), static_cast<const T*>(grad), grad_stride, dim, scale,
+                  nullptr, static_cast<T*>(out), st);
+    }
+    return check_launch("embedding_grad");
+  });
+}
+
+size_t gs_embedding_sparse_grad_workspace_bytes(int64_t n, int64_t dim, int type) {
+  if (n <= 0) return 256;
+  return grad_bytes(SumPlan(n, dim > 0 ? dim : 1, type), type, true);
+}
+
+int gs_embedding_sparse_grad_count(const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t dim, int type,
+                                   gs_mailbox* mailbox, int64_t ticket, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  GS_RETURN_IF_ERROR(check_rows("gs_embedding_sparse_grad_count", nullptr, 0, dim, type, n, num_rows));
+  GS_RETURN_IF_ERROR(check_ids("gs_embedding_sparse_grad_count", ids, id_bytes, n));
+  GS_REQUIRE(n > 0, "gs_embedding_sparse_grad_count: no ids");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const SumPlan plan(n, dim > 0 ? dim : 1, type);
+  GradSpace space;
+  Carver ws(workspace, workspace_bytes);
+  const uint32_t rows = static_cast<uint32_t>(num_rows);
+  if (!carve_grad(ws, plan, type, rows, true, &space)) {
+    set_error_text("gs_embedding_sparse_grad_count: workspace needs %zu bytes, 256-byte aligned",
+                   gs_embedding_sparse_grad_workspace_bytes(n, dim, type));
+    return GS_ERR_WORKSPACE;
+  }
+  with_id_type(id_bytes, [&](auto id) {
+    using IdT = decltype(id);
+    sort_ids(static_cast<const IdT*>(ids), n, rows, space, st);
+    return 0;
+  });
+  return exclusive_scan(RunHeads{space.sorted, rows}, n, space.rank, space.scan_tiles, st, mailbox, ticket);
+}
+
+int gs_embedding_sparse_grad_fill(const void* grad, int64_t grad_stride, int64_t dim, int type, int64_t n,
+                                  int64_t num_rows, float scale, int64_t* met, void* values, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  GS_RETURN_IF_ERROR(check_rows("gs_embedding_sparse_grad_fill", grad, grad_stride, dim, type, n, num_rows));
+  GS_REQUIRE(n > 0 && met && ((grad && values) || dim == 0), "gs_embedding_sparse_grad_fill: no ids or null array");
+  GS_REQUIRE(aligned_to(values, value_bytes(type)), "gs_embedding_sparse_grad_fill: values not aligned to their type");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const SumPlan plan(n, dim > 0 ? dim : 1, type);
+  GS_RETURN_IF_ERROR(check_plan("gs_embedding_sparse_grad_fill", plan));
+  GradSpace space;
+  Carver ws(workspace, workspace_bytes);
+  const uint32_t rows = static_cast<uint32_t>(num_rows);
+  if (!carve_grad(ws, plan, type, rows, true, &space)) {
+    set_error_text("gs_embedding_sparse_grad_fill: workspace needs %zu bytes, 256-byte aligned",
+                   gs_embedding_sparse_grad_workspace_bytes(n, dim, type));
+    return GS_ERR_WORKSPACE;
+  }
+  return with_value_type(type, "gs_embedding_sparse_grad_fill", [&](auto zero) {
+    using T = decltype(zero);
+    launch_sums(plan, space, rows, static_cast<const T*>(grad), grad_stride, dim, scale, met, static_cast<T*>(values), st);
+    return check_launch("embedding_sparse_grad_fill");
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,413 @@
+// Rows sorted by expert and back, with weights applied, and the gradients, on gfx950.
+//
+// T tokens choose K experts of E each; item t * K + k is token t's k-th choice.  The items sorted by
+// expert, stably, are the order in which the experts' rows lie:
+//   place[t, k]            where item t * K + k lies, -1 when its choice names no expert
+//   order[place[t, k]]     = t * K + k, -1 behind the last
+//   gather   rows[place[t, k], :] = x[t, :], zeros behind the last
+//   combine  out[t, :]     = sum over k of weights[t, k] * y[place[t, k], :]
+//   its gradient: dy[place[t, k], :] = weights[t, k] * dout[t, :], dweights[t, k] = <dout[t, :], y[place[t, k], :]>
+//   (the gradient of the gather is a combine without weights).
+// No counterpart in the reference.  With one choice each, the experts may be node types or relations.
+// Every row moves once: the kernels go by token, read its row once, and reach the experts' rows through
+// `place`.  What bounds them is the rows' bytes; products and sums are fp32, rounded once at the end.
+#include "gs_key_sort.hpp"
+#include "gs_rows.hpp"
+
+namespace gs {
+namespace {
+
+constexpr int kThreads = 256;
+
+// -------------------------------------------------------------------- sort ----
+// Sorted items of fewer than 256 experts (one pass, which knows where every expert begins).
+struct OrderOut {
+  int32_t* order;
+  int32_t* place;
+  int64_t* offsets;
+  uint32_t experts;
+  __device__ __forceinline__ void digit(uint32_t d, uint32_t start) const {
+    if (d <= experts) offsets[d] = start;
+  }
+  __device__ __forceinline__ void item(uint32_t at, key_sort::Word w) const {
+    const bool there = key_sort::key_of(w) < experts;
+    place[key_sort::position_of(w)] = there ? static_cast<int32_t>(at) : -1;
+    order[at] = there ? static_cast<int32_t>(key_sort::position_of(w)) : -1;
+  }
+};
+
+// The same from words sorted in several passes, and where the experts begin, by search.
+__global__ void __launch_bounds__(kThreads)
+order_kernel(const key_sort::Word* __restrict__ words, int64_t n, OrderOut out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i < n) out.item(static_cast<uint32_t>(i), words[i]);
+  if (i <= static_cast<int64_t>(out.experts)) {
+    int64_t lo = 0, hi = n;  // items of the experts before i
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (key_sort::key_of(words[mid]) < static_cast<uint32_t>(i)) lo = mid + 1; else hi = mid;
+    }
+    out.offsets[i] = lo;
+  }
+}
+__global__ void __launch_bounds__(kThreads) no_items_kernel(int64_t* __restrict__ offsets, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads)
+    offsets[i] = 0;
+}
+
+// ------------------------------------------------------------------ gather ----
+// Zeros in the rows from `live` (read on the device) to n, a share of them by every workgroup.
+template <typename T>
+__device__ __forceinline__ void zero_rows_behind(const int64_t* __restrict__ live, int64_t n, int64_t dim,
+                                                 const Divider& chunks, T* __restrict__ rows) {
+  const int64_t from = *live;
+  if (from >= n || from < 0) return;
+  const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
+    const int64_t row = i / chunks.d;
+    store_chunk(rows + (from + row) * dim + chunk_start<T>(dim, i - row * chunks.d), Values<T>{}, dim);
+  }
+}
+
+// A chunk of a token a lane (ITEMS of them): read once, written to every choice's place.
+template <typename T, int ITEMS>
+__global__ void __launch_bounds__(kThreads)
+gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
+              int64_t total, int choices, int64_t n, const int64_t* __restrict__ live, T* __restrict__ rows) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * ITEMS);
+  const RowRange range(chunks, first);
+  int64_t token[ITEMS], at[ITEMS];
+  Values<T> v[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const uint32_t j = i * kThreads + threadIdx.x;
+    uint32_t c;
+    token[i] = range.row(first + j < total ? j : 0, &c);
+    at[i] = chunk_start<T>(dim, c);
+    v[i] = load_chunk(x + token[i] * stride + at[i], dim);
+    if (first + j >= total) token[i] = -1;
+  }
+  for (int k = 0; k < choices; ++k) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if (token[i] < 0) continue;
+      const int64_t to = place[token[i] * choices + k];
+      if (to >= 0 && to < n) store_chunk(rows + to * dim + at[i], v[i], dim);
+    }
+  }
+  zero_rows_behind(live, n, dim, chunks, rows);
+}
+
+// ----------------------------------------------------------------- combine ----
+template <typename W>
+__device__ __forceinline__ float weight_of(const W* weights, int64_t item) {
+  return weights ? static_cast<float>(weights[item]) : 1.0f;
+}
+
+// A chunk of a token's sum a lane; the rows of KU choices are asked for together.
+template <typename T, typename W, int KU>
+__global__ void __launch_bounds__(kThreads)
+combine_kernel(const T* __restrict__ y, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
+               int64_t total, int choices, int64_t n, const W* __restrict__ weights, T* __restrict__ out) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+  if (first + threadIdx.x >= total) return;
+  const RowRange range(chunks, first);
+  uint32_t c;
+  const int64_t token = range.row(threadIdx.x, &c), at = chunk_start<T>(dim, c);
+  Wide<T> sum = {};
+  for (int k0 = 0; k0 < choices; k0 += KU) {
+    Values<T> v[KU];
+    float w[KU];
+    bool there[KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+      const int64_t item = token * choices + (k0 + u < choices ? k0 + u : k0);
+      const int64_t from = place[item];
+      there[u] = k0 + u < choices && from >= 0 && from < n;
+      w[u] = weight_of(weights, item);
+      v[u] = Values<T>{};
+      if (there[u]) v[u] = load_chunk(y + from * stride + at, dim);
+    }
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+      if (there[u]) sum += widen<T>(v[u]) * w[u];
+  }
+  store_chunk(out + token * dim + at, narrow<T>(sum), dim);
+}
+
+// ---------------------------------------------------- gradient of the combine ----
+// A group of G lanes a token (or a whole workgroup, WAVES = 4): dout's chunk is read once for KU
+// choices, y's rows give the weights' gradients, dy's rows are written.
+template <typename T, typename W, int G, int WAVES, int KU>
+__global__ void __launch_bounds__(kThreads)
+combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ y, int64_t y_stride,
+                    int64_t dim, Divider chunks, const int32_t* __restrict__ place, int64_t tokens, int choices,
+                    int64_t n, const int64_t* __restrict__ live, const W* __restrict__ weights, T* __restrict__ dy,
+                    W* __restrict__ dweights) {
+  constexpr int kLanes = G * WAVES;               // of a token
+  constexpr int kTokens = kThreads / kLanes;      // of a workgroup
+  __shared__ float s_dots[WAVES > 1 ? WAVES * KU : 1];
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t token = t < tokens ? t : tokens - 1;  // (works along, writes nothing)
+  for (int k0 = 0; k0 < choices; k0 += KU) {
+    int64_t from[KU];
+    float w[KU], dot[KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+      const int64_t item = token * choices + (k0 + u < choices ? k0 + u : k0);
+      from[u] = place[item];
+      w[u] = weight_of(weights, item);
+      dot[u] = 0.0f;
+      if (k0 + u >= choices || from[u] < 0 || from[u] >= n || t >= tokens) from[u] = -1;
+    }
+    for (int64_t c = lane; c < chunks.d; c += kLanes) {
+      const int64_t at = chunk_start<T>(dim, c);
+      const int64_t overlap = c * Chunk<T>::kVec - at;  // values of the chunk before
+      const Wide<T> d = widen<T>(load_chunk(dout + token * dout_stride + at, dim));
+      Values<T> v[KU];
+      if (dweights) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+          v[u] = Values<T>{};
+          if (from[u] >= 0) v[u] = load_chunk(y + from[u] * y_stride + at, dim);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        if (dweights && from[u] >= 0) {
+          const Wide<T> b = widen<T>(v[u]);
+#pragma unroll
+          for (int i = 0; i < Chunk<T>::kVec; ++i)
+            if (i >= overlap) dot[u] = __fmaf_rn(d[i], b[i], dot[u]);
+        }
+        if (dy && from[u] >= 0) store_chunk(dy + from[u] * dim + at, narrow<T>(d * w[u]), dim);
+      }
+    }
+    if (!dweights) continue;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int m = G / 2; m > 0; m /= 2) dot[u] += __shfl_xor(dot[u], m, kWave);
+    if (WAVES > 1) {
+      if (lane % kWave == 0) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) s_dots[(lane / kWave) * KU + u] = dot[u];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        dot[u] = 0.0f;
+        for (int wv = 0; wv < WAVES; ++wv) dot[u] += s_dots[wv * KU + u];
+      }
+      __syncthreads();
+    }
+    if (lane == 0 && t < tokens) {
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        if (k0 + u < choices) dweights[token * choices + k0 + u] = static_cast<W>(from[u] >= 0 ? dot[u] : 0.0f);
+    }
+  }
+  if (dy) zero_rows_behind(live, n, dim, chunks, dy);
+}
+
+// ------------------------------------------------------------------- checks ----
+int check_shape(const char* what, int64_t tokens, int64_t choices, int64_t experts) {
+  GS_REQUIRE(tokens >= 0 && choices >= 0 && experts >= 0, "%s: negative size", what);
+  GS_REQUIRE(choices < (int64_t(1) << 31) && (choices == 0 || tokens <= ((int64_t(1) << 31) - 1) / choices),
+             "%s: tokens x choices, at most 2^31 - 1 are taken", what);
+  GS_REQUIRE(experts < (int64_t(1) << 31), "%s: %lld experts, at most 2^31 - 1 are taken", what,
+             static_cast<long long>(experts));
+  return GS_OK;
+}
+int check_values(const char* what, int type, int64_t dim, int64_t stride) {
+  GS_REQUIRE(type == GS_F32 || type == GS_F16 || type == GS_BF16, "%s: value type %d is none of GS_F32, GS_F16, GS_BF16",
+             what, type);
+  GS_REQUIRE(dim >= 0 && dim < (int64_t(1) << 24), "%s: rows of %lld values, at most 2^24 - 1 are taken", what,
+             static_cast<long long>(dim));
+  GS_REQUIRE(stride >= 0, "%s: negative stride", what);
+  return GS_OK;
+}
+int check_grid(const char* what, int64_t blocks) {
+  if (blocks < (int64_t(1) << 31)) return GS_OK;
+  set_error_text("%s: more rows and values than one launch takes", what);
+  return GS_ERR_UNSUPPORTED;
+}
+
+// weights are fp32 or of the rows' type
+template <typename T, typename F>
+int with_weight_type(int type, int weight_type, const char* what, F&& f) {
+  if (weight_type == GS_F32) return f(float(0));
+  if (weight_type == type) return f(T(0));
+  set_error_text("%s: weights are fp32 or of the rows' type", what);
+  return GS_ERR_INVALID_ARG;
+}
+template <typename F>
+void with_choices(int64_t choices, F&& f) {
+  if (choices <= 1) f(std::integral_constant<int, 1>());
+  else if (choices == 2) f(std::integral_constant<int, 2>());
+  else if (choices <= 4) f(std::integral_constant<int, 4>());
+  else f(std::integral_constant<int, 8>());
+}
+
+template <typename T>
+int launch_gather(const T* x, int64_t stride, int64_t dim, const int32_t* place, int64_t tokens, int64_t choices,
+                  const int64_t* live, T* rows, hipStream_t st, const char* what) {
+  const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks;
+  constexpr int kMany = 4;
+  const bool many = total >= int64_t(256) * 4 * kThreads * kMany;
+  const int64_t blocks = (total + kThreads * (many ? kMany : 1) - 1) / (kThreads * (many ? kMany : 1));
+  GS_RETURN_IF_ERROR(check_grid(what, blocks));
+  auto* kernel = many ? gather_kernel<T, kMany> : gather_kernel<T, 1>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, x, stride, dim,
+                     Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices), tokens * choices, live,
+                     rows);
+  return check_launch(what);
+}
+
+template <typename T, typename W, int G, int WAVES>
+int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t y_stride, int64_t dim,
+                        const int32_t* place, int64_t tokens, int64_t choices, const int64_t* live, const W* weights,
+                        T* dy, W* dweights, hipStream_t st) {
+  constexpr int kTokens = kThreads / (G * WAVES);
+  const dim3 grid(static_cast<unsigned>((tokens + kTokens - 1) / kTokens));
+  with_choices(choices, [&](auto ku) {
+    hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st, dout,
+                       dout_stride, y, y_stride, dim, Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place, tokens,
+                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights);
+  });
+  return check_launch("expert_combine_grad");
+}
+
+template <typename IdT>
+int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOut& out, void* workspace,
+               size_t workspace_bytes, hipStream_t st) {
+  if (n == 0) {
+    hipLaunchKernelGGL(no_items_kernel, dim3(blocks_for(num_experts + 1 < (1 << 20) ? num_experts + 1 : (1 << 20), kThreads)),
+                       dim3(kThreads), 0, st, out.offsets, num_experts + 1);
+    return check_launch("expert_sort");
+  }
+  const uint32_t num = static_cast<uint32_t>(num_experts);
+  const int passes = key_sort::passes_for(num);
+  Carver ws(workspace, workspace_bytes);
+  key_sort::Space space;
+  key_sort::carve(ws, n, passes > 1 ? 2 : 0, &space);
+  if (!ws.ok) {
+    set_error_text("gs_expert_sort: workspace needs %zu bytes, 256-byte aligned",
+                   gs_expert_sort_workspace_bytes(n, num_experts));
+    return GS_ERR_WORKSPACE;
+  }
+  const key_sort::IdWords<IdT> src{experts, num};
+  if (passes == 1) {
+    key_sort::sort(src, n, num, space, out, st);
+  } else {
+    key_sort::Word* sorted = space.word[(passes - 1) & 1];
+    key_sort::sort(src, n, num, space, key_sort::WordsOut{sorted}, st);
+    const int64_t threads = n > num_experts + 1 ? n : num_experts + 1;
+    hipLaunchKernelGGL(order_kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
+                       st, sorted, n, out);
+  }
+  return check_launch("expert_sort");
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" {
+
+size_t gs_expert_sort_workspace_bytes(int64_t n, int64_t num_experts) {
+  if (n <= 0 || num_experts < 0) return 256;
+  const uint32_t num = static_cast<uint32_t>(num_experts);
+  return key_sort::space_bytes(n, key_sort::passes_for(num) > 1 ? 2 : 0);
+}
+
+int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_experts, int32_t* order, int32_t* place,
+                   int64_t* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+  GS_RETURN_IF_ERROR(check_shape("gs_expert_sort", n, 1, num_experts));
+  GS_REQUIRE(valid_id_bytes(id_bytes), "gs_expert_sort: id_bytes must be 4 or 8, got %d", id_bytes);
+  GS_REQUIRE(offsets && (n == 0 || (experts && order && place)), "gs_expert_sort: null array");
+  GS_REQUIRE(aligned_to(experts, id_bytes), "gs_expert_sort: ids not aligned to their type");
+  const OrderOut out{order, place, offsets, static_cast<uint32_t>(num_experts)};
+  return with_id_type(id_bytes, [&](auto id) {
+    using IdT = decltype(id);
+    return sort_items(static_cast<const IdT*>(experts), n, num_experts, out, workspace, workspace_bytes,
+                      static_cast<hipStream_t>(stream));
+  });
+}
+
+int gs_expert_gather(const void* x, int64_t x_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
+                     int64_t choices, const int64_t* live, void* rows, void* stream) {
+  GS_RETURN_IF_ERROR(check_shape("gs_expert_gather", tokens, choices, 0));
+  GS_RETURN_IF_ERROR(check_values("gs_expert_gather", type, dim, x_stride));
+  if (tokens == 0 || choices == 0 || dim == 0) return GS_OK;
+  GS_REQUIRE(x && place && live && rows, "gs_expert_gather: null array");
+  GS_REQUIRE(aligned_to(x, value_bytes(type)) && aligned_to(rows, value_bytes(type)),
+             "gs_expert_gather: rows not aligned to their type");
+  return with_value_type(type, "gs_expert_gather", [&](auto zero) {
+    using T = decltype(zero);
+    return launch_gather(static_cast<const T*>(x), x_stride, dim, place, tokens, choices, live, static_cast<T*>(rows),
+                         static_cast<hipStream_t>(stream), "gs_expert_gather");
+  });
+}
+
+int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
+                      int64_t choices, const void* weights, int weight_type, void* out, void* stream) {
+  GS_RETURN_IF_ERROR(check_shape("gs_expert_combine", tokens, choices, 0));
+  GS_RETURN_IF_ERROR(check_values("gs_expert_combine", type, dim, y_stride));
+  if (tokens == 0 || dim == 0) return GS_OK;
+  GS_REQUIRE(out && (choices == 0 || (y && place)), "gs_expert_combine: null array");
+  GS_REQUIRE(aligned_to(y, value_bytes(type)) && aligned_to(out, value_bytes(type)),
+             "gs_expert_combine: rows not aligned to their type");
+  return with_value_type(type, "gs_expert_combine", [&](auto zero) {
+    using T = decltype(zero);
+    return with_weight_type<T>(type, weights ? weight_type : GS_F32, "gs_expert_combine", [&](auto wzero) {
+      using W = decltype(wzero);
+      const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks;
+      const int64_t blocks = (total + kThreads - 1) / kThreads;
+      GS_RETURN_IF_ERROR(check_grid("gs_expert_combine", blocks));
+      with_choices(choices, [&](auto ku) {
+        hipLaunchKernelGGL((combine_kernel<T, W, decltype(ku)::value>), dim3(static_cast<unsigned>(blocks)),
+                           dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(y), y_stride, dim,
+                           Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices),
+                           tokens * choices, static_cast<const W*>(weights), static_cast<T*>(out));
+      });
+      return check_launch("expert_combine");
+    });
+  });
+}
+
+int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int64_t dim, int type,
+                           const int32_t* place, int64_t tokens, int64_t choices, const int64_t* live,
+                           const void* weights, int weight_type, void* dy, void* dweights, void* stream) {
+  GS_RETURN_IF_ERROR(check_shape("gs_expert_combine_grad", tokens, choices, 0));
+  GS_RETURN_IF_ERROR(check_values("gs_expert_combine_grad", type, dim, dout_stride));
+  GS_REQUIRE(y_stride >= 0, "gs_expert_combine_grad: negative stride");
+  if (tokens == 0 || choices == 0 || (!dy && !dweights)) return GS_OK;
+  GS_REQUIRE(place && live, "gs_expert_combine_grad: null array");
+  GS_REQUIRE(dim == 0 || (dout && (!dweights || y)), "gs_expert_combine_grad: null array");
+  GS_REQUIRE(aligned_to(dout, value_bytes(type)) && aligned_to(y, value_bytes(type)) && aligned_to(dy, value_bytes(type)),
+             "gs_expert_combine_grad: rows not aligned to their type");
+  return with_value_type(type, "gs_expert_combine_grad", [&](auto zero) {
+    using T = decltype(zero);
+    return with_weight_type<T>(type, weights || dweights ? weight_type : GS_F32, "gs_expert_combine_grad", [&](auto wzero) {
+      using W = decltype(wzero);
+      const int64_t chunks = chunks_of<T>(dim);
+      auto go = [&](auto lanes, auto waves) {
+        return launch_combine_grad<T, W, decltype(lanes)::value, decltype(waves)::value>(
+            static_cast<const T*>(dout), dout_stride, static_cast<const T*>(y), y_stride, dim, place, tokens, choices,
+            live, static_cast<const W*>(weights), static_cast<T*>(dy), static_cast<W*>(dweights),
+            static_cast<hipStream_t>(stream));
+      };
+      using One = std::integral_constant<int, 1>;
+      if (chunks <= 4) return go(std::integral_constant<int, 4>(), One());
+      if (chunks <= 16) return go(std::integral_constant<int, 16>(), One());
+      if (chunks <= kWave || tokens >= 4096) return go(std::integral_constant<int, kWave>(), One());
+      return go(std::integral_constant<int, kWave>(), std::integral_constant<int, kThreads / kWave>());
+    });
+  });
+}
+
+}  // extern "C"

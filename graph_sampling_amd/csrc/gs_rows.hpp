@@ -1,0 +1,129 @@
+// Rows of values moved by ids (embedding rows, rows sent to experts): the pieces that
+// gs_embedding.hip and gs_experts.hip share.
+#pragma once
+
+#include "gs_common.hpp"
+
+namespace gs {
+
+// A row is moved in chunks of 16 bytes, one a lane.  Chunks are aligned like the values, not like
+// themselves: rows of an odd width are read in the same way (the memory pipeline takes 16 bytes from
+// any address here).  The last chunk of a row whose width is no multiple of the chunk starts
+// earlier and overlaps the one before; its values are read, or written the same, twice.
+template <typename T>
+struct Chunk {
+  static constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  typedef T Values __attribute__((ext_vector_type(kVec)));
+  typedef float Wide __attribute__((ext_vector_type(kVec)));
+};
+template <typename T>
+using Values = typename Chunk<T>::Values;
+template <typename T>
+using Wide = typename Chunk<T>::Wide;
+
+// chunks of a row, at least one
+template <typename T>
+constexpr int64_t chunks_of(int64_t dim) {
+  return dim <= Chunk<T>::kVec ? 1 : (dim + Chunk<T>::kVec - 1) / Chunk<T>::kVec;
+}
+// where chunk c of a row begins
+template <typename T>
+__device__ __forceinline__ int64_t chunk_start(int64_t dim, int64_t c) {
+  const int64_t at = c * Chunk<T>::kVec, last = dim - Chunk<T>::kVec;
+  return at < last ? at : (last > 0 ? last : 0);
+}
+
+// p: the chunk's first value; dim: the row's width (narrower rows than a chunk go value by value)
+template <typename T>
+__device__ __forceinline__ Values<T> load_chunk(const T* p, int64_t dim) {
+  Values<T> v = {};
+  if (dim >= Chunk<T>::kVec) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::kVec; ++i)
+      if (i < dim) v[i] = p[i];
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, Values<T> v, int64_t dim) {
+  if (dim >= Chunk<T>::kVec) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::kVec; ++i)
+      if (i < dim) p[i] = v[i];
+  }
+}
+template <typename T>
+__device__ __forceinline__ Wide<T> widen(Values<T> v) {
+  return __builtin_convertvector(v, Wide<T>);
+}
+template <typename T>  // one rounding, to nearest, ties to even
+__device__ __forceinline__ Values<T> narrow(Wide<T> v) {
+  return __builtin_convertvector(v, Values<T>);
+}
+
+// x / d for x < 2^31 by a product (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", 1994), 1 <= d < 2^31.
+struct Divider {
+  uint32_t mul = 1, shift = 0, d = 1;
+  Divider() = default;
+  explicit Divider(uint32_t by) : d(by) {
+    while ((uint64_t(1) << shift) < by) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+    return (__umulhi(mul, x) + x) >> shift;
+  }
+};
+
+// The chunks of all rows side by side, a workgroup a range of them: the row and the chunk in it of the
+// j-th chunk (j below 2^31 - d) behind the range's first one.
+struct RowRange {
+  Divider by;
+  int64_t row0;
+  uint32_t c0;
+  __device__ __forceinline__ RowRange(const Divider& chunks, int64_t first) : by(chunks) {
+    if (first < (int64_t(1) << 31)) {
+      const uint32_t q = chunks.quotient(static_cast<uint32_t>(first));
+      row0 = q;
+      c0 = static_cast<uint32_t>(first) - q * chunks.d;
+    } else {
+      row0 = first / chunks.d;
+      c0 = static_cast<uint32_t>(first - row0 * chunks.d);
+    }
+  }
+  __device__ __forceinline__ int64_t row(uint32_t j, uint32_t* chunk) const {
+    const uint32_t x = c0 + j, q = by.quotient(x);
+    *chunk = x - q * by.d;
+    return row0 + q;
+  }
+};
+
+// Which value type an entry point was given: calls f with a zero of the type.
+template <typename F>
+int with_value_type(int type, const char* what, F&& f) {
+  switch (type) {
+    case GS_F32:
+      return f(float(0));
+    case GS_F16:
+      return f(_Float16(0));
+    case GS_BF16:
+      return f(__bf16(0));
+    default:
+      set_error_text("%s: value type %d is none of GS_F32, GS_F16, GS_BF16", what, type);
+      return GS_ERR_INVALID_ARG;
+  }
+}
+template <typename F>
+int with_id_type(int id_bytes, F&& f) {
+  return id_bytes == 4 ? f(int32_t(0)) : f(int64_t(0));
+}
+inline int value_bytes(int type) { return type == GS_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) == 0;
+}
+
+}  // namespace gs

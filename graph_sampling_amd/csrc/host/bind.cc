@@ -10,6 +10,7 @@
 #include "graph_ops.h"
 #include "hetero_graph.h"
 #include "hip_ops.h"
+#include "row_ops.h"
 #include "sampler_pool.h"
 #include "tensor_ops.h"
 
@@ -158,6 +159,23 @@ TORCH_LIBRARY(gs_ops, m) {
   m.def("batch_list_sampling_with_probs", &BatchListSamplingProbs);
   m.def("_CAPI_IndexSearch", &IndexSearch);
   m.def("index_search", &IndexSearch);
+  // not in the reference: rows of values moved by ids, with gradients (row_ops.h)
+  m.def("_CAPI_Embedding", &Embedding);
+  m.def("embedding", &Embedding);
+  m.def("_CAPI_EmbeddingGrad", &gs::EmbeddingGrad);
+  m.def("embedding_grad", &gs::EmbeddingGrad);
+  m.def("_CAPI_EmbeddingSparseGrad", &gs::EmbeddingSparseGrad);
+  m.def("embedding_sparse_grad", &gs::EmbeddingSparseGrad);
+  m.def("_CAPI_ExpertSort", &gs::ExpertSort);
+  m.def("expert_sort", &gs::ExpertSort);
+  m.def("_CAPI_ExpertGather", &gs::ExpertGather);
+  m.def("expert_gather", &gs::ExpertGather);
+  m.def("_CAPI_ExpertDispatch", &ExpertDispatch);
+  m.def("expert_dispatch", &ExpertDispatch);
+  m.def("_CAPI_ExpertCombine", &gs::ExpertCombine);
+  m.def("expert_combine", &gs::ExpertCombine);
+  m.def("_CAPI_ExpertCombineGrad", &gs::ExpertCombineGrad);
+  m.def("expert_combine_grad", &gs::ExpertCombineGrad);
   // not in the reference: reproducible sampling (its seeds are compile-time constants)
   m.def("_CAPI_SetSeed", &SetSeed);
   m.def("_CAPI_SetThreadSeed", &SetThreadSeed);

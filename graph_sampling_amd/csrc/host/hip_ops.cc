@@ -1,6 +1,7 @@
 #include "hip_ops.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
@@ -1888,6 +1889,220 @@ torch::Tensor IndexSearch(const torch::Tensor& data, const torch::Tensor& keys) 
                         out.data_ptr(), ws.data_ptr(), ws.numel(), Stream(data)),
         "gs_index_search");
   return out;
+}
+
+// ------------------------------------------------------- rows moved by ids ----
+namespace {
+int ValueType(const torch::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return GS_F32;
+    case torch::kFloat16: return GS_F16;
+    case torch::kBFloat16: return GS_BF16;
+    default:
+      TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  }
+}
+
+// A 2-D tensor whose rows the kernels can walk: values of a row side by side, rows any distance apart.
+struct Rows {
+  torch::Tensor t;  // keeps a copy alive
+  int64_t stride;
+  int type;
+  Rows(const torch::Tensor& rows, const char* name) : t(rows) {
+    TORCH_CHECK(t.defined(), name, " is undefined");
+    TORCH_CHECK(t.is_cuda(), "Not implemented warning: ", name, " must be a GPU tensor");
+    TORCH_CHECK(t.layout() == torch::kStrided, name, " must be a dense tensor");
+    TORCH_CHECK(t.dim() == 2, name, " must have two dimensions, got ", t.dim());
+    type = ValueType(t, name);
+    if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
+    if (t.is_neg()) t = t.resolve_neg();
+    stride = t.size(0) > 1 ? t.stride(0) : t.size(1);
+  }
+};
+
+torch::Tensor FlatIds(const torch::Tensor& ids, const torch::Device& device, const char* name) {
+  TORCH_CHECK(ids.defined(), name, " is undefined");
+  TORCH_CHECK(ids.is_cuda(), "Not implemented warning: ", name, " must be a GPU tensor");
+  TORCH_CHECK(ids.device() == device, name, " must be on ", device, ", got ", ids.device());
+  auto flat = ids.contiguous();
+  IdBytes(flat, name);
+  return flat;
+}
+
+torch::TensorOptions Like(const torch::Tensor& t) { return torch::dtype(t.scalar_type()).device(t.device()); }
+
+// tokens and choices of the places, which a caller may have made by itself
+struct Places {
+  int64_t tokens, choices;
+  torch::Tensor place;
+  Places(const torch::Tensor& p, const torch::Device& device) : place(p) {
+    NeedDevice(place, "place");
+    TORCH_CHECK(place.scalar_type() == torch::kInt32, "place must be int32, got ", place.scalar_type());
+    TORCH_CHECK(place.dim() == 1 || place.dim() == 2, "place must be [tokens] or [tokens, choices]");
+    TORCH_CHECK(place.device() == device, "place must be on ", device, ", got ", place.device());
+    tokens = place.size(0);
+    choices = place.dim() == 2 ? place.size(1) : 1;
+  }
+  const int32_t* data() const { return place.data_ptr<int32_t>(); }
+};
+const int64_t* LiveRows(const torch::Tensor& offsets, const torch::Device& device) {
+  NeedI64(offsets, "offsets");
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must be [experts + 1]");
+  TORCH_CHECK(offsets.device() == device, "offsets must be on ", device, ", got ", offsets.device());
+  return offsets.data_ptr<int64_t>() + offsets.numel() - 1;
+}
+struct Weights {
+  torch::Tensor t;
+  int type = GS_F32;
+  Weights(const torch::optional<torch::Tensor>& w, const Places& p, const torch::Tensor& rows) {
+    if (!w.has_value() || !w.value().defined()) return;
+    TORCH_CHECK(w.value().is_cuda(), "Not implemented warning: weights must be a GPU tensor");
+    TORCH_CHECK(w.value().device() == rows.device(), "weights must be on ", rows.device(), ", got ", w.value().device());
+    TORCH_CHECK(w.value().sizes() == p.place.sizes(), "weights must have the shape of place, ", p.place.sizes(), ", got ",
+                w.value().sizes());
+    TORCH_CHECK(w.value().scalar_type() == torch::kFloat32 || w.value().scalar_type() == rows.scalar_type(),
+                "weights must be float32 or of the rows' type, got ", w.value().scalar_type());
+    t = w.value().contiguous();
+    type = ValueType(t, "weights");
+  }
+  const void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+}  // namespace
+
+bool Capturing(const torch::Tensor& t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(Stream(t)), &status) == hipSuccess,
+              "hipStreamIsCapturing failed");
+  return status != hipStreamCaptureStatusNone;
+}
+
+torch::Tensor EmbeddingLookup(const torch::Tensor& table, const torch::Tensor& ids, double scale) {
+  const Rows w(table, "embedding table");
+  const auto flat = FlatIds(ids, table.device(), "ids");
+  c10::hip::HIPGuard on(table.device().index());
+  const int64_t dim = w.t.size(1);
+  auto sizes = ids.sizes().vec();
+  sizes.push_back(dim);
+  auto out = torch::empty(sizes, Like(table));
+  Check(gs_embedding_lookup(w.t.data_ptr(), w.t.size(0), w.stride, dim, w.type, flat.data_ptr(), IdBytes(flat, "ids"),
+                            flat.numel(), static_cast<float>(scale), out.data_ptr(), Stream(table)),
+        "gs_embedding_lookup");
+  return out;
+}
+
+torch::Tensor EmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& ids, int64_t num_rows, double scale) {
+  const Rows g(grad, "gradient");
+  const auto flat = FlatIds(ids, grad.device(), "ids");
+  TORCH_CHECK(flat.numel() == g.t.size(0), "a gradient of ", g.t.size(0), " rows for ", flat.numel(), " ids");
+  TORCH_CHECK(num_rows >= 0, "num_rows must be non-negative");
+  c10::hip::HIPGuard on(grad.device().index());
+  const int64_t n = flat.numel(), dim = g.t.size(1);
+  auto out = torch::empty({num_rows, dim}, Like(grad));
+  auto ws = Scratch(gs_embedding_grad_workspace_bytes(n, dim, g.type), grad);
+  Check(gs_embedding_grad(g.t.data_ptr(), g.stride, dim, g.type, flat.data_ptr(), IdBytes(flat, "ids"), n, num_rows,
+                          static_cast<float>(scale), out.data_ptr(), ws.data_ptr(), ws.numel(), Stream(grad)),
+        "gs_embedding_grad");
+  return out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(const torch::Tensor& grad, const torch::Tensor& ids,
+                                                             int64_t num_rows, double scale) {
+  const Rows g(grad, "gradient");
+  const auto flat = FlatIds(ids, grad.device(), "ids");
+  TORCH_CHECK(flat.numel() == g.t.size(0), "a gradient of ", g.t.size(0), " rows for ", flat.numel(), " ids");
+  TORCH_CHECK(num_rows >= 0, "num_rows must be non-negative");
+  TORCH_CHECK(!Capturing(grad), "a sparse gradient waits for the number of rows it holds: it cannot be recorded into "
+              "a graph (a dense one can)");
+  c10::hip::HIPGuard on(grad.device().index());
+  const int64_t n = flat.numel(), dim = g.t.size(1);
+  if (n == 0) return {torch::empty({0}, I64(grad)), torch::empty({0, dim}, Like(grad))};
+  void* st = Stream(grad);
+  auto ws = Scratch(gs_embedding_sparse_grad_workspace_bytes(n, dim, g.type), grad);
+  HostBoxes& boxes = Boxes(grad.get_device());
+  const int64_t ticket = boxes.next++;
+  Check(gs_embedding_sparse_grad_count(flat.data_ptr(), IdBytes(flat, "ids"), n, num_rows, dim, g.type,
+                                       boxes.slot(ticket), ticket, ws.data_ptr(), ws.numel(), st),
+        "gs_embedding_sparse_grad_count");
+  const int64_t met = WaitBox(boxes.slot(ticket), ticket, st, "gs_embedding_sparse_grad_count");
+  TORCH_CHECK(met >= 0 && met <= n, "gs_embedding_sparse_grad_count reported ", met, " rows of ", n, " ids");
+  auto rows = torch::empty({met}, I64(grad));
+  auto values = torch::empty({met, dim}, Like(grad));
+  if (met > 0)
+    Check(gs_embedding_sparse_grad_fill(g.t.data_ptr(), g.stride, dim, g.type, n, num_rows, static_cast<float>(scale),
+                                        rows.data_ptr<int64_t>(), values.data_ptr(), ws.data_ptr(), ws.numel(), st),
+          "gs_embedding_sparse_grad_fill");
+  return {rows, values};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> ExpertSort(const torch::Tensor& experts, int64_t num_experts) {
+  TORCH_CHECK(experts.defined(), "experts is undefined");
+  TORCH_CHECK(experts.dim() == 1 || experts.dim() == 2, "experts must be [tokens] or [tokens, choices], got ",
+              experts.sizes());
+  TORCH_CHECK(num_experts >= 0, "num_experts must be non-negative");
+  const auto flat = FlatIds(experts, experts.device(), "experts");
+  c10::hip::HIPGuard on(experts.device().index());
+  const int64_t n = flat.numel();
+  const auto i32 = torch::dtype(torch::kInt32).device(experts.device());
+  auto order = torch::empty({n}, i32);
+  auto place = torch::empty(experts.sizes(), i32);
+  auto offsets = torch::empty({num_experts + 1}, I64(experts));
+  auto ws = Scratch(gs_expert_sort_workspace_bytes(n, num_experts), experts);
+  Check(gs_expert_sort(flat.data_ptr(), IdBytes(flat, "experts"), n, num_experts, order.data_ptr<int32_t>(),
+                       place.data_ptr<int32_t>(), offsets.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(),
+                       Stream(experts)),
+        "gs_expert_sort");
+  return {order, place, offsets};
+}
+
+torch::Tensor ExpertGather(const torch::Tensor& x, const torch::Tensor& place, const torch::Tensor& offsets) {
+  const Rows r(x, "rows");
+  const Places p(place, x.device());
+  TORCH_CHECK(r.t.size(0) == p.tokens, "rows of ", r.t.size(0), " tokens, places of ", p.tokens);
+  const int64_t* live = LiveRows(offsets, x.device());
+  c10::hip::HIPGuard on(x.device().index());
+  auto out = torch::empty({place.numel(), r.t.size(1)}, Like(x));
+  Check(gs_expert_gather(r.t.data_ptr(), r.stride, r.t.size(1), r.type, p.data(), p.tokens, p.choices, live,
+                         out.data_ptr(), Stream(x)),
+        "gs_expert_gather");
+  return out;
+}
+
+torch::Tensor ExpertCombine(const torch::Tensor& y, const torch::Tensor& place,
+                            const torch::optional<torch::Tensor>& weights) {
+  const Rows r(y, "rows");
+  const Places p(place, y.device());
+  TORCH_CHECK(r.t.size(0) == place.numel(), "rows of ", r.t.size(0), " items, places of ", place.numel());
+  const Weights w(weights, p, y);
+  c10::hip::HIPGuard on(y.device().index());
+  auto out = torch::empty({p.tokens, r.t.size(1)}, Like(y));
+  Check(gs_expert_combine(r.t.data_ptr(), r.stride, r.t.size(1), r.type, p.data(), p.tokens, p.choices, w.data(), w.type,
+                          out.data_ptr(), Stream(y)),
+        "gs_expert_combine");
+  return out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& dout, const torch::Tensor& y,
+                                                           const torch::Tensor& place, const torch::Tensor& offsets,
+                                                           const torch::optional<torch::Tensor>& weights,
+                                                           bool of_rows, bool of_weights) {
+  const Rows d(dout, "gradient"), r(y, "rows");
+  const Places p(place, dout.device());
+  TORCH_CHECK(y.device() == dout.device(), "rows and gradient are on different devices");
+  TORCH_CHECK(d.type == r.type, "rows and gradient differ in type");
+  TORCH_CHECK(d.t.size(0) == p.tokens && r.t.size(0) == place.numel() && d.t.size(1) == r.t.size(1),
+              "a gradient of ", d.t.sizes(), " and rows of ", r.t.sizes(), " for places of ", place.sizes());
+  const Weights w(weights, p, dout);
+  TORCH_CHECK(!of_weights || w.t.defined(), "no weights to take the gradient of");
+  const int64_t* live = LiveRows(offsets, dout.device());
+  c10::hip::HIPGuard on(dout.device().index());
+  torch::Tensor dy, dw;
+  if (of_rows) dy = torch::empty({place.numel(), d.t.size(1)}, Like(dout));
+  if (of_weights) dw = torch::empty(place.sizes(), Like(w.t));
+  Check(gs_expert_combine_grad(d.t.data_ptr(), d.stride, r.t.data_ptr(), r.stride, d.t.size(1), d.type, p.data(),
+                               p.tokens, p.choices, live, w.data(), w.type, of_rows ? dy.data_ptr() : nullptr,
+                               of_weights ? dw.data_ptr() : nullptr, Stream(dout)),
+        "gs_expert_combine_grad");
+  return {dy, dw};
 }
 
 }  // namespace hip

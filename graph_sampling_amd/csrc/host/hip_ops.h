@@ -359,5 +359,31 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> CooFilter
 // position of each key in data, -1 when absent
 torch::Tensor IndexSearch(const torch::Tensor& data, const torch::Tensor& keys);
 
+// ---- rows of values (fp32, fp16, bf16) moved by ids: embeddings, rows sorted by expert.  Ids are taken
+// flat; a table, gradient or set of rows is 2-D, and is copied when its rows are not contiguous.
+// [number of ids, dim]: scale * the table's rows
+torch::Tensor EmbeddingLookup(const torch::Tensor& table, const torch::Tensor& ids, double scale);
+// [num_rows, dim]: scale * the sums of grad's rows by id
+torch::Tensor EmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& ids, int64_t num_rows,
+                            double scale);
+// {ids met, ascending; a row of sums each}; waits for how many there are
+std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(const torch::Tensor& grad,
+                                                             const torch::Tensor& ids, int64_t num_rows,
+                                                             double scale);
+// {order, place, offsets} (int32 like the items, int32 like experts, int64 [num_experts + 1])
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> ExpertSort(const torch::Tensor& experts,
+                                                                   int64_t num_experts);
+torch::Tensor ExpertGather(const torch::Tensor& x, const torch::Tensor& place, const torch::Tensor& offsets);
+torch::Tensor ExpertCombine(const torch::Tensor& y, const torch::Tensor& place,
+                            const torch::optional<torch::Tensor>& weights);
+// {gradient of y, gradient of weights}, undefined where not wanted
+std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& dout, const torch::Tensor& y,
+                                                           const torch::Tensor& place,
+                                                           const torch::Tensor& offsets,
+                                                           const torch::optional<torch::Tensor>& weights,
+                                                           bool of_rows, bool of_weights);
+// whether the current stream of t's device is being recorded into a graph
+bool Capturing(const torch::Tensor& t);
+
 }  // namespace hip
 }  // namespace gs

@@ -1020,6 +1020,65 @@ int gs_batch_split(const void* data, const int64_t* data_ptr, const void* data_k
                    int64_t n, int64_t num_batches, void* const* out_data_host,
                    const int64_t* const* out_ptrs_host, int num_segments, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Rows of values moved by ids: embedding lookup and its gradient, rows sorted by */
+/* expert (or node type) and back.  No counterpart in the reference, whose examples */
+/* index feature matrices with torch.                                             */
+/* ------------------------------------------------------------------------- */
+/* Type of a row's values.  Products and sums are fp32 whatever it is, rounded once. */
+typedef enum gs_value_type { GS_F32 = 0, GS_F16 = 1, GS_BF16 = 2 } gs_value_type;
+
+/* out[i, :] = scale * table[ids[i], :] for n ids (below 2^31).  table: num_rows (below 2^32 - 1)
+ * rows of dim values (below 2^24), row r from table + r * row_stride values; out: n x dim.  An id outside
+ * [0, num_rows) stands for no row and gives zeros.  Rows are aligned to their type, no more. */
+int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride, int64_t dim, int type,
+                        const void* ids, int id_bytes, int64_t n, float scale, void* out, void* stream);
+
+/* Its gradient, out[v, :] = scale * sum of grad[i, :] over the i with ids[i] == v: num_rows x dim, every
+ * row written.  Row i of grad from grad + i * grad_stride values (0: the same row for all).  Sums in an
+ * order that follows from the ids alone: the same bits every time. */
+size_t gs_embedding_grad_workspace_bytes(int64_t n, int64_t dim, int type);
+int gs_embedding_grad(const void* grad, int64_t grad_stride, int64_t dim, int type, const void* ids, int id_bytes,
+                      int64_t n, int64_t num_rows, float scale, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* The same for the rows that are met only, n > 0.  _count sorts the ids and posts how many different rows
+ * they name to the mailbox; _fill, on the same workspace, untouched in between, and with the same n,
+ * num_rows, dim and type, writes those rows' ids, ascending, to met and their sums to values, a row each. */
+size_t gs_embedding_sparse_grad_workspace_bytes(int64_t n, int64_t dim, int type);
+int gs_embedding_sparse_grad_count(const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t dim, int type,
+                                   gs_mailbox* mailbox, int64_t ticket, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+int gs_embedding_sparse_grad_fill(const void* grad, int64_t grad_stride, int64_t dim, int type, int64_t n,
+                                  int64_t num_rows, float scale, int64_t* met, void* values, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* n items (below 2^31) sorted by expert, stably: order[p] = the item at place p, place[i] = where item i
+ * lies, offsets[0..num_experts] = where each expert's items begin and the last one's end.  An item whose
+ * expert lies outside [0, num_experts) has no place: place[i] = -1, and order is -1 from
+ * offsets[num_experts] on.  (No counterpart in the reference.) */
+size_t gs_expert_sort_workspace_bytes(int64_t n, int64_t num_experts);
+int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_experts, int32_t* order, int32_t* place,
+                   int64_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+
+/* rows[place[t, k], :] = x[t, :] for tokens x choices places (below 2^31 together), zeros in the rows from
+ * *live (device; offsets[num_experts] of the sort) to tokens * choices.  A place outside
+ * [0, tokens * choices) is left out. */
+int gs_expert_gather(const void* x, int64_t x_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
+                     int64_t choices, const int64_t* live, void* rows, void* stream);
+
+/* out[t, :] = sum over k of weights[t, k] * y[place[t, k], :], in the order of k; weights NULL: ones; of type
+ * GS_F32 or `type`.  A place outside [0, tokens * choices) adds nothing.  Also the gradient of gs_expert_gather. */
+int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
+                      int64_t choices, const void* weights, int weight_type, void* out, void* stream);
+
+/* Its gradients (either may be NULL): dy[place[t, k], :] = weights[t, k] * dout[t, :], zeros in the rows from
+ * *live on; dweights[t, k] = <dout[t, :], y[place[t, k], :]>, zero where there is no place, of type weight_type.
+ * y is read for dweights only. */
+int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int64_t dim, int type,
+                           const int32_t* place, int64_t tokens, int64_t choices, const int64_t* live,
+                           const void* weights, int weight_type, void* dy, void* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,401 @@
+"""gs.ops.embedding against the formulas in 64 bits.
+
+Tolerances.  A looked-up value is one fp32 product (relative error 2^-24) rounded once (eps / 2 of its type).
+A gradient is a sum of m fp32 values by sums of sums: at most 32 + 64 * 5 additions lie on any value's way
+(tiles of up to 32 positions, then up to 64 entries a level), each off by 2^-24 of a partial sum that is
+at most the sum S of the magnitudes, and one product; so it is off by (min(m, 352) + 1) * 2^-24 * scale * S before it
+is rounded once."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import graph_sampling_amd as gs
+from graph_sampling_amd import capi
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+F32 = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def smallest(dtype):  # half of the least subnormal: what rounding near zero is off by
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def rows(n, dim, dtype, dev, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(n, dim, generator=g).to(dtype).to(dev)
+
+
+def ids_of(kind, n, num_rows, seed, idt=np.int64):
+    rng = np.random.default_rng(seed)
+    if kind == "even":
+        ids = rng.integers(0, num_rows, n)
+    elif kind == "skewed":
+        ids = (num_rows ** rng.random(n)).astype(np.int64) - 1
+    elif kind == "one":
+        ids = np.full(n, num_rows // 2)
+    elif kind == "none":
+        ids = np.full(n, -1)
+    elif kind == "outside":  # beyond both ends, and as far as the type goes
+        ids = rng.integers(-2, num_rows + 2, n)
+        ids[rng.random(n) < 0.1] = np.iinfo(idt).max
+        ids[rng.random(n) < 0.1] = np.iinfo(idt).min
+    elif kind == "sorted":
+        ids = np.sort(rng.integers(0, num_rows, n))
+    elif kind == "hub":  # half of all on one row, the rest anywhere, a few nowhere
+        ids = np.where(rng.random(n) < 0.5, num_rows - 1, rng.integers(0, num_rows, n))
+        ids[rng.random(n) < 0.05] = -1
+    return ids.astype(idt)
+
+
+def check_lookup(out, table, ids, scale):
+    t = table.double().cpu().numpy()
+    there = (ids >= 0) & (ids < t.shape[0])
+    want = np.zeros(ids.shape + (t.shape[1],))
+    want[there] = t[ids[there]] * float(np.float32(scale))
+    got = out.detach().double().cpu().numpy()
+    assert got.shape == want.shape
+    assert np.all(np.abs(got - want) <= np.abs(want) * (half_step(out.dtype) + 2 * F32) + smallest(out.dtype))
+    assert np.all(got[~there] == 0)
+
+
+def sums_by_id(grad, ids, num_rows, scale):
+    """(sums, tolerance before rounding)"""
+    g = grad.double().cpu().numpy().reshape(ids.size, grad.shape[-1])
+    flat = ids.reshape(-1)
+    there = np.flatnonzero((flat >= 0) & (flat < num_rows))
+    want = np.zeros((num_rows, g.shape[1]))
+    size = np.zeros_like(want)
+    np.add.at(want, flat[there], g[there])
+    np.add.at(size, flat[there], np.abs(g[there]))
+    m = np.bincount(flat[there], minlength=num_rows)[:, None]
+    s = abs(float(np.float32(scale)))
+    return want * float(np.float32(scale)), (np.minimum(m, 352) + 1) * F32 * s * size
+
+
+def check_sums(got, want, tol, dtype):
+    got = got.detach().double().cpu().numpy()
+    assert got.shape == want.shape
+    assert np.all(np.abs(got - want) <= tol + (np.abs(want) + tol) * half_step(dtype) + smallest(dtype))
+
+
+CASES = [
+    # rows, width, ids, kind
+    (1, 1, 1, "even"), (7, 3, 5, "outside"), (100, 8, 64, "even"), (50, 4, 300, "skewed"), (33, 17, 1000, "outside"),
+    (1000, 64, 4096, "hub"), (1000, 64, 4097, "hub"), (3000, 97, 5000, "skewed"), (70000, 16, 9000, "even"),
+    (300, 520, 700, "one"), (255, 1001, 333, "none"), (256, 1032, 2000, "sorted"), (257, 130, 50000, "one"),
+    (12, 2, 200000, "hub"), (1 << 17, 5, 30000, "even"), (5, 4096, 9, "even"), (20, 8, 0, "even"), (20000000, 1, 5000, "even"),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("num_rows,dim,n,kind", CASES)
+def test_lookup_and_gradients(dev, num_rows, dim, n, kind, dtype):
+    idt = np.int32 if (n + dim) % 2 else np.int64
+    ids = ids_of(kind, n, num_rows, n + dim, idt)
+    table = rows(num_rows, dim, dtype, dev, 1).requires_grad_(True)
+    d_ids = torch.from_numpy(ids).to(dev)
+    scale = math.sqrt(dim) if n % 2 else 1.0
+    out = gs.ops.embedding(table, d_ids, scale)
+    assert out.dtype == dtype
+    check_lookup(out, table.detach(), ids, scale)
+    grad = rows(n, dim, dtype, dev, 2)
+    want, tol = sums_by_id(grad, ids, num_rows, scale)
+    dense, = torch.autograd.grad(out, table, grad)
+    assert dense.dtype == dtype and dense.layout == torch.strided
+    check_sums(dense, want, tol, dtype)
+    again, = torch.autograd.grad(gs.ops.embedding(table, d_ids, scale), table, grad)
+    assert torch.equal(dense.view(torch.uint8), again.view(torch.uint8))
+    sparse, = torch.autograd.grad(gs.ops.embedding(table, d_ids, scale, sparse_grad=True), table, grad)
+    met = np.unique(ids[(ids >= 0) & (ids < num_rows)])
+    assert sparse.is_sparse and sparse.is_coalesced() and sparse.shape == table.shape and sparse.dtype == dtype
+    assert np.array_equal(sparse.indices()[0].cpu().numpy(), met)
+    # the same sums in the same order: the same bits
+    assert torch.equal(sparse.values(), dense[sparse.indices()[0]])
+    # and through the C ABI by itself
+    assert torch.equal(capi.embedding_lookup(table.detach(), d_ids, scale), out)
+    assert torch.equal(capi.embedding_grad(grad, d_ids, num_rows, scale), dense)
+    c_met, c_values = capi.embedding_sparse_grad(grad, d_ids, num_rows, scale)
+    assert torch.equal(c_met, sparse.indices()[0]) and torch.equal(c_values, sparse.values())
+
+
+@gpu
+def test_rows_any_distance_apart_and_off_their_alignment(dev):
+    for dtype in TYPES:
+        base = rows(400, 61, dtype, dev, 3)
+        for view in (base[:, 1:60], base[:, 3:35], base[::3, :40], base[5:, 7:8], base.t()[:50]):
+            n = view.shape[0]
+            ids = ids_of("outside", 777, n, 4)
+            table = view.detach().requires_grad_(True)
+            out = gs.ops.embedding(table, torch.from_numpy(ids).to(dev), 1.5)
+            check_lookup(out, view, ids, 1.5)
+            wide = rows(777, 2 * view.shape[1] + 1, dtype, dev, 5)
+            grad = wide[:, 1:view.shape[1] + 1]
+            got, = torch.autograd.grad(out, table, grad)
+            check_sums(got, *sums_by_id(grad, ids, n, 1.5), dtype)
+    # the same gradient row for every id, and one value for all of them
+    table = rows(30, 12, torch.float32, dev, 6).requires_grad_(True)
+    ids = ids_of("even", 100, 30, 7)
+    d_ids = torch.from_numpy(ids).to(dev)
+    row = rows(1, 12, torch.float32, dev, 8)
+    got, = torch.autograd.grad(gs.ops.embedding(table, d_ids), table, row.expand(100, 12))
+    check_sums(got, *sums_by_id(row.expand(100, 12).contiguous(), ids, 30, 1.0), torch.float32)
+    got, = torch.autograd.grad(gs.ops.embedding(table, d_ids).sum(), table)
+    check_sums(got, *sums_by_id(torch.ones(100, 12), ids, 30, 1.0), torch.float32)
+
+
+@gpu
+def test_ids_of_any_shape_and_order(dev):
+    table = rows(40, 6, torch.float32, dev, 9).requires_grad_(True)
+    ids = ids_of("even", 60, 40, 10).reshape(4, 5, 3)
+    d_ids = torch.from_numpy(ids).to(dev)
+    for view, host in ((d_ids, ids), (d_ids.transpose(0, 2), ids.transpose(2, 1, 0)), (d_ids[:, ::2], ids[:, ::2]),
+                       (d_ids[1, 2, 0], ids[1, 2, 0]), (d_ids[:0], ids[:0]), (d_ids[0, 0, :1].expand(7), np.repeat(ids[0, 0, :1], 7))):
+        host = np.asarray(host)
+        out = gs.ops.embedding(table, view, 2.0)
+        assert out.shape == host.shape + (6,)
+        check_lookup(out, table.detach(), host, 2.0)
+        grad = rows(host.size, 6, torch.float32, dev, 11).view(out.shape)
+        got, = torch.autograd.grad(out, table, grad)
+        check_sums(got, *sums_by_id(grad, host, 40, 2.0), torch.float32)
+
+
+@gpu
+def test_rows_that_no_id_names_do_not_matter(dev):
+    """Infinities and NaN in rows of the table, and of the gradient, that stand for nothing."""
+    table = rows(10, 20, torch.bfloat16, dev, 12)
+    table[3] = float("nan")
+    table[4] = float("inf")
+    table.requires_grad_(True)
+    ids = np.array([1, -1, 2, 10, 9, 1])
+    out = gs.ops.embedding(table, torch.from_numpy(ids).to(dev), 0.0)
+    assert torch.equal(out, torch.zeros_like(out))  # (a scale of zero, finite rows)
+    out = gs.ops.embedding(table, torch.from_numpy(ids).to(dev), 3.0)
+    check_lookup(out, torch.nan_to_num(table.detach(), 0, 0, 0), ids, 3.0)
+    grad = rows(6, 20, torch.bfloat16, dev, 13)
+    grad[1] = float("nan")
+    grad[3] = float("inf")
+    got, = torch.autograd.grad(out, table, grad)
+    clean = grad.clone()
+    clean[1] = clean[3] = 0
+    check_sums(got, *sums_by_id(clean, ids, 10, 3.0), torch.bfloat16)
+    # where they are named, they come through
+    out = gs.ops.embedding(table, torch.tensor([3, 4], device=dev), 2.0)
+    assert out[0].isnan().all() and out[1].isinf().all()
+
+
+@gpu
+def test_gradient_against_differences(dev):
+    table = rows(9, 5, torch.float32, dev, 14)
+    ids = torch.tensor([0, 3, 3, 8, -1, 3, 20], device=dev)
+    grad, way = rows(7, 5, torch.float32, dev, 15), rows(9, 5, torch.float32, dev, 16)
+    table.requires_grad_(True)
+    got, = torch.autograd.grad(gs.ops.embedding(table, ids, 0.5), table, grad)
+    with torch.no_grad():  # linear: any step will do; powers of two keep the steps exact to rounding
+        up = (gs.ops.embedding(table + 4 * way, ids, 0.5).double() * grad.double()).sum()
+        down = (gs.ops.embedding(table - 4 * way, ids, 0.5).double() * grad.double()).sum()
+    # 14 looked-up rows of values below 32, each off by two roundings, times gradients below 8
+    assert abs((up - down).item() / 8 - (got.double() * way.double()).sum().item()) < 35 * 32 * 8 * 2 * F32
+
+
+@gpu
+def test_accumulates_and_steps_like_a_parameter(dev):
+    table = torch.nn.Parameter(rows(50, 8, torch.float32, dev, 17))
+    ids = ids_of("hub", 40, 50, 18)
+    d_ids = torch.from_numpy(ids).to(dev)
+    gs.ops.embedding(table, d_ids).sum().backward()
+    gs.ops.embedding(table, d_ids).sum().backward()  # twice the same: exactly twice the sums
+    once, = torch.autograd.grad(gs.ops.embedding(table, d_ids).sum(), table)
+    assert torch.equal(table.grad, 2 * once)
+    table.grad = None
+    before = table.detach().clone()
+    optimizer = torch.optim.SparseAdam([table], lr=0.5)
+    gs.ops.embedding(table, d_ids, sparse_grad=True).sum().backward()
+    optimizer.step()
+    moved = (table.detach() != before).any(1).cpu().numpy()
+    assert np.array_equal(np.flatnonzero(moved), np.unique(ids[ids >= 0]))
+
+
+@gpu
+def test_recorded_lookup_and_gradient_follow_their_inputs(dev):
+    """Forward and gradient in one HIP graph, ids and values rewritten between replays, eager work between."""
+    for n, num_rows, dim in ((50, 30, 16), (6000, 500, 40), (9000, 70000, 8)):
+        table = rows(num_rows, dim, torch.float32, dev, 19)
+        grad = rows(n, dim, torch.float32, dev, 20)
+        ids = torch.from_numpy(ids_of("hub", n, num_rows, 21)).to(dev)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            gs.ops.embedding(table, ids, 2.0)
+            torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, ids, num_rows, 2.0)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = gs.ops.embedding(table, ids, 2.0)
+            got = torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, ids, num_rows, 2.0)
+        for rep in range(4):
+            ids.copy_(torch.from_numpy(ids_of("outside" if rep % 2 else "skewed", n, num_rows, 30 + rep)))
+            grad.copy_(rows(n, dim, torch.float32, dev, 40 + rep))
+            want = torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, ids, num_rows, 2.0)
+            want_out = gs.ops.embedding(table, ids, 2.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want_out) and torch.equal(got, want)
+
+
+@gpu
+def test_recorded_backward_pass(dev):
+    """forward + backward through autograd, recorded: no eager graph of the leaf lives."""
+    table = rows(300, 24, torch.float32, dev, 22).requires_grad_(True)
+    grad = rows(700, 24, torch.float32, dev, 23)
+    ids = torch.from_numpy(ids_of("skewed", 700, 300, 24)).to(dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(gs.ops.embedding(table, ids, 1.5), table, grad)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(gs.ops.embedding(table, ids, 1.5), table, grad)
+    for rep in range(3):
+        grad.copy_(rows(700, 24, torch.float32, dev, 50 + rep))
+        want, = torch.autograd.grad(gs.ops.embedding(table, ids, 1.5), table, grad)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@gpu
+def test_recording_is_refused_where_it_would_end_the_process(dev):
+    table = rows(30, 8, torch.float32, dev, 25).requires_grad_(True)
+    ids = torch.arange(10, device=dev)
+    eager = gs.ops.embedding(table, ids)  # lives through the recording, on the default stream
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    message = None
+    with torch.cuda.graph(graph):
+        try:
+            gs.ops.embedding(table, ids)
+        except RuntimeError as error:
+            message = str(error)
+        plain = gs.ops.embedding(table.detach(), ids)  # nothing flows back: recorded
+    assert message and "eager graph of the same leaf" in message
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, eager)
+    torch.autograd.grad(eager.sum(), table)
+
+
+@gpu
+def test_sparse_gradient_is_not_recorded(dev):
+    grad, ids = rows(10, 8, torch.float32, dev, 26), torch.arange(10, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    message = None
+    with torch.cuda.graph(graph):
+        kept = grad * 2
+        try:
+            torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(grad, ids, 30, 1.0)
+        except RuntimeError as error:
+            message = str(error)
+    assert message and "cannot be recorded" in message
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept, grad * 2)
+
+
+@gpu
+def test_on_another_stream(dev):
+    table = rows(2000, 32, torch.float32, dev, 27).requires_grad_(True)
+    ids = torch.from_numpy(ids_of("hub", 20000, 2000, 28)).to(dev)
+    grad = rows(20000, 32, torch.float32, dev, 29)
+    want, = torch.autograd.grad(gs.ops.embedding(table, ids), table, grad)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, = torch.autograd.grad(gs.ops.embedding(table, ids), table, grad)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_refusals(dev):
+    table, ids = rows(5, 4, torch.float32, dev, 30), torch.zeros(3, dtype=torch.int64, device=dev)
+    for bad, match in (((table.double(), ids), "float32, float16 or bfloat16"), ((table, ids.float()), "int64"),
+                       ((table[0], ids), "two dimensions"), ((table.cpu(), ids), "GPU tensor"),
+                       ((table, ids.cpu()), "GPU tensor"), ((table.to_sparse(), ids), "dense|subclasses")):
+        with pytest.raises(RuntimeError, match=match):
+            gs.ops.embedding(*bad)
+    with pytest.raises(RuntimeError, match="for 3 ids|shape"):
+        torch.ops.gs_ops._CAPI_EmbeddingGrad(rows(4, 4, torch.float32, dev, 31), ids, 5, 1.0)
+    with pytest.raises(RuntimeError, match="non-negative"):
+        torch.ops.gs_ops._CAPI_EmbeddingGrad(rows(3, 4, torch.float32, dev, 31), ids, -1, 1.0)
+    leaf = table.clone().requires_grad_(True)
+    out = gs.ops.embedding(leaf, ids)
+    dout = rows(3, 4, torch.float32, dev, 32).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="once more"):
+        torch.autograd.grad(out, leaf, dout, create_graph=True)
+    with pytest.raises(RuntimeError, match="once more"):
+        torch.ops.gs_ops._CAPI_EmbeddingGrad(dout, ids, 5, 1.0)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: gs.ops.embedding(t, ids).sum())(table)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        gs.ops.embedding(torch.autograd.forward_ad.make_dual(table, table), ids)
+
+
+@gpu
+def test_null_and_empty(dev):
+    ids = torch.zeros(4, dtype=torch.int32, device=dev)
+    empty = torch.empty(0, 6, device=dev, requires_grad=True)
+    out = gs.ops.embedding(empty, ids)
+    assert torch.equal(out, torch.zeros(4, 6, device=dev))
+    assert torch.autograd.grad(out.sum(), empty)[0].shape == (0, 6)
+    sparse, = torch.autograd.grad(gs.ops.embedding(empty, ids, sparse_grad=True).sum(), empty)
+    assert sparse.is_sparse and sparse._nnz() == 0
+    thin = torch.empty(5, 0, device=dev, requires_grad=True)
+    out = gs.ops.embedding(thin, ids)
+    assert out.shape == (4, 0)
+    assert torch.autograd.grad(out.sum(), thin)[0].shape == (5, 0)
+    sparse, = torch.autograd.grad(gs.ops.embedding(thin, ids, sparse_grad=True).sum(), thin)
+    assert sparse.indices().tolist() == [[0]] and sparse.values().shape == (1, 0)
+
+
+# ------------------------------------------------------------------ no GPU ----
+def test_bad_arguments_are_refused_before_anything_is_launched():
+    import ctypes
+    lib, i64 = capi.lib(), ctypes.c_int64
+    buf = (ctypes.c_int64 * 64)()
+    at = ctypes.addressof(buf)
+
+    def lookup(table=buf, rows=4, stride=8, dim=8, kind=0, ids=buf, id_bytes=8, n=2, out=buf):
+        return lib.gs_embedding_lookup(table, i64(rows), i64(stride), i64(dim), kind, ids, id_bytes, i64(n),
+                                       ctypes.c_float(1), out, None)
+
+    assert lookup(n=0) == 0 and lookup(dim=0) == 0
+    for bad, match in ((dict(kind=3), b"value type"), (dict(id_bytes=2), b"id_bytes"), (dict(n=-1), b"ids"),
+                       (dict(n=1 << 31), b"ids"), (dict(rows=(1 << 32) - 1), b"rows"), (dict(dim=1 << 24), b"values"),
+                       (dict(stride=-1), b"stride"), (dict(ids=None), b"null"), (dict(out=None), b"null"),
+                       (dict(table=None), b"null"), (dict(table=ctypes.c_void_p(at + 2)), b"aligned"),
+                       (dict(ids=ctypes.c_void_p(at + 4)), b"aligned"), (dict(kind=1, out=ctypes.c_void_p(at + 1)), b"aligned")):
+        status = lookup(**bad)
+        assert status < 0 and match in lib.gs_status_string(status), (bad, lib.gs_status_string(status))
+    assert lib.gs_embedding_grad_workspace_bytes(i64(1000), i64(64), 0) > 16000
+    status = lib.gs_embedding_grad(buf, i64(8), i64(8), 0, buf, 8, i64(2), i64(4), ctypes.c_float(1), buf, buf,
+                                   ctypes.c_size_t(16), None)
+    assert status == -2 and b"workspace" in lib.gs_status_string(status)
+    status = lib.gs_embedding_sparse_grad_count(buf, 8, i64(0), i64(4), i64(8), 0, None, i64(1), buf, ctypes.c_size_t(16),
+                                                None)
+    assert status == -1 and b"no ids" in lib.gs_status_string(status)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        gs.ops.embedding(torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
