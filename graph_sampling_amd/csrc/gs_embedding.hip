@@ -9,9 +9,10 @@
 //
 // The gradient adds in an order that follows from the ids alone, without atomics: the positions are
 // sorted by id (gs_key_sort.hpp), a group of lanes adds up a tile of consecutive sorted positions run
-// by run, and writes a row when the run lies inside its tile.  Runs that cross tiles leave partial
-// sums, at most two a tile, which are themselves a sorted list: the next launch adds them up in the
-// same way, and so on until one tile holds all.  So a row that half of the ids name costs no more
+// by run, and writes a row when the run lies inside its tile.  Runs that cross tiles are joined in
+// LDS by the workgroup's groups, and those that cross workgroups leave partial sums, at most two a
+// workgroup, which are themselves a sorted list: the next launch adds them up in the same way, and
+// so on until one workgroup holds all.  So a row that half of the ids name costs no more
 // than any other, and sums of many addends are sums of sums, which keeps fp32 exact enough.
 #include "gs_key_sort.hpp"
 #include "gs_rows.hpp"
@@ -78,189 +79,221 @@ struct RunsOut {
   float scale;
   int64_t dim;
   int64_t chunks;        // of a row
-  int slices;            // groups side by side over a row
+  int slices;            // workgroups side by side over a row
   int64_t* met;          // sparse: ids of the rows by their rank (null: dense)
   const int64_t* rank;   // sparse: met rows before a sorted position
-  Entry* entries;        // 2 a tile (null where there is one tile)
-  float* sums;           // [2 * tiles, chunks * kVec]
+  Entry* entries;        // 2 a workgroup (null where there is one)
+  float* sums;           // [2 * workgroups, chunks * kVec]
 };
 
-// where a group's lane works: G lanes a group, 64 / G groups a wave
-struct GroupPlace {
-  int64_t tile;
-  int64_t chunk;  // of this lane; may lie behind the row's last
-  bool in;
-  template <int G>
-  static __device__ __forceinline__ GroupPlace of(int64_t tiles, int slices, int64_t chunks) {
-    const int64_t g = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
-    GroupPlace p;
-    p.tile = g / slices;
-    p.chunk = (g - p.tile * slices) * G + (threadIdx.x & (G - 1));
-    p.in = p.tile < tiles && p.chunk < chunks;
-    if (p.tile >= tiles) p.tile = tiles - 1;  // (works along, writes nothing)
-    if (p.chunk >= chunks) p.chunk = 0;
-    return p;
-  }
-};
+// A workgroup is up to 64 groups of G lanes, a chunk of the row a lane, group after group along the list.
+template <int G>
+constexpr int kGroups = 1024 / G < 64 ? 1024 / G : 64;
+template <int G>
+constexpr int kSumThreads = kGroups<G>* G;
 
-// A run that ends: its row when it is whole, a partial sum when it crosses a tile's edge.
-template <typename T>
-struct RunWriter {
+template <typename T, int G>
+struct Runs {
+  static constexpr int kEntries = 2 * kGroups<G>;
+  struct Shared {
+    Entry entry[kEntries];
+    Entry left[2];  // the workgroup's own
+    Wide<T> sum[kEntries][G];
+  };
   const RunsOut& o;
-  T* out;
-  const GroupPlace& p;
-  Entry first{0, kNone}, last{0, kNone};
+  Shared& s;
+  T* out;          // at this lane's chunk
+  int64_t part;    // workgroup along the list
+  int64_t chunk;
+  int group, lane;
+  bool in;         // whether the lane has a chunk
 
+  __device__ __forceinline__ Runs(const RunsOut& o_, Shared& s_, T* out_) : o(o_), s(s_) {
+    part = blockIdx.x / o.slices;
+    group = threadIdx.x / G;
+    lane = threadIdx.x & (G - 1);
+    chunk = (blockIdx.x - part * o.slices) * G + lane;
+    in = chunk < o.chunks;
+    if (!in) chunk = 0;  // (works along, writes nothing)
+    out = out_ + chunk_start<T>(o.dim, chunk);
+    if (lane == 0) s.entry[2 * group] = s.entry[2 * group + 1] = Entry{0, kNone};
+    if (threadIdx.x < 2) s.left[threadIdx.x] = Entry{0, kNone};
+  }
+  __device__ __forceinline__ void write(uint32_t row, const Wide<T>& sum) {
+    if (in) store_chunk(out + static_cast<int64_t>(row) * o.dim, narrow<T>(sum * o.scale), o.dim);
+  }
+  // a run of this group's tile that ends; left, right: it began before the tile, goes on behind it
   __device__ __forceinline__ void finish(uint32_t row, const Wide<T>& sum, bool left, bool right) {
-    if (!left && !right) {
-      const int64_t at = chunk_start<T>(o.dim, p.chunk);
-      if (p.in) store_chunk(out + static_cast<int64_t>(row) * o.dim + at, narrow<T>(sum * o.scale), o.dim);
-      return;
-    }
-    const int slot = left ? 0 : 1;
-    float* to = o.sums + ((2 * p.tile + slot) * o.chunks + p.chunk) * Chunk<T>::kVec;
-    if (p.in) __builtin_memcpy(to, &sum, sizeof(sum));
-    if (left) {
-      first = Entry{row, kSum};
-      if (right) last = Entry{row, kThrough};
-    } else {
-      last = Entry{row, kSum};
+    if (!left && !right) return write(row, sum);
+    const int slot = 2 * group + (left ? 0 : 1);
+    s.sum[slot][lane] = sum;
+    if (lane == 0) {
+      s.entry[slot] = Entry{row, kSum};
+      if (left && right) s.entry[slot + 1] = Entry{row, kThrough};
     }
   }
-  __device__ __forceinline__ void entries() {
-    if (o.entries && p.in && p.chunk == 0) {
-      o.entries[2 * p.tile] = first;
-      o.entries[2 * p.tile + 1] = last;
+  // the run whose first piece here is entry i, added up over the groups it goes through
+  __device__ __forceinline__ void walk(int i) {
+    const uint32_t row = s.entry[i].row;
+    const bool left = i == 0;
+    Wide<T> sum = s.sum[i][lane];
+    int j = i + 1;
+    for (; j < kEntries; ++j) {
+      const Entry e = s.entry[j];
+      if (e.state == kNone || e.row != row) break;
+      if (e.state == kSum) sum += s.sum[j][lane];
     }
+    const bool right = j == kEntries;
+    if (!left && !right) return write(row, sum);
+    const int slot = left ? 0 : 1;
+    if (in) {
+      float* to = o.sums + ((2 * part + slot) * o.chunks + chunk) * Chunk<T>::kVec;
+      __builtin_memcpy(to, &sum, sizeof(sum));
+    }
+    if (lane == 0) {
+      s.left[slot] = Entry{row, kSum};
+      if (left && right) s.left[1] = Entry{row, kThrough};
+    }
+  }
+  // behind every group's tile: every thread of the workgroup calls this
+  __device__ __forceinline__ void join() {
+    __syncthreads();
+    if (group == 0 && s.entry[0].state == kSum) walk(0);
+    if (s.entry[2 * group + 1].state == kSum) walk(2 * group + 1);
+    __syncthreads();
+    if (o.entries && threadIdx.x < 2 && blockIdx.x == part * o.slices)
+      o.entries[2 * part + threadIdx.x] = s.left[threadIdx.x];
   }
 };
 
 constexpr int kBatch = 8;  // rows a group asks for together
 
-// Tiles of `size` sorted positions.
+// A tile of `size` sorted positions a group.
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kSumThreads<G>)
 sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t num_rows, const T* __restrict__ grad,
-                int64_t stride, int size, int64_t tiles, RunsOut o, T* __restrict__ out) {
-  const GroupPlace p = GroupPlace::of<G>(tiles, o.slices, o.chunks);
-  const int64_t base = p.tile * size;
-  const int count = n - base < size ? static_cast<int>(n - base) : size;
-  const int64_t at = chunk_start<T>(o.dim, p.chunk);
-  RunWriter<T> writer{o, out, p};
-  uint32_t key = key_sort::key_of(words[base]);
-  bool left = base > 0 && key_sort::key_of(words[base > 0 ? base - 1 : 0]) == key;
-  const uint32_t behind = base + count < n ? key_sort::key_of(words[base + count]) : num_rows;
-  int64_t row = key;
-  if (o.rank) row = o.rank[base] - (left ? 1 : 0);
-  if (o.met && !left && key < num_rows && p.in && p.chunk == 0) o.met[row] = key;
-  Wide<T> sum = {};
-  for (int j0 = 0; j0 < count; j0 += kBatch) {
-    key_sort::Word w[kBatch];
-    Values<T> v[kBatch];
+                int64_t stride, int size, RunsOut o, T* __restrict__ out) {
+  __shared__ typename Runs<T, G>::Shared s_runs;
+  Runs<T, G> runs(o, s_runs, out);
+  const int64_t base = (runs.part * kGroups<G> + runs.group) * size;
+  const T* const from = grad + chunk_start<T>(o.dim, runs.chunk);
+  const int count = n - base < size ? (n > base ? static_cast<int>(n - base) : 0) : size;
+  uint32_t key = count > 0 ? key_sort::key_of(words[base]) : num_rows;
+  if (key < num_rows) {
+    bool left = base > 0 && key_sort::key_of(words[base - 1]) == key;
+    const uint32_t behind = base + count < n ? key_sort::key_of(words[base + count]) : num_rows;
+    uint32_t row = key;
+    if (o.rank) row = static_cast<uint32_t>(o.rank[base]) - (left ? 1 : 0);
+    const bool names = o.met && runs.in && runs.chunk == 0;  // this lane writes the rows' ids
+    if (names && !left) o.met[row] = key;
+    Wide<T> sum = {};
+    for (int j0 = 0; j0 < count && key < num_rows; j0 += kBatch) {
+      key_sort::Word w[kBatch];
+      Values<T> v[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) w[k] = words[base + (j0 + k < count ? j0 + k : count - 1)];
-    if (key_sort::key_of(w[0]) >= num_rows) {  // no rows from here on
-      if (j0 > 0 && key < num_rows) writer.finish(static_cast<uint32_t>(row), sum, left, false);
-      key = num_rows;
-      break;
-    }
+      for (int k = 0; k < kBatch; ++k) w[k] = words[base + (j0 + k < count ? j0 + k : count - 1)];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) v[k] = load_chunk(grad + key_sort::position_of(w[k]) * stride + at, o.dim);
+      for (int k = 0; k < kBatch; ++k) v[k] = load_chunk(from + key_sort::position_of(w[k]) * stride, o.dim);
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (j0 + k >= count) break;
-      const uint32_t next = key_sort::key_of(w[k]);
-      if (next != key) {
-        writer.finish(static_cast<uint32_t>(row), sum, left, false);
-        left = false;
-        key = next;
-        row = o.rank ? row + 1 : static_cast<int64_t>(key);
-        if (o.met && key < num_rows && p.in && p.chunk == 0) o.met[row] = key;
-        sum = Wide<T>{};
-        if (key >= num_rows) break;
+      for (int k = 0; k < kBatch; ++k) {
+        if (j0 + k >= count) break;
+        const uint32_t next = key_sort::key_of(w[k]);
+        if (next != key) {
+          runs.finish(row, sum, left, false);
+          left = false;
+          key = next;
+          row = o.rank ? row + 1 : key;
+          if (key >= num_rows) break;  // (no rows from here on)
+          if (names) o.met[row] = key;
+          sum = Wide<T>{};
+        }
+        sum += widen<T>(v[k]);
       }
-      sum += widen<T>(v[k]);
     }
-    if (key >= num_rows) break;
+    if (key < num_rows) runs.finish(row, sum, left, behind == key);
   }
-  if (key < num_rows) writer.finish(static_cast<uint32_t>(row), sum, left, behind == key);
-  writer.entries();
+  runs.join();
 }
 
-// Tiles of `size` entries that an earlier launch left, m of them; sums_in as RunsOut::sums.
+// A tile of kJoinSize entries that an earlier launch left a group, of m; sums_in as RunsOut::sums.
+constexpr int kJoinSize = 16;
+
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads)
-join_runs_kernel(const Entry* __restrict__ in, int64_t m, const float* __restrict__ sums_in, int size, int64_t tiles,
-                 RunsOut o, T* __restrict__ out) {
-  const GroupPlace p = GroupPlace::of<G>(tiles, o.slices, o.chunks);
-  const int64_t base = p.tile * size;
-  const int count = m - base < size ? static_cast<int>(m - base) : size;
-  RunWriter<T> writer{o, out, p};
-  const Entry before = base > 0 ? in[base - 1] : Entry{0, kNone};
-  const Entry behind = base + count < m ? in[base + count] : Entry{0, kNone};
+__global__ void __launch_bounds__(kSumThreads<G>)
+join_runs_kernel(const Entry* __restrict__ in, int64_t m, const float* __restrict__ sums_in, RunsOut o,
+                 T* __restrict__ out) {
+  __shared__ typename Runs<T, G>::Shared s_runs;
+  Runs<T, G> runs(o, s_runs, out);
+  const int64_t base = (runs.part * kGroups<G> + runs.group) * kJoinSize;
+  const Entry none{0, kNone};
+  const Entry before = base > 0 && base <= m ? in[base - 1] : none;
+  const Entry behind = base + kJoinSize < m ? in[base + kJoinSize] : none;
+  Entry e[kJoinSize];
+#pragma unroll
+  for (int k = 0; k < kJoinSize; ++k) {
+    e[k] = in[base + k < m ? base + k : m - 1];
+    if (base + k >= m) e[k] = none;
+  }
   bool open = false, left = false;
   uint32_t row = 0;
   Wide<T> sum = {};
-  for (int j0 = 0; j0 < count; j0 += kBatch) {
-    Entry e[kBatch];
+#pragma unroll
+  for (int j0 = 0; j0 < kJoinSize; j0 += kBatch) {
     Wide<T> v[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) e[k] = in[base + (j0 + k < count ? j0 + k : count - 1)];
-#pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (j0 + k >= count) e[k].state = kNone;
       v[k] = Wide<T>{};
-      if (e[k].state == kSum)
-        __builtin_memcpy(&v[k], sums_in + ((base + j0 + k) * o.chunks + p.chunk) * Chunk<T>::kVec, sizeof(v[k]));
+      if (e[j0 + k].state == kSum)
+        __builtin_memcpy(&v[k], sums_in + ((base + j0 + k) * o.chunks + runs.chunk) * Chunk<T>::kVec, sizeof(v[k]));
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (e[k].state == kNone) continue;  // (never inside a run)
-      if (!open || e[k].row != row) {
-        if (open) writer.finish(row, sum, left, false);
+      if (e[j0 + k].state == kNone) continue;  // (never inside a run)
+      if (!open || e[j0 + k].row != row) {
+        if (open) runs.finish(row, sum, left, false);
         open = true;
-        row = e[k].row;
+        row = e[j0 + k].row;
         left = j0 + k == 0 && before.state != kNone && before.row == row;
         sum = Wide<T>{};
       }
       sum += v[k];
     }
   }
-  if (open) writer.finish(row, sum, left, behind.state != kNone && behind.row == row);
-  writer.entries();
+  if (open) runs.finish(row, sum, left, behind.state != kNone && behind.row == row);
+  runs.join();
 }
 
 // ------------------------------------------------------------------- plans ----
-// The tiles of every launch: a function of the sizes alone.
-constexpr int kJoinSize = 64;
+// The workgroups of every launch: a function of the sizes alone.
 constexpr int kMaxLevels = 8;
 
 struct SumPlan {
   int64_t n, chunks;
-  int group, slices;  // lanes a group, groups over a row
-  int size;           // positions a tile of the first launch
+  int group, slices;  // lanes a group, workgroups over a row
+  int size;           // positions a group of the first launch
   int levels;
-  int64_t tiles[kMaxLevels];
+  int64_t parts[kMaxLevels];  // workgroups along the list
 
   SumPlan(int64_t n_, int64_t dim, int type) : n(n_) {
     chunks = type == GS_F32 ? chunks_of<float>(dim) : chunks_of<_Float16>(dim);
     group = 1;
     while (group < kWave && group < chunks) group *= 2;
     slices = static_cast<int>((chunks + group - 1) / group);
+    const int groups = 1024 / group < 64 ? 1024 / group : 64;
     // as long as there are waves enough for the chip, longer tiles leave fewer partial sums
     size = 32;
     while (size > 8 && (n / size) * slices * group < int64_t(256) * 16 * kWave) size /= 2;
     levels = 0;
-    int64_t t = (n + size - 1) / size;
-    tiles[levels++] = t;
-    while (t > 1) {
-      t = (2 * t + kJoinSize - 1) / kJoinSize;
-      tiles[levels++] = t;
+    int64_t p = (n + int64_t(size) * groups - 1) / (int64_t(size) * groups);
+    parts[levels++] = p;
+    while (p > 1) {
+      p = (2 * p + kJoinSize * groups - 1) / (kJoinSize * groups);
+      parts[levels++] = p;
     }
   }
   int vec(int type) const { return 16 / value_bytes(type); }
   size_t sums_bytes(int level, int type) const {
-    return static_cast<size_t>(2 * tiles[level]) * chunks * vec(type) * sizeof(float);
+    return static_cast<size_t>(2 * parts[level]) * chunks * vec(type) * sizeof(float);
   }
 };
 
@@ -278,7 +311,7 @@ size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
   size_t bytes = key_sort::space_bytes(p.n, 2);
   if (sparse) bytes += padded(static_cast<size_t>(p.n + 1) * 8) + scan_workspace_bytes(p.n);
   for (int l = 0; l < 2 && l + 1 < p.levels; ++l)
-    bytes += padded(static_cast<size_t>(2 * p.tiles[l]) * sizeof(Entry)) + padded(p.sums_bytes(l, type));
+    bytes += padded(static_cast<size_t>(2 * p.parts[l]) * sizeof(Entry)) + padded(p.sums_bytes(l, type));
   return bytes;
 }
 
@@ -291,7 +324,7 @@ bool carve_grad(Carver& ws, const SumPlan& p, int type, uint32_t num_rows, bool 
     s->entries[l] = nullptr;
     s->sums[l] = nullptr;
     if (l + 1 < p.levels) {
-      s->entries[l] = ws.take<Entry>(static_cast<size_t>(2 * p.tiles[l]));
+      s->entries[l] = ws.take<Entry>(static_cast<size_t>(2 * p.parts[l]));
       s->sums[l] = ws.take<float>(p.sums_bytes(l, type) / sizeof(float));
     }
   }
@@ -320,13 +353,13 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
       const bool last = l == p.levels - 1;
       const RunsOut o{scale, dim, p.chunks, p.slices, l == 0 ? met : nullptr, s.rank,
                       last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
-      const dim3 grid(static_cast<unsigned>((p.tiles[l] * p.slices + kThreads / G - 1) / (kThreads / G)));
+      const dim3 grid(static_cast<unsigned>(p.parts[l] * p.slices));
       if (l == 0)
-        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(kThreads), 0, st, s.sorted, p.n, num_rows, grad, stride,
-                           p.size, p.tiles[0], o, out);
+        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(kSumThreads<G>), 0, st, s.sorted, p.n, num_rows, grad,
+                           stride, p.size, o, out);
       else
-        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(kThreads), 0, st, s.entries[(l - 1) & 1],
-                           2 * p.tiles[l - 1], s.sums[(l - 1) & 1], kJoinSize, p.tiles[l], o, out);
+        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(kSumThreads<G>), 0, st, s.entries[(l - 1) & 1],
+                           2 * p.parts[l - 1], s.sums[(l - 1) & 1], o, out);
     }
   });
 }
@@ -367,7 +400,7 @@ int check_ids(const char* what, const void* ids, int id_bytes, int64_t n) {
 }
 // whether every launch of the sums has a grid that can be launched
 int check_plan(const char* what, const SumPlan& p) {
-  if (p.tiles[0] * p.slices < (int64_t(1) << 31)) return GS_OK;
+  if (p.parts[0] * p.slices < (int64_t(1) << 31)) return GS_OK;
   set_error_text("%s: %lld rows of %lld chunks are more than one launch takes", what, static_cast<long long>(p.n),
                  static_cast<long long>(p.chunks));
   return GS_ERR_UNSUPPORTED;

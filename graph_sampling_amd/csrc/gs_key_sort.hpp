@@ -185,10 +185,19 @@ pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restr
   if (SELF) {  // four threads a digit, a quarter of the tiles each
     const int part = threadIdx.x / kDigits;
     uint32_t all = 0, before = 0;
-    for (int64_t b = part; b < tiles; b += kThreads / kDigits) {
-      const uint32_t c = counts[b * kDigits + digit];
-      all += c;
-      before += b < tile ? c : 0;
+    for (int64_t b0 = part; b0 < tiles; b0 += 8 * (kThreads / kDigits)) {
+      uint32_t c[8];  // (asked for together)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t b = b0 + k * (kThreads / kDigits);
+        c[k] = counts[(b < tiles ? b : tiles - 1) * kDigits + digit];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t b = b0 + k * (kThreads / kDigits);
+        all += b < tiles ? c[k] : 0;
+        before += b < tile ? c[k] : 0;
+      }
     }
     s_all[part][digit] = all;
     s_before[part][digit] = before;
