@@ -87,14 +87,15 @@ struct RunsOut {
 };
 
 // A workgroup is up to 64 groups of G lanes, a chunk of the row a lane, group after group along the list.
-template <int G>
-constexpr int kGroups = 1024 / G < 64 ? 1024 / G : 64;
-template <int G>
-constexpr int kSumThreads = kGroups<G>* G;
+// Those that sum rows have up to 512 threads, so that four of them share a compute unit; those that
+// join what is left up to 1024, so that few launches do.  (A group that took 32 entries one after the other
+// needed 11 us for the 256 of 16 k ids where two a group need 4.)
+constexpr int kSumMost = 512, kJoinMost = 1024;
+constexpr int groups_in(int most, int lanes) { return most / lanes < 64 ? most / lanes : 64; }
 
-template <typename T, int G>
+template <typename T, int G, int GROUPS>
 struct Runs {
-  static constexpr int kEntries = 2 * kGroups<G>;
+  static constexpr int kEntries = 2 * GROUPS;
   struct Shared {
     Entry entry[kEntries];
     Entry left[2];  // the workgroup's own
@@ -137,13 +138,25 @@ struct Runs {
     const uint32_t row = s.entry[i].row;
     const bool left = i == 0;
     Wide<T> sum = s.sum[i][lane];
-    int j = i + 1;
-    for (; j < kEntries; ++j) {
-      const Entry e = s.entry[j];
-      if (e.state == kNone || e.row != row) break;
-      if (e.state == kSum) sum += s.sum[j][lane];
+    bool right = i + 1 == kEntries;
+    for (int j0 = i + 1; j0 < kEntries; j0 += 4) {
+      Entry e[4];
+      Wide<T> v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        e[k] = s.entry[j0 + k < kEntries ? j0 + k : kEntries - 1];
+        v[k] = s.sum[j0 + k < kEntries ? j0 + k : kEntries - 1][lane];  // (what is no sum is not added)
+      }
+      bool on = true;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (j0 + k >= kEntries) break;
+        on = on && e[k].state != kNone && e[k].row == row;
+        if (on && e[k].state == kSum) sum += v[k];
+        if (on && j0 + k + 1 == kEntries) right = true;
+      }
+      if (!on) break;
     }
-    const bool right = j == kEntries;
     if (!left && !right) return write(row, sum);
     const int slot = left ? 0 : 1;
     if (in) {
@@ -158,27 +171,38 @@ struct Runs {
   // behind every group's tile: every thread of the workgroup calls this
   __device__ __forceinline__ void join() {
     __syncthreads();
-    if (group == 0 && s.entry[0].state == kSum) walk(0);
-    if (s.entry[2 * group + 1].state == kSum) walk(2 * group + 1);
+    for (int i = 2 * group; i < 2 * group + 2; ++i)  // where a run's first piece is
+      if (s.entry[i].state == kSum && (i == 0 || s.entry[i - 1].state == kNone || s.entry[i - 1].row != s.entry[i].row))
+        walk(i);
     __syncthreads();
     if (o.entries && threadIdx.x < 2 && blockIdx.x == part * o.slices)
       o.entries[2 * part + threadIdx.x] = s.left[threadIdx.x];
   }
 };
 
-constexpr int kBatch = 8;  // rows a group asks for together
+constexpr int kBatch = 8;      // rows a group asks for together
+constexpr int kMostSize = 32;  // positions of a tile at most
 
 // A tile of `size` sorted positions a group.
 template <typename T, int G>
-__global__ void __launch_bounds__(kSumThreads<G>)
+__global__ void __launch_bounds__(groups_in(kSumMost, G) * G)
 sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t num_rows, const T* __restrict__ grad,
                 int64_t stride, int size, RunsOut o, T* __restrict__ out) {
-  __shared__ typename Runs<T, G>::Shared s_runs;
-  Runs<T, G> runs(o, s_runs, out);
-  const int64_t base = (runs.part * kGroups<G> + runs.group) * size;
+  constexpr int kGroups = groups_in(kSumMost, G);
+  __shared__ typename Runs<T, G, kGroups>::Shared s_runs;
+  __shared__ key_sort::Word s_words[kGroups * kMostSize];
+  Runs<T, G, kGroups> runs(o, s_runs, out);
+  {  // the workgroup's words, once
+    const int64_t first = runs.part * kGroups * size;
+    for (int j = threadIdx.x; j < kGroups * size; j += kGroups * G)
+      s_words[j] = words[first + j < n ? first + j : n - 1];
+    __syncthreads();
+  }
+  const key_sort::Word* const mine = s_words + runs.group * size;
+  const int64_t base = (runs.part * kGroups + runs.group) * size;
   const T* const from = grad + chunk_start<T>(o.dim, runs.chunk);
   const int count = n - base < size ? (n > base ? static_cast<int>(n - base) : 0) : size;
-  uint32_t key = count > 0 ? key_sort::key_of(words[base]) : num_rows;
+  uint32_t key = count > 0 ? key_sort::key_of(mine[0]) : num_rows;
   if (key < num_rows) {
     bool left = base > 0 && key_sort::key_of(words[base - 1]) == key;
     const uint32_t behind = base + count < n ? key_sort::key_of(words[base + count]) : num_rows;
@@ -191,7 +215,7 @@ sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t nu
       key_sort::Word w[kBatch];
       Values<T> v[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) w[k] = words[base + (j0 + k < count ? j0 + k : count - 1)];
+      for (int k = 0; k < kBatch; ++k) w[k] = mine[j0 + k < count ? j0 + k : count - 1];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) v[k] = load_chunk(from + key_sort::position_of(w[k]) * stride, o.dim);
 #pragma unroll
@@ -215,51 +239,23 @@ sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t nu
   runs.join();
 }
 
-// A tile of kJoinSize entries that an earlier launch left a group, of m; sums_in as RunsOut::sums.
-constexpr int kJoinSize = 16;
-
+// Two entries that an earlier launch left a group, of m; sums_in as RunsOut::sums.
 template <typename T, int G>
-__global__ void __launch_bounds__(kSumThreads<G>)
+__global__ void __launch_bounds__(groups_in(kJoinMost, G) * G)
 join_runs_kernel(const Entry* __restrict__ in, int64_t m, const float* __restrict__ sums_in, RunsOut o,
                  T* __restrict__ out) {
-  __shared__ typename Runs<T, G>::Shared s_runs;
-  Runs<T, G> runs(o, s_runs, out);
-  const int64_t base = (runs.part * kGroups<G> + runs.group) * kJoinSize;
-  const Entry none{0, kNone};
-  const Entry before = base > 0 && base <= m ? in[base - 1] : none;
-  const Entry behind = base + kJoinSize < m ? in[base + kJoinSize] : none;
-  Entry e[kJoinSize];
+  constexpr int kGroups = groups_in(kJoinMost, G);
+  __shared__ typename Runs<T, G, kGroups>::Shared s_runs;
+  Runs<T, G, kGroups> runs(o, s_runs, out);
+  const int64_t base = 2 * (runs.part * kGroups + runs.group);
 #pragma unroll
-  for (int k = 0; k < kJoinSize; ++k) {
-    e[k] = in[base + k < m ? base + k : m - 1];
-    if (base + k >= m) e[k] = none;
+  for (int k = 0; k < 2; ++k) {
+    const Entry e = base + k < m ? in[base + k] : Entry{0, kNone};
+    if (e.state == kSum)
+      __builtin_memcpy(&s_runs.sum[2 * runs.group + k][runs.lane],
+                       sums_in + ((base + k) * o.chunks + runs.chunk) * Chunk<T>::kVec, sizeof(Wide<T>));
+    if (runs.lane == 0) s_runs.entry[2 * runs.group + k] = e;
   }
-  bool open = false, left = false;
-  uint32_t row = 0;
-  Wide<T> sum = {};
-#pragma unroll
-  for (int j0 = 0; j0 < kJoinSize; j0 += kBatch) {
-    Wide<T> v[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      v[k] = Wide<T>{};
-      if (e[j0 + k].state == kSum)
-        __builtin_memcpy(&v[k], sums_in + ((base + j0 + k) * o.chunks + runs.chunk) * Chunk<T>::kVec, sizeof(v[k]));
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (e[j0 + k].state == kNone) continue;  // (never inside a run)
-      if (!open || e[j0 + k].row != row) {
-        if (open) runs.finish(row, sum, left, false);
-        open = true;
-        row = e[j0 + k].row;
-        left = j0 + k == 0 && before.state != kNone && before.row == row;
-        sum = Wide<T>{};
-      }
-      sum += v[k];
-    }
-  }
-  if (open) runs.finish(row, sum, left, behind.state != kNone && behind.row == row);
   runs.join();
 }
 
@@ -279,15 +275,15 @@ struct SumPlan {
     group = 1;
     while (group < kWave && group < chunks) group *= 2;
     slices = static_cast<int>((chunks + group - 1) / group);
-    const int groups = 1024 / group < 64 ? 1024 / group : 64;
+    const int groups = groups_in(kSumMost, group), joins = groups_in(kJoinMost, group);
     // as long as there are waves enough for the chip, longer tiles leave fewer partial sums
-    size = 32;
+    size = kMostSize;
     while (size > 8 && (n / size) * slices * group < int64_t(256) * 16 * kWave) size /= 2;
     levels = 0;
     int64_t p = (n + int64_t(size) * groups - 1) / (int64_t(size) * groups);
     parts[levels++] = p;
     while (p > 1) {
-      p = (2 * p + kJoinSize * groups - 1) / (kJoinSize * groups);
+      p = (p + joins - 1) / joins;
       parts[levels++] = p;
     }
   }
@@ -355,10 +351,10 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
                       last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
       const dim3 grid(static_cast<unsigned>(p.parts[l] * p.slices));
       if (l == 0)
-        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(kSumThreads<G>), 0, st, s.sorted, p.n, num_rows, grad,
+        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(groups_in(kSumMost, G) * G), 0, st, s.sorted, p.n, num_rows, grad,
                            stride, p.size, o, out);
       else
-        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(kSumThreads<G>), 0, st, s.entries[(l - 1) & 1],
+        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(groups_in(kJoinMost, G) * G), 0, st, s.entries[(l - 1) & 1],
                            2 * p.parts[l - 1], s.sums[(l - 1) & 1], o, out);
     }
   });
