@@ -29,10 +29,11 @@ struct OrderOut {
   __device__ __forceinline__ void digit(uint32_t d, uint32_t start) const {
     if (d <= experts) offsets[d] = start;
   }
+  __device__ __forceinline__ void from(key_sort::Word w, uint32_t at) const {
+    place[key_sort::position_of(w)] = key_sort::key_of(w) < experts ? static_cast<int32_t>(at) : -1;
+  }
   __device__ __forceinline__ void item(uint32_t at, key_sort::Word w) const {
-    const bool there = key_sort::key_of(w) < experts;
-    place[key_sort::position_of(w)] = there ? static_cast<int32_t>(at) : -1;
-    order[at] = there ? static_cast<int32_t>(key_sort::position_of(w)) : -1;
+    order[at] = key_sort::key_of(w) < experts ? static_cast<int32_t>(key_sort::position_of(w)) : -1;
   }
 };
 
@@ -40,7 +41,10 @@ struct OrderOut {
 __global__ void __launch_bounds__(kThreads)
 order_kernel(const key_sort::Word* __restrict__ words, int64_t n, OrderOut out) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i < n) out.item(static_cast<uint32_t>(i), words[i]);
+  if (i < n) {
+    out.from(words[i], static_cast<uint32_t>(i));
+    out.item(static_cast<uint32_t>(i), words[i]);
+  }
   if (i <= static_cast<int64_t>(out.experts)) {
     int64_t lo = 0, hi = n;  // items of the experts before i
     while (lo < hi) {
@@ -289,7 +293,7 @@ int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOu
     return check_launch("expert_sort");
   }
   const uint32_t num = static_cast<uint32_t>(num_experts);
-  const int passes = key_sort::passes_for(num);
+  const int passes = key_sort::Digits(num).passes;
   Carver ws(workspace, workspace_bytes);
   key_sort::Space space;
   key_sort::carve(ws, n, passes > 1 ? 2 : 0, &space);
@@ -321,7 +325,7 @@ extern "C" {
 size_t gs_expert_sort_workspace_bytes(int64_t n, int64_t num_experts) {
   if (n <= 0 || num_experts < 0) return 256;
   const uint32_t num = static_cast<uint32_t>(num_experts);
-  return key_sort::space_bytes(n, key_sort::passes_for(num) > 1 ? 2 : 0);
+  return key_sort::space_bytes(n, key_sort::Digits(num).passes > 1 ? 2 : 0);
 }
 
 int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_experts, int32_t* order, int32_t* place,

@@ -1,6 +1,6 @@
 // Stable sort of the positions 0..n-1 by a key, for keys of a few bits: what the gradient of an
 // embedding and the sending of rows to experts start from.  One 64-bit word per item, the key
-// above its position, eight bits of the key a pass; nothing here keeps a state between calls or
+// above its position, eight or nine bits of the key a pass; nothing here keeps a state between calls or
 // waits for another workgroup, so that a call can be captured into a graph.
 #pragma once
 
@@ -9,14 +9,15 @@
 namespace gs {
 namespace key_sort {
 
-constexpr int kBits = 8;
-constexpr int kDigits = 1 << kBits;
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kItems = 4;
-constexpr int kTile = kThreads * kItems;
-// tiles whose counts every workgroup of a pass adds up by itself
-constexpr int64_t kSelfTiles = 256;
+constexpr int kItems = 4;  // of a thread
+// A tile is 512 threads' items, or 1024's: comparing the items of a tile by ballots is what a pass
+// takes longest for, so as long as there are compute units without a tile, tiles are small.
+constexpr int kSmall = 512, kLarge = 1024;
+constexpr int64_t kAlone = kLarge * kItems;           // items that one workgroup sorts alone
+constexpr int64_t kFewItems = 8 * kSmall * kItems;    // items that every workgroup of a pass counts by itself
+constexpr int64_t kSelfTiles = 256;  // tiles whose counts every workgroup of a pass adds up by itself
+constexpr int kMostDigits = 512;
+inline int threads_for(int64_t n) { return n <= kSelfTiles * kSmall * kItems ? kSmall : kLarge; }
 
 using Word = unsigned long long;
 
@@ -38,19 +39,36 @@ struct StoredWords {
 
 __device__ __forceinline__ uint32_t key_of(Word w) { return static_cast<uint32_t>(w >> 32); }
 __device__ __forceinline__ uint32_t position_of(Word w) { return static_cast<uint32_t>(w); }
+
+// Digits of eight bits, or of nine where that is a pass less (keys of 17 and 18 bits, of 25 to 27): 400 k
+// keys of 18 bits take two passes of 16 us for three of 13.
+struct Digits {
+  int bits, passes;
+  explicit Digits(uint32_t num) {
+    int key_bits = 1;
+    while (key_bits < 32 && (num >> key_bits) != 0) ++key_bits;
+    const int eight = (key_bits + 7) / 8, nine = (key_bits + 8) / 9;
+    bits = nine < eight ? 9 : 8;
+    passes = nine < eight ? nine : eight;
+  }
+};
+template <int BITS>
 __device__ __forceinline__ uint32_t digit_of(Word w, int pass) {
-  return (key_of(w) >> (kBits * pass)) & (kDigits - 1);
+  return (key_of(w) >> (BITS * pass)) & ((1u << BITS) - 1);
 }
 
-// passes for the keys 0..num
-inline int passes_for(uint32_t num) {
-  int passes = 1;
-  while (passes < 4 && (static_cast<uint64_t>(num) >> (kBits * passes)) != 0) ++passes;
-  return passes;
-}
+// Work that has nothing to do with the sort and runs beside it, in workgroups of their own: a sort of
+// a few thousand items occupies a few compute units.
+struct NoWork {
+  static constexpr bool kAny = false;
+  __device__ __forceinline__ void run(int64_t, int64_t, int) const {}
+};
 
+template <int BITS, int THREADS>
 struct TileTables {
-  uint32_t count[kWaves][kDigits];  // of a wave's items, then of the waves before it
+  static constexpr int kDigits = 1 << BITS, kWaves = THREADS / kWave;
+  static_assert(kDigits <= THREADS, "a thread a digit");
+  uint16_t count[kWaves][kDigits];  // of a wave's items, then of the waves before it
   uint32_t scan[kDigits / kWave];
 };
 
@@ -59,52 +77,60 @@ __device__ __forceinline__ uint32_t item_of(int r) {
   return (threadIdx.x / kWave) * (kWave * kItems) + r * kWave + (threadIdx.x & (kWave - 1));
 }
 
-// Rank of each item among the earlier items of the tile with its digit, and in `total` (threads
-// below 256) how many items the tile holds of digit threadIdx.x.  A round's 64 items are compared by
-// eight ballots; only the wave itself touches its counts until the barrier.  Items from `live`
+// Rank of each item among the earlier items of the tile with its digit, and in `total` (a thread a
+// digit) how many items the tile holds of digit threadIdx.x.  A round's 64 items are compared by a
+// ballot a bit; only the wave itself touches its counts until the barrier.  Items from `live`
 // on are not counted.  Every thread of the workgroup calls this.
-__device__ __forceinline__ void rank_tile(const uint32_t (&digit)[kItems], uint32_t live, TileTables& t,
+template <int BITS, int THREADS>
+__device__ __forceinline__ void rank_tile(const uint32_t (&digit)[kItems], uint32_t live, TileTables<BITS, THREADS>& t,
                                           uint32_t (&rank)[kItems], uint32_t* total) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  for (int j = threadIdx.x; j < kWaves * kDigits; j += kThreads) (&t.count[0][0])[j] = 0;
+  constexpr int kDigits = 1 << BITS, kWaves = THREADS / kWave;
+  const int wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int j = threadIdx.x; j < kWaves * kDigits / 2; j += THREADS)
+    reinterpret_cast<uint32_t*>(&t.count[0][0])[j] = 0;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kItems; ++r) {
     const bool in = item_of(r) < live;
-    unsigned long long same = __ballot(in);
+    const unsigned long long there = __ballot(in);
+    // lanes with this digit: per bit, the lanes whose bit equals this lane's (and-not-xor in one instruction)
+    uint32_t lo = static_cast<uint32_t>(there), hi = static_cast<uint32_t>(there >> 32);
 #pragma unroll
-    for (int b = 0; b < kBits; ++b) {
-      const unsigned long long set = __ballot((digit[r] >> b) & 1u);
-      same &= (digit[r] >> b) & 1u ? set : ~set;
+    for (int b = 0; b < BITS; ++b) {
+      const int mine = static_cast<int>(digit[r] << (31 - b)) >> 31;
+      const unsigned long long set = __ballot(mine);
+      lo = __builtin_amdgcn_bitop3_b32(lo, static_cast<uint32_t>(set), mine, 0x90);
+      hi = __builtin_amdgcn_bitop3_b32(hi, static_cast<uint32_t>(set >> 32), mine, 0x90);
     }
-    uint32_t earlier = 0;
-    if (in) earlier = t.count[wave][digit[r]];
-    const uint32_t in_round = __popcll(same & ((1ull << lane) - 1));
+    const uint32_t in_round = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+    const uint32_t earlier = t.count[wave][digit[r]];  // (LDS operations of a wave keep their order)
     rank[r] = earlier + in_round;
-    __builtin_amdgcn_wave_barrier();  // (all have read before the last of the equal ones adds them)
-    if (in && (same >> lane) == 1ull) t.count[wave][digit[r]] = rank[r] + 1;
-    __builtin_amdgcn_wave_barrier();
+    if (in && in_round == 0) t.count[wave][digit[r]] = static_cast<uint16_t>(earlier + __popc(lo) + __popc(hi));
   }
   __syncthreads();
   uint32_t sum = 0;
   if (threadIdx.x < kDigits) {
+    uint32_t c[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) c[w] = t.count[w][threadIdx.x];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const uint32_t c = t.count[w][threadIdx.x];
-      t.count[w][threadIdx.x] = sum;
-      sum += c;
+      t.count[w][threadIdx.x] = static_cast<uint16_t>(sum);
+      sum += c[w];
     }
   }
   *total = sum;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kItems; ++r)
-    if (item_of(r) < live) rank[r] += t.count[wave][digit[r]];
+  for (int r = 0; r < kItems; ++r) rank[r] += t.count[wave][digit[r]];
 }
 
-// Exclusive prefix over the digits, one a thread (threads below 256 hold a value); ends with a barrier
+// Exclusive prefix over the digits, one a thread (the first threads hold a value); ends with a barrier
 // for all.
-__device__ __forceinline__ uint32_t scan_digits(uint32_t v, TileTables& t) {
+template <int BITS, int THREADS>
+__device__ __forceinline__ uint32_t scan_digits(uint32_t v, TileTables<BITS, THREADS>& t) {
+  constexpr int kDigits = 1 << BITS;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   uint32_t incl = v;
 #pragma unroll
@@ -115,29 +141,34 @@ __device__ __forceinline__ uint32_t scan_digits(uint32_t v, TileTables& t) {
   if (threadIdx.x < kDigits && lane == kWave - 1) t.scan[wave] = incl;
   __syncthreads();
   uint32_t before = 0;
-  if (threadIdx.x < kDigits)
-    for (int w = 0; w < wave; ++w) before += t.scan[w];
+  if (threadIdx.x < kDigits) {
+#pragma unroll
+    for (int w = 0; w < kDigits / kWave; ++w) before += w < wave ? t.scan[w] : 0;
+  }
   __syncthreads();
   return before + incl - v;
 }
 
-// counts[tile * 256 + d] = items of the tile with digit d
-template <typename Src>
-__global__ void __launch_bounds__(kThreads)
-count_kernel(Src src, int64_t n, int pass, uint32_t* __restrict__ counts) {
+// counts[tile * digits + d] = items of the tile with digit d
+template <int BITS, int THREADS, typename Src, typename Beside>
+__global__ void __launch_bounds__(THREADS)
+count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__ counts, Beside beside) {
+  constexpr int kDigits = 1 << BITS;
+  if (Beside::kAny && blockIdx.x >= tiles) return beside.run(blockIdx.x - tiles, gridDim.x - tiles, THREADS);
   __shared__ uint32_t s_hist[4][kDigits];
-  for (int j = threadIdx.x; j < 4 * kDigits; j += kThreads) (&s_hist[0][0])[j] = 0;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (THREADS * kItems);
   Word w[kItems];
 #pragma unroll
   for (int r = 0; r < kItems; ++r) {
-    const int64_t i = base + r * kThreads + threadIdx.x;
+    const int64_t i = base + r * THREADS + threadIdx.x;
     w[r] = src(i < n ? i : n - 1);
   }
+#pragma unroll
+  for (int j = threadIdx.x; j < 4 * kDigits; j += THREADS) (&s_hist[0][0])[j] = 0;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kItems; ++r)
-    if (base + r * kThreads + threadIdx.x < n) atomicAdd(&s_hist[threadIdx.x & 3][digit_of(w[r], pass)], 1u);
+    if (base + r * THREADS + threadIdx.x < n) atomicAdd(&s_hist[threadIdx.x & 3][digit_of<BITS>(w[r], pass)], 1u);
   __syncthreads();
   if (threadIdx.x < kDigits) {
     uint32_t all = 0;
@@ -149,30 +180,40 @@ count_kernel(Src src, int64_t n, int pass, uint32_t* __restrict__ counts) {
 
 // For sorts of more than kSelfTiles tiles: in place of every count, how many items of its digit the
 // tiles before hold, and in totals[d] how many all hold.  A workgroup a digit.
-static __global__ void __launch_bounds__(kThreads)
-prefix_kernel(uint32_t* __restrict__ counts, int64_t tiles, uint32_t* __restrict__ totals) {
-  __shared__ int64_t s_scan[kWaves + 1];
+static __global__ void __launch_bounds__(kLarge)
+prefix_kernel(uint32_t* __restrict__ counts, int64_t tiles, int digits, uint32_t* __restrict__ totals) {
+  __shared__ int64_t s_scan[kLarge / kWave + 1];
   const int digit = blockIdx.x;
   int64_t run = 0;
-  for (int64_t t0 = 0; t0 < tiles; t0 += kThreads) {
+  for (int64_t t0 = 0; t0 < tiles; t0 += kLarge) {
     const int64_t t = t0 + threadIdx.x;
-    const int64_t c = t < tiles ? counts[t * kDigits + digit] : 0;
+    const int64_t c = t < tiles ? counts[t * digits + digit] : 0;
     int64_t all;
-    const int64_t at = block_exclusive_scan<kThreads>(c, &all, s_scan);
-    if (t < tiles) counts[t * kDigits + digit] = static_cast<uint32_t>(run + at);
+    const int64_t at = block_exclusive_scan<kLarge>(c, &all, s_scan);
+    if (t < tiles) counts[t * digits + digit] = static_cast<uint32_t>(run + at);
     run += all;
   }
   if (threadIdx.x == 0) totals[digit] = static_cast<uint32_t>(run);
 }
 
-// One pass over one tile.  Out: what becomes of an item at its place (and, of the first tile, of the
-// places where the digits start).
-template <typename Src, bool SELF, typename Out>
-__global__ void __launch_bounds__(kThreads)
+// Where a pass gets the counts of all tiles from: it counts all items by itself (a launch less, for few),
+// adds up the tiles' counts, or finds them added up.
+enum class Counts { kHere, kTiles, kPrefixes };
+
+// One pass over one tile.  Out: what becomes of an item at its place -- `item`, in the order of their
+// places, so that neighbours are written together, and `from`, in the order in which they came -- and, of
+// the first tile, of the places where the digits start.  The tile is put in order in LDS first.
+template <int BITS, int THREADS, typename Src, Counts COUNTS, typename Out, typename Beside>
+__global__ void __launch_bounds__(THREADS)
 pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restrict__ counts,
-            const uint32_t* __restrict__ totals, Out out) {
-  __shared__ TileTables s_tables;
-  __shared__ uint32_t s_all[4][kDigits], s_before[4][kDigits], s_base[kDigits];
+            const uint32_t* __restrict__ totals, Out out, Beside beside) {
+  constexpr int kDigits = 1 << BITS, kParts = THREADS / kDigits, kTile = THREADS * kItems;
+  if (Beside::kAny && blockIdx.x >= tiles) return beside.run(blockIdx.x - tiles, gridDim.x - tiles, THREADS);
+  __shared__ TileTables<BITS, THREADS> s_tables;
+  __shared__ uint32_t s_all[kParts][kDigits], s_before[kParts][kDigits];
+  __shared__ uint32_t s_start[kDigits];  // where a digit's items start in the tile
+  __shared__ uint32_t s_shift[kDigits];  // from a place in the tile's order to the place in memory, modulo 2^32
+  __shared__ Word s_word[kTile];
   const int64_t tile = blockIdx.x, base = tile * kTile;
   const uint32_t live = n - base < kTile ? static_cast<uint32_t>(n - base) : kTile;
   Word w[kItems];
@@ -181,22 +222,40 @@ pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restr
     const uint32_t j = item_of(r);
     w[r] = src(base + (j < live ? j : live - 1));
   }
-  const int digit = threadIdx.x & (kDigits - 1);
-  if (SELF) {  // four threads a digit, a quarter of the tiles each
-    const int part = threadIdx.x / kDigits;
-    uint32_t all = 0, before = 0;
-    for (int64_t b0 = part; b0 < tiles; b0 += 8 * (kThreads / kDigits)) {
-      uint32_t c[8];  // (asked for together)
+  const int digit = threadIdx.x & (kDigits - 1), part = threadIdx.x / kDigits;
+  if constexpr (COUNTS == Counts::kHere) {
+    constexpr int kAhead = 8;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t b = b0 + k * (kThreads / kDigits);
-        c[k] = counts[(b < tiles ? b : tiles - 1) * kDigits + digit];
+    for (int j = threadIdx.x; j < kParts * kDigits; j += THREADS) (&s_all[0][0])[j] = (&s_before[0][0])[j] = 0;
+    __syncthreads();
+    for (int64_t i0 = threadIdx.x; i0 < n; i0 += kAhead * THREADS) {
+      Word other[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) other[k] = src(i0 + k * THREADS < n ? i0 + k * THREADS : n - 1);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t i = i0 + k * THREADS;
+        if (i >= n) continue;
+        atomicAdd(i < base ? &s_before[threadIdx.x % kParts][digit_of<BITS>(other[k], pass)]
+                           : &s_all[threadIdx.x % kParts][digit_of<BITS>(other[k], pass)], 1u);
+      }
+    }
+    // (s_all: of this tile and those behind it)
+  } else if constexpr (COUNTS == Counts::kTiles) {  // a share of the tiles a thread, kAhead counts asked for together
+    constexpr int kAhead = 16;
+    uint32_t all = 0, before = 0;
+    for (int b0 = part; b0 < static_cast<int>(tiles); b0 += kAhead * kParts) {
+      uint32_t c[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int b = b0 + k * kParts;
+        c[k] = counts[(b < static_cast<int>(tiles) ? b : b0) * kDigits + digit];
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t b = b0 + k * (kThreads / kDigits);
-        all += b < tiles ? c[k] : 0;
-        before += b < tile ? c[k] : 0;
+      for (int k = 0; k < kAhead; ++k) {
+        const int b = b0 + k * kParts;
+        all += b < static_cast<int>(tiles) && b >= static_cast<int>(tile) ? c[k] : 0;
+        before += b < static_cast<int>(tile) ? c[k] : 0;
       }
     }
     s_all[part][digit] = all;
@@ -204,73 +263,96 @@ pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restr
   }
   uint32_t d[kItems], rank[kItems], total;
 #pragma unroll
-  for (int r = 0; r < kItems; ++r) d[r] = digit_of(w[r], pass);
-  rank_tile(d, live, s_tables, rank, &total);
+  for (int r = 0; r < kItems; ++r) d[r] = digit_of<BITS>(w[r], pass);
+  rank_tile<BITS, THREADS>(d, live, s_tables, rank, &total);
   uint32_t all = 0, before = 0;
   if (threadIdx.x < kDigits) {
-    if (SELF) {
+    if (COUNTS == Counts::kPrefixes) {
+      all = totals[digit];
+      before = counts[tile * kDigits + digit];
+    } else {
 #pragma unroll
-      for (int p = 0; p < kThreads / kDigits; ++p) {
+      for (int p = 0; p < kParts; ++p) {
         all += s_all[p][digit];
         before += s_before[p][digit];
       }
-    } else {
-      all = totals[digit];
-      before = counts[tile * kDigits + digit];
+      all += before;
     }
   }
-  const uint32_t start = scan_digits(all, s_tables);
+  const uint32_t start = scan_digits<BITS, THREADS>(all, s_tables);
+  const uint32_t here = scan_digits<BITS, THREADS>(total, s_tables);
   if (threadIdx.x < kDigits) {
-    s_base[digit] = start + before;
+    s_start[digit] = here;
+    s_shift[digit] = start + before - here;
     if (tile == 0) out.digit(digit, start);
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kItems; ++r)
-    if (item_of(r) < live) out.item(s_base[d[r]] + rank[r], w[r]);
+  for (int r = 0; r < kItems; ++r) {
+    if (item_of(r) >= live) continue;
+    const uint32_t at = s_start[d[r]] + rank[r];
+    s_word[at] = w[r];
+    out.from(w[r], at + s_shift[d[r]]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const uint32_t at = r * THREADS + threadIdx.x;
+    if (at >= live) continue;
+    const Word word = s_word[at];
+    out.item(at + s_shift[digit_of<BITS>(word, pass)], word);
+  }
 }
 
-// All passes of a sort of one tile, by one workgroup in LDS: one launch.
-template <typename Src, typename Out>
-__global__ void __launch_bounds__(kThreads)
-one_tile_kernel(Src src, uint32_t n, int passes, Out out) {
-  __shared__ TileTables s_tables;
-  __shared__ uint32_t s_base[kDigits];
-  __shared__ Word s_word[kTile];
+// All passes of a sort of up to kItems * THREADS items, by one workgroup in LDS: one launch.
+template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
+__global__ void __launch_bounds__(THREADS)
+alone_kernel(Src src, uint32_t n, int passes, Out out, Beside beside) {
+  constexpr int kDigits = 1 << BITS;
+  if (Beside::kAny && blockIdx.x >= 1) return beside.run(blockIdx.x - 1, gridDim.x - 1, THREADS);
+  __shared__ TileTables<BITS, THREADS> s_tables;
+  __shared__ uint32_t s_start[kDigits];
+  __shared__ Word s_word[THREADS * kItems];
   Word w[kItems];
 #pragma unroll
   for (int r = 0; r < kItems; ++r) w[r] = src(item_of(r) < n ? item_of(r) : n - 1);
-  for (int pass = 0;; ++pass) {
+  for (int pass = 0; pass < passes; ++pass) {
     const bool last = pass == passes - 1;
     uint32_t d[kItems], rank[kItems], total;
 #pragma unroll
-    for (int r = 0; r < kItems; ++r) d[r] = digit_of(w[r], pass);
-    rank_tile(d, n, s_tables, rank, &total);
-    const uint32_t start = scan_digits(total, s_tables);
+    for (int r = 0; r < kItems; ++r) d[r] = digit_of<BITS>(w[r], pass);
+    rank_tile<BITS, THREADS>(d, n, s_tables, rank, &total);
+    const uint32_t start = scan_digits<BITS, THREADS>(total, s_tables);
     if (threadIdx.x < kDigits) {
-      s_base[threadIdx.x] = start;
+      s_start[threadIdx.x] = start;
       if (last) out.digit(threadIdx.x, start);
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kItems; ++r) {
       if (item_of(r) >= n) continue;
-      const uint32_t at = s_base[d[r]] + rank[r];
-      if (last) out.item(at, w[r]);
-      else s_word[at] = w[r];
+      const uint32_t at = s_start[d[r]] + rank[r];
+      s_word[at] = w[r];
+      if (last) out.from(w[r], at);
     }
-    if (last) return;
     __syncthreads();
+    if (!last) {
 #pragma unroll
-    for (int r = 0; r < kItems; ++r)
-      if (item_of(r) < n) w[r] = s_word[item_of(r)];
-    __syncthreads();
+      for (int r = 0; r < kItems; ++r) w[r] = s_word[item_of(r) < n ? item_of(r) : n - 1];
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const uint32_t at = r * THREADS + threadIdx.x;
+    if (at < n) out.item(at, s_word[at]);
   }
 }
 
 struct WordsOut {
   Word* word;
   __device__ __forceinline__ void digit(uint32_t, uint32_t) const {}
+  __device__ __forceinline__ void from(Word, uint32_t) const {}
   __device__ __forceinline__ void item(uint32_t at, Word w) const { word[at] = w; }
 };
 
@@ -279,51 +361,85 @@ struct Space {
   uint32_t* counts;
   uint32_t* totals;
 };
-inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+inline int64_t tiles_of(int64_t n) {
+  const int64_t tile = threads_for(n) * kItems;
+  return (n + tile - 1) / tile;
+}
 // words: of the two buffers, how many the sort needs (a last pass that writes elsewhere: passes - 1, at most 2)
 inline size_t space_bytes(int64_t n, int words) {
-  return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(tiles_of(n)) * kDigits * 4) +
-         padded(kDigits * 4);
+  return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(tiles_of(n)) * kMostDigits * 4) +
+         padded(kMostDigits * 4);
 }
 inline void carve(Carver& ws, int64_t n, int words, Space* s) {
   for (int i = 0; i < 2; ++i) s->word[i] = i < words ? ws.take<Word>(static_cast<size_t>(n)) : nullptr;
-  s->counts = ws.take<uint32_t>(static_cast<size_t>(tiles_of(n)) * kDigits);
-  s->totals = ws.take<uint32_t>(kDigits);
+  s->counts = ws.take<uint32_t>(static_cast<size_t>(tiles_of(n)) * kMostDigits);
+  s->totals = ws.take<uint32_t>(kMostDigits);
 }
 
-template <typename Src, typename Out>
-void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, hipStream_t st) {
+// a launch of `tiles` workgroups and those of the work beside it, as its next part
+template <typename Beside, typename Kernel, typename... Args>
+void launch_beside(Kernel kernel, int64_t tiles, int threads, hipStream_t st, Beside& beside, Args... args) {
+  int64_t blocks = tiles;
+  if constexpr (Beside::kAny) blocks += beside.blocks(threads);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, args..., beside);
+  if constexpr (Beside::kAny) ++beside.part;
+}
+
+template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
+void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& beside, hipStream_t st) {
   const int64_t tiles = tiles_of(n);
-  const dim3 grid(static_cast<unsigned>(tiles));
-  hipLaunchKernelGGL(count_kernel<Src>, grid, dim3(kThreads), 0, st, src, n, pass, s.counts);
-  if (tiles <= kSelfTiles) {
-    hipLaunchKernelGGL((pass_kernel<Src, true, Out>), grid, dim3(kThreads), 0, st, src, n, pass, tiles, s.counts,
-                       s.totals, out);
+  const uint32_t *counts = s.counts, *totals = s.totals;
+  if (n <= kFewItems) {
+    launch_beside(pass_kernel<BITS, THREADS, Src, Counts::kHere, Out, Beside>, tiles, THREADS, st, beside, src, n, pass,
+                  tiles, counts, totals, out);
+    return;
+  }
+  launch_beside(count_kernel<BITS, THREADS, Src, Beside>, tiles, THREADS, st, beside, src, n, pass, tiles, s.counts);
+  const bool self = tiles <= kSelfTiles;
+  if (!self)
+    hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(kLarge), 0, st, s.counts, tiles, 1 << BITS, s.totals);
+  launch_beside(self ? pass_kernel<BITS, THREADS, Src, Counts::kTiles, Out, Beside>
+                     : pass_kernel<BITS, THREADS, Src, Counts::kPrefixes, Out, Beside>,
+                tiles, THREADS, st, beside, src, n, pass, tiles, counts, totals, out);
+}
+
+template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
+void sort_tiles(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
+  if constexpr (Beside::kAny) beside.parts = n <= kFewItems ? passes : 2 * passes;
+  for (int p = 0; p < passes; ++p) {
+    const StoredWords stored{s.word[(p + 1) & 1]};
+    const WordsOut next{s.word[p & 1]};
+    if (p == 0 && passes == 1) launch_pass<BITS, THREADS>(src, n, p, s, out, beside, st);
+    else if (p == 0) launch_pass<BITS, THREADS>(src, n, p, s, next, beside, st);
+    else if (p == passes - 1) launch_pass<BITS, THREADS>(stored, n, p, s, out, beside, st);
+    else launch_pass<BITS, THREADS>(stored, n, p, s, next, beside, st);
+  }
+}
+
+template <int BITS, typename Src, typename Out, typename Beside>
+void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
+  if (n <= kAlone) {
+    if constexpr (Beside::kAny) beside.parts = 1;
+    const uint32_t count = static_cast<uint32_t>(n);
+    if (n <= kSmall * kItems)
+      launch_beside(alone_kernel<BITS, kSmall, Src, Out, Beside>, 1, kSmall, st, beside, src, count, passes, out);
+    else
+      launch_beside(alone_kernel<BITS, kLarge, Src, Out, Beside>, 1, kLarge, st, beside, src, count, passes, out);
+  } else if (threads_for(n) == kSmall) {
+    sort_tiles<BITS, kSmall>(src, n, passes, s, out, beside, st);
   } else {
-    hipLaunchKernelGGL(prefix_kernel, dim3(kDigits), dim3(kThreads), 0, st, s.counts, tiles, s.totals);
-    hipLaunchKernelGGL((pass_kernel<Src, false, Out>), grid, dim3(kThreads), 0, st, src, n, pass, tiles, s.counts,
-                       s.totals, out);
+    sort_tiles<BITS, kLarge>(src, n, passes, s, out, beside, st);
   }
 }
 
 // Sorts n >= 1 items (below 2^31), keys 0..num; the last pass hands every word with its place to `out`.  Where
-// the sort has two passes it uses word[0] of the space, three or four word[0] and word[1].
-template <typename Src, typename Out>
-void sort(Src src, int64_t n, uint32_t num, const Space& s, Out out, hipStream_t st) {
-  const int passes = passes_for(num);
-  if (n <= kTile) {
-    hipLaunchKernelGGL((one_tile_kernel<Src, Out>), dim3(1), dim3(kThreads), 0, st, src, static_cast<uint32_t>(n),
-                       passes, out);
-    return;
-  }
-  for (int p = 0; p < passes; ++p) {
-    const StoredWords stored{s.word[(p + 1) & 1]};
-    const WordsOut next{s.word[p & 1]};
-    if (p == 0 && passes == 1) launch_pass(src, n, p, s, out, st);
-    else if (p == 0) launch_pass(src, n, p, s, next, st);
-    else if (p == passes - 1) launch_pass(stored, n, p, s, out, st);
-    else launch_pass(stored, n, p, s, next, st);
-  }
+// the sort has two passes it uses word[0] of the space, three or four word[0] and word[1].  beside: run in as many
+// equal parts as there are launches.
+template <typename Src, typename Out, typename Beside = NoWork>
+void sort(Src src, int64_t n, uint32_t num, const Space& s, Out out, hipStream_t st, Beside beside = Beside()) {
+  const Digits digits(num);
+  if (digits.bits == 9) sort_by<9>(src, n, digits.passes, s, out, beside, st);
+  else sort_by<8>(src, n, digits.passes, s, out, beside, st);
 }
 
 }  // namespace key_sort

@@ -56,6 +56,12 @@ __device__ __forceinline__ void store_chunk(T* p, Values<T> v, int64_t dim) {
       if (i < dim) p[i] = v[i];
   }
 }
+// the same past the caches, of a whole chunk
+template <typename T>
+__device__ __forceinline__ void store_past(T* p, Values<T> v) {
+  typedef Values<T> Loose __attribute__((aligned(sizeof(T))));
+  __builtin_nontemporal_store(v, reinterpret_cast<Loose*>(p));
+}
 template <typename T>
 __device__ __forceinline__ Wide<T> widen(Values<T> v) {
   return __builtin_convertvector(v, Wide<T>);
