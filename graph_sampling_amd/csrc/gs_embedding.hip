@@ -99,8 +99,8 @@ struct RunsOut {
   int64_t dim;
   int64_t chunks;        // of a row
   int slices;            // workgroups side by side over a row
-  int64_t* met;          // sparse: ids of the rows by their rank (null: dense)
-  const int64_t* rank;   // sparse: met rows before a sorted position
+  int64_t* met;          // sparse: ids of the rows by their rank
+  const int64_t* heads;  // sparse: runs that begin before a workgroup's positions
   Entry* entries;        // 2 a workgroup (null where there is one)
   float* sums;           // [2 * workgroups, chunks * kVec]
 };
@@ -202,58 +202,114 @@ struct Runs {
 constexpr int kBatch = 8;      // rows a group asks for together
 constexpr int kMostSize = 32;  // positions of a tile at most
 
-// A tile of `size` sorted positions a group.
+// A row's chunk, past the caches where a line holds no other row's: every row is read once (207 MB of random rows
+// of 256 B, added up by 32s: 43 us plain, 38 so).
 template <typename T, int G>
+__device__ __forceinline__ Values<T> load_once(const T* p, int64_t dim) {
+  if (G >= 16 && dim >= Chunk<T>::kVec) return load_past(p);
+  return load_chunk(p, dim);
+}
+
+// Whether a run of a row that is there begins at sorted position i.
+__device__ __forceinline__ bool run_begins(const key_sort::Word* __restrict__ words, int64_t i, uint32_t num_rows) {
+  const uint32_t key = key_sort::key_of(words[i]), before = key_sort::key_of(words[i > 0 ? i - 1 : 0]);
+  return key < num_rows && (i == 0 || before != key);
+}
+
+// Runs that begin among a workgroup's positions of the kernel below.
+__global__ void __launch_bounds__(kThreads)
+count_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t num_rows, int per_part,
+                  int64_t* __restrict__ counts) {
+  __shared__ int s_count;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_part;
+  int count = 0;
+  for (int j = threadIdx.x; j < per_part; j += kThreads)
+    count += first + j < n && run_begins(words, first + j, num_rows) ? 1 : 0;
+#pragma unroll
+  for (int m = kWave / 2; m > 0; m /= 2) count += __shfl_xor(count, m, kWave);
+  if (threadIdx.x % kWave == 0) atomicAdd(&s_count, count);
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = s_count;
+}
+
+// A tile of `size` sorted positions a group.  The workgroup's words lie in LDS as {output row, position of the
+// row in grad, top bit: a run begins}; the output row is the key, or its rank among the rows that are met (SPARSE),
+// and ~0 where there is none.
+template <typename T, int G, bool SPARSE>
 __global__ void __launch_bounds__(groups_in(kSumMost, G) * G)
 sum_runs_kernel(const key_sort::Word* __restrict__ words, int64_t n, uint32_t num_rows, const T* __restrict__ grad,
                 int64_t stride, int size, RunsOut o, T* __restrict__ out) {
-  constexpr int kGroups = groups_in(kSumMost, G);
+  constexpr int kGroups = groups_in(kSumMost, G), kThreadsHere = kGroups * G, kMost = kGroups * kMostSize;
+  constexpr uint32_t kNowhere = ~0u, kBegins = 1u << 31;
   __shared__ typename Runs<T, G, kGroups>::Shared s_runs;
-  __shared__ key_sort::Word s_words[kGroups * kMostSize];
+  __shared__ uint2 s_words[kMost + 1];
+  __shared__ int s_heads[SPARSE ? kMost / kWave + 1 : 1];
   Runs<T, G, kGroups> runs(o, s_runs, out);
-  {  // the workgroup's words, once
-    const int64_t first = runs.part * kGroups * size;
-    for (int j = threadIdx.x; j < kGroups * size; j += kGroups * G)
-      s_words[j] = words[first + j < n ? first + j : n - 1];
+  const int here = kGroups * size;
+  const int64_t first = runs.part * here;
+  for (int j0 = 0; j0 <= here; j0 += kThreadsHere) {
+    const int j = j0 + threadIdx.x;
+    const int64_t i = first + j;
+    uint2 w = make_uint2(kNowhere, kBegins);
+    if (j <= here && i < n) {
+      const key_sort::Word word = words[i];
+      const bool begins = i == 0 || key_sort::key_of(words[i > 0 ? i - 1 : 0]) != key_sort::key_of(word);
+      w.x = key_sort::key_of(word) < num_rows ? key_sort::key_of(word) : kNowhere;
+      w.y = key_sort::position_of(word) | (begins ? kBegins : 0u);
+    }
+    if (SPARSE) {
+      const unsigned long long heads = __ballot(w.x != kNowhere && (w.y & kBegins) && j < here);
+      if (j % kWave == 0 && j < here) s_heads[j / kWave] = __popcll(heads);
+    }
+    if (j <= here) s_words[j] = w;
+  }
+  __syncthreads();
+  if (SPARSE) {
+    const int64_t before = o.heads[runs.part];
+    for (int j0 = 0; j0 < here; j0 += kThreadsHere) {
+      const int j = j0 + threadIdx.x;
+      const uint2 w = s_words[j < here ? j : here - 1];
+      const bool begins = j < here && w.x != kNowhere && (w.y & kBegins);
+      const unsigned long long heads = __ballot(begins);
+      int upto = __popcll(heads & (~0ull >> (kWave - 1 - threadIdx.x % kWave)));  // up to this position
+      for (int c = 0; c < j / kWave && j < here; ++c) upto += s_heads[c];
+      const uint32_t rank = static_cast<uint32_t>(before + upto - 1);
+      if (begins && blockIdx.x == runs.part * o.slices) o.met[rank] = w.x;
+      if (j < here && w.x != kNowhere) s_words[j].x = rank;
+    }
     __syncthreads();
   }
-  const key_sort::Word* const mine = s_words + runs.group * size;
-  const int64_t base = (runs.part * kGroups + runs.group) * size;
+  const uint2* const mine = s_words + runs.group * size;
   const T* const from = grad + chunk_start<T>(o.dim, runs.chunk);
-  const int count = n - base < size ? (n > base ? static_cast<int>(n - base) : 0) : size;
-  uint32_t key = count > 0 ? key_sort::key_of(mine[0]) : num_rows;
-  if (key < num_rows) {
-    bool left = base > 0 && key_sort::key_of(words[base - 1]) == key;
-    const uint32_t behind = base + count < n ? key_sort::key_of(words[base + count]) : num_rows;
-    uint32_t row = key;
-    if (o.rank) row = static_cast<uint32_t>(o.rank[base]) - (left ? 1 : 0);
-    const bool names = o.met && runs.in && runs.chunk == 0;  // this lane writes the rows' ids
-    if (names && !left) o.met[row] = key;
+  uint32_t row = mine[0].x;
+  if (row != kNowhere) {
+    bool left = !(mine[0].y & kBegins);
     Wide<T> sum = {};
-    for (int j0 = 0; j0 < count && key < num_rows; j0 += kBatch) {
-      key_sort::Word w[kBatch];
+    for (int j0 = 0; j0 < size && row != kNowhere; j0 += kBatch) {
+      uint2 w[kBatch];
       Values<T> v[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) w[k] = mine[j0 + k < count ? j0 + k : count - 1];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) v[k] = load_chunk(from + key_sort::position_of(w[k]) * stride, o.dim);
+      for (int k = 0; k < kBatch; ++k) w[k] = mine[j0 + k];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        if (j0 + k >= count) break;
-        const uint32_t next = key_sort::key_of(w[k]);
-        if (next != key) {
+        const uint32_t at = w[k].x != kNowhere ? w[k].y & ~kBegins : w[0].y & ~kBegins;
+        v[k] = load_once<T, G>(from + at * stride, o.dim);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if ((w[k].y & kBegins) && j0 + k > 0) {
           runs.finish(row, sum, left, false);
           left = false;
-          key = next;
-          row = o.rank ? row + 1 : key;
-          if (key >= num_rows) break;  // (no rows from here on)
-          if (names) o.met[row] = key;
+          row = w[k].x;
+          if (row == kNowhere) break;  // (no rows from here on)
           sum = Wide<T>{};
         }
         sum += widen<T>(v[k]);
       }
     }
-    if (key < num_rows) runs.finish(row, sum, left, behind == key);
+    if (row != kNowhere) runs.finish(row, sum, left, !(mine[size].y & kBegins));
   }
   runs.join();
 }
@@ -316,7 +372,8 @@ struct SumPlan {
 struct GradSpace {
   key_sort::Space sort;
   key_sort::Word* sorted;
-  int64_t* rank;        // sparse
+  int64_t* counts;      // sparse: runs that begin in each workgroup's positions
+  int64_t* heads;       // sparse: and before them
   int64_t* scan_tiles;  // sparse
   Entry* entries[2];
   float* sums[2];
@@ -325,7 +382,9 @@ struct GradSpace {
 // even levels write buffer 0, odd ones buffer 1, each sized for the first of them
 size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
   size_t bytes = key_sort::space_bytes(p.n, 2);
-  if (sparse) bytes += padded(static_cast<size_t>(p.n + 1) * 8) + scan_workspace_bytes(p.n);
+  if (sparse)
+    bytes += padded(static_cast<size_t>(p.parts[0]) * 8) + padded(static_cast<size_t>(p.parts[0] + 1) * 8) +
+             scan_workspace_bytes(p.parts[0]);
   for (int l = 0; l < 2 && l + 1 < p.levels; ++l)
     bytes += padded(static_cast<size_t>(2 * p.parts[l]) * sizeof(Entry)) + padded(p.sums_bytes(l, type));
   return bytes;
@@ -334,8 +393,9 @@ size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
 bool carve_grad(Carver& ws, const SumPlan& p, int type, uint32_t num_rows, bool sparse, GradSpace* s) {
   key_sort::carve(ws, p.n, 2, &s->sort);
   s->sorted = s->sort.word[(key_sort::Digits(num_rows).passes - 1) & 1];
-  s->rank = sparse ? ws.take<int64_t>(static_cast<size_t>(p.n + 1)) : nullptr;
-  s->scan_tiles = sparse ? ws.take<int64_t>(scan_workspace_bytes(p.n) / 8) : nullptr;
+  s->counts = sparse ? ws.take<int64_t>(static_cast<size_t>(p.parts[0])) : nullptr;
+  s->heads = sparse ? ws.take<int64_t>(static_cast<size_t>(p.parts[0] + 1)) : nullptr;
+  s->scan_tiles = sparse ? ws.take<int64_t>(scan_workspace_bytes(p.parts[0]) / 8) : nullptr;
   for (int l = 0; l < 2; ++l) {
     s->entries[l] = nullptr;
     s->sums[l] = nullptr;
@@ -367,11 +427,11 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
     constexpr int G = decltype(g)::value;
     for (int l = 0; l < p.levels; ++l) {
       const bool last = l == p.levels - 1;
-      const RunsOut o{scale, dim, p.chunks, p.slices, l == 0 ? met : nullptr, s.rank,
+      const RunsOut o{scale, dim, p.chunks, p.slices, met, s.heads,
                       last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
       const dim3 grid(static_cast<unsigned>(p.parts[l] * p.slices));
       if (l == 0)
-        hipLaunchKernelGGL((sum_runs_kernel<T, G>), grid, dim3(groups_in(kSumMost, G) * G), 0, st, s.sorted, p.n, num_rows, grad,
+        hipLaunchKernelGGL((met ? sum_runs_kernel<T, G, true> : sum_runs_kernel<T, G, false>), grid, dim3(groups_in(kSumMost, G) * G), 0, st, s.sorted, p.n, num_rows, grad,
                            stride, p.size, o, out);
       else
         hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(groups_in(kJoinMost, G) * G), 0, st, s.entries[(l - 1) & 1],
@@ -380,15 +440,9 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
   });
 }
 
-// heads of the sorted runs of rows that are there
-struct RunHeads {
-  const key_sort::Word* word;
-  uint32_t num_rows;
-  __device__ __forceinline__ int64_t operator()(int64_t i) const {
-    const uint32_t key = key_sort::key_of(word[i]);
-    const uint32_t before = key_sort::key_of(word[i > 0 ? i - 1 : 0]);
-    return key < num_rows && (i == 0 || before != key);
-  }
+struct Numbers {
+  const int64_t* number;
+  __device__ __forceinline__ int64_t operator()(int64_t i) const { return number[i]; }
 };
 
 template <typename IdT, typename Beside>
@@ -530,7 +584,9 @@ int gs_embedding_sparse_grad_count(const void* ids, int id_bytes, int64_t n, int
     sort_ids(static_cast<const IdT*>(ids), n, rows, space, key_sort::NoWork(), st);
     return 0;
   });
-  return exclusive_scan(RunHeads{space.sorted, rows}, n, space.rank, space.scan_tiles, st, mailbox, ticket);
+  hipLaunchKernelGGL(count_runs_kernel, dim3(static_cast<unsigned>(plan.parts[0])), dim3(kThreads), 0, st, space.sorted, n,
+                     rows, plan.size * groups_in(kSumMost, plan.group), space.counts);
+  return exclusive_scan(Numbers{space.counts}, plan.parts[0], space.heads, space.scan_tiles, st, mailbox, ticket);
 }
 
 int gs_embedding_sparse_grad_fill(const void* grad, int64_t grad_stride, int64_t dim, int type, int64_t n,

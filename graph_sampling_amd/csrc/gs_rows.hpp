@@ -63,6 +63,11 @@ __device__ __forceinline__ void store_past(T* p, Values<T> v) {
   __builtin_nontemporal_store(v, reinterpret_cast<Loose*>(p));
 }
 template <typename T>
+__device__ __forceinline__ Values<T> load_past(const T* p) {
+  typedef Values<T> Loose __attribute__((aligned(sizeof(T))));
+  return __builtin_nontemporal_load(reinterpret_cast<const Loose*>(p));
+}
+template <typename T>
 __device__ __forceinline__ Wide<T> widen(Values<T> v) {
   return __builtin_convertvector(v, Wide<T>);
 }
