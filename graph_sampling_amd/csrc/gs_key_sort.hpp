@@ -10,15 +10,18 @@ namespace gs {
 namespace key_sort {
 
 constexpr int kItems = 4;  // of a thread
-// A tile is 512 threads' items, or 1024's: comparing the items of a tile by ballots is what a pass
-// takes longest for, but every tile reads the counts of all (400 k items in 196 small tiles 17 us a pass, in
-// 98 large ones 14; 30 k items in 15 small tiles 6 us, in 8 large ones 8).
-constexpr int kSmall = 512, kLarge = 1024;
-constexpr int64_t kAlone = kLarge * kItems;           // items that one workgroup sorts alone
-constexpr int64_t kFewItems = 8 * kSmall * kItems;    // items that every workgroup of a pass counts by itself
+// A tile is the items of 256, 512 or 1024 threads: comparing them by ballots is what a pass takes longest
+// for, and small tiles spread that over more compute units, but every tile reads the counts of all.  Us a
+// pass: 16 k items 4.9 / 5.9 / 8.1; 131 k 8.8 / 6.3 / -; 400 k - / 17 / 14.
+constexpr int64_t kMostTiles = 64;  // of the smaller sizes
+constexpr int64_t kAlone = 1024 * kItems;        // items that one workgroup sorts alone
+constexpr int64_t kFewItems = 2 * kAlone;        // items that every workgroup of a pass counts by itself
 constexpr int64_t kSelfTiles = 256;  // tiles whose counts every workgroup of a pass adds up by itself
 constexpr int kMostDigits = 512;
-inline int threads_for(int64_t n) { return n <= 64 * kSmall * kItems ? kSmall : kLarge; }
+// (a thread a digit at least)
+inline int threads_for(int64_t n, int bits, int64_t tiles) {
+  return bits == 8 && n <= tiles * 256 * kItems ? 256 : n <= tiles * 512 * kItems ? 512 : 1024;
+}
 
 using Word = unsigned long long;
 
@@ -189,16 +192,16 @@ count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__
 
 // For sorts of more than kSelfTiles tiles: in place of every count, how many items of its digit the
 // tiles before hold, and in totals[d] how many all hold.  A workgroup a digit.
-static __global__ void __launch_bounds__(kLarge)
+static __global__ void __launch_bounds__(1024)
 prefix_kernel(uint32_t* __restrict__ counts, int64_t tiles, int digits, uint32_t* __restrict__ totals) {
-  __shared__ int64_t s_scan[kLarge / kWave + 1];
+  __shared__ int64_t s_scan[1024 / kWave + 1];
   const int digit = blockIdx.x;
   int64_t run = 0;
-  for (int64_t t0 = 0; t0 < tiles; t0 += kLarge) {
+  for (int64_t t0 = 0; t0 < tiles; t0 += 1024) {
     const int64_t t = t0 + threadIdx.x;
     const int64_t c = t < tiles ? counts[t * digits + digit] : 0;
     int64_t all;
-    const int64_t at = block_exclusive_scan<kLarge>(c, &all, s_scan);
+    const int64_t at = block_exclusive_scan<1024>(c, &all, s_scan);
     if (t < tiles) counts[t * digits + digit] = static_cast<uint32_t>(run + at);
     run += all;
   }
@@ -371,18 +374,18 @@ struct Space {
   uint32_t* counts;
   uint32_t* totals;
 };
-inline int64_t tiles_of(int64_t n) {
-  const int64_t tile = threads_for(n) * kItems;
+// words: of the two buffers, how many the sort needs (a last pass that writes elsewhere: passes - 1, at most 2)
+inline int64_t most_tiles(int64_t n) {  // whatever the digits
+  const int64_t tile = threads_for(n, 8, kMostTiles) * kItems;
   return (n + tile - 1) / tile;
 }
-// words: of the two buffers, how many the sort needs (a last pass that writes elsewhere: passes - 1, at most 2)
 inline size_t space_bytes(int64_t n, int words) {
-  return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(tiles_of(n)) * kMostDigits * 4) +
+  return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(most_tiles(n)) * kMostDigits * 4) +
          padded(kMostDigits * 4);
 }
 inline void carve(Carver& ws, int64_t n, int words, Space* s) {
   for (int i = 0; i < 2; ++i) s->word[i] = i < words ? ws.take<Word>(static_cast<size_t>(n)) : nullptr;
-  s->counts = ws.take<uint32_t>(static_cast<size_t>(tiles_of(n)) * kMostDigits);
+  s->counts = ws.take<uint32_t>(static_cast<size_t>(most_tiles(n)) * kMostDigits);
   s->totals = ws.take<uint32_t>(kMostDigits);
 }
 
@@ -397,7 +400,7 @@ void launch_beside(Kernel kernel, int64_t tiles, int threads, hipStream_t st, Be
 
 template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
 void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& beside, hipStream_t st) {
-  const int64_t tiles = tiles_of(n);
+  const int64_t tiles = (n + THREADS * kItems - 1) / (THREADS * kItems);
   const uint32_t *counts = s.counts, *totals = s.totals;
   if (n <= kFewItems) {
     launch_beside(pass_kernel<BITS, THREADS, Src, Counts::kHere, Out, Beside>, tiles, THREADS, st, beside, src, n, pass,
@@ -407,7 +410,7 @@ void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& 
   launch_beside(count_kernel<BITS, THREADS, Src, Beside>, tiles, THREADS, st, beside, src, n, pass, tiles, s.counts);
   const bool self = tiles <= kSelfTiles;
   if (!self)
-    hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(kLarge), 0, st, s.counts, tiles, 1 << BITS, s.totals);
+    hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(1024), 0, st, s.counts, tiles, 1 << BITS, s.totals);
   launch_beside(self ? pass_kernel<BITS, THREADS, Src, Counts::kTiles, Out, Beside>
                      : pass_kernel<BITS, THREADS, Src, Counts::kPrefixes, Out, Beside>,
                 tiles, THREADS, st, beside, src, n, pass, tiles, counts, totals, out);
@@ -426,20 +429,22 @@ void sort_tiles(Src src, int64_t n, int passes, const Space& s, Out out, Beside 
   }
 }
 
+template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
+void sort_with(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
+  if (n > kAlone) return sort_tiles<BITS, THREADS>(src, n, passes, s, out, beside, st);
+  if constexpr (Beside::kAny) beside.parts = 1;
+  launch_beside(alone_kernel<BITS, THREADS, Src, Out, Beside>, 1, THREADS, st, beside, src, static_cast<uint32_t>(n),
+                passes, out);
+}
+
 template <int BITS, typename Src, typename Out, typename Beside>
 void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
-  if (n <= kAlone) {
-    if constexpr (Beside::kAny) beside.parts = 1;
-    const uint32_t count = static_cast<uint32_t>(n);
-    if (n <= kSmall * kItems)
-      launch_beside(alone_kernel<BITS, kSmall, Src, Out, Beside>, 1, kSmall, st, beside, src, count, passes, out);
-    else
-      launch_beside(alone_kernel<BITS, kLarge, Src, Out, Beside>, 1, kLarge, st, beside, src, count, passes, out);
-  } else if (threads_for(n) == kSmall) {
-    sort_tiles<BITS, kSmall>(src, n, passes, s, out, beside, st);
-  } else {
-    sort_tiles<BITS, kLarge>(src, n, passes, s, out, beside, st);
+  const int threads = threads_for(n, BITS, n <= kAlone ? 1 : kMostTiles);
+  if constexpr (BITS == 8) {
+    if (threads == 256) return sort_with<BITS, 256>(src, n, passes, s, out, beside, st);
   }
+  if (threads == 512) return sort_with<BITS, 512>(src, n, passes, s, out, beside, st);
+  sort_with<BITS, 1024>(src, n, passes, s, out, beside, st);
 }
 
 // Sorts n >= 1 items (below 2^31), keys 0..num; the last pass hands every word with its place to `out`.  Where
