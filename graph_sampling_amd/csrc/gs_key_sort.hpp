@@ -15,7 +15,7 @@ constexpr int kItems = 4;  // of a thread
 // pass: 16 k items 4.9 / 5.9 / 8.1; 131 k 8.8 / 6.3 / -; 400 k - / 17 / 14.
 constexpr int64_t kMostTiles = 64;  // of the smaller sizes
 constexpr int64_t kAlone = 1024 * kItems;        // items that one workgroup sorts alone
-constexpr int64_t kFewItems = 2 * kAlone;        // items that every workgroup of a pass counts by itself
+constexpr int64_t kFewItems = 4 * kAlone;        // items that every workgroup of a pass counts by itself
 constexpr int64_t kSelfTiles = 256;  // tiles whose counts every workgroup of a pass adds up by itself
 constexpr int kMostDigits = 512;
 // (a thread a digit at least)
@@ -219,7 +219,8 @@ template <int BITS, int THREADS, typename Src, Counts COUNTS, typename Out, type
 __global__ void __launch_bounds__(THREADS)
 pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restrict__ counts,
             const uint32_t* __restrict__ totals, Out out, Beside beside) {
-  constexpr int kDigits = 1 << BITS, kParts = THREADS / kDigits, kTile = THREADS * kItems;
+  // (kHere: copies of the counts, lane by lane in turn: where many items hold one digit, additions queue up)
+  constexpr int kDigits = 1 << BITS, kParts = COUNTS == Counts::kHere ? 8 : THREADS / kDigits, kTile = THREADS * kItems;
   if (Beside::kAny && blockIdx.x >= tiles) return beside.run(blockIdx.x - tiles, gridDim.x - tiles, THREADS);
   __shared__ TileTables<BITS, THREADS> s_tables;
   __shared__ uint32_t s_all[kParts][kDigits], s_before[kParts][kDigits];
@@ -439,7 +440,7 @@ void sort_with(Src src, int64_t n, int passes, const Space& s, Out out, Beside b
 
 template <int BITS, typename Src, typename Out, typename Beside>
 void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
-  const int threads = threads_for(n, BITS, n <= kAlone ? 1 : kMostTiles);
+  const int threads = n > kAlone && n <= kFewItems ? 512 : threads_for(n, BITS, n <= kAlone ? 1 : kMostTiles);
   if constexpr (BITS == 8) {
     if (threads == 256) return sort_with<BITS, 256>(src, n, passes, s, out, beside, st);
   }
