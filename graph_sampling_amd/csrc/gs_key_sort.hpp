@@ -11,16 +11,20 @@ namespace key_sort {
 
 constexpr int kItems = 4;  // of a thread
 // A tile is the items of 256, 512 or 1024 threads: comparing them by ballots is what a pass takes longest
-// for, and small tiles spread that over more compute units, but every tile reads the counts of all.  Us a
-// pass: 16 k items 4.9 / 5.9 / 8.1; 131 k 8.8 / 6.3 / -; 400 k - / 17 / 14.
-constexpr int64_t kMostTiles = 64;  // of the smaller sizes
+// for, and small tiles spread that over more compute units, as long as their counts are few.  Up to 64 tiles
+// every workgroup of a pass adds up the counts of all by itself; more are added up by a launch between.  Us a
+// count and pass (8 bits, 4 M keys), by itself / with that launch: 131 k items in 256-thread tiles 12.3 / 9.4,
+// 512 8.5 / 9.7, 1024 10.9 / 11.0; 400 k 31.6 / 12.3, 14.9 / 10.8, 11.6 / 11.6; 810 k -, 31.2 / 13.9, 15.9 / 13.2;
+// 2 M -, 106 / 21.4, 39.5 / 19.0.  (16 k items, the pass alone: 256 threads 4.9, 512 5.9, 1024 8.1.)
+constexpr int64_t kSelfTiles = 64;
 constexpr int64_t kAlone = 1024 * kItems;        // items that one workgroup sorts alone
 constexpr int64_t kFewItems = 4 * kAlone;        // items that every workgroup of a pass counts by itself
-constexpr int64_t kSelfTiles = 256;  // tiles whose counts every workgroup of a pass adds up by itself
 constexpr int kMostDigits = 512;
 // (a thread a digit at least)
-inline int threads_for(int64_t n, int bits, int64_t tiles) {
-  return bits == 8 && n <= tiles * 256 * kItems ? 256 : n <= tiles * 512 * kItems ? 512 : 1024;
+inline int threads_for(int64_t n, int bits) {
+  if (n <= kAlone) return bits == 8 && n <= 256 * kItems ? 256 : n <= 512 * kItems ? 512 : 1024;
+  if (n <= kFewItems) return 512;
+  return bits == 8 && n <= kSelfTiles * 256 * kItems ? 256 : n <= 4 * kSelfTiles * 512 * kItems ? 512 : 1024;
 }
 
 using Word = unsigned long long;
@@ -377,7 +381,7 @@ struct Space {
 };
 // words: of the two buffers, how many the sort needs (a last pass that writes elsewhere: passes - 1, at most 2)
 inline int64_t most_tiles(int64_t n) {  // whatever the digits
-  const int64_t tile = threads_for(n, 8, kMostTiles) * kItems;
+  const int64_t tile = threads_for(n, 8) * kItems;
   return (n + tile - 1) / tile;
 }
 inline size_t space_bytes(int64_t n, int words) {
@@ -440,7 +444,7 @@ void sort_with(Src src, int64_t n, int passes, const Space& s, Out out, Beside b
 
 template <int BITS, typename Src, typename Out, typename Beside>
 void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
-  const int threads = n > kAlone && n <= kFewItems ? 512 : threads_for(n, BITS, n <= kAlone ? 1 : kMostTiles);
+  const int threads = threads_for(n, BITS);
   if constexpr (BITS == 8) {
     if (threads == 256) return sort_with<BITS, 256>(src, n, passes, s, out, beside, st);
   }
