@@ -64,13 +64,13 @@ __global__ void __launch_bounds__(kThreads) no_items_kernel(int64_t* __restrict_
 // Zeros in the rows from `live` (read on the device) to n, a share of them by every workgroup.
 template <typename T>
 __device__ __forceinline__ void zero_rows_behind(const int64_t* __restrict__ live, int64_t n, int64_t dim,
-                                                 const Divider& chunks, T* __restrict__ rows) {
+                                                 const Divider& chunks, T* __restrict__ rows, bool past) {
   const int64_t from = *live;
   if (from >= n || from < 0) return;
   const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
     const int64_t row = i / chunks.d;
-    store_chunk(rows + (from + row) * dim + chunk_start<T>(dim, i - row * chunks.d), Values<T>{}, dim);
+    store_result(rows + (from + row) * dim + chunk_start<T>(dim, i - row * chunks.d), Values<T>{}, dim, past);
   }
 }
 
@@ -78,7 +78,7 @@ __device__ __forceinline__ void zero_rows_behind(const int64_t* __restrict__ liv
 template <typename T, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
-              int64_t total, int choices, int64_t n, const int64_t* __restrict__ live, T* __restrict__ rows) {
+              int64_t total, int choices, int64_t n, const int64_t* __restrict__ live, T* __restrict__ rows, bool past) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * ITEMS);
   const RowRange range(chunks, first);
   int64_t token[ITEMS], at[ITEMS];
@@ -97,10 +97,10 @@ gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chun
     for (int i = 0; i < ITEMS; ++i) {
       if (token[i] < 0) continue;
       const int64_t to = place[token[i] * choices + k];
-      if (to >= 0 && to < n) store_chunk(rows + to * dim + at[i], v[i], dim);
+      if (to >= 0 && to < n) store_result(rows + to * dim + at[i], v[i], dim, past);
     }
   }
-  zero_rows_behind(live, n, dim, chunks, rows);
+  zero_rows_behind(live, n, dim, chunks, rows, past);
 }
 
 // ----------------------------------------------------------------- combine ----
@@ -113,7 +113,7 @@ __device__ __forceinline__ float weight_of(const W* weights, int64_t item) {
 template <typename T, typename W, int KU>
 __global__ void __launch_bounds__(kThreads)
 combine_kernel(const T* __restrict__ y, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
-               int64_t total, int choices, int64_t n, const W* __restrict__ weights, T* __restrict__ out) {
+               int64_t total, int choices, int64_t n, const W* __restrict__ weights, T* __restrict__ out, bool past) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
   if (first + threadIdx.x >= total) return;
   const RowRange range(chunks, first);
@@ -137,7 +137,7 @@ combine_kernel(const T* __restrict__ y, int64_t stride, int64_t dim, Divider chu
     for (int u = 0; u < KU; ++u)
       if (there[u]) sum += widen<T>(v[u]) * w[u];
   }
-  store_chunk(out + token * dim + at, narrow<T>(sum), dim);
+  store_result(out + token * dim + at, narrow<T>(sum), dim, past);
 }
 
 // ---------------------------------------------------- gradient of the combine ----
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads)
 combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ y, int64_t y_stride,
                     int64_t dim, Divider chunks, const int32_t* __restrict__ place, int64_t tokens, int choices,
                     int64_t n, const int64_t* __restrict__ live, const W* __restrict__ weights, T* __restrict__ dy,
-                    W* __restrict__ dweights) {
+                    W* __restrict__ dweights, bool past) {
   constexpr int kLanes = G * WAVES;               // of a token
   constexpr int kTokens = kThreads / kLanes;      // of a workgroup
   __shared__ float s_dots[WAVES > 1 ? WAVES * KU : 1];
@@ -186,7 +186,7 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
           for (int i = 0; i < Chunk<T>::kVec; ++i)
             if (i >= overlap) dot[u] = __fmaf_rn(d[i], b[i], dot[u]);
         }
-        if (dy && from[u] >= 0) store_chunk(dy + from[u] * dim + at, narrow<T>(d * w[u]), dim);
+        if (dy && from[u] >= 0) store_result(dy + from[u] * dim + at, narrow<T>(d * w[u]), dim, past);
       }
     }
     if (!dweights) continue;
@@ -213,7 +213,7 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
         if (k0 + u < choices) dweights[token * choices + k0 + u] = static_cast<W>(from[u] >= 0 ? dot[u] : 0.0f);
     }
   }
-  if (dy) zero_rows_behind(live, n, dim, chunks, dy);
+  if (dy) zero_rows_behind(live, n, dim, chunks, dy, past);
 }
 
 // ------------------------------------------------------------------- checks ----
@@ -266,7 +266,7 @@ int launch_gather(const T* x, int64_t stride, int64_t dim, const int32_t* place,
   auto* kernel = many ? gather_kernel<T, kMany> : gather_kernel<T, 1>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, x, stride, dim,
                      Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices), tokens * choices, live,
-                     rows);
+                     rows, results_past(rows, dim));
   return check_launch(what);
 }
 
@@ -279,7 +279,7 @@ int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t 
   with_choices(choices, [&](auto ku) {
     hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st, dout,
                        dout_stride, y, y_stride, dim, Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place, tokens,
-                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights);
+                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights, results_past(dy, dim));
   });
   return check_launch("expert_combine_grad");
 }
@@ -376,7 +376,8 @@ int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, co
         hipLaunchKernelGGL((combine_kernel<T, W, decltype(ku)::value>), dim3(static_cast<unsigned>(blocks)),
                            dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(y), y_stride, dim,
                            Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices),
-                           tokens * choices, static_cast<const W*>(weights), static_cast<T*>(out));
+                           tokens * choices, static_cast<const W*>(weights), static_cast<T*>(out),
+                           results_past(static_cast<const T*>(out), dim));
       });
       return check_launch("expert_combine");
     });
