@@ -1388,6 +1388,25 @@ def expert_sort(experts, num_experts):
     return order, place, offsets
 
 
+def expert_dispatch(x, experts, num_experts):
+    """(rows, order, place, offsets): expert_sort and expert_gather in one call."""
+    ptr, stride, dim, kind = _rows(x, "x")
+    idb = _ids(experts, "experts")
+    n, dev = experts.numel(), experts.device
+    tokens, choices = experts.size(0), experts.size(1) if experts.dim() == 2 else 1
+    if x.size(0) != tokens:
+        raise GsError("x has %d rows for experts of %s" % (x.size(0), tuple(experts.shape)))
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    place = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
+    rows = torch.empty(n, x.size(1), dtype=x.dtype, device=dev)
+    ws = workspace(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
+    _check(lib().gs_expert_dispatch(ptr, stride, dim, kind, _ptr(experts), idb, _i64(tokens), _i64(choices),
+                                    _i64(num_experts), _ptr(order), _ptr(place), _ptr(offsets), _ptr(rows), _ptr(ws),
+                                    ctypes.c_size_t(ws.numel()), _stream(dev)), "gs_expert_dispatch")
+    return rows, order, place, offsets
+
+
 def _choices(place, rows, num_rows, name):
     """(tokens, choices) of int32 places for a tensor of num_rows(tokens, choices) rows."""
     _need(place, torch.int32, "place")

@@ -155,28 +155,31 @@ struct Runs {
   }
   // the run whose first piece here is entry i, added up over the groups it goes through
   __device__ __forceinline__ void walk(int i) {
+    constexpr int kAhead = 8;  // groups asked about together
     const uint32_t row = s.entry[i].row;
     const bool left = i == 0;
     Wide<T> sum = s.sum[i][lane];
-    bool right = i + 1 == kEntries;
-    for (int j0 = i + 1; j0 < kEntries; j0 += 4) {
-      Entry e[4];
-      Wide<T> v[4];
+    // (on: the run goes on into the next group)
+    bool on = (i & 1) != 0 || (s.entry[1].state != kNone && s.entry[1].row == row);
+    for (int g0 = i / 2 + 1; on && g0 < GROUPS; g0 += kAhead) {
+      Entry e[kAhead][2];
+      Wide<T> v[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        e[k] = s.entry[j0 + k < kEntries ? j0 + k : kEntries - 1];
-        v[k] = s.sum[j0 + k < kEntries ? j0 + k : kEntries - 1][lane];  // (what is no sum is not added)
+      for (int k = 0; k < kAhead; ++k) {
+        const int g = g0 + k < GROUPS ? g0 + k : GROUPS - 1;
+        e[k][0] = s.entry[2 * g];
+        e[k][1] = s.entry[2 * g + 1];
+        v[k] = s.sum[2 * g][lane];  // (what is no sum is not added)
       }
-      bool on = true;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (j0 + k >= kEntries) break;
-        on = on && e[k].state != kNone && e[k].row == row;
-        if (on && e[k].state == kSum) sum += v[k];
-        if (on && j0 + k + 1 == kEntries) right = true;
+      for (int k = 0; k < kAhead; ++k) {
+        if (g0 + k >= GROUPS) break;
+        on = on && e[k][0].state == kSum && e[k][0].row == row;
+        if (on) sum += v[k];
+        on = on && e[k][1].state == kThrough;
       }
-      if (!on) break;
     }
+    const bool right = on;
     if (!left && !right) return write(row, sum);
     const int slot = left ? 0 : 1;
     if (in) {
@@ -188,12 +191,12 @@ struct Runs {
       if (left && right) s.left[1] = Entry{row, kThrough};
     }
   }
-  // behind every group's tile: every thread of the workgroup calls this
+  // behind every group's tile: every thread of the workgroup calls this.  A run begins here in the first group's first
+  // entry (it began in an earlier workgroup) or in a group's last one that holds a sum.
   __device__ __forceinline__ void join() {
     __syncthreads();
-    for (int i = 2 * group; i < 2 * group + 2; ++i)  // where a run's first piece is
-      if (s.entry[i].state == kSum && (i == 0 || s.entry[i - 1].state == kNone || s.entry[i - 1].row != s.entry[i].row))
-        walk(i);
+    if (group == 0 && s.entry[0].state == kSum) walk(0);
+    if (s.entry[2 * group + 1].state == kSum) walk(2 * group + 1);
     __syncthreads();
     if (o.entries && threadIdx.x < 2 && blockIdx.x == part * o.slices)
       o.entries[2 * part + threadIdx.x] = s.left[threadIdx.x];
@@ -382,7 +385,8 @@ struct GradSpace {
 
 // even levels write buffer 0, odd ones buffer 1, each sized for the first of them
 size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
-  size_t bytes = key_sort::space_bytes(p.n, 2);
+  // (sorted lies in one of the sort's own buffers where it has any)
+  size_t bytes = p.n <= key_sort::kAlone ? padded(static_cast<size_t>(p.n) * 8) : key_sort::space_bytes(p.n, 2);
   if (sparse)
     bytes += padded(static_cast<size_t>(p.parts[0]) * 8) + padded(static_cast<size_t>(p.parts[0] + 1) * 8) +
              scan_workspace_bytes(p.parts[0]);
@@ -393,7 +397,8 @@ size_t grad_bytes(const SumPlan& p, int type, bool sparse) {
 
 bool carve_grad(Carver& ws, const SumPlan& p, int type, uint32_t num_rows, bool sparse, GradSpace* s) {
   key_sort::carve(ws, p.n, 2, &s->sort);
-  s->sorted = s->sort.word[(key_sort::Digits(num_rows).passes - 1) & 1];
+  s->sorted = p.n <= key_sort::kAlone ? ws.take<key_sort::Word>(static_cast<size_t>(p.n))
+                                      : s->sort.word[(key_sort::Digits(num_rows).passes - 1) & 1];
   s->counts = sparse ? ws.take<int64_t>(static_cast<size_t>(p.parts[0])) : nullptr;
   s->heads = sparse ? ws.take<int64_t>(static_cast<size_t>(p.parts[0] + 1)) : nullptr;
   s->scan_tiles = sparse ? ws.take<int64_t>(scan_workspace_bytes(p.parts[0]) / 8) : nullptr;

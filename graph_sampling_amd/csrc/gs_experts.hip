@@ -61,11 +61,10 @@ __global__ void __launch_bounds__(kThreads) no_items_kernel(int64_t* __restrict_
 }
 
 // ------------------------------------------------------------------ gather ----
-// Zeros in the rows from `live` (read on the device) to n, a share of them by every workgroup.
+// Zeros in the rows from `from` to n, a share of them by every workgroup.
 template <typename T>
-__device__ __forceinline__ void zero_rows_behind(const int64_t* __restrict__ live, int64_t n, int64_t dim,
-                                                 const Divider& chunks, T* __restrict__ rows, bool past) {
-  const int64_t from = *live;
+__device__ __forceinline__ void zero_rows_behind(int64_t from, int64_t n, int64_t dim, const Divider& chunks,
+                                                 T* __restrict__ rows, bool past) {
   if (from >= n || from < 0) return;
   const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
@@ -100,7 +99,66 @@ gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chun
       if (to >= 0 && to < n) store_result(rows + to * dim + at[i], v[i], dim, past);
     }
   }
-  zero_rows_behind(live, n, dim, chunks, rows, past);
+  zero_rows_behind(*live, n, dim, chunks, rows, past);
+}
+
+// The same with the sort, for a few items: every workgroup ranks all of them in LDS, which takes less than a launch,
+// and goes on with its chunks; the first one writes the order down.  16 items of 64 experts: 4 us where two launches
+// take 6 and the space between them.
+constexpr int64_t kDispatchItems = kThreads * key_sort::kItems;
+
+template <typename T, typename IdT>
+__global__ void __launch_bounds__(kThreads)
+sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks,
+                   int64_t total, int choices, uint32_t n, OrderOut out, T* __restrict__ rows, bool past) {
+  constexpr int kBits = 8, kDigits = 1 << kBits;
+  static_assert(kDigits == kThreads, "a digit a thread");
+  __shared__ key_sort::TileTables<kBits, kThreads> s_tables;
+  __shared__ uint32_t s_start[kDigits];
+  __shared__ int32_t s_place[kDispatchItems];
+  // the token's chunk is on its way meanwhile
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+  const bool in = first + threadIdx.x < total;
+  const RowRange range(chunks, first);
+  uint32_t c;
+  const int64_t token = range.row(in ? threadIdx.x : 0, &c), at = chunk_start<T>(dim, c);
+  const Values<T> v = load_chunk(x + token * stride + at, dim);
+
+  const key_sort::IdWords<IdT> src{experts, out.experts};
+  key_sort::Word w[key_sort::kItems];
+  uint32_t d[key_sort::kItems], rank[key_sort::kItems], here;
+#pragma unroll
+  for (int r = 0; r < key_sort::kItems; ++r) {
+    const uint32_t i = key_sort::item_of(r);
+    w[r] = src(i < n ? i : n - 1);
+    d[r] = key_sort::digit_of<kBits>(w[r], 0);
+  }
+  key_sort::rank_tile<kBits, kThreads>(d, n, s_tables, rank, &here);
+  uint32_t start = here, none = 0;
+  key_sort::scan_digits(start, none, s_tables);
+  s_start[threadIdx.x] = start;
+  if (blockIdx.x == 0) out.digit(threadIdx.x, start);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < key_sort::kItems; ++r) {
+    const uint32_t i = key_sort::item_of(r);
+    if (i >= n) continue;
+    const uint32_t to = s_start[d[r]] + rank[r];
+    s_place[i] = key_sort::key_of(w[r]) < out.experts ? static_cast<int32_t>(to) : -1;
+    if (blockIdx.x == 0) {
+      out.from(w[r], to);
+      out.item(to, w[r]);
+    }
+  }
+  __syncthreads();
+  if (in) {
+    for (int k = 0; k < choices; ++k) {
+      const int32_t to = s_place[token * choices + k];
+      if (to >= 0) store_result(rows + to * dim + at, v, dim, past);
+    }
+  }
+  const int64_t live = s_start[out.experts];
+  if (live < n) zero_rows_behind(live, static_cast<int64_t>(n), dim, chunks, rows, past);
 }
 
 // ----------------------------------------------------------------- combine ----
@@ -213,7 +271,7 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
         if (k0 + u < choices) dweights[token * choices + k0 + u] = static_cast<W>(from[u] >= 0 ? dot[u] : 0.0f);
     }
   }
-  if (dy) zero_rows_behind(live, n, dim, chunks, dy, past);
+  if (dy) zero_rows_behind(*live, n, dim, chunks, dy, past);
 }
 
 // ------------------------------------------------------------------- checks ----
@@ -297,6 +355,9 @@ int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOu
   Carver ws(workspace, workspace_bytes);
   key_sort::Space space;
   key_sort::carve(ws, n, passes > 1 ? 2 : 0, &space);
+  key_sort::Word* sorted = nullptr;  // (in one of the sort's own buffers where it has any)
+  if (passes > 1)
+    sorted = n <= key_sort::kAlone ? ws.take<key_sort::Word>(static_cast<size_t>(n)) : space.word[(passes - 1) & 1];
   if (!ws.ok) {
     set_error_text("gs_expert_sort: workspace needs %zu bytes, 256-byte aligned",
                    gs_expert_sort_workspace_bytes(n, num_experts));
@@ -306,7 +367,6 @@ int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOu
   if (passes == 1) {
     key_sort::sort(src, n, num, space, out, st);
   } else {
-    key_sort::Word* sorted = space.word[(passes - 1) & 1];
     key_sort::sort(src, n, num, space, key_sort::WordsOut{sorted}, st);
     const int64_t threads = n > num_experts + 1 ? n : num_experts + 1;
     hipLaunchKernelGGL(order_kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
@@ -325,7 +385,9 @@ extern "C" {
 size_t gs_expert_sort_workspace_bytes(int64_t n, int64_t num_experts) {
   if (n <= 0 || num_experts < 0) return 256;
   const uint32_t num = static_cast<uint32_t>(num_experts);
-  return key_sort::space_bytes(n, key_sort::Digits(num).passes > 1 ? 2 : 0);
+  const bool words = key_sort::Digits(num).passes > 1;
+  if (n <= key_sort::kAlone) return words ? padded(static_cast<size_t>(n) * 8) : 0;
+  return key_sort::space_bytes(n, words ? 2 : 0);
 }
 
 int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_experts, int32_t* order, int32_t* place,
@@ -354,6 +416,38 @@ int gs_expert_gather(const void* x, int64_t x_stride, int64_t dim, int type, con
     using T = decltype(zero);
     return launch_gather(static_cast<const T*>(x), x_stride, dim, place, tokens, choices, live, static_cast<T*>(rows),
                          static_cast<hipStream_t>(stream), "gs_expert_gather");
+  });
+}
+
+int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, const void* experts, int id_bytes,
+                       int64_t tokens, int64_t choices, int64_t num_experts, int32_t* order, int32_t* place,
+                       int64_t* offsets, void* rows, void* workspace, size_t workspace_bytes, void* stream) {
+  GS_RETURN_IF_ERROR(check_shape("gs_expert_dispatch", tokens, choices, num_experts));
+  GS_RETURN_IF_ERROR(check_values("gs_expert_dispatch", type, dim, x_stride));
+  const int64_t n = tokens * choices;
+  if (n == 0 || n > kDispatchItems || num_experts >= 256 || dim == 0) {
+    GS_RETURN_IF_ERROR(gs_expert_sort(experts, id_bytes, n, num_experts, order, place, offsets, workspace,
+                                      workspace_bytes, stream));
+    return gs_expert_gather(x, x_stride, dim, type, place, tokens, choices, offsets + num_experts, rows, stream);
+  }
+  GS_REQUIRE(valid_id_bytes(id_bytes), "gs_expert_dispatch: id_bytes must be 4 or 8, got %d", id_bytes);
+  GS_REQUIRE(x && experts && order && place && offsets && rows, "gs_expert_dispatch: null array");
+  GS_REQUIRE(aligned_to(experts, id_bytes) && aligned_to(x, value_bytes(type)) && aligned_to(rows, value_bytes(type)),
+             "gs_expert_dispatch: ids or rows not aligned to their type");
+  const OrderOut out{order, place, offsets, static_cast<uint32_t>(num_experts)};
+  return with_value_type(type, "gs_expert_dispatch", [&](auto zero) {
+    using T = decltype(zero);
+    return with_id_type(id_bytes, [&](auto id) {
+      using IdT = decltype(id);
+      const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks, blocks = (total + kThreads - 1) / kThreads;
+      GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks));
+      hipLaunchKernelGGL((sort_gather_kernel<T, IdT>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const IdT*>(experts), static_cast<const T*>(x),
+                         x_stride, dim, Divider(static_cast<uint32_t>(chunks)), total, static_cast<int>(choices),
+                         static_cast<uint32_t>(n), out, static_cast<T*>(rows),
+                         results_past(static_cast<const T*>(rows), dim));
+      return check_launch("expert_dispatch");
+    });
   });
 }
 

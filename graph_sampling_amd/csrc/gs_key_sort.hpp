@@ -196,16 +196,17 @@ count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__
 
 // For sorts of more than kSelfTiles tiles: in place of every count, how many items of its digit the
 // tiles before hold, and in totals[d] how many all hold.  A workgroup a digit.
-static __global__ void __launch_bounds__(1024)
+constexpr int kPrefixThreads = 256;
+static __global__ void __launch_bounds__(kPrefixThreads)
 prefix_kernel(uint32_t* __restrict__ counts, int64_t tiles, int digits, uint32_t* __restrict__ totals) {
-  __shared__ int64_t s_scan[1024 / kWave + 1];
+  __shared__ int64_t s_scan[kPrefixThreads / kWave + 1];
   const int digit = blockIdx.x;
   int64_t run = 0;
-  for (int64_t t0 = 0; t0 < tiles; t0 += 1024) {
+  for (int64_t t0 = 0; t0 < tiles; t0 += kPrefixThreads) {
     const int64_t t = t0 + threadIdx.x;
     const int64_t c = t < tiles ? counts[t * digits + digit] : 0;
     int64_t all;
-    const int64_t at = block_exclusive_scan<1024>(c, &all, s_scan);
+    const int64_t at = block_exclusive_scan<kPrefixThreads>(c, &all, s_scan);
     if (t < tiles) counts[t * digits + digit] = static_cast<uint32_t>(run + at);
     run += all;
   }
@@ -385,10 +386,13 @@ inline int64_t most_tiles(int64_t n) {  // whatever the digits
   return (n + tile - 1) / tile;
 }
 inline size_t space_bytes(int64_t n, int words) {
+  if (n <= kAlone) return 0;  // (one workgroup does it in LDS)
   return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(most_tiles(n)) * kMostDigits * 4) +
          padded(kMostDigits * 4);
 }
 inline void carve(Carver& ws, int64_t n, int words, Space* s) {
+  *s = Space{};
+  if (n <= kAlone) return;
   for (int i = 0; i < 2; ++i) s->word[i] = i < words ? ws.take<Word>(static_cast<size_t>(n)) : nullptr;
   s->counts = ws.take<uint32_t>(static_cast<size_t>(most_tiles(n)) * kMostDigits);
   s->totals = ws.take<uint32_t>(kMostDigits);
@@ -415,7 +419,7 @@ void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& 
   launch_beside(count_kernel<BITS, THREADS, Src, Beside>, tiles, THREADS, st, beside, src, n, pass, tiles, s.counts);
   const bool self = tiles <= kSelfTiles;
   if (!self)
-    hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(1024), 0, st, s.counts, tiles, 1 << BITS, s.totals);
+    hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(kPrefixThreads), 0, st, s.counts, tiles, 1 << BITS, s.totals);
   launch_beside(self ? pass_kernel<BITS, THREADS, Src, Counts::kTiles, Out, Beside>
                      : pass_kernel<BITS, THREADS, Src, Counts::kPrefixes, Out, Beside>,
                 tiles, THREADS, st, beside, src, n, pass, tiles, counts, totals, out);

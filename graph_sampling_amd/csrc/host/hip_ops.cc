@@ -2034,24 +2034,52 @@ std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(const torch::Tensor
   return {rows, values};
 }
 
+namespace {
+// outputs and scratch of a sort of experts
+struct SortedExperts {
+  torch::Tensor flat, order, place, offsets, workspace;
+  SortedExperts(const torch::Tensor& experts, int64_t num_experts, const torch::Device& device) {
+    TORCH_CHECK(experts.defined(), "experts is undefined");
+    TORCH_CHECK(experts.dim() == 1 || experts.dim() == 2, "experts must be [tokens] or [tokens, choices], got ",
+                experts.sizes());
+    TORCH_CHECK(num_experts >= 0, "num_experts must be non-negative");
+    flat = FlatIds(experts, device, "experts");
+    const auto i32 = torch::dtype(torch::kInt32).device(device);
+    order = torch::empty({flat.numel()}, i32);
+    place = torch::empty(experts.sizes(), i32);
+    offsets = torch::empty({num_experts + 1}, I64(experts));
+    const size_t bytes = gs_expert_sort_workspace_bytes(flat.numel(), num_experts);
+    if (bytes > 0) workspace = Scratch(bytes, experts);
+  }
+  void* scratch() const { return workspace.defined() ? workspace.data_ptr() : nullptr; }
+  size_t scratch_bytes() const { return workspace.defined() ? static_cast<size_t>(workspace.numel()) : 0; }
+};
+}  // namespace
+
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> ExpertSort(const torch::Tensor& experts, int64_t num_experts) {
-  TORCH_CHECK(experts.defined(), "experts is undefined");
-  TORCH_CHECK(experts.dim() == 1 || experts.dim() == 2, "experts must be [tokens] or [tokens, choices], got ",
-              experts.sizes());
-  TORCH_CHECK(num_experts >= 0, "num_experts must be non-negative");
-  const auto flat = FlatIds(experts, experts.device(), "experts");
+  const SortedExperts s(experts, num_experts, experts.device());
   c10::hip::HIPGuard on(experts.device().index());
-  const int64_t n = flat.numel();
-  const auto i32 = torch::dtype(torch::kInt32).device(experts.device());
-  auto order = torch::empty({n}, i32);
-  auto place = torch::empty(experts.sizes(), i32);
-  auto offsets = torch::empty({num_experts + 1}, I64(experts));
-  auto ws = Scratch(gs_expert_sort_workspace_bytes(n, num_experts), experts);
-  Check(gs_expert_sort(flat.data_ptr(), IdBytes(flat, "experts"), n, num_experts, order.data_ptr<int32_t>(),
-                       place.data_ptr<int32_t>(), offsets.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(),
-                       Stream(experts)),
+  Check(gs_expert_sort(s.flat.data_ptr(), IdBytes(s.flat, "experts"), s.flat.numel(), num_experts,
+                       s.order.data_ptr<int32_t>(), s.place.data_ptr<int32_t>(), s.offsets.data_ptr<int64_t>(),
+                       s.scratch(), s.scratch_bytes(), Stream(experts)),
         "gs_expert_sort");
-  return {order, place, offsets};
+  return {s.order, s.place, s.offsets};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> ExpertDispatch(const torch::Tensor& x,
+                                                                                      const torch::Tensor& experts,
+                                                                                      int64_t num_experts) {
+  const Rows r(x, "rows");
+  const SortedExperts s(experts, num_experts, x.device());
+  const int64_t tokens = experts.size(0), choices = experts.dim() == 2 ? experts.size(1) : 1;
+  TORCH_CHECK(r.t.size(0) == tokens, "rows of ", r.t.size(0), " tokens, experts of ", tokens);
+  c10::hip::HIPGuard on(x.device().index());
+  auto out = torch::empty({s.flat.numel(), r.t.size(1)}, Like(x));
+  Check(gs_expert_dispatch(r.t.data_ptr(), r.stride, r.t.size(1), r.type, s.flat.data_ptr(), IdBytes(s.flat, "experts"),
+                           tokens, choices, num_experts, s.order.data_ptr<int32_t>(), s.place.data_ptr<int32_t>(),
+                           s.offsets.data_ptr<int64_t>(), out.data_ptr(), s.scratch(), s.scratch_bytes(), Stream(x)),
+        "gs_expert_dispatch");
+  return {out, s.order, s.place, s.offsets};
 }
 
 torch::Tensor ExpertGather(const torch::Tensor& x, const torch::Tensor& place, const torch::Tensor& offsets) {

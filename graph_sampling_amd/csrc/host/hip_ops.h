@@ -374,6 +374,10 @@ std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(const torch::Tensor
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> ExpertSort(const torch::Tensor& experts,
                                                                    int64_t num_experts);
 torch::Tensor ExpertGather(const torch::Tensor& x, const torch::Tensor& place, const torch::Tensor& offsets);
+// both: {rows, order, place, offsets}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> ExpertDispatch(const torch::Tensor& x,
+                                                                                      const torch::Tensor& experts,
+                                                                                      int64_t num_experts);
 torch::Tensor ExpertCombine(const torch::Tensor& y, const torch::Tensor& place,
                             const torch::optional<torch::Tensor>& weights);
 // {gradient of y, gradient of weights}, undefined where not wanted

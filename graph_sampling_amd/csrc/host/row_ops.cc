@@ -84,6 +84,19 @@ struct GatherFunction : public torch::autograd::Function<GatherFunction> {
   }
 };
 
+struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& experts,
+                               int64_t num_experts) {
+    const auto [rows, order, place, offsets] = hip::ExpertDispatch(x, experts, num_experts);
+    ctx->save_for_backward({place});
+    ctx->mark_non_differentiable({order, place, offsets});
+    return {rows, order, place, offsets};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return GatherFunction::backward(ctx, {grads[0]});
+  }
+};
+
 struct CombineFunction : public torch::autograd::Function<CombineFunction> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& y, const torch::Tensor& place,
                                const torch::Tensor& offsets, const torch::optional<torch::Tensor>& weights) {
@@ -142,9 +155,9 @@ torch::Tensor ExpertGather(torch::Tensor x, torch::Tensor order, torch::Tensor p
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> ExpertDispatch(torch::Tensor x,
                                                                                       torch::Tensor experts,
                                                                                       int64_t num_experts) {
-  auto [order, place, offsets] = hip::ExpertSort(experts, num_experts);
-  auto rows = Followed(x) ? GatherFunction::apply(x, place, offsets) : hip::ExpertGather(x, place, offsets);
-  return {rows, order, place, offsets};
+  if (!Followed(x)) return hip::ExpertDispatch(x, experts, num_experts);
+  const auto out = DispatchFunction::apply(x, experts, num_experts);
+  return {out[0], out[1], out[2], out[3]};
 }
 
 torch::Tensor ExpertCombine(torch::Tensor y, torch::Tensor order, torch::Tensor place, torch::Tensor offsets,

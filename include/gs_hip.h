@@ -1067,6 +1067,13 @@ int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_exp
 int gs_expert_gather(const void* x, int64_t x_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
                      int64_t choices, const int64_t* live, void* rows, void* stream);
 
+/* gs_expert_sort of experts [tokens, choices] and gs_expert_gather of x by it, in one call (one launch for up to 1024
+ * items of fewer than 256 experts).  Workspace: as gs_expert_sort's for tokens * choices items.  (No
+ * counterpart in the reference.) */
+int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, const void* experts, int id_bytes,
+                       int64_t tokens, int64_t choices, int64_t num_experts, int32_t* order, int32_t* place,
+                       int64_t* offsets, void* rows, void* workspace, size_t workspace_bytes, void* stream);
+
 /* out[t, :] = sum over k of weights[t, k] * y[place[t, k], :], in the order of k; weights NULL: ones; of type
  * GS_F32 or `type`.  A place outside [0, tokens * choices) adds nothing.  Also the gradient of gs_expert_gather. */
 int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,

@@ -387,7 +387,7 @@ def test_bad_arguments_are_refused_before_anything_is_launched():
                        (dict(ids=ctypes.c_void_p(at + 4)), b"aligned"), (dict(kind=1, out=ctypes.c_void_p(at + 1)), b"aligned")):
         status = lookup(**bad)
         assert status < 0 and match in lib.gs_status_string(status), (bad, lib.gs_status_string(status))
-    assert lib.gs_embedding_grad_workspace_bytes(i64(1000), i64(64), 0) > 16000
+    assert lib.gs_embedding_grad_workspace_bytes(i64(1000), i64(64), 0) > 8000  # a word an id
     status = lib.gs_embedding_grad(buf, i64(8), i64(8), 0, buf, 8, i64(2), i64(4), ctypes.c_float(1), buf, buf,
                                    ctypes.c_size_t(16), None)
     assert status == -2 and b"workspace" in lib.gs_status_string(status)

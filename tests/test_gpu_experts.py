@@ -145,6 +145,7 @@ def test_there_and_back(dev, tokens, choices, num, dim, kind, dtype):
         assert torch.equal(c_dy, grads[0]) and (w is None or torch.equal(c_dw, grads[1]))
     assert all(torch.equal(a, b) for a, b in zip(capi.expert_sort(d_e, num), got))
     assert torch.equal(capi.expert_gather(x.detach(), got.place, got.offsets), got_rows)
+    assert all(torch.equal(a, b) for a, b in zip(capi.expert_dispatch(x.detach(), d_e, num), (got_rows,) + tuple(got)))
 
 
 @gpu
@@ -378,7 +379,9 @@ def test_bad_arguments_are_refused_before_anything_is_launched():
     def sort(ids=buf, id_bytes=8, n=4, num=3, order=buf, place=buf, offsets=buf, ws=buf, ws_bytes=16):
         return lib.gs_expert_sort(ids, id_bytes, i64(n), i64(num), order, place, offsets, ws, ctypes.c_size_t(ws_bytes), None)
 
-    fails(sort(), b"workspace")
+    assert lib.gs_expert_sort_workspace_bytes(i64(4), i64(3)) == 0  # one workgroup's, in LDS
+    fails(sort(n=5000), b"workspace")
+    fails(sort(n=5, num=300), b"workspace")
     fails(sort(n=-1), b"negative")
     fails(sort(n=1 << 31), b"2^31")
     fails(sort(num=1 << 31), b"experts")
