@@ -233,7 +233,10 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
           v[u] = Values<T>{};
-          if (from[u] >= 0) v[u] = load_chunk(y + from[u] * y_stride + at, dim);
+          // (past the caches: y is read for the last time, and dy needs their room: 50 k tokens, 4 rows of 500
+          // bf16 each, 102 us plain and 77 so)
+          if (from[u] >= 0)
+            v[u] = dim >= Chunk<T>::kVec ? load_past(y + from[u] * y_stride + at) : load_chunk(y + from[u] * y_stride + at, dim);
         }
       }
 #pragma unroll
@@ -334,7 +337,8 @@ int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t 
                         T* dy, W* dweights, hipStream_t st) {
   constexpr int kTokens = kThreads / (G * WAVES);
   const dim3 grid(static_cast<unsigned>((tokens + kTokens - 1) / kTokens));
-  with_choices(choices, [&](auto ku) {
+  // (rows of eight choices at once take registers that waves need: 50 k tokens, 4 of 8 choices, 139 us; of 4 101)
+  with_choices(choices < 4 ? choices : 4, [&](auto ku) {
     hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st, dout,
                        dout_stride, y, y_stride, dim, Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place, tokens,
                        static_cast<int>(choices), tokens * choices, live, weights, dy, dweights, results_past(dy, dim));
@@ -503,6 +507,9 @@ int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y,
       using One = std::integral_constant<int, 1>;
       if (chunks <= 4) return go(std::integral_constant<int, 4>(), One());
       if (chunks <= 16) return go(std::integral_constant<int, 16>(), One());
+      // (half a wave, too, where a whole one would idle for a third of its time: rows of 77 chunks 59 us for 68)
+      if (chunks <= 32 || (tokens >= 4096 && chunks > kWave && chunks <= 85))
+        return go(std::integral_constant<int, 32>(), One());
       if (chunks <= kWave || tokens >= 4096) return go(std::integral_constant<int, kWave>(), One());
       return go(std::integral_constant<int, kWave>(), std::integral_constant<int, kThreads / kWave>());
     });

@@ -90,6 +90,7 @@ struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
     const auto [rows, order, place, offsets] = hip::ExpertDispatch(x, experts, num_experts);
     ctx->save_for_backward({place});
     ctx->mark_non_differentiable({order, place, offsets});
+    ctx->set_materialize_grads(false);  // (zeros for the three that have none)
     return {rows, order, place, offsets};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
