@@ -1962,7 +1962,7 @@ struct Weights {
                 w.value().sizes());
     TORCH_CHECK(w.value().scalar_type() == torch::kFloat32 || w.value().scalar_type() == rows.scalar_type(),
                 "weights must be float32 or of the rows' type, got ", w.value().scalar_type());
-    t = w.value().contiguous();
+    t = w.value().contiguous().resolve_neg();
     type = ValueType(t, "weights");
   }
   const void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
@@ -1971,8 +1971,10 @@ struct Weights {
 
 bool Capturing(const torch::Tensor& t) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(Stream(t)), &status) == hipSuccess,
-              "hipStreamIsCapturing failed");
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(Stream(t)), &status) != hipSuccess) {
+    (void)hipGetLastError();  // (the default stream may not be asked while another stream is recorded: not this one)
+    return false;
+  }
   return status != hipStreamCaptureStatusNone;
 }
 

@@ -127,6 +127,98 @@ def test_lookup_and_gradients(dev, num_rows, dim, n, kind, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("num_rows", [1, 200, 255, 256, 65535, 70000, (1 << 18) - 1, 1 << 18, 5_000_000, 140_000_000, 2 ** 32 - 2])
+def test_sorts_of_every_size_and_key(dev, num_rows):
+    """Both sides of every size at which the sort changes its tiles or launches, with keys of one to four digits of
+    eight and nine bits.  Whole numbers, whose sums fp32 holds exactly whatever the order."""
+    rng = np.random.default_rng(num_rows % 1000)
+    for n in (1, 63, 1024, 1025, 2049, 4096, 4097, 16384, 16385, 65536, 65537, 131072, 131073, 524288, 524289):
+        ids = rng.integers(-1, num_rows, n)
+        if n > 2000:  # a run that goes through many tiles
+            ids[n // 3:n // 2] = num_rows - 1
+        grad = rng.integers(-8, 9, (n, 1)).astype(np.float32)
+        met, values = torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(torch.from_numpy(grad).to(dev),
+                                                                 torch.from_numpy(ids).to(dev), num_rows, 1.0)
+        want, which = np.unique(ids[ids >= 0], return_inverse=True)
+        assert np.array_equal(met.cpu().numpy(), want)
+        assert np.array_equal(values[:, 0].cpu().numpy(), np.bincount(which, grad[ids >= 0, 0], want.size))
+        if num_rows <= 5_000_000:
+            dense = torch.ops.gs_ops._CAPI_EmbeddingGrad(torch.from_numpy(grad).to(dev), torch.from_numpy(ids).to(dev),
+                                                         num_rows, 1.0)
+            assert torch.equal(dense[met], values) and int(dense.count_nonzero()) == int(values.count_nonzero())
+
+
+@gpu
+def test_values_near_zero_are_kept(dev):
+    """Results below the smallest normal number are rounded, not dropped."""
+    for dtype, power in ((torch.float32, -120), (torch.bfloat16, -120), (torch.float16, -12)):
+        table = rows(20, 33, dtype, dev, 33).requires_grad_(True)
+        ids = ids_of("even", 50, 20, 34)
+        scale = 2.0 ** power * 2.0 ** (-9 if dtype != torch.float16 else -4)
+        out = gs.ops.embedding(table, torch.from_numpy(ids).to(dev), scale)
+        assert (out.detach().abs() < torch.finfo(dtype).smallest_normal).any() and out.detach().count_nonzero() > 0
+        check_lookup(out, table.detach(), ids, scale)
+        grad = rows(50, 33, dtype, dev, 35)
+        got, = torch.autograd.grad(out, table, grad)
+        want, tol = sums_by_id(grad, ids, 20, scale)
+        check_sums(got, want, tol + smallest(torch.float32), dtype)  # (the product with the scale is fp32 and may be tiny)
+
+
+@gpu
+def test_offsets_beyond_32_bits(dev):
+    """Tables, results and gradients of more than 2^32 values, the last rows among those that are named."""
+    if torch.cuda.mem_get_info(dev)[0] < 80 << 30:
+        pytest.skip("needs about 40 GB of free device memory")
+    num_rows, dim = 70_000_000, 64
+    table = torch.zeros(num_rows, dim, dtype=torch.float16, device=dev)
+    named = torch.tensor([0, 1, 33_554_432, 67_108_863, 67_108_864, num_rows - 1], device=dev)
+    table[named] = rows(named.numel(), dim, torch.float16, dev, 36)
+    assert torch.equal(gs.ops.embedding(table, named), table[named])
+    n = 68_000_000  # ids: the result is as large as the table
+    ids = (torch.arange(n, device=dev, dtype=torch.int32) % 1000)
+    ids[-3:] = torch.tensor([num_rows - 1, 67_108_864, -1], dtype=torch.int32, device=dev)
+    out = gs.ops.embedding(table, ids)
+    assert torch.equal(out[-3:-1], table[[num_rows - 1, 67_108_864]]) and not out[-1].any()
+    assert torch.equal(out[66_999_000:67_000_000], table[:1000]) and torch.equal(out[:1000], table[:1000])
+    # that result as a gradient: 68 k rows for each of a thousand ids, summed to 68 k (or fewer) times the same
+    out.fill_(2.0 ** -17)
+    met, sums = torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(out, ids, num_rows, 1.0)
+    counts = torch.bincount(ids[ids >= 0].long(), minlength=num_rows)
+    assert torch.equal(met, counts.nonzero()[:, 0])
+    want = counts[met].double() * 2.0 ** -17  # (exact in fp32: counts below 2^24)
+    assert (sums.double() - want[:, None]).abs().max() <= want.max() * half_step(torch.float16)
+    dense = torch.ops.gs_ops._CAPI_EmbeddingGrad(out, ids, num_rows, 1.0)
+    assert torch.equal(dense[met], sums) and int(dense[:, 0].count_nonzero()) == met.numel()
+
+
+@gpu
+def test_two_threads_at_once(dev):
+    """Gradients of both kinds by two threads on a stream each: nothing is shared between calls."""
+    import threading
+    work = []
+    for seed in (37, 38):
+        grad, ids = rows(30000, 24, torch.float32, dev, seed), torch.from_numpy(ids_of("hub", 30000, 900, seed)).to(dev)
+        work.append((grad, ids, torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, ids, 900, 1.0)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(grad, ids, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                met, values = torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(grad, ids, 900, 1.0)
+                dense = torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, ids, 900, 1.0)
+                if not (torch.equal(dense, want) and torch.equal(dense[met], values)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@gpu
 def test_rows_any_distance_apart_and_off_their_alignment(dev):
     for dtype in TYPES:
         base = rows(400, 61, dtype, dev, 3)

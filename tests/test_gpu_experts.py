@@ -79,7 +79,9 @@ CASES = [
     (128, 8, 255, 33, "skewed"), (513, 8, 256, 20, "even"), (600, 7, 300, 9, "outside"), (1000, 4, 16, 97, "one"),
     (1025, 4, 3, 1001, "none"), (2000, 3, 7, 130, "outside"), (9000, 9, 160, 12, "skewed"), (40000, 1, 5, 64, "skewed"),
     (5000, 2, 70000, 8, "even"), (30, 20, 40, 4096, "skewed"), (5, 11, 4, 1500, "outside"), (0, 3, 4, 8, "even"),
-    (7, 0, 4, 8, "even"), (6, 2, 0, 8, "none"),
+    (7, 0, 4, 8, "even"), (6, 2, 0, 8, "none"), (50, 4, 1000, 16, "outside"), (4096, 1, 256, 4, "even"),
+    (1024, 1, 255, 100, "outside"), (205, 5, 17, 100, "skewed"), (140000, 1, 3, 8, "outside"), (270000, 2, 700, 2, "skewed"),
+    (3, 3, 5, 70001, "outside"),
 ]
 
 
@@ -187,6 +189,39 @@ def test_rows_any_distance_apart(dev):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
         same = rows(1, 16, dtype, dev, 13).expand(100, 16)
         assert torch.equal(gs.ops.expert_gather(same, order), gs.ops.expert_gather(same.contiguous(), order))
+
+
+@gpu
+def test_offsets_beyond_32_bits(dev):
+    """More than 2^32 values sent, combined and in the gradients: rows at both ends against the formulas."""
+    if torch.cuda.mem_get_info(dev)[0] < 120 << 30:
+        pytest.skip("needs about 60 GB of free device memory")
+    tokens, choices, num, dim = 2_200_000, 2, 4, 1024
+    g = torch.Generator(device=dev)
+    g.manual_seed(33)
+    e = torch.randint(-1, num, (tokens, choices), generator=g, device=dev, dtype=torch.int32)
+    e[-1] = torch.tensor([num - 1, 0], device=dev)
+    x = torch.randn(tokens, dim, generator=g, device=dev, dtype=torch.bfloat16)
+    got, order = gs.ops.expert_dispatch(x, e, num)
+    live = int(order.offsets[-1])
+    assert live * dim > 2 ** 31 and got.numel() > 2 ** 32
+    some = torch.cat([torch.arange(1000, device=dev), torch.arange(live - 1000, live, device=dev),
+                      torch.randint(live, (1000,), generator=g, device=dev)])
+    assert torch.equal(got[some], x[order.order[some].long() // choices]) and not got[live:].any()
+    w = torch.rand(tokens, choices, generator=g, device=dev)
+    out = gs.ops.expert_combine(got, order, w)
+    t = torch.cat([torch.arange(500, device=dev), torch.arange(tokens - 500, tokens, device=dev)])
+    there = (e[t] >= 0).float()
+    within(out[t], (x[t].double() * (w[t] * there).sum(1, keepdim=True).double()).cpu().numpy(),
+           6 * F32 * (x[t].abs().double() * w[t].sum(1, keepdim=True).double()).cpu().numpy(), torch.bfloat16)
+    dy, dw = torch.ops.gs_ops._CAPI_ExpertCombineGrad(x, got, order.order, order.place, order.offsets, w)
+    item = order.order[some].long()
+    want = x[item // choices].double() * w.view(-1)[item, None].double()
+    within(dy[some], want.cpu().numpy(), want.abs().cpu().numpy() * F32, torch.bfloat16)
+    assert not dy[live:].any()
+    square = (x[t].double() ** 2).sum(1, keepdim=True)
+    within(dw[t], (square * there.double()).cpu().numpy(), ((dim + 12) * F32 * square).cpu().numpy() * np.ones((1, choices)),
+           torch.float32)
 
 
 @gpu
