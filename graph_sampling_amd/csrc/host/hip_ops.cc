@@ -1969,13 +1969,24 @@ struct Weights {
 };
 }  // namespace
 
-bool Capturing(const torch::Tensor& t) {
+namespace {
+bool StreamRecorded(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(static_cast<hipStream_t>(Stream(t)), &status) != hipSuccess) {
-    (void)hipGetLastError();  // (the default stream may not be asked while another stream is recorded: not this one)
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();  // (the default stream may not be asked while another is recorded: it is not itself)
     return false;
   }
   return status != hipStreamCaptureStatusNone;
+}
+}  // namespace
+
+bool Capturing(const torch::Tensor& t) { return StreamRecorded(static_cast<hipStream_t>(Stream(t))); }
+
+bool RecordedWith(const torch::Tensor& t, c10::StreamId id) {
+  const auto current = c10::hip::getCurrentHIPStream(t.device().index());
+  if (current.id() == id) return true;
+  const c10::Stream other(c10::Stream::UNSAFE, current.unwrap().device(), id);
+  return StreamRecorded(c10::hip::HIPStream(other).stream());
 }
 
 torch::Tensor EmbeddingLookup(const torch::Tensor& table, const torch::Tensor& ids, double scale) {

@@ -388,6 +388,8 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& 
                                                            bool of_rows, bool of_weights);
 // whether the current stream of t's device is being recorded into a graph
 bool Capturing(const torch::Tensor& t);
+// whether the stream with this id is the current one of t's device, or is being recorded as well
+bool RecordedWith(const torch::Tensor& t, c10::StreamId id);
 
 }  // namespace hip
 }  // namespace gs

@@ -1,7 +1,6 @@
 #include "row_ops.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "hip_ops.h"
@@ -11,17 +10,18 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// A tensor that a gradient may flow back to, and a call recorded into a graph: the engine makes the
-// stream of the leaf's accumulator wait, which ends the process when that stream is outside the recording.
+// A tensor that a gradient may flow back to, and a call recorded into a graph: the backward pass makes the
+// stream of the node that made t (the accumulator of a leaf) wait for the recording one, which ends the process
+// when that stream is outside the recording.
 void CheckRecording(const torch::Tensor& t) {
-  if (!t.is_cuda() || !t.is_leaf() || !hip::Capturing(t)) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!accumulator) return;
-  const auto stream = accumulator->stream();
-  TORCH_CHECK(!stream.has_value() ||
-                  *stream == c10::hip::getCurrentHIPStream(t.device().index()).unwrap(),
-              "a graph is being recorded, and an eager graph of the same leaf lives on another stream: its gradient "
-              "cannot be recorded (drop the eager outputs first, or run them on the recording stream)");
+  if (!t.is_cuda() || !hip::Capturing(t)) return;
+  const auto node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(stream.has_value() && hip::RecordedWith(t, stream->id()),
+              "a graph is being recorded, and an eager graph of the same leaf lives, or the tensor was made, on a "
+              "stream outside the recording: its gradient cannot be recorded (drop the eager outputs first, or "
+              "make them on the recording stream)");
 }
 
 // whether somebody follows what becomes of t: only then is a node made

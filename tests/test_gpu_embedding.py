@@ -388,6 +388,57 @@ def test_recording_is_refused_where_it_would_end_the_process(dev):
 
 
 @gpu
+def test_recording_with_several_uses_of_a_leaf(dev):
+    """Two lookups of one table, and one of a table made inside the recording: their nodes are on the recording
+    stream.  A tensor made outside, and followed, is refused."""
+    table = rows(40, 8, torch.float32, dev, 44).requires_grad_(True)
+    a, b = torch.arange(30, device=dev), torch.arange(5, 25, device=dev)
+
+    def step():
+        first, second = gs.ops.embedding(table, a), gs.ops.embedding(table, b, 2.0)
+        third = gs.ops.embedding(table * 3, a)
+        return torch.autograd.grad((first * first).sum() + second.sum() + third.sum(), table)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for rep in range(3):
+        with torch.no_grad():
+            table.copy_(rows(40, 8, torch.float32, dev, 45 + rep))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    made = table * 2  # outside
+    graph, message = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(graph):
+        kept = made.detach() + 1
+        try:
+            gs.ops.embedding(made, a)
+        except RuntimeError as error:
+            message = str(error)
+    assert message and "outside the recording" in message
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept, made.detach() + 1)
+
+
+@gpu
+def test_inference_mode(dev):
+    with torch.inference_mode():
+        table = rows(40, 8, torch.float32, dev, 47)
+        ids = torch.arange(30, device=dev)
+        assert torch.equal(gs.ops.embedding(table, ids), table[:30])
+
+
+@gpu
 def test_sparse_gradient_is_not_recorded(dev):
     grad, ids = rows(10, 8, torch.float32, dev, 26), torch.arange(10, device=dev)
     graph = torch.cuda.CUDAGraph()

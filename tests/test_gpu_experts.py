@@ -322,6 +322,64 @@ def test_recorded_and_replayed(dev):
 
 
 @gpu
+def test_recorded_backward_pass(dev):
+    """There, back with weights, and the gradients of rows and weights through autograd, recorded."""
+    x, w = rows(200, 16, torch.float32, dev, 34).requires_grad_(True), torch.rand(200, 3, device=dev).requires_grad_(True)
+    e = torch.from_numpy(experts_of("outside", 200, 3, 7, 35)).to(dev)
+    dout = rows(200, 16, torch.float32, dev, 36)
+
+    def step():
+        got, order = gs.ops.expert_dispatch(x, e, 7)
+        out = gs.ops.expert_combine(torch.tanh(got), order, w)
+        return torch.autograd.grad(out, (x, w), dout)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for rep in range(3):
+        e.copy_(torch.from_numpy(experts_of("skewed" if rep % 2 else "outside", 200, 3, 7, 37 + rep)))
+        dout.copy_(rows(200, 16, torch.float32, dev, 40 + rep))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+def test_two_threads_at_once(dev):
+    import threading
+    work = []
+    for seed in (43, 44):
+        x, e = rows(9000, 24, torch.float32, dev, seed), torch.from_numpy(experts_of("skewed", 9000, 2, 300, seed)).to(dev)
+        got, order = gs.ops.expert_dispatch(x, e, 300)
+        work.append((x, e, got, order, gs.ops.expert_combine(got, order)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(x, e, want, want_order, want_out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got, order = gs.ops.expert_dispatch(x, e, 300)
+                same = all(torch.equal(a, b) for a, b in zip((got,) + tuple(order), (want,) + tuple(want_order)))
+                if not (same and torch.equal(gs.ops.expert_combine(got, order), want_out)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=run, args=t) for t in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@gpu
 def test_a_layer_of_typed_nodes_end_to_end(dev):
     """Embeddings of a frontier, rows by type, a product per type, back with weights, and the gradients of
     every leaf against the same layer written in 64-bit torch."""
