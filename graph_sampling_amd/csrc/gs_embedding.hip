@@ -454,7 +454,7 @@ struct Numbers {
 
 template <typename IdT, typename Beside>
 void sort_ids(const IdT* ids, int64_t n, uint32_t num_rows, const GradSpace& s, Beside beside, hipStream_t st) {
-  key_sort::sort(key_sort::IdWords<IdT>{ids, num_rows}, n, num_rows, s.sort, key_sort::WordsOut{s.sorted}, st, beside);
+  key_sort::sort<false>(key_sort::IdWords<IdT>{ids, num_rows}, n, num_rows, s.sort, key_sort::WordsOut{s.sorted}, st, beside);
 }
 
 int check_rows(const char* what, const void* rows, int64_t stride, int64_t dim, int type, int64_t n, int64_t num_rows) {

@@ -107,13 +107,12 @@ gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chun
 // take 6 and the space between them.
 constexpr int64_t kDispatchItems = kThreads * key_sort::kItems;
 
-template <typename T, typename IdT>
+template <typename T, typename IdT, int BITS>
 __global__ void __launch_bounds__(kThreads)
 sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks,
                    int64_t total, int choices, uint32_t n, OrderOut out, T* __restrict__ rows, bool past) {
-  constexpr int kBits = 8, kDigits = 1 << kBits;
-  static_assert(kDigits == kThreads, "a digit a thread");
-  __shared__ key_sort::TileTables<kBits, kThreads> s_tables;
+  constexpr int kDigits = 1 << BITS;
+  __shared__ key_sort::TileTables<BITS, kThreads> s_tables;
   __shared__ uint32_t s_start[kDigits];
   __shared__ int32_t s_place[kDispatchItems];
   // the token's chunk is on its way meanwhile
@@ -131,13 +130,15 @@ sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int
   for (int r = 0; r < key_sort::kItems; ++r) {
     const uint32_t i = key_sort::item_of(r);
     w[r] = src(i < n ? i : n - 1);
-    d[r] = key_sort::digit_of<kBits>(w[r], 0);
+    d[r] = key_sort::digit_of<BITS>(w[r], 0);
   }
-  key_sort::rank_tile<kBits, kThreads>(d, n, s_tables, rank, &here);
+  key_sort::rank_tile<BITS, kThreads>(d, n, s_tables, rank, &here);
   uint32_t start = here, none = 0;
   key_sort::scan_digits(start, none, s_tables);
-  s_start[threadIdx.x] = start;
-  if (blockIdx.x == 0) out.digit(threadIdx.x, start);
+  if (threadIdx.x < kDigits) {
+    s_start[threadIdx.x] = start;
+    if (blockIdx.x == 0) out.digit(threadIdx.x, start);
+  }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < key_sort::kItems; ++r) {
@@ -369,9 +370,9 @@ int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOu
   }
   const key_sort::IdWords<IdT> src{experts, num};
   if (passes == 1) {
-    key_sort::sort(src, n, num, space, out, st);
+    key_sort::sort<true>(src, n, num, space, out, st);
   } else {
-    key_sort::sort(src, n, num, space, key_sort::WordsOut{sorted}, st);
+    key_sort::sort<false>(src, n, num, space, key_sort::WordsOut{sorted}, st);
     const int64_t threads = n > num_experts + 1 ? n : num_experts + 1;
     hipLaunchKernelGGL(order_kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
                        st, sorted, n, out);
@@ -445,7 +446,11 @@ int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, c
       using IdT = decltype(id);
       const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks, blocks = (total + kThreads - 1) / kThreads;
       GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks));
-      hipLaunchKernelGGL((sort_gather_kernel<T, IdT>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+      const int bits = key_sort::Digits(static_cast<uint32_t>(num_experts), true).bits;
+      auto* kernel = bits == 4   ? sort_gather_kernel<T, IdT, 4>
+                     : bits == 7 ? sort_gather_kernel<T, IdT, 7>
+                                 : sort_gather_kernel<T, IdT, 8>;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
                          static_cast<hipStream_t>(stream), static_cast<const IdT*>(experts), static_cast<const T*>(x),
                          x_stride, dim, Divider(static_cast<uint32_t>(chunks)), total, static_cast<int>(choices),
                          static_cast<uint32_t>(n), out, static_cast<T*>(rows),

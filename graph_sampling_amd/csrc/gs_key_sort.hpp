@@ -11,20 +11,29 @@ namespace key_sort {
 
 constexpr int kItems = 4;  // of a thread
 // A tile is the items of 256, 512 or 1024 threads: comparing them by ballots is what a pass takes longest
-// for, and small tiles spread that over more compute units, as long as their counts are few.  Up to 64 tiles
-// every workgroup of a pass adds up the counts of all by itself; more are added up by a launch between.  Us a
-// count and pass (8 bits, 4 M keys), by itself / with that launch: 131 k items in 256-thread tiles 12.3 / 9.4,
-// 512 8.5 / 9.7, 1024 10.9 / 11.0; 400 k 31.6 / 12.3, 14.9 / 10.8, 11.6 / 11.6; 810 k -, 31.2 / 13.9, 15.9 / 13.2;
-// 2 M -, 106 / 21.4, 39.5 / 19.0.  (16 k items, the pass alone: 256 threads 4.9, 512 5.9, 1024 8.1.)
-constexpr int64_t kSelfTiles = 64;
+// for, and small tiles spread that over more compute units, as long as their counts are few.  Up to 16 k counts
+// every workgroup of a pass adds up all of them by itself, if a thread reads no more than it asks for at once;
+// more are added up by a launch between.  Us a count and pass (8 bits, 4 M keys), by itself / with that launch:
+// 131 k items in 256-thread tiles 12.3 / 9.4, 512 8.5 / 9.7, 1024 10.9 / 11.0; 400 k 31.6 / 12.3, 14.9 / 10.8,
+// 11.6 / 11.6; 810 k -, 31.2 / 13.9, 15.9 / 13.2; 2 M -, 106 / 21.4, 39.5 / 19.0.  (16 k items, the pass alone:
+// 256 threads 4.9, 512 5.9, 1024 8.1.)
 constexpr int64_t kAlone = 1024 * kItems;        // items that one workgroup sorts alone
 constexpr int64_t kFewItems = 4 * kAlone;        // items that every workgroup of a pass counts by itself
+constexpr int64_t kSelfCounts = int64_t(1) << 14;
 constexpr int kMostDigits = 512;
+constexpr int ahead_of(int bits) { return bits <= 4 ? 8 : 32; }  // counts a thread asks for at once
+inline int64_t tiles_of(int64_t n, int threads) { return (n + threads * kItems - 1) / (threads * kItems); }
+inline bool adds_up_itself(int64_t tiles, int bits, int threads) {
+  return tiles <= ahead_of(bits) * (threads >> bits) && (tiles << bits) <= kSelfCounts;
+}
 // (a thread a digit at least)
 inline int threads_for(int64_t n, int bits) {
-  if (n <= kAlone) return bits == 8 && n <= 256 * kItems ? 256 : n <= 512 * kItems ? 512 : 1024;
+  const int least = bits == 9 ? 512 : 256;
+  if (n <= kAlone) return n <= 256 * kItems && least == 256 ? 256 : n <= 512 * kItems ? 512 : 1024;
   if (n <= kFewItems) return 512;
-  return bits == 8 && n <= kSelfTiles * 256 * kItems ? 256 : n <= 4 * kSelfTiles * 512 * kItems ? 512 : 1024;
+  for (int threads = least; threads <= 1024; threads *= 2)
+    if (adds_up_itself(tiles_of(n, threads), bits, threads)) return threads;
+  return n <= (int64_t(1) << 19) ? 512 : 1024;
 }
 
 using Word = unsigned long long;
@@ -49,17 +58,22 @@ __device__ __forceinline__ uint32_t key_of(Word w) { return static_cast<uint32_t
 __device__ __forceinline__ uint32_t position_of(Word w) { return static_cast<uint32_t>(w); }
 
 // Digits of eight bits, or of nine where that is a pass less (keys of 17 and 18 bits, of 25 to 27): 400 k
-// keys of 18 bits take two passes of 16 us for three of 13.
+// keys of 18 bits take two passes of 14 us for three of 13.  Few keys (FEW: a caller that expects some) have digits
+// of four or seven bits: fewer ballots and fewer counts.
 struct Digits {
   int bits, passes;
-  explicit Digits(uint32_t num) {
+  explicit Digits(uint32_t num, bool few = false) {
     int key_bits = 1;
     while (key_bits < 32 && (num >> key_bits) != 0) ++key_bits;
     const int eight = (key_bits + 7) / 8, nine = (key_bits + 8) / 9;
     bits = nine < eight ? 9 : 8;
     passes = nine < eight ? nine : eight;
+    if (few && key_bits <= 7) bits = key_bits <= 4 ? 4 : 7;
   }
 };
+// copies of a table of counts that many threads add to: where many items hold one digit, additions queue up
+template <int BITS>
+constexpr int kCopies = BITS <= 7 ? 16 : 4;
 template <int BITS>
 __device__ __forceinline__ uint32_t digit_of(Word w, int pass) {
   return (key_of(w) >> (BITS * pass)) & ((1u << BITS) - 1);
@@ -77,7 +91,7 @@ struct TileTables {
   static constexpr int kDigits = 1 << BITS, kWaves = THREADS / kWave;
   static_assert(kDigits <= THREADS, "a thread a digit");
   uint16_t count[kWaves][kDigits];  // of a wave's items, then of the waves before it
-  uint2 scan[kDigits / kWave];
+  uint2 scan[kDigits > kWave ? kDigits / kWave : 1];
 };
 
 // item r of this thread: a wave owns 64 * kItems consecutive items, 64 of them a round
@@ -150,12 +164,12 @@ __device__ __forceinline__ void scan_digits(uint32_t& v, uint32_t& u, TileTables
         ui += uo;
       }
     }
-    if (lane == kWave - 1) t.scan[wave] = make_uint2(vi, ui);
+    if (kDigits > kWave && lane == kWave - 1) t.scan[wave] = make_uint2(vi, ui);
   }
   __syncthreads();
   v = vi - v;
   u = ui - u;
-  if (threadIdx.x < kDigits) {
+  if (threadIdx.x < kDigits && kDigits > kWave) {
 #pragma unroll
     for (int w = 0; w < kDigits / kWave; ++w) {
       const uint2 s = t.scan[w];
@@ -171,7 +185,7 @@ __global__ void __launch_bounds__(THREADS)
 count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__ counts, Beside beside) {
   constexpr int kDigits = 1 << BITS;
   if (Beside::kAny && blockIdx.x >= tiles) return beside.run(blockIdx.x - tiles, gridDim.x - tiles, THREADS);
-  __shared__ uint32_t s_hist[4][kDigits];
+  __shared__ uint32_t s_hist[kCopies<BITS>][kDigits + 1];
   const int64_t base = static_cast<int64_t>(blockIdx.x) * (THREADS * kItems);
   Word w[kItems];
 #pragma unroll
@@ -180,21 +194,21 @@ count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__
     w[r] = src(i < n ? i : n - 1);
   }
 #pragma unroll
-  for (int j = threadIdx.x; j < 4 * kDigits; j += THREADS) (&s_hist[0][0])[j] = 0;
+  for (int j = threadIdx.x; j < kCopies<BITS> * (kDigits + 1); j += THREADS) (&s_hist[0][0])[j] = 0;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kItems; ++r)
-    if (base + r * THREADS + threadIdx.x < n) atomicAdd(&s_hist[threadIdx.x & 3][digit_of<BITS>(w[r], pass)], 1u);
+    if (base + r * THREADS + threadIdx.x < n) atomicAdd(&s_hist[threadIdx.x % kCopies<BITS>][digit_of<BITS>(w[r], pass)], 1u);
   __syncthreads();
   if (threadIdx.x < kDigits) {
     uint32_t all = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) all += s_hist[c][threadIdx.x];
+    for (int c = 0; c < kCopies<BITS>; ++c) all += s_hist[c][threadIdx.x];
     counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = all;
   }
 }
 
-// For sorts of more than kSelfTiles tiles: in place of every count, how many items of its digit the
+// For sorts of many tiles: in place of every count, how many items of its digit the
 // tiles before hold, and in totals[d] how many all hold.  A workgroup a digit.
 constexpr int kPrefixThreads = 256;
 static __global__ void __launch_bounds__(kPrefixThreads)
@@ -224,11 +238,11 @@ template <int BITS, int THREADS, typename Src, Counts COUNTS, typename Out, type
 __global__ void __launch_bounds__(THREADS)
 pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restrict__ counts,
             const uint32_t* __restrict__ totals, Out out, Beside beside) {
-  // (kHere: copies of the counts, lane by lane in turn: where many items hold one digit, additions queue up)
-  constexpr int kDigits = 1 << BITS, kParts = COUNTS == Counts::kHere ? 8 : THREADS / kDigits, kTile = THREADS * kItems;
+  constexpr int kDigits = 1 << BITS, kTile = THREADS * kItems;
+  constexpr int kParts = COUNTS == Counts::kHere ? 2 * kCopies<BITS> : THREADS / kDigits;
   if (Beside::kAny && blockIdx.x >= tiles) return beside.run(blockIdx.x - tiles, gridDim.x - tiles, THREADS);
   __shared__ TileTables<BITS, THREADS> s_tables;
-  __shared__ uint32_t s_all[kParts][kDigits], s_before[kParts][kDigits];
+  __shared__ uint32_t s_all[kParts][kDigits + 1], s_before[kParts][kDigits + 1];
   __shared__ uint32_t s_start[kDigits];  // where a digit's items start in the tile
   __shared__ uint32_t s_shift[kDigits];  // from a place in the tile's order to the place in memory, modulo 2^32
   __shared__ Word s_word[kTile];
@@ -244,7 +258,7 @@ pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restr
   if constexpr (COUNTS == Counts::kHere) {
     constexpr int kAhead = 8;
 #pragma unroll
-    for (int j = threadIdx.x; j < kParts * kDigits; j += THREADS) (&s_all[0][0])[j] = (&s_before[0][0])[j] = 0;
+    for (int j = threadIdx.x; j < kParts * (kDigits + 1); j += THREADS) (&s_all[0][0])[j] = (&s_before[0][0])[j] = 0;
     __syncthreads();
     for (int64_t i0 = threadIdx.x; i0 < n; i0 += kAhead * THREADS) {
       Word other[kAhead];
@@ -260,7 +274,7 @@ pass_kernel(Src src, int64_t n, int pass, int64_t tiles, const uint32_t* __restr
     }
     // (s_all: of this tile and those behind it)
   } else if constexpr (COUNTS == Counts::kTiles) {  // a share of the tiles a thread, kAhead counts asked for together
-    constexpr int kAhead = 32;
+    constexpr int kAhead = ahead_of(BITS);
     uint32_t all = 0, before = 0;
     for (int b0 = part; b0 < static_cast<int>(tiles); b0 += kAhead * kParts) {
       uint32_t c[kAhead];
@@ -381,20 +395,17 @@ struct Space {
   uint32_t* totals;
 };
 // words: of the two buffers, how many the sort needs (a last pass that writes elsewhere: passes - 1, at most 2)
-inline int64_t most_tiles(int64_t n) {  // whatever the digits
-  const int64_t tile = threads_for(n, 8) * kItems;
-  return (n + tile - 1) / tile;
-}
+// (a tile's counts are no more than a quarter of its items: 512 of 512 threads, 256 of 256)
+inline size_t most_counts(int64_t n) { return static_cast<size_t>(n / 4 + kMostDigits); }
 inline size_t space_bytes(int64_t n, int words) {
   if (n <= kAlone) return 0;  // (one workgroup does it in LDS)
-  return words * padded(static_cast<size_t>(n) * 8) + padded(static_cast<size_t>(most_tiles(n)) * kMostDigits * 4) +
-         padded(kMostDigits * 4);
+  return words * padded(static_cast<size_t>(n) * 8) + padded(most_counts(n) * 4) + padded(kMostDigits * 4);
 }
 inline void carve(Carver& ws, int64_t n, int words, Space* s) {
   *s = Space{};
   if (n <= kAlone) return;
   for (int i = 0; i < 2; ++i) s->word[i] = i < words ? ws.take<Word>(static_cast<size_t>(n)) : nullptr;
-  s->counts = ws.take<uint32_t>(static_cast<size_t>(most_tiles(n)) * kMostDigits);
+  s->counts = ws.take<uint32_t>(most_counts(n));
   s->totals = ws.take<uint32_t>(kMostDigits);
 }
 
@@ -409,7 +420,7 @@ void launch_beside(Kernel kernel, int64_t tiles, int threads, hipStream_t st, Be
 
 template <int BITS, int THREADS, typename Src, typename Out, typename Beside>
 void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& beside, hipStream_t st) {
-  const int64_t tiles = (n + THREADS * kItems - 1) / (THREADS * kItems);
+  const int64_t tiles = tiles_of(n, THREADS);
   const uint32_t *counts = s.counts, *totals = s.totals;
   if (n <= kFewItems) {
     launch_beside(pass_kernel<BITS, THREADS, Src, Counts::kHere, Out, Beside>, tiles, THREADS, st, beside, src, n, pass,
@@ -417,7 +428,7 @@ void launch_pass(Src src, int64_t n, int pass, const Space& s, Out out, Beside& 
     return;
   }
   launch_beside(count_kernel<BITS, THREADS, Src, Beside>, tiles, THREADS, st, beside, src, n, pass, tiles, s.counts);
-  const bool self = tiles <= kSelfTiles;
+  const bool self = adds_up_itself(tiles, BITS, THREADS);
   if (!self)
     hipLaunchKernelGGL(prefix_kernel, dim3(1 << BITS), dim3(kPrefixThreads), 0, st, s.counts, tiles, 1 << BITS, s.totals);
   launch_beside(self ? pass_kernel<BITS, THREADS, Src, Counts::kTiles, Out, Beside>
@@ -449,7 +460,7 @@ void sort_with(Src src, int64_t n, int passes, const Space& s, Out out, Beside b
 template <int BITS, typename Src, typename Out, typename Beside>
 void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside beside, hipStream_t st) {
   const int threads = threads_for(n, BITS);
-  if constexpr (BITS == 8) {
+  if constexpr (BITS <= 8) {
     if (threads == 256) return sort_with<BITS, 256>(src, n, passes, s, out, beside, st);
   }
   if (threads == 512) return sort_with<BITS, 512>(src, n, passes, s, out, beside, st);
@@ -458,10 +469,14 @@ void sort_by(Src src, int64_t n, int passes, const Space& s, Out out, Beside bes
 
 // Sorts n >= 1 items (below 2^31), keys 0..num; the last pass hands every word with its place to `out`.  Where
 // the sort has two passes it uses word[0] of the space, three or four word[0] and word[1].  beside: run in as many
-// equal parts as there are launches.
-template <typename Src, typename Out, typename Beside = NoWork>
+// equal parts as there are launches.  FEW: as in Digits.
+template <bool FEW, typename Src, typename Out, typename Beside = NoWork>
 void sort(Src src, int64_t n, uint32_t num, const Space& s, Out out, hipStream_t st, Beside beside = Beside()) {
-  const Digits digits(num);
+  const Digits digits(num, FEW);
+  if constexpr (FEW) {
+    if (digits.bits == 4) return sort_by<4>(src, n, 1, s, out, beside, st);
+    if (digits.bits == 7) return sort_by<7>(src, n, 1, s, out, beside, st);
+  }
   if (digits.bits == 9) sort_by<9>(src, n, digits.passes, s, out, beside, st);
   else sort_by<8>(src, n, digits.passes, s, out, beside, st);
 }

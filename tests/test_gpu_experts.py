@@ -151,6 +151,16 @@ def test_there_and_back(dev, tokens, choices, num, dim, kind, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("num", [1, 2, 14, 15, 16, 60, 126, 127, 128, 255, 256, 511, 512, 3000, 65536])
+def test_sorts_of_every_size_and_number_of_experts(dev, num):
+    """Both sides of every size at which the sort changes its tiles or launches, with digits of every width."""
+    for n in (1, 255, 1024, 1025, 2048, 4096, 4097, 16384, 16385, 32769, 65537, 131073, 262145, 524289, 1_048_577):
+        for kind in ("outside", "skewed"):
+            e = experts_of(kind, n, 1, num, n % 1000 + num, np.int32)
+            check_order(gs.ops.expert_sort(torch.from_numpy(e).to(dev), num), e, num)
+
+
+@gpu
 def test_one_choice_each_without_a_second_dimension(dev):
     """Node types: experts, places and weights of shape [tokens]."""
     e = experts_of("skewed", 777, 1, 6, 6)[:, 0]
