@@ -4,7 +4,7 @@
 bench.py measures the GraphSAGE minibatch; this script times the other rows of the scope
 table at the sizes of their configurations -- induced-subgraph slicing, format conversions,
 weighted sampling with and without replacement, list sampling, the super-batch helpers,
-walks, SDDMM, segment and COO sums, row slicing -- through the same C ABI
+walks, SDDMM, rows moved by ids, segment and COO sums, row slicing -- through the same C ABI
 (graph_sampling_amd/capi.py), with `algorithmic` = the bytes the operator must move at the
 least (stated per line) over the median of the timed calls, and four whole samplers (LADIES
 and GraphSAGE written against Matrix, as written and through jit.compile) by wall clock.
@@ -216,6 +216,24 @@ def main():
     run("sddmm_dot", "gs_sddmm_coo u_dot_v, 64-d fp32 features, 8M random edges; 532 B per edge",
         lambda: capi.sddmm_coo("dot", er, ec, None, feat, feat, out_e, 0, 2, 64, 64, 1, 64, None, None),
         lambda o: (8_000_000 * 532, 8_000_000, "edges"))
+    # rows moved by ids: a frontier's features, the gradient of a table's rows, rows by type and back
+    front = perm_ids(600_000)
+    run("embedding_lookup", "gs_embedding_lookup: 600 k rows of 64 fp32 by id; 2 x 256 B + b per row",
+        lambda: capi.embedding_lookup(feat, front), lambda o: (600_000 * (512 + b), 600_000, "rows"))
+    g_ids, g_rows = rand_ids(400_000, 1 << 17), feat[:400_000]
+    run("embedding_grad", "gs_embedding_grad: 400 k rows of 64 fp32 into 131 072; 256 B + b per row, 256 B per sum",
+        lambda: capi.embedding_grad(g_rows, g_ids, 1 << 17),
+        lambda o: (400_000 * (256 + b) + (1 << 17) * 256, 400_000, "rows"))
+    kinds = rand_ids(600_000, 5)
+    run("expert_dispatch", "gs_expert_dispatch: 600 k rows of 64 fp32 by one of 5 types; 2 x 256 B + b + 8 B per row",
+        lambda: capi.expert_dispatch(feat[:600_000], kinds, 5), lambda o: (600_000 * (512 + b + 8), 600_000, "rows"))
+    t_rows, _, t_place, t_offsets = capi.expert_dispatch(feat[:600_000], kinds, 5)
+    run("expert_combine", "gs_expert_combine: the same rows brought back; 2 x 256 B + 4 B per row",
+        lambda: capi.expert_combine(t_rows, t_place), lambda o: (600_000 * (512 + 4), 600_000, "rows"))
+    t_weights = torch.rand(600_000, generator=gen, device=dev)
+    run("expert_combine_grad", "gs_expert_combine_grad: with weights, both gradients; 3 x 256 B + 12 B per row",
+        lambda: capi.expert_combine_grad(feat[:600_000], t_rows, t_place, t_offsets, t_weights),
+        lambda o: (600_000 * (768 + 12), 600_000, "rows"))
     # Divide(divisor, axis=0) on the CSC: out[e] = w[e] / divisor[column of e], scalar per edge
     out_w = torch.empty(E, 1, device=dev)
     run("sddmm_div_csc", "gs_sddmm_csc e_div_v over the whole graph (edge weight / per-column scalar): "

@@ -61,7 +61,8 @@ lookup_kernel(const T* __restrict__ table, int64_t num_rows, int64_t stride, int
 // ---------------------------------------------------------------- gradient ----
 // Zeros in the whole gradient, before the rows that are met are written: beside the sort, whose launches leave
 // most of the chip idle.  16 k tokens, us: the sort alone 17.1, 64 MB of zeros alone 10.6, one after the other 27.9,
-// beside each other 21.7 (with 512 workgroups of zeros instead of 128 23.4, with 32 23.3: the sort waits for memory).
+// beside each other 21.7.  64 k threads, which fill at the rate that memory takes: with 256 k the sort waits for
+// memory (23.4), with 16 k it is done before the zeros are (23.3).
 template <typename T>
 struct Zeros {
   static constexpr bool kAny = true;
@@ -71,7 +72,7 @@ struct Zeros {
   // workgroups a launch
   int blocks(int threads) const {
     const int64_t chunks = (n / Chunk<T>::kVec + parts - 1) / parts, most = (chunks + 4 * threads - 1) / (4 * threads);
-    return static_cast<int>(most < 1 ? 1 : most > 128 ? 128 : most);
+    return static_cast<int>(most < 1 ? 1 : most > (1 << 16) / threads ? (1 << 16) / threads : most);
   }
   __device__ __forceinline__ void run(int64_t block, int64_t of, int threads) const {
     const int64_t whole = n / Chunk<T>::kVec, share = (whole + parts - 1) / parts;
@@ -207,7 +208,7 @@ struct Runs {
 constexpr int kBatch = 8;      // rows a group asks for together
 constexpr int kMostSize = 32;  // positions of a tile at most
 
-// A row's chunk, past the caches where a line holds no other row's: every row is read once (207 MB of random rows
+// A row's chunk, past the caches where rows are longer than a line: every row is read once (207 MB of random rows
 // of 256 B, added up by 32s: 43 us plain, 38 so).
 template <typename T, int G>
 __device__ __forceinline__ Values<T> load_once(const T* p, int64_t dim) {
@@ -438,11 +439,11 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
                       last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
       const dim3 grid(static_cast<unsigned>(p.parts[l] * p.slices));
       if (l == 0)
-        hipLaunchKernelGGL((met ? sum_runs_kernel<T, G, true> : sum_runs_kernel<T, G, false>), grid, dim3(groups_in(kSumMost, G) * G), 0, st, s.sorted, p.n, num_rows, grad,
-                           stride, p.size, o, out);
+        hipLaunchKernelGGL((met ? sum_runs_kernel<T, G, true> : sum_runs_kernel<T, G, false>), grid,
+                           dim3(groups_in(kSumMost, G) * G), 0, st, s.sorted, p.n, num_rows, grad, stride, p.size, o, out);
       else
-        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(groups_in(kJoinMost, G) * G), 0, st, s.entries[(l - 1) & 1],
-                           2 * p.parts[l - 1], s.sums[(l - 1) & 1], o, out);
+        hipLaunchKernelGGL((join_runs_kernel<T, G>), grid, dim3(groups_in(kJoinMost, G) * G), 0, st,
+                           s.entries[(l - 1) & 1], 2 * p.parts[l - 1], s.sums[(l - 1) & 1], o, out);
     }
   });
 }

@@ -20,7 +20,7 @@ namespace {
 constexpr int kThreads = 256;
 
 // -------------------------------------------------------------------- sort ----
-// Sorted items of fewer than 256 experts (one pass, which knows where every expert begins).
+// Sorted items of fewer than 512 experts (one pass, which knows where every expert begins).
 struct OrderOut {
   int32_t* order;
   int32_t* place;
@@ -236,8 +236,8 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
           v[u] = Values<T>{};
           // (past the caches: y is read for the last time, and dy needs their room: 50 k tokens, 4 rows of 500
           // bf16 each, 102 us plain and 77 so)
-          if (from[u] >= 0)
-            v[u] = dim >= Chunk<T>::kVec ? load_past(y + from[u] * y_stride + at) : load_chunk(y + from[u] * y_stride + at, dim);
+          const T* const at_y = y + (from[u] >= 0 ? from[u] * y_stride + at : 0);
+          if (from[u] >= 0) v[u] = dim >= Chunk<T>::kVec ? load_past(at_y) : load_chunk(at_y, dim);
         }
       }
 #pragma unroll

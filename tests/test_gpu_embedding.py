@@ -431,6 +431,33 @@ def test_recording_with_several_uses_of_a_leaf(dev):
 
 
 @gpu
+def test_in_a_compiled_sampler(dev):
+    """A sampler that hands out its frontier's rows, as written and through jit.compile."""
+    from tests.util import rmat_csc_np
+    indptr, indices = rmat_csc_np(1 << 12, 1 << 16, seed=1)
+    A = gs.Matrix().load_csc(torch.from_numpy(indptr).to(dev), torch.from_numpy(indices).to(dev))
+    table = rows(1 << 12, 24, torch.bfloat16, dev, 48)
+
+    def sampler(A, seeds, fanouts, table):
+        blocks = []
+        for k in fanouts:
+            sub = A[:, seeds].columnwise_sampling(k, False)
+            seeds = sub.all_indices()
+            blocks.insert(0, sub.to_dgl_block())
+        return seeds, blocks, gs.ops.embedding(table, seeds, 2.0)
+
+    seeds = torch.randperm(1 << 12, device=dev)[:200]
+    compiled = gs.jit.compile(sampler, (A, seeds[:4], [5, 3], table))
+    for trial in range(2):
+        gs.set_seed(60 + trial)
+        nodes, _, h = sampler(A, seeds, [5, 3], table)
+        gs.set_seed(60 + trial)
+        got_nodes, _, got = compiled(A, seeds, [5, 3], table)
+        assert torch.equal(nodes, got_nodes) and torch.equal(h, got)
+        assert torch.equal(h, (table[nodes].float() * 2).bfloat16())
+
+
+@gpu
 def test_inference_mode(dev):
     with torch.inference_mode():
         table = rows(40, 8, torch.float32, dev, 47)
