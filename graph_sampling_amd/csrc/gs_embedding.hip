@@ -28,7 +28,7 @@ constexpr int kThreads = 256;
 template <typename T, typename IdT, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 lookup_kernel(const T* __restrict__ table, int64_t num_rows, int64_t stride, int64_t dim, Divider chunks,
-              const IdT* __restrict__ ids, int64_t total, float scale, T* __restrict__ out, bool past) {
+              const IdT* __restrict__ ids, int64_t total, float scale, T* __restrict__ out, Past past) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * ITEMS);
   const RowRange range(chunks, first);
   int64_t id[ITEMS], to[ITEMS], at[ITEMS];
@@ -54,7 +54,7 @@ lookup_kernel(const T* __restrict__ table, int64_t num_rows, int64_t stride, int
     const Values<T> w = scale == 1.0f ? v[k] : narrow<T>(widen<T>(v[k]) * scale);
     // (0 * inf where there is no row would be NaN)
     const bool there = id[k] >= 0 && id[k] < num_rows;
-    if (to[k] >= 0) store_result(out + to[k], there ? w : Values<T>{}, dim, past);
+    if (to[k] >= 0) store_result(out + to[k], there ? w : Values<T>{}, at[k], dim, past);
   }
 }
 
@@ -98,7 +98,7 @@ constexpr uint32_t kNone = 0, kSum = 1, kThrough = 2;  // (through: the run goes
 
 struct RunsOut {
   float scale;
-  bool past;             // (results_past)
+  Past past;             // (results_past)
   int64_t dim;
   int64_t chunks;        // of a row
   int slices;            // workgroups side by side over a row
@@ -143,7 +143,9 @@ struct Runs {
     if (threadIdx.x < 2) s.left[threadIdx.x] = Entry{0, kNone};
   }
   __device__ __forceinline__ void write(uint32_t row, const Wide<T>& sum) {
-    if (in) store_result(out + static_cast<int64_t>(row) * o.dim, narrow<T>(sum * o.scale), o.dim, o.past);
+    if (!in) return;
+    store_result(out + static_cast<int64_t>(row) * o.dim, narrow<T>(sum * o.scale), chunk_start<T>(o.dim, chunk), o.dim,
+                 o.past);
   }
   // a run of this group's tile that ends; left, right: it began before the tile, goes on behind it
   __device__ __forceinline__ void finish(uint32_t row, const Wide<T>& sum, bool left, bool right) {
@@ -435,7 +437,7 @@ void launch_sums(const SumPlan& p, const GradSpace& s, uint32_t num_rows, const 
     constexpr int G = decltype(g)::value;
     for (int l = 0; l < p.levels; ++l) {
       const bool last = l == p.levels - 1;
-      const RunsOut o{scale, results_past(out, dim), dim, p.chunks, p.slices, met, s.heads,
+      const RunsOut o{scale, results_past(out, dim, false), dim, p.chunks, p.slices, met, s.heads,
                       last ? nullptr : s.entries[l & 1], last ? nullptr : s.sums[l & 1]};
       const dim3 grid(static_cast<unsigned>(p.parts[l] * p.slices));
       if (l == 0)
@@ -517,7 +519,7 @@ int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride,
       auto* kernel = many ? lookup_kernel<T, IdT, kMany> : lookup_kernel<T, IdT, 1>;
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st,
                          static_cast<const T*>(table), num_rows, row_stride, dim, by, static_cast<const IdT*>(ids), total,
-                         scale, static_cast<T*>(out), results_past(static_cast<const T*>(out), dim));
+                         scale, static_cast<T*>(out), results_past(static_cast<const T*>(out), dim, true));
       return check_launch("embedding_lookup");
     });
   });

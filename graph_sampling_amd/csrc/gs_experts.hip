@@ -64,12 +64,13 @@ __global__ void __launch_bounds__(kThreads) no_items_kernel(int64_t* __restrict_
 // Zeros in the rows from `from` to n, a share of them by every workgroup.
 template <typename T>
 __device__ __forceinline__ void zero_rows_behind(int64_t from, int64_t n, int64_t dim, const Divider& chunks,
-                                                 T* __restrict__ rows, bool past) {
+                                                 T* __restrict__ rows, Past past) {
   if (from >= n || from < 0) return;
   const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
     const int64_t row = i / chunks.d;
-    store_result(rows + (from + row) * dim + chunk_start<T>(dim, i - row * chunks.d), Values<T>{}, dim, past);
+    const int64_t at = chunk_start<T>(dim, i - row * chunks.d);
+    store_result(rows + (from + row) * dim + at, Values<T>{}, at, dim, past);
   }
 }
 
@@ -77,7 +78,7 @@ __device__ __forceinline__ void zero_rows_behind(int64_t from, int64_t n, int64_
 template <typename T, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
-              int64_t total, int choices, int64_t n, const int64_t* __restrict__ live, T* __restrict__ rows, bool past) {
+              int64_t total, int choices, int64_t n, const int64_t* __restrict__ live, T* __restrict__ rows, Past past) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * ITEMS);
   const RowRange range(chunks, first);
   int64_t token[ITEMS], at[ITEMS];
@@ -96,7 +97,7 @@ gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chun
     for (int i = 0; i < ITEMS; ++i) {
       if (token[i] < 0) continue;
       const int64_t to = place[token[i] * choices + k];
-      if (to >= 0 && to < n) store_result(rows + to * dim + at[i], v[i], dim, past);
+      if (to >= 0 && to < n) store_result(rows + to * dim + at[i], v[i], at[i], dim, past);
     }
   }
   zero_rows_behind(*live, n, dim, chunks, rows, past);
@@ -110,7 +111,7 @@ constexpr int64_t kDispatchItems = kThreads * key_sort::kItems;
 template <typename T, typename IdT, int BITS>
 __global__ void __launch_bounds__(kThreads)
 sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks,
-                   int64_t total, int choices, uint32_t n, OrderOut out, T* __restrict__ rows, bool past) {
+                   int64_t total, int choices, uint32_t n, OrderOut out, T* __restrict__ rows, Past past) {
   constexpr int kDigits = 1 << BITS;
   __shared__ key_sort::TileTables<BITS, kThreads> s_tables;
   __shared__ uint32_t s_start[kDigits];
@@ -155,7 +156,7 @@ sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int
   if (in) {
     for (int k = 0; k < choices; ++k) {
       const int32_t to = s_place[token * choices + k];
-      if (to >= 0) store_result(rows + to * dim + at, v, dim, past);
+      if (to >= 0) store_result(rows + to * dim + at, v, at, dim, past);
     }
   }
   const int64_t live = s_start[out.experts];
@@ -172,7 +173,7 @@ __device__ __forceinline__ float weight_of(const W* weights, int64_t item) {
 template <typename T, typename W, int KU>
 __global__ void __launch_bounds__(kThreads)
 combine_kernel(const T* __restrict__ y, int64_t stride, int64_t dim, Divider chunks, const int32_t* __restrict__ place,
-               int64_t total, int choices, int64_t n, const W* __restrict__ weights, T* __restrict__ out, bool past) {
+               int64_t total, int choices, int64_t n, const W* __restrict__ weights, T* __restrict__ out, Past past) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
   if (first + threadIdx.x >= total) return;
   const RowRange range(chunks, first);
@@ -196,7 +197,7 @@ combine_kernel(const T* __restrict__ y, int64_t stride, int64_t dim, Divider chu
     for (int u = 0; u < KU; ++u)
       if (there[u]) sum += widen<T>(v[u]) * w[u];
   }
-  store_result(out + token * dim + at, narrow<T>(sum), dim, past);
+  store_result(out + token * dim + at, narrow<T>(sum), at, dim, past);
 }
 
 // ---------------------------------------------------- gradient of the combine ----
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kThreads)
 combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ y, int64_t y_stride,
                     int64_t dim, Divider chunks, const int32_t* __restrict__ place, int64_t tokens, int choices,
                     int64_t n, const int64_t* __restrict__ live, const W* __restrict__ weights, T* __restrict__ dy,
-                    W* __restrict__ dweights, bool past) {
+                    W* __restrict__ dweights, Past past) {
   constexpr int kLanes = G * WAVES;               // of a token
   constexpr int kTokens = kThreads / kLanes;      // of a workgroup
   __shared__ float s_dots[WAVES > 1 ? WAVES * KU : 1];
@@ -248,7 +249,7 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
           for (int i = 0; i < Chunk<T>::kVec; ++i)
             if (i >= overlap) dot[u] = __fmaf_rn(d[i], b[i], dot[u]);
         }
-        if (dy && from[u] >= 0) store_result(dy + from[u] * dim + at, narrow<T>(d * w[u]), dim, past);
+        if (dy && from[u] >= 0) store_result(dy + from[u] * dim + at, narrow<T>(d * w[u]), at, dim, past);
       }
     }
     if (!dweights) continue;
@@ -328,7 +329,7 @@ int launch_gather(const T* x, int64_t stride, int64_t dim, const int32_t* place,
   auto* kernel = many ? gather_kernel<T, kMany> : gather_kernel<T, 1>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, x, stride, dim,
                      Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices), tokens * choices, live,
-                     rows, results_past(rows, dim));
+                     rows, results_past(rows, dim, false));
   return check_launch(what);
 }
 
@@ -342,7 +343,8 @@ int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t 
   with_choices(choices < 4 ? choices : 4, [&](auto ku) {
     hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st, dout,
                        dout_stride, y, y_stride, dim, Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place, tokens,
-                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights, results_past(dy, dim));
+                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights,
+                       results_past(dy, dim, false));
   });
   return check_launch("expert_combine_grad");
 }
@@ -454,7 +456,7 @@ int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, c
                          static_cast<hipStream_t>(stream), static_cast<const IdT*>(experts), static_cast<const T*>(x),
                          x_stride, dim, Divider(static_cast<uint32_t>(chunks)), total, static_cast<int>(choices),
                          static_cast<uint32_t>(n), out, static_cast<T*>(rows),
-                         results_past(static_cast<const T*>(rows), dim));
+                         results_past(static_cast<const T*>(rows), dim, false));
       return check_launch("expert_dispatch");
     });
   });
@@ -480,7 +482,7 @@ int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, co
                            dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(y), y_stride, dim,
                            Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices),
                            tokens * choices, static_cast<const W*>(weights), static_cast<T*>(out),
-                           results_past(static_cast<const T*>(out), dim));
+                           results_past(static_cast<const T*>(out), dim, true));
       });
       return check_launch("expert_combine");
     });

@@ -67,20 +67,36 @@ __device__ __forceinline__ Values<T> load_past(const T* p) {
   typedef Values<T> Loose __attribute__((aligned(sizeof(T))));
   return __builtin_nontemporal_load(reinterpret_cast<const Loose*>(p));
 }
-// Results go past the caches where rows fill whole lines (results_past), and leave the caches to what is read.
-// 600 k rows of 256 B looked up in 627 MB: 51 us with plain stores, 38 so (with plain stores and loads past the
-// caches 58), and with a kernel behind that reads the result 75 and 72; 75 k rows 6.5 and 5.5, with that kernel 11.0
-// and 10.8.  Lines written in two parts go to memory twice: 30 k rows of 2002 B sent to experts 14 us plain, 20 so, and
-// 162 k rows of 1286 B looked up 44 and 52 with only the lines inside a row past the caches.
+// Whether results go past the caches, and leave those to what is read: as they come, where rows fill whole lines; in
+// the lines that lie inside a row, where no chunk crosses a line; or not at all.  600 k rows of 256 B looked up in
+// 627 MB: 51 us with plain stores, 38 so (with plain stores and loads past the caches 58), and with a kernel behind
+// that reads the result 75 and 72; 75 k rows 6.5 and 5.5, with that kernel 11.0 and 10.8.  94 k rows of 400 B sent to
+// 4 experts each, and the gradient: 107 plain, 88 with the inner lines so.  Lines written in two parts go to memory
+// twice: 30 k rows of 2002 B sent to experts 14 us plain, 20 so; 162 k rows of 1286 B looked up 44 and 52.
+enum class Past { kNo, kInside, kAll };
+
+// p: the chunk `at` values into a row of dim values
 template <typename T>
-__device__ __forceinline__ void store_result(T* p, Values<T> v, int64_t dim, bool past) {
-  if (past) store_past(p, v);
+__device__ __forceinline__ void store_result(T* p, Values<T> v, int64_t at, int64_t dim, Past past) {
+  bool whole = past == Past::kAll;
+  if (past == Past::kInside) {
+    constexpr int64_t kLine = 128;
+    constexpr int64_t kSize = static_cast<int64_t>(sizeof(T));
+    const int64_t in_line = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) % kLine);
+    whole = in_line <= at * kSize && kLine - in_line <= (dim - at) * kSize;
+  }
+  if (whole) store_past(p, v);
   else store_chunk(p, v, dim);
 }
+// contiguous: the rows lie side by side and are written in order
 template <typename T>
-bool results_past(const T* rows, int64_t dim) {
+Past results_past(const T* rows, int64_t dim, bool contiguous) {
   constexpr int64_t kLine = 128;
-  return dim > 0 && dim * static_cast<int64_t>(sizeof(T)) % kLine == 0 && reinterpret_cast<uintptr_t>(rows) % kLine == 0;
+  const int64_t bytes = dim * static_cast<int64_t>(sizeof(T));
+  const uintptr_t base = reinterpret_cast<uintptr_t>(rows);
+  if (dim <= 0 || bytes % 16 != 0 || base % 16 != 0) return Past::kNo;
+  if (base % kLine == 0 && (contiguous || bytes % kLine == 0)) return Past::kAll;
+  return bytes >= 2 * kLine ? Past::kInside : Past::kNo;
 }
 template <typename T>
 __device__ __forceinline__ Wide<T> widen(Values<T> v) {
