@@ -129,6 +129,8 @@ __device__ __forceinline__ void rank_tile(const uint32_t (&digit)[kItems], uint3
     const uint32_t earlier = t.count[wave][digit[r]];  // (LDS operations of a wave keep their order)
     rank[r] = earlier + in_round;
     if (in && in_round == 0) t.count[wave][digit[r]] = static_cast<uint16_t>(earlier + __popc(lo) + __popc(hi));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (keeps the next round's reads behind this one's writes)
+    __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
   uint32_t sum = 0;
@@ -198,7 +200,8 @@ count_kernel(Src src, int64_t n, int pass, int64_t tiles, uint32_t* __restrict__
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kItems; ++r)
-    if (base + r * THREADS + threadIdx.x < n) atomicAdd(&s_hist[threadIdx.x % kCopies<BITS>][digit_of<BITS>(w[r], pass)], 1u);
+    if (base + r * THREADS + threadIdx.x < n)
+      atomicAdd(&s_hist[threadIdx.x % kCopies<BITS>][digit_of<BITS>(w[r], pass)], 1u);
   __syncthreads();
   if (threadIdx.x < kDigits) {
     uint32_t all = 0;
