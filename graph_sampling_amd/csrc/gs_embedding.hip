@@ -457,7 +457,8 @@ struct Numbers {
 
 template <typename IdT, typename Beside>
 void sort_ids(const IdT* ids, int64_t n, uint32_t num_rows, const GradSpace& s, Beside beside, hipStream_t st) {
-  key_sort::sort<false>(key_sort::IdWords<IdT>{ids, num_rows}, n, num_rows, s.sort, key_sort::WordsOut{s.sorted}, st, beside);
+  const key_sort::IdWords<IdT> src{ids, num_rows};
+  key_sort::sort<false>(src, n, num_rows, s.sort, key_sort::WordsOut{s.sorted}, st, beside);
 }
 
 int check_rows(const char* what, const void* rows, int64_t stride, int64_t dim, int type, int64_t n, int64_t num_rows) {
@@ -480,10 +481,8 @@ int check_ids(const char* what, const void* ids, int id_bytes, int64_t n) {
 }
 // whether every launch of the sums has a grid that can be launched
 int check_plan(const char* what, const SumPlan& p) {
-  if (p.parts[0] * p.slices < (int64_t(1) << 31)) return GS_OK;
-  set_error_text("%s: %lld rows of %lld chunks are more than one launch takes", what, static_cast<long long>(p.n),
-                 static_cast<long long>(p.chunks));
-  return GS_ERR_UNSUPPORTED;
+  GS_RETURN_IF_ERROR(check_grid(what, p.parts[0] * p.slices, groups_in(kSumMost, p.group) * p.group));
+  return p.levels > 1 ? check_grid(what, p.parts[1] * p.slices, groups_in(kJoinMost, p.group) * p.group) : int(GS_OK);
 }
 
 }  // namespace
@@ -508,11 +507,7 @@ int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride,
     constexpr int kMany = 4;
     const bool many = total >= int64_t(256) * kThreads * kMany;
     const int64_t blocks = (total + kThreads * (many ? kMany : 1) - 1) / (kThreads * (many ? kMany : 1));
-    if (blocks >= (int64_t(1) << 31)) {
-      set_error_text("gs_embedding_lookup: %lld rows of %lld values are more than one launch takes",
-                     static_cast<long long>(n), static_cast<long long>(dim));
-      return static_cast<int>(GS_ERR_UNSUPPORTED);
-    }
+    GS_RETURN_IF_ERROR(check_grid("gs_embedding_lookup", blocks, kThreads));
     const Divider by(static_cast<uint32_t>(chunks));
     return with_id_type(id_bytes, [&](auto id) {
       using IdT = decltype(id);

@@ -296,11 +296,6 @@ int check_values(const char* what, int type, int64_t dim, int64_t stride) {
   GS_REQUIRE(stride >= 0, "%s: negative stride", what);
   return GS_OK;
 }
-int check_grid(const char* what, int64_t blocks) {
-  if (blocks < (int64_t(1) << 31)) return GS_OK;
-  set_error_text("%s: more rows and values than one launch takes", what);
-  return GS_ERR_UNSUPPORTED;
-}
 
 // weights are fp32 or of the rows' type
 template <typename T, typename F>
@@ -325,7 +320,7 @@ int launch_gather(const T* x, int64_t stride, int64_t dim, const int32_t* place,
   constexpr int kMany = 4;
   const bool many = total >= int64_t(256) * 4 * kThreads * kMany;
   const int64_t blocks = (total + kThreads * (many ? kMany : 1) - 1) / (kThreads * (many ? kMany : 1));
-  GS_RETURN_IF_ERROR(check_grid(what, blocks));
+  GS_RETURN_IF_ERROR(check_grid(what, blocks, kThreads));
   auto* kernel = many ? gather_kernel<T, kMany> : gather_kernel<T, 1>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, x, stride, dim,
                      Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices), tokens * choices, live,
@@ -338,23 +333,31 @@ int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t 
                         const int32_t* place, int64_t tokens, int64_t choices, const int64_t* live, const W* weights,
                         T* dy, W* dweights, hipStream_t st) {
   constexpr int kTokens = kThreads / (G * WAVES);
-  const dim3 grid(static_cast<unsigned>((tokens + kTokens - 1) / kTokens));
+  constexpr int64_t kMost = most_blocks(kThreads) * kTokens;  // tokens a launch
+  const auto past = results_past(dy, dim, false);
   // (rows of eight choices at once take registers that waves need: 50 k tokens, 4 of 8 choices, 139 us; of 4 101)
-  with_choices(choices < 4 ? choices : 4, [&](auto ku) {
-    hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st, dout,
-                       dout_stride, y, y_stride, dim, Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place, tokens,
-                       static_cast<int>(choices), tokens * choices, live, weights, dy, dweights,
-                       results_past(dy, dim, false));
-  });
-  return check_launch("expert_combine_grad");
+  for (int64_t t = 0; t < tokens; t += kMost) {
+    const int64_t here = tokens - t < kMost ? tokens - t : kMost, item = t * choices;
+    const dim3 grid(static_cast<unsigned>((here + kTokens - 1) / kTokens));
+    with_choices(choices < 4 ? choices : 4, [&](auto ku) {
+      hipLaunchKernelGGL((combine_grad_kernel<T, W, G, WAVES, decltype(ku)::value>), grid, dim3(kThreads), 0, st,
+                         dout + t * dout_stride, dout_stride, y, y_stride, dim,
+                         Divider(static_cast<uint32_t>(chunks_of<T>(dim))), place + item, here,
+                         static_cast<int>(choices), tokens * choices, live, weights ? weights + item : nullptr, dy,
+                         dweights ? dweights + item : nullptr, past);
+    });
+    GS_RETURN_IF_ERROR(check_launch("expert_combine_grad"));
+  }
+  return GS_OK;
 }
 
 template <typename IdT>
 int sort_items(const IdT* experts, int64_t n, int64_t num_experts, const OrderOut& out, void* workspace,
                size_t workspace_bytes, hipStream_t st) {
   if (n == 0) {
-    hipLaunchKernelGGL(no_items_kernel, dim3(blocks_for(num_experts + 1 < (1 << 20) ? num_experts + 1 : (1 << 20), kThreads)),
-                       dim3(kThreads), 0, st, out.offsets, num_experts + 1);
+    const int64_t offsets = num_experts + 1;
+    hipLaunchKernelGGL(no_items_kernel, dim3(blocks_for(offsets < (1 << 20) ? offsets : (1 << 20), kThreads)),
+                       dim3(kThreads), 0, st, out.offsets, offsets);
     return check_launch("expert_sort");
   }
   const uint32_t num = static_cast<uint32_t>(num_experts);
@@ -447,7 +450,7 @@ int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, c
     return with_id_type(id_bytes, [&](auto id) {
       using IdT = decltype(id);
       const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks, blocks = (total + kThreads - 1) / kThreads;
-      GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks));
+      GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks, kThreads));
       const int bits = key_sort::Digits(static_cast<uint32_t>(num_experts), true).bits;
       auto* kernel = bits == 4   ? sort_gather_kernel<T, IdT, 4>
                      : bits == 7 ? sort_gather_kernel<T, IdT, 7>
@@ -474,17 +477,22 @@ int gs_expert_combine(const void* y, int64_t y_stride, int64_t dim, int type, co
     using T = decltype(zero);
     return with_weight_type<T>(type, weights ? weight_type : GS_F32, "gs_expert_combine", [&](auto wzero) {
       using W = decltype(wzero);
-      const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks;
-      const int64_t blocks = (total + kThreads - 1) / kThreads;
-      GS_RETURN_IF_ERROR(check_grid("gs_expert_combine", blocks));
-      with_choices(choices, [&](auto ku) {
-        hipLaunchKernelGGL((combine_kernel<T, W, decltype(ku)::value>), dim3(static_cast<unsigned>(blocks)),
-                           dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(y), y_stride, dim,
-                           Divider(static_cast<uint32_t>(chunks)), place, total, static_cast<int>(choices),
-                           tokens * choices, static_cast<const W*>(weights), static_cast<T*>(out),
-                           results_past(static_cast<const T*>(out), dim, true));
-      });
-      return check_launch("expert_combine");
+      const int64_t chunks = chunks_of<T>(dim), most = most_blocks(kThreads) * kThreads / chunks;  // tokens a launch
+      const auto past = results_past(static_cast<const T*>(out), dim, true);
+      for (int64_t t = 0; t < tokens; t += most) {
+        const int64_t here = tokens - t < most ? tokens - t : most, total = here * chunks, item = t * choices;
+        const dim3 grid(static_cast<unsigned>((total + kThreads - 1) / kThreads));
+        with_choices(choices, [&](auto ku) {
+          hipLaunchKernelGGL((combine_kernel<T, W, decltype(ku)::value>), grid, dim3(kThreads), 0,
+                             static_cast<hipStream_t>(stream), static_cast<const T*>(y), y_stride, dim,
+                             Divider(static_cast<uint32_t>(chunks)), place ? place + item : nullptr, total,
+                             static_cast<int>(choices), tokens * choices,
+                             weights ? static_cast<const W*>(weights) + item : nullptr,
+                             static_cast<T*>(out) + t * dim, past);
+        });
+        GS_RETURN_IF_ERROR(check_launch("expert_combine"));
+      }
+      return static_cast<int>(GS_OK);
     });
   });
 }

@@ -163,6 +163,13 @@ template <typename F>
 int with_id_type(int id_bytes, F&& f) {
   return id_bytes == 4 ? f(int32_t(0)) : f(int64_t(0));
 }
+// Workgroups of `threads` that one launch takes: it counts its threads in 32 bits.
+constexpr int64_t most_blocks(int threads) { return ((int64_t(1) << 32) - 1) / threads; }
+inline int check_grid(const char* what, int64_t blocks, int threads) {
+  if (blocks <= most_blocks(threads)) return GS_OK;
+  set_error_text("%s: more rows and values than one launch takes", what);
+  return GS_ERR_UNSUPPORTED;
+}
 inline int value_bytes(int type) { return type == GS_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) == 0;

@@ -2126,22 +2126,27 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& 
                                                            const torch::Tensor& place, const torch::Tensor& offsets,
                                                            const torch::optional<torch::Tensor>& weights,
                                                            bool of_rows, bool of_weights) {
-  const Rows d(dout, "gradient"), r(y, "rows");
+  const Rows d(dout, "gradient");
   const Places p(place, dout.device());
-  TORCH_CHECK(y.device() == dout.device(), "rows and gradient are on different devices");
-  TORCH_CHECK(d.type == r.type, "rows and gradient differ in type");
-  TORCH_CHECK(d.t.size(0) == p.tokens && r.t.size(0) == place.numel() && d.t.size(1) == r.t.size(1),
-              "a gradient of ", d.t.sizes(), " and rows of ", r.t.sizes(), " for places of ", place.sizes());
+  TORCH_CHECK(d.t.size(0) == p.tokens, "a gradient of ", d.t.sizes(), " for places of ", place.sizes());
   const Weights w(weights, p, dout);
   TORCH_CHECK(!of_weights || w.t.defined(), "no weights to take the gradient of");
+  torch::optional<Rows> r;
+  if (y.defined() || of_weights) {
+    r.emplace(y, "rows");
+    TORCH_CHECK(y.device() == dout.device(), "rows and gradient are on different devices");
+    TORCH_CHECK(d.type == r->type, "rows and gradient differ in type");
+    TORCH_CHECK(r->t.size(0) == place.numel() && d.t.size(1) == r->t.size(1), "a gradient of ", d.t.sizes(),
+                " and rows of ", r->t.sizes(), " for places of ", place.sizes());
+  }
   const int64_t* live = LiveRows(offsets, dout.device());
   c10::hip::HIPGuard on(dout.device().index());
   torch::Tensor dy, dw;
   if (of_rows) dy = torch::empty({place.numel(), d.t.size(1)}, Like(dout));
   if (of_weights) dw = torch::empty(place.sizes(), Like(w.t));
-  Check(gs_expert_combine_grad(d.t.data_ptr(), d.stride, r.t.data_ptr(), r.stride, d.t.size(1), d.type, p.data(),
-                               p.tokens, p.choices, live, w.data(), w.type, of_rows ? dy.data_ptr() : nullptr,
-                               of_weights ? dw.data_ptr() : nullptr, Stream(dout)),
+  Check(gs_expert_combine_grad(d.t.data_ptr(), d.stride, r ? r->t.data_ptr() : nullptr, r ? r->stride : 0, d.t.size(1),
+                               d.type, p.data(), p.tokens, p.choices, live, w.data(), w.type,
+                               of_rows ? dy.data_ptr() : nullptr, of_weights ? dw.data_ptr() : nullptr, Stream(dout)),
         "gs_expert_combine_grad");
   return {dy, dw};
 }

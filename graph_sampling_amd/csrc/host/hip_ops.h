@@ -380,7 +380,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> ExpertDis
                                                                                       int64_t num_experts);
 torch::Tensor ExpertCombine(const torch::Tensor& y, const torch::Tensor& place,
                             const torch::optional<torch::Tensor>& weights);
-// {gradient of y, gradient of weights}, undefined where not wanted
+// {gradient of y, gradient of weights}, undefined where not wanted (y may be, unless the second one is)
 std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& dout, const torch::Tensor& y,
                                                            const torch::Tensor& place,
                                                            const torch::Tensor& offsets,

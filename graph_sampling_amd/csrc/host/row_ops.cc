@@ -101,9 +101,12 @@ struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
 struct CombineFunction : public torch::autograd::Function<CombineFunction> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& y, const torch::Tensor& place,
                                const torch::Tensor& offsets, const torch::optional<torch::Tensor>& weights) {
-    ctx->save_for_backward({y, place, offsets, weights.has_value() ? weights.value() : torch::Tensor()});
-    ctx->saved_data["weights"] = weights.has_value() && weights.value().requires_grad();
-    ctx->saved_data["rows"] = y.requires_grad();
+    const bool of_rows = y.requires_grad(), of_weights = weights.has_value() && weights.value().requires_grad();
+    // (y, the larger, is kept for the weights' gradient only)
+    ctx->save_for_backward({of_weights ? y : torch::Tensor(), place, offsets,
+                            weights.has_value() ? weights.value() : torch::Tensor()});
+    ctx->saved_data["weights"] = of_weights;
+    ctx->saved_data["rows"] = of_rows;
     return hip::ExpertCombine(y, place, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {

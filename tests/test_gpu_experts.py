@@ -235,6 +235,65 @@ def test_offsets_beyond_32_bits(dev):
 
 
 @gpu
+def test_more_lanes_than_one_launch_takes(dev):
+    """Sums and gradients of more than 2^32 lanes go in several launches: tokens at both ends and beside the cut."""
+    if torch.cuda.mem_get_info(dev)[0] < 120 << 30:
+        pytest.skip("needs about 70 GB of free device memory")
+    def near(n, cut):
+        return torch.cat([torch.arange(1000, device=dev), torch.arange(cut - 1000, cut + 1000, device=dev),
+                          torch.arange(n - 1000, n, device=dev)])
+
+    # rows of 17 fp16 values are three lanes each, every token's place the same row
+    cut = (2 ** 32 - 1) // 256 * 256 // 3
+    tokens = cut + 300_000
+    row = torch.arange(1, 18, device=dev).half()
+    weights = (torch.arange(tokens, device=dev, dtype=torch.int32) % 64).half().view(tokens, 1)
+    place = torch.zeros(tokens, 1, dtype=torch.int32, device=dev)
+    at = gs.ops.ExpertOrder(place.view(-1), place, torch.tensor([0, tokens], device=dev))
+    out = gs.ops.expert_combine(row.expand(tokens, 17), at, weights)
+    t = near(tokens, cut)
+    assert torch.equal(out[t], weights[t] * row)  # (whole numbers up to 63 * 17: exact)
+    del out, weights, place, at
+    # rows of one value have four lanes in the gradient
+    cut = (2 ** 32 - 1) // 256 * 64
+    tokens = cut + 5000
+    weights = (torch.arange(tokens, device=dev, dtype=torch.int32) % 64).half().view(tokens, 1)
+    dout = (torch.arange(tokens, device=dev, dtype=torch.int32) % 31).half().view(tokens, 1)
+    place = torch.arange(tokens - 1, -1, -1, device=dev, dtype=torch.int32).view(tokens, 1)
+    offsets = torch.tensor([0, tokens], device=dev)
+    dy, dw = torch.ops.gs_ops._CAPI_ExpertCombineGrad(dout, weights, place.view(-1), place, offsets, weights)
+    t = near(tokens, cut)
+    back = tokens - 1 - t
+    assert torch.equal(dy[back], weights[t] * dout[t]) and torch.equal(dw[t], dout[t] * weights[back])
+    assert bool((dy.view(-1).flip(0) == (weights * dout).view(-1)).all())
+
+
+@gpu
+def test_rows_are_kept_for_the_gradient_of_weights_only(dev):
+    """Rows that nobody's gradient needs may be overwritten after they were added up."""
+    e = torch.randint(-1, 5, (50, 3), device=dev)
+    x = rows(50, 24, torch.float32, dev, 3).requires_grad_(True)
+    sent, order = gs.ops.expert_dispatch(x, e, 5)
+    w = rows(50, 3, torch.float32, dev, 4)
+    dout = rows(50, 24, torch.float32, dev, 5)
+    want, = torch.autograd.grad(gs.ops.expert_combine(sent, order, w), x, dout, retain_graph=True)
+    for weights in (None, w):
+        y = sent * 1.0
+        out = gs.ops.expert_combine(y, order, weights)
+        y.detach().zero_()
+        got, = torch.autograd.grad(out, x, dout, retain_graph=True)
+        if weights is not None:
+            assert torch.equal(got, want)
+    kept = w.clone().requires_grad_(True)
+    y = sent * 1.0
+    out = gs.ops.expert_combine(y, order, kept)
+    with torch.no_grad():
+        y.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, (x, kept), dout)
+
+
+@gpu
 def test_what_has_no_place_does_not_matter(dev):
     """NaN and infinities in rows and weights of choices that name no expert, and behind the last row."""
     e = np.array([[0, -1], [-1, -1], [5, 1], [1, 0]])
