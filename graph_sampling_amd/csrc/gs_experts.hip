@@ -62,12 +62,12 @@ __global__ void __launch_bounds__(kThreads) no_items_kernel(int64_t* __restrict_
 
 // ------------------------------------------------------------------ gather ----
 // Zeros in the rows from `from` to n, a share of them by every workgroup.
-template <typename T>
+template <int THREADS = kThreads, typename T>
 __device__ __forceinline__ void zero_rows_behind(int64_t from, int64_t n, int64_t dim, const Divider& chunks,
                                                  T* __restrict__ rows, Past past) {
   if (from >= n || from < 0) return;
-  const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
+  const int64_t total = (n - from) * chunks.d, stride = static_cast<int64_t>(gridDim.x) * THREADS;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; i < total; i += stride) {
     const int64_t row = i / chunks.d;
     const int64_t at = chunk_start<T>(dim, i - row * chunks.d);
     store_result(rows + (from + row) * dim + at, Values<T>{}, at, dim, past);
@@ -105,19 +105,20 @@ gather_kernel(const T* __restrict__ x, int64_t stride, int64_t dim, Divider chun
 
 // The same with the sort, for a few items: every workgroup ranks all of them in LDS, which takes less than a launch,
 // and goes on with its chunks; the first one writes the order down.  16 items of 64 experts: 4 us where two launches
-// take 6 and the space between them.
+// take 6 and the space between them; 8 of 256 experts, the whole call: 8.9 us for 16.5.
 constexpr int64_t kDispatchItems = kThreads * key_sort::kItems;
+constexpr int dispatch_threads(int bits) { return bits == 9 ? 512 : kThreads; }  // (a thread a digit)
 
 template <typename T, typename IdT, int BITS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(dispatch_threads(BITS))
 sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int64_t stride, int64_t dim, Divider chunks,
                    int64_t total, int choices, uint32_t n, OrderOut out, T* __restrict__ rows, Past past) {
-  constexpr int kDigits = 1 << BITS;
-  __shared__ key_sort::TileTables<BITS, kThreads> s_tables;
+  constexpr int kDigits = 1 << BITS, kThreadsHere = dispatch_threads(BITS);
+  __shared__ key_sort::TileTables<BITS, kThreadsHere> s_tables;
   __shared__ uint32_t s_start[kDigits];
   __shared__ int32_t s_place[kDispatchItems];
   // the token's chunk is on its way meanwhile
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreadsHere;
   const bool in = first + threadIdx.x < total;
   const RowRange range(chunks, first);
   uint32_t c;
@@ -133,7 +134,7 @@ sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int
     w[r] = src(i < n ? i : n - 1);
     d[r] = key_sort::digit_of<BITS>(w[r], 0);
   }
-  key_sort::rank_tile<BITS, kThreads>(d, n, s_tables, rank, &here);
+  key_sort::rank_tile<BITS, kThreadsHere>(d, n, s_tables, rank, &here);
   uint32_t start = here, none = 0;
   key_sort::scan_digits(start, none, s_tables);
   if (threadIdx.x < kDigits) {
@@ -160,7 +161,7 @@ sort_gather_kernel(const IdT* __restrict__ experts, const T* __restrict__ x, int
     }
   }
   const int64_t live = s_start[out.experts];
-  if (live < n) zero_rows_behind(live, static_cast<int64_t>(n), dim, chunks, rows, past);
+  if (live < n) zero_rows_behind<kThreadsHere>(live, static_cast<int64_t>(n), dim, chunks, rows, past);
 }
 
 // ----------------------------------------------------------------- combine ----
@@ -435,7 +436,7 @@ int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, c
   GS_RETURN_IF_ERROR(check_shape("gs_expert_dispatch", tokens, choices, num_experts));
   GS_RETURN_IF_ERROR(check_values("gs_expert_dispatch", type, dim, x_stride));
   const int64_t n = tokens * choices;
-  if (n == 0 || n > kDispatchItems || num_experts >= 256 || dim == 0) {
+  if (n == 0 || n > kDispatchItems || num_experts >= 512 || dim == 0) {
     GS_RETURN_IF_ERROR(gs_expert_sort(experts, id_bytes, n, num_experts, order, place, offsets, workspace,
                                       workspace_bytes, stream));
     return gs_expert_gather(x, x_stride, dim, type, place, tokens, choices, offsets + num_experts, rows, stream);
@@ -449,13 +450,14 @@ int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, c
     using T = decltype(zero);
     return with_id_type(id_bytes, [&](auto id) {
       using IdT = decltype(id);
-      const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks, blocks = (total + kThreads - 1) / kThreads;
-      GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks, kThreads));
-      const int bits = key_sort::Digits(static_cast<uint32_t>(num_experts), true).bits;
+      const int bits = key_sort::Digits(static_cast<uint32_t>(num_experts), true).bits, threads = dispatch_threads(bits);
+      const int64_t chunks = chunks_of<T>(dim), total = tokens * chunks, blocks = (total + threads - 1) / threads;
+      GS_RETURN_IF_ERROR(check_grid("gs_expert_dispatch", blocks, threads));
       auto* kernel = bits == 4   ? sort_gather_kernel<T, IdT, 4>
                      : bits == 7 ? sort_gather_kernel<T, IdT, 7>
-                                 : sort_gather_kernel<T, IdT, 8>;
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                     : bits == 8 ? sort_gather_kernel<T, IdT, 8>
+                                 : sort_gather_kernel<T, IdT, 9>;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0,
                          static_cast<hipStream_t>(stream), static_cast<const IdT*>(experts), static_cast<const T*>(x),
                          x_stride, dim, Divider(static_cast<uint32_t>(chunks)), total, static_cast<int>(choices),
                          static_cast<uint32_t>(n), out, static_cast<T*>(rows),

@@ -161,6 +161,20 @@ def test_sorts_of_every_size_and_number_of_experts(dev, num):
 
 
 @gpu
+@pytest.mark.parametrize("num", [1, 15, 16, 127, 128, 255, 256, 257, 511, 512])
+def test_few_items_of_any_number_of_experts(dev, num):
+    """Both sides of every number of experts at which the one launch for few items changes its digits, or ends."""
+    for tokens, choices, dim in ((1, 1, 3), (1, 8, 4096), (9, 7, 1000), (128, 8, 40), (1024, 1, 17), (1025, 1, 17)):
+        for kind in ("outside", "skewed", "none"):
+            e = experts_of(kind, tokens, choices, num, tokens + num)
+            x = rows(tokens, dim, torch.bfloat16, dev, num)
+            got, order = gs.ops.expert_dispatch(x, torch.from_numpy(e).to(dev), num)
+            items, _, offsets = check_order(order, e, num)
+            live = int(offsets[-1])
+            assert torch.equal(got[:live], x[torch.from_numpy(items[:live] // choices).to(dev)]) and not got[live:].any()
+
+
+@gpu
 def test_one_choice_each_without_a_second_dimension(dev):
     """Node types: experts, places and weights of shape [tokens]."""
     e = experts_of("skewed", 777, 1, 6, 6)[:, 0]
