@@ -2008,6 +2008,7 @@ torch::Tensor EmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& ids,
   const auto flat = FlatIds(ids, grad.device(), "ids");
   TORCH_CHECK(flat.numel() == g.t.size(0), "a gradient of ", g.t.size(0), " rows for ", flat.numel(), " ids");
   TORCH_CHECK(num_rows >= 0, "num_rows must be non-negative");
+  TORCH_CHECK(num_rows < (int64_t(1) << 32) - 1, "at most 2^32 - 2 rows are taken, got ", num_rows);
   c10::hip::HIPGuard on(grad.device().index());
   const int64_t n = flat.numel(), dim = g.t.size(1);
   auto out = torch::empty({num_rows, dim}, Like(grad));
@@ -2024,6 +2025,7 @@ std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(const torch::Tensor
   const auto flat = FlatIds(ids, grad.device(), "ids");
   TORCH_CHECK(flat.numel() == g.t.size(0), "a gradient of ", g.t.size(0), " rows for ", flat.numel(), " ids");
   TORCH_CHECK(num_rows >= 0, "num_rows must be non-negative");
+  TORCH_CHECK(num_rows < (int64_t(1) << 32) - 1, "at most 2^32 - 2 rows are taken, got ", num_rows);
   TORCH_CHECK(!Capturing(grad), "a sparse gradient waits for the number of rows it holds: it cannot be recorded into "
               "a graph (a dense one can)");
   c10::hip::HIPGuard on(grad.device().index());
@@ -2056,6 +2058,7 @@ struct SortedExperts {
     TORCH_CHECK(experts.dim() == 1 || experts.dim() == 2, "experts must be [tokens] or [tokens, choices], got ",
                 experts.sizes());
     TORCH_CHECK(num_experts >= 0, "num_experts must be non-negative");
+    TORCH_CHECK(num_experts < (int64_t(1) << 31), "at most 2^31 - 1 experts are taken, got ", num_experts);
     flat = FlatIds(experts, device, "experts");
     const auto i32 = torch::dtype(torch::kInt32).device(device);
     order = torch::empty({flat.numel()}, i32);

@@ -515,6 +515,22 @@ def test_recording_is_refused_where_it_would_end_the_process(dev):
 
 
 @gpu
+def test_sizes_beyond_the_limits_are_refused_before_anything_is_allocated(dev):
+    e = torch.zeros(4, dtype=torch.int32, device=dev)
+    x = torch.zeros(4, 3, device=dev)
+    held = torch.cuda.memory_allocated(dev)
+    for num in (1 << 31, 1 << 40, (1 << 63) - 1):
+        with pytest.raises(RuntimeError, match="experts are taken"):
+            gs.ops.expert_sort(e, num)
+        with pytest.raises(RuntimeError, match="experts are taken"):
+            gs.ops.expert_dispatch(x, e, num)
+        for entry in (torch.ops.gs_ops._CAPI_EmbeddingGrad, torch.ops.gs_ops._CAPI_EmbeddingSparseGrad):
+            with pytest.raises(RuntimeError, match="rows are taken"):
+                entry(x, e, max(num, 1 << 33), 1.0)
+    assert torch.cuda.memory_allocated(dev) == held
+
+
+@gpu
 def test_refusals(dev):
     x, e = rows(5, 4, torch.float32, dev, 32), torch.zeros(5, 2, dtype=torch.int64, device=dev)
     for bad, match in (((x.double(), e, 3), "float32, float16 or bfloat16"), ((x, e.float(), 3), "int64"),
