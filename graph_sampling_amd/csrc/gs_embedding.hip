@@ -346,6 +346,20 @@ join_runs_kernel(const Entry* __restrict__ in, int64_t m, const float* __restric
 // ------------------------------------------------------------------- plans ----
 // The workgroups of every launch: a function of the sizes alone.
 constexpr int kMaxLevels = 8;
+// n below 2^31 (short tiles are for lists of fewer than 2^23 lanes, which need no more levels than the longest one)
+constexpr int most_levels(int lanes) {
+  const int64_t joins = groups_in(kJoinMost, lanes);
+  int64_t p = (int64_t(1) << 31) / (kMostSize * groups_in(kSumMost, lanes));
+  int levels = 1;
+  for (; p > 1; p = (p + joins - 1) / joins) ++levels;
+  return levels;
+}
+static_assert(most_levels(1) <= kMaxLevels && most_levels(16) <= kMaxLevels && most_levels(32) <= kMaxLevels &&
+              most_levels(kWave) <= kMaxLevels, "launches of the longest list");
+// Whether a call takes these sizes: what it does not take has no plan.
+bool has_plan(int64_t n, int64_t dim, int type) {
+  return n > 0 && n < (int64_t(1) << 31) && dim < (int64_t(1) << 24) && (type == GS_F32 || type == GS_F16 || type == GS_BF16);
+}
 
 struct SumPlan {
   int64_t n, chunks;
@@ -521,7 +535,7 @@ int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride,
 }
 
 size_t gs_embedding_grad_workspace_bytes(int64_t n, int64_t dim, int type) {
-  if (n <= 0 || dim <= 0) return 256;
+  if (!has_plan(n, dim, type) || dim <= 0) return 256;  // (the call needs none, or refuses)
   return grad_bytes(SumPlan(n, dim, type), type, false);
 }
 
@@ -564,7 +578,7 @@ int gs_embedding_grad(const void* grad, int64_t grad_stride, int64_t dim, int ty
 }
 
 size_t gs_embedding_sparse_grad_workspace_bytes(int64_t n, int64_t dim, int type) {
-  if (n <= 0) return 256;
+  if (!has_plan(n, dim, type)) return 256;
   return grad_bytes(SumPlan(n, dim > 0 ? dim : 1, type), type, true);
 }
 

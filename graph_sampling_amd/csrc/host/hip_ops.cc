@@ -1914,6 +1914,7 @@ struct Rows {
     TORCH_CHECK(t.layout() == torch::kStrided, name, " must be a dense tensor");
     TORCH_CHECK(t.dim() == 2, name, " must have two dimensions, got ", t.dim());
     type = ValueType(t, name);
+    TORCH_CHECK(t.size(1) < (int64_t(1) << 24), name, ": rows of at most 2^24 - 1 values are taken, got ", t.size(1));
     if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
     if (t.is_neg()) t = t.resolve_neg();
     stride = t.size(0) > 1 ? t.stride(0) : t.size(1);
@@ -1924,6 +1925,7 @@ torch::Tensor FlatIds(const torch::Tensor& ids, const torch::Device& device, con
   TORCH_CHECK(ids.defined(), name, " is undefined");
   TORCH_CHECK(ids.is_cuda(), "Not implemented warning: ", name, " must be a GPU tensor");
   TORCH_CHECK(ids.device() == device, name, " must be on ", device, ", got ", ids.device());
+  TORCH_CHECK(ids.numel() < (int64_t(1) << 31), name, ": at most 2^31 - 1 are taken, got ", ids.numel());
   auto flat = ids.contiguous();
   IdBytes(flat, name);
   return flat;

@@ -1036,7 +1036,8 @@ int gs_embedding_lookup(const void* table, int64_t num_rows, int64_t row_stride,
 
 /* Its gradient, out[v, :] = scale * sum of grad[i, :] over the i with ids[i] == v: num_rows x dim, every
  * row written.  Row i of grad from grad + i * grad_stride values (0: the same row for all).  Sums in an
- * order that follows from the ids alone: the same bits every time. */
+ * order that follows from the ids alone: the same bits every time.  The workspace of sizes that no call takes is
+ * given as 256 bytes; the call itself refuses them. */
 size_t gs_embedding_grad_workspace_bytes(int64_t n, int64_t dim, int type);
 int gs_embedding_grad(const void* grad, int64_t grad_stride, int64_t dim, int type, const void* ids, int id_bytes,
                       int64_t n, int64_t num_rows, float scale, void* out, void* workspace, size_t workspace_bytes,

@@ -569,3 +569,43 @@ def test_bad_arguments_are_refused_before_anything_is_launched():
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="GPU tensor"):
         gs.ops.embedding(torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
+
+
+def test_workspaces_of_sizes_that_no_call_takes():
+    """They have no plan: a size comes back all the same, and the call with it refuses."""
+    import ctypes
+    lib, i64 = capi.lib(), ctypes.c_int64
+    buf = (ctypes.c_int64 * 64)()
+    sizes = (lib.gs_embedding_grad_workspace_bytes, lib.gs_embedding_sparse_grad_workspace_bytes)
+    for dim in (1, 64, 2048, (1 << 24) - 1):
+        for kind in (0, 1, 2):
+            for size in sizes:
+                # the most ids that are taken: a word each at least, and then the launches that join the sums
+                assert size(i64((1 << 31) - 1), i64(dim), kind) > 8 << 31
+                for n in (1 << 31, 1 << 37, 1 << 45, 1 << 62, (1 << 63) - 1, -1, 0):
+                    assert size(i64(n), i64(dim), kind) == 256
+    for size in sizes:
+        assert size(i64(1000), i64(1 << 24), 0) == size(i64(1000), i64(1 << 62), 0) == size(i64(1000), i64(64), 9) == 256
+    for n, dim, kind, match in ((1 << 37, 64, 0, b"ids"), (2, 1 << 24, 0, b"values"), (2, 8, 9, b"value type")):
+        status = lib.gs_embedding_grad(buf, i64(8), i64(dim), kind, buf, 8, i64(n), i64(4), ctypes.c_float(1), buf, buf,
+                                       ctypes.c_size_t(256), None)
+        assert status < 0 and match in lib.gs_status_string(status)
+        status = lib.gs_embedding_sparse_grad_count(buf, 8, i64(n), i64(4), i64(dim), kind, None, i64(1), buf,
+                                                    ctypes.c_size_t(256), None)
+        assert status < 0 and match in lib.gs_status_string(status)
+
+
+@gpu
+def test_more_ids_than_are_taken_are_refused_before_anything_is_allocated(dev):
+    ids = torch.zeros(1, dtype=torch.int32, device=dev).expand(1 << 31)
+    row, wide = torch.zeros(1, 1, device=dev), torch.zeros(1, 1, device=dev).expand(1, 1 << 24)
+    held = torch.cuda.memory_allocated(dev)
+    for call in (lambda: gs.ops.embedding(row, ids), lambda: gs.ops.expert_sort(ids, 4),
+                 lambda: gs.ops.expert_dispatch(row.expand(1 << 31, 1), ids, 4),
+                 lambda: torch.ops.gs_ops._CAPI_EmbeddingGrad(row.expand(1 << 31, 1), ids, 4, 1.0),
+                 lambda: torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(row.expand(1 << 31, 1), ids, 4, 1.0)):
+        with pytest.raises(RuntimeError, match=r"(ids|experts): at most 2\^31 - 1 are taken"):
+            call()
+    with pytest.raises(RuntimeError, match=r"at most 2\^24 - 1 values are taken"):
+        gs.ops.embedding(wide, ids[:4])
+    assert torch.cuda.memory_allocated(dev) == held
