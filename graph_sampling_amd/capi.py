@@ -1315,6 +1315,13 @@ def coo2csc(key, value, num_keys, is_sorted, num_values=None):
 _VALUE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+def _scratch(nbytes, device):
+    """Scratch of one call.  The buffer that workspace() keeps is the device's: a call on another stream, or of
+    another thread while this one waits for the stream between two of the library's, would write over it, and
+    places and positions are read back from it as addresses."""
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
 def _rows(t, name):
     """(pointer, values between rows, width, value type) of a 2-D tensor whose rows are contiguous."""
     if not t.is_cuda:
@@ -1342,7 +1349,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0):
     if grad.size(0) != ids.numel():
         raise GsError("a gradient of %d rows for %d ids" % (grad.size(0), ids.numel()))
     out = torch.empty(num_rows, grad.size(1), dtype=grad.dtype, device=grad.device)
-    ws = workspace(lib().gs_embedding_grad_workspace_bytes(_i64(ids.numel()), dim, kind), grad.device)
+    ws = _scratch(lib().gs_embedding_grad_workspace_bytes(_i64(ids.numel()), dim, kind), grad.device)
     _check(lib().gs_embedding_grad(ptr, stride, dim, kind, _ptr(ids), idb, _i64(ids.numel()), _i64(num_rows),
                                    ctypes.c_float(scale), _ptr(out), _ptr(ws), ctypes.c_size_t(ws.numel()),
                                    _stream(grad.device)), "gs_embedding_grad")
@@ -1359,7 +1366,7 @@ def embedding_sparse_grad(grad, ids, num_rows, scale=1.0):
     if n == 0:
         return (torch.empty(0, dtype=torch.int64, device=dev),
                 torch.empty(0, grad.size(1), dtype=grad.dtype, device=dev))
-    ws = workspace(lib().gs_embedding_sparse_grad_workspace_bytes(_i64(n), dim, kind), dev)
+    ws = _scratch(lib().gs_embedding_sparse_grad_workspace_bytes(_i64(n), dim, kind), dev)
     box = torch.zeros(2, dtype=torch.int64, pin_memory=True)
     st = _stream(dev)
     _check(lib().gs_embedding_sparse_grad_count(_ptr(ids), idb, _i64(n), _i64(num_rows), dim, kind, _ptr(box), _i64(1),
@@ -1382,7 +1389,7 @@ def expert_sort(experts, num_experts):
     order = torch.empty(n, dtype=torch.int32, device=dev)
     place = torch.empty(experts.shape, dtype=torch.int32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
-    ws = workspace(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
+    ws = _scratch(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
     _check(lib().gs_expert_sort(_ptr(experts), idb, _i64(n), _i64(num_experts), _ptr(order), _ptr(place), _ptr(offsets),
                                 _ptr(ws), ctypes.c_size_t(ws.numel()), _stream(dev)), "gs_expert_sort")
     return order, place, offsets
@@ -1400,7 +1407,7 @@ def expert_dispatch(x, experts, num_experts):
     place = torch.empty(experts.shape, dtype=torch.int32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
     rows = torch.empty(n, x.size(1), dtype=x.dtype, device=dev)
-    ws = workspace(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
+    ws = _scratch(lib().gs_expert_sort_workspace_bytes(_i64(n), _i64(num_experts)), dev)
     _check(lib().gs_expert_dispatch(ptr, stride, dim, kind, _ptr(experts), idb, _i64(tokens), _i64(choices),
                                     _i64(num_experts), _ptr(order), _ptr(place), _ptr(offsets), _ptr(rows), _ptr(ws),
                                     ctypes.c_size_t(ws.numel()), _stream(dev)), "gs_expert_dispatch")

@@ -609,3 +609,82 @@ def test_more_ids_than_are_taken_are_refused_before_anything_is_allocated(dev):
     with pytest.raises(RuntimeError, match=r"at most 2\^24 - 1 values are taken"):
         gs.ops.embedding(wide, ids[:4])
     assert torch.cuda.memory_allocated(dev) == held
+
+
+class CountingLibrary:
+    """Stands in for the kernel library: notes the scratch that every call is given, and what a fill finds in it."""
+    def __init__(self):
+        self.scratch, self.held = [], None
+
+    def __getattr__(self, name):
+        import ctypes
+        if name.endswith("_workspace_bytes"):
+            return lambda *args: 4096
+
+        def call(*args):
+            at = [i for i, a in enumerate(args) if isinstance(a, ctypes.c_size_t)][0] - 1
+            self.scratch.append(args[at].value)
+            if name == "gs_embedding_sparse_grad_count":
+                ctypes.memset(args[at], 7, 4096)
+                ctypes.cast(args[6], ctypes.POINTER(ctypes.c_int64))[0] = 2
+            elif name == "gs_embedding_sparse_grad_fill":
+                self.held = ctypes.string_at(args[at], 4096)
+            return 0
+        return call
+
+
+def test_scratch_of_the_binding_is_the_calls_own(monkeypatch):
+    """What one call has in its scratch is not written over by another of the binding's calls, by any thread."""
+    import ctypes
+    import types
+    library, cpu, zeros = CountingLibrary(), torch.device("cpu"), torch.zeros
+    monkeypatch.setattr(capi, "lib", lambda: library)
+    monkeypatch.setattr(capi, "_ids", lambda t, name: 8)
+    monkeypatch.setattr(capi, "_stream", lambda device: None)
+    monkeypatch.setattr(capi, "_rows", lambda t, name: (ctypes.c_void_p(t.data_ptr()), capi._i64(t.stride(0)),
+                                                        capi._i64(t.size(1)), 0))
+    monkeypatch.setattr(torch, "zeros", lambda *args, pin_memory=False, **kw: zeros(*args, **kw))
+    grad, ids = torch.zeros(3, 4), torch.zeros(3, dtype=torch.int64)
+
+    def another_call():  # while the first one waits for its stream
+        capi.workspace(4096, cpu).fill_(255)
+        capi.embedding_grad(grad, ids, 5)
+        capi.expert_sort(ids, 4)
+        capi.expert_dispatch(grad, ids, 4)
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: types.SimpleNamespace(synchronize=another_call))
+    capi.embedding_sparse_grad(grad, ids, 5)
+    assert library.held == bytes([7]) * 4096
+    count, *others, fill = library.scratch
+    assert count == fill and len(others) == 3
+    assert capi.workspace(4096, cpu).data_ptr() not in library.scratch
+
+
+@gpu
+def test_two_threads_through_the_binding(dev):
+    """Both gradients, sorts and rows sent by two threads on a stream each, through the C ABI's binding."""
+    import threading
+    work = []
+    for seed in (51, 52):
+        grad, ids = rows(30000, 24, torch.float32, dev, seed), torch.from_numpy(ids_of("hub", 30000, 900, seed)).to(dev)
+        work.append((grad, ids, capi.embedding_grad(grad, ids, 900), capi.expert_dispatch(grad, ids, 900)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(grad, ids, want, want_sent):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                met, values = capi.embedding_sparse_grad(grad, ids, 900)
+                dense = capi.embedding_grad(grad, ids, 900)
+                sent = capi.expert_dispatch(grad, ids, 900)
+                same = all(torch.equal(a, b) for a, b in zip(sent, want_sent))
+                same = same and all(torch.equal(a, b) for a, b in zip(capi.expert_sort(ids, 900), want_sent[1:]))
+                if not (same and torch.equal(dense, want) and torch.equal(dense[met], values)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
