@@ -1436,6 +1436,8 @@ def expert_gather(x, place, offsets):
 def _weights(weights, place):
     if weights is None:
         return _ptr(None), 0
+    if not weights.is_cuda or weights.device != place.device:
+        raise GsError("weights must live on the GPU, beside place (%s), got %s" % (place.device, weights.device))
     if weights.dtype not in _VALUE_TYPES or weights.shape != place.shape or not weights.is_contiguous():
         raise GsError("weights must be contiguous, of a value type and of the shape of place")
     return _ptr(weights), _VALUE_TYPES[weights.dtype]

@@ -599,3 +599,19 @@ def test_bad_arguments_are_refused_before_anything_is_launched():
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="GPU tensor"):
         gs.ops.expert_dispatch(torch.zeros(3, 4), torch.zeros(3, 2, dtype=torch.int64), 4)
+
+
+def test_the_binding_refuses_weights_in_host_memory(monkeypatch):
+    """They would be read, and their gradient written, by a kernel."""
+    import ctypes
+    monkeypatch.setattr(capi, "_rows", lambda t, name: (ctypes.c_void_p(t.data_ptr()), capi._i64(t.stride(0)),
+                                                        capi._i64(t.size(1)), 0))
+    monkeypatch.setattr(capi, "_need", lambda t, dtype, name: None)  # (as if the others were on the GPU)
+    monkeypatch.setattr(capi, "_stream", lambda device: None)
+    y, x, weights = torch.zeros(6, 4), torch.zeros(3, 4), torch.ones(3, 2)
+    place, offsets = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(5, dtype=torch.int64)
+    monkeypatch.setattr(capi, "lib", lambda: pytest.fail("a library call"))
+    with pytest.raises(capi.GsError, match="weights must live on the GPU"):
+        capi.expert_combine(y, place, weights)
+    with pytest.raises(capi.GsError, match="weights must live on the GPU"):
+        capi.expert_combine_grad(x, y, place, offsets, weights)
