@@ -558,6 +558,51 @@ def test_refusals(dev):
         torch.func.grad(lambda t: gs.ops.expert_gather(t, order).sum())(x)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("choices,kind", [(1, "outside"), (2, "skewed")])
+def test_many_tokens_with_a_part_of_a_workgroup_behind(dev, choices, kind, dtype):
+    """Four chunks a lane are taken from 2^20 chunks on: 300 001 rows of 33 values are 2 700 009 in fp32 and 1 500 005 in
+    the others, 745 and 869 behind the last whole workgroup of 1024."""
+    tokens, dim, num = 300_001, 33, 9
+    e = experts_of(kind, tokens, choices, num, choices)
+    x = rows(tokens, dim, dtype, dev, 53)
+    got, order = gs.ops.expert_dispatch(x, torch.from_numpy(e).to(dev), num)
+    items, _, offsets = check_order(order, e, num)
+    live = int(offsets[-1])
+    assert live < e.size
+    assert torch.equal(got[:live], x[torch.from_numpy(items[:live] // choices).to(dev)]) and not got[live:].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+# rows of 65, 77, 85, 86 and 129 chunks of four values (fp32) and of eight: both sides of where half a wave a token gives
+# way to a whole one, and where either goes around more than once, the last time in part; then tokens too few for that
+@pytest.mark.parametrize("tokens,dim", [(4099, 257), (4099, 307), (4099, 339), (4099, 341), (4099, 513), (4099, 611),
+                                        (4099, 675), (4099, 681), (4099, 1025), (4096, 340), (130, 300), (130, 511)])
+def test_gradients_of_sums_of_long_rows(dev, tokens, dim, dtype):
+    choices, num = 3, 9
+    e = torch.from_numpy(experts_of("outside", tokens, choices, num, dim)).to(dev)
+    order = gs.ops.expert_sort(e, num)
+    live = int(order.offsets[-1])
+    at = order.place.long()
+    there = at >= 0
+    assert 0 < live < at.numel()
+    dout = rows(tokens, dim, dtype, dev, 55)
+    d64 = dout.double()
+    for wtype, shift in ((torch.float32, 0), (dtype, 1)):
+        y = rows(tokens * choices, dim + shift, dtype, dev, 54)[:, shift:].requires_grad_(True)
+        w = rows(tokens, choices, wtype, dev, 56).requires_grad_(True)
+        dy, dw = torch.autograd.grad(gs.ops.expert_combine(y, order, w), (y, w), dout)
+        want = torch.zeros(tokens * choices, dim, dtype=torch.float64, device=dev)
+        want[at[there]] = (d64[:, None, :] * w.detach().double()[:, :, None])[there]
+        off = (dy.double() - want).abs()
+        assert bool((off <= want.abs() * (F32 + half_step(dtype)) * (1 + F32) + smallest(dtype)).all())
+        assert not dy[live:].any()
+        terms = torch.where(there[:, :, None], d64[:, None, :] * y.detach().double()[at.clamp(min=0)], 0.0)
+        within(dw, terms.sum(2).cpu().numpy(), ((dim + 12) * F32 * terms.abs().sum(2)).cpu().numpy(), wtype)
+
+
 # ------------------------------------------------------------------ no GPU ----
 def test_bad_arguments_are_refused_before_anything_is_launched():
     import ctypes
