@@ -236,8 +236,9 @@ combine_grad_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
           v[u] = Values<T>{};
-          // (past the caches: y is read for the last time, and dy needs their room: 50 k tokens, 4 rows of 500
-          // bf16 each, 102 us plain and 77 so)
+          // (past the caches: y is read for the last time, and dy needs their room: 50 k tokens, 4 rows of 512
+          // bf16 each, from memory 91 us plain and 86 so; of 500, whose dy is written plainly, 101 and 106, and the same
+          // rows every call 100 and 88)
           const T* const at_y = y + (from[u] >= 0 ? from[u] * y_stride + at : 0);
           if (from[u] >= 0) v[u] = dim >= Chunk<T>::kVec ? load_past(at_y) : load_chunk(at_y, dim);
         }
@@ -336,7 +337,7 @@ int launch_combine_grad(const T* dout, int64_t dout_stride, const T* y, int64_t 
   constexpr int kTokens = kThreads / (G * WAVES);
   constexpr int64_t kMost = most_blocks(kThreads) * kTokens;  // tokens a launch
   const auto past = results_past(dy, dim, false);
-  // (rows of eight choices at once take registers that waves need: 50 k tokens, 4 of 8 choices, 139 us; of 4 101)
+  // (rows of eight choices at once take registers that waves need: 25 k tokens, 8 choices of 500 bf16, 123 us; four 107)
   for (int64_t t = 0; t < tokens; t += kMost) {
     const int64_t here = tokens - t < kMost ? tokens - t : kMost, item = t * choices;
     const dim3 grid(static_cast<unsigned>((here + kTokens - 1) / kTokens));
@@ -524,7 +525,9 @@ int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y,
       using One = std::integral_constant<int, 1>;
       if (chunks <= 4) return go(std::integral_constant<int, 4>(), One());
       if (chunks <= 16) return go(std::integral_constant<int, 16>(), One());
-      // (half a wave, too, where a whole one would idle for a third of its time: rows of 77 chunks 59 us for 68)
+      // (half a wave, too, where a whole one would idle for a third of its time: rows of 77 chunks, 8192 tokens of 3
+      // choices 18.5 us for 22.4, 20 k of 4 62.6 for 61.6 from memory and 50.8 for 54.7 from the caches, 50 k of 2 86 for 77
+      // and 62 for 64)
       if (chunks <= 32 || (tokens >= 4096 && chunks > kWave && chunks <= 85))
         return go(std::integral_constant<int, 32>(), One());
       if (chunks <= kWave || tokens >= 4096) return go(std::integral_constant<int, kWave>(), One());

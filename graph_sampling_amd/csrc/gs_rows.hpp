@@ -68,11 +68,13 @@ __device__ __forceinline__ Values<T> load_past(const T* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const Loose*>(p));
 }
 // Whether results go past the caches, and leave those to what is read: as they come, where rows fill whole lines; in
-// the lines that lie inside a row, where no chunk crosses a line; or not at all.  600 k rows of 256 B looked up in
-// 627 MB: 51 us with plain stores, 38 so (with plain stores and loads past the caches 58), and with a kernel behind
-// that reads the result 75 and 72; 75 k rows 6.5 and 5.5, with that kernel 11.0 and 10.8.  94 k rows of 400 B sent to
-// 4 experts each, and the gradient: 107 plain, 88 with the inner lines so.  Lines written in two parts go to memory
-// twice: 30 k rows of 2002 B sent to experts 14 us plain, 20 so; 162 k rows of 1286 B looked up 44 and 52.
+// the lines that lie inside a row, where no chunk crosses a line; or not at all.  Kernel times, other ids and results
+// every call, so that nothing is left in the memory-side cache: 600 k rows of 256 B looked up in 627 MB 60 us with plain
+// stores, 48 so (with plain stores and loads past the caches 58), and with a kernel behind that reads the result 115 and
+// 113; 75 k rows 12.0 and 10.0.  94 k rows of 400 B sent to 4 experts each, and the gradient: 45 + 53 plain, 48 + 43 with
+// the inner lines so, 67 + 36 with all.  Rows that are no multiple of 16 bytes, whose lines are written in two parts, go
+// plainly: 30 k rows of 2002 B sent to experts 29 us either way (the same rows every call 20 and 22); a
+// lookup alone is the other way round, 162 k rows of 1286 B 78 plain and 69 so.
 enum class Past { kNo, kInside, kAll };
 
 // p: the chunk `at` values into a row of dim values

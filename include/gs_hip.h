@@ -1064,12 +1064,12 @@ int gs_expert_sort(const void* experts, int id_bytes, int64_t n, int64_t num_exp
 
 /* rows[place[t, k], :] = x[t, :] for tokens x choices places (below 2^31 together), zeros in the rows from
  * *live (device; offsets[num_experts] of the sort) to tokens * choices.  A place outside
- * [0, tokens * choices) is left out. */
+ * [0, tokens * choices) is left out; a row before *live that no place names stays as it was. */
 int gs_expert_gather(const void* x, int64_t x_stride, int64_t dim, int type, const int32_t* place, int64_t tokens,
                      int64_t choices, const int64_t* live, void* rows, void* stream);
 
 /* gs_expert_sort of experts [tokens, choices] and gs_expert_gather of x by it, in one call (one launch for up to 1024
- * items of fewer than 256 experts).  Workspace: as gs_expert_sort's for tokens * choices items.  (No
+ * items of fewer than 512 experts).  Workspace: as gs_expert_sort's for tokens * choices items.  (No
  * counterpart in the reference.) */
 int gs_expert_dispatch(const void* x, int64_t x_stride, int64_t dim, int type, const void* experts, int id_bytes,
                        int64_t tokens, int64_t choices, int64_t num_experts, int32_t* order, int32_t* place,
