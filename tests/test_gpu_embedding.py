@@ -639,6 +639,7 @@ def test_scratch_of_the_binding_is_the_calls_own(monkeypatch):
     import types
     library, cpu, zeros = CountingLibrary(), torch.device("cpu"), torch.zeros
     monkeypatch.setattr(capi, "lib", lambda: library)
+    monkeypatch.setattr(capi, "_ws", capi._Workspace())  # (a buffer in host memory is not left for calls on a GPU)
     monkeypatch.setattr(capi, "_ids", lambda t, name: 8)
     monkeypatch.setattr(capi, "_stream", lambda device: None)
     monkeypatch.setattr(capi, "_rows", lambda t, name: (ctypes.c_void_p(t.data_ptr()), capi._i64(t.stride(0)),
