@@ -1468,3 +1468,82 @@ def expert_combine_grad(dout, y, place, offsets, weights=None):
                                         _ptr(offsets[-1:]), w, wkind, _ptr(dy), _ptr(dw), _stream(dout.device)),
            "gs_expert_combine_grad")
     return dy, dw
+
+
+# --------------------------------------------- experts: choice, products, dropout ----
+def expert_choose(logits, choices, normalize=True):
+    """(experts int32, weights float32), [tokens, choices] each."""
+    ptr, stride, num, kind = _rows(logits, "logits")
+    tokens, dev = logits.size(0), logits.device
+    experts = torch.empty(tokens, choices, dtype=torch.int32, device=dev)
+    weights = torch.empty(tokens, choices, dtype=torch.float32, device=dev)
+    _check(lib().gs_expert_choose(ptr, stride, kind, _i64(tokens), num, _i64(choices), int(bool(normalize)), _ptr(experts),
+                                  _ptr(weights), _stream(dev)), "gs_expert_choose")
+    return experts, weights
+
+
+def expert_choose_grad(dweights, logits, experts, weights, normalize=True):
+    ptr, stride, num, kind = _rows(logits, "logits")
+    _need(experts, torch.int32, "experts")
+    _need(weights, torch.float32, "weights")
+    _need(dweights, torch.float32, "dweights")
+    if experts.dim() != 2 or experts.size(0) != logits.size(0) or not experts.shape == weights.shape == dweights.shape:
+        raise GsError("experts, weights and their gradient must be [tokens, choices]")
+    if not experts.device == weights.device == dweights.device == logits.device:
+        raise GsError("logits, experts, weights and their gradient are on different devices")
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _check(lib().gs_expert_choose_grad(ptr, stride, kind, _ptr(experts), _ptr(weights), _ptr(dweights),
+                                       _i64(logits.size(0)), num, _i64(experts.size(1)), int(bool(normalize)), _ptr(out),
+                                       _stream(logits.device)), "gs_expert_choose_grad")
+    return out
+
+
+def expert_matmul(rows, offsets, weight):
+    """rows [n, inner] of expert e times weight[e]; weight [experts, inner, outer], either of the last two contiguous."""
+    ptr, stride, inner, kind = _rows(rows, "rows")
+    _need(offsets, torch.int64, "offsets")
+    if not weight.is_cuda or not weight.device == offsets.device == rows.device:
+        raise GsError("rows, offsets and weight must live on one GPU")
+    if weight.dim() != 3 or weight.dtype != rows.dtype or weight.size(1) != rows.size(1):
+        raise GsError("weight must be [experts, inner, outer] of the rows' type")
+    if offsets.numel() != weight.size(0) + 1:
+        raise GsError("offsets must be [experts + 1]")
+    transposed = weight.size(2) > 1 and weight.stride(2) != 1
+    if transposed and weight.size(1) > 1 and weight.stride(1) != 1:
+        raise GsError("the rows or the columns of weight must be contiguous")
+    out = torch.empty(rows.size(0), weight.size(2), dtype=rows.dtype, device=rows.device)
+    _check(lib().gs_expert_matmul(ptr, stride, _i64(rows.size(0)), inner, kind, _ptr(weight), _i64(weight.stride(0)),
+                                  _i64(weight.stride(2 if transposed else 1)), int(transposed), _i64(weight.size(0)),
+                                  _i64(weight.size(2)), _ptr(offsets), _ptr(out), _stream(rows.device)), "gs_expert_matmul")
+    return out
+
+
+def expert_matmul_grad(grad, rows, offsets):
+    """The gradient of weight, [experts, inner, outer]."""
+    ptr, stride, inner, kind = _rows(rows, "rows")
+    gptr, gstride, outer, gkind = _rows(grad, "grad")
+    _need(offsets, torch.int64, "offsets")
+    if grad.size(0) != rows.size(0) or gkind != kind or not offsets.device == grad.device == rows.device:
+        raise GsError("rows, grad and offsets do not belong together")
+    num = offsets.numel() - 1
+    out = torch.empty(num, rows.size(1), grad.size(1), dtype=rows.dtype, device=rows.device)
+    _check(lib().gs_expert_matmul_grad(ptr, stride, inner, gptr, gstride, outer, kind, _i64(rows.size(0)), _ptr(offsets),
+                                       _i64(num), _ptr(out), _stream(rows.device)), "gs_expert_matmul_grad")
+    return out
+
+
+def dropout(x, p, seed, residual=None):
+    """seed: a number, or a one-element int64 tensor on x's device."""
+    for t in (x, residual):
+        if t is not None and not (t.is_cuda and t.device == x.device and t.is_contiguous() and t.dtype == x.dtype and
+                                  t.dtype in _VALUE_TYPES and t.shape == x.shape):
+            raise GsError("x and residual must be contiguous GPU tensors of one value type and shape")
+    at = seed if isinstance(seed, torch.Tensor) else None
+    if at is not None:
+        _need(at, torch.int64, "seed")
+        if at.numel() != 1 or at.device != x.device:
+            raise GsError("seed must be one int64 beside x")
+    out = torch.empty_like(x)
+    _check(lib().gs_dropout(_ptr(x), _ptr(residual), _i64(x.numel()), _VALUE_TYPES[x.dtype], ctypes.c_double(p),
+                            _u64(0 if at is not None else seed), _ptr(at), _ptr(out), _stream(x.device)), "gs_dropout")
+    return out

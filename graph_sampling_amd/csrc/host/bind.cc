@@ -176,6 +176,17 @@ TORCH_LIBRARY(gs_ops, m) {
   m.def("expert_combine", &gs::ExpertCombine);
   m.def("_CAPI_ExpertCombineGrad", &gs::ExpertCombineGrad);
   m.def("expert_combine_grad", &gs::ExpertCombineGrad);
+  // and what experts do in between
+  m.def("_CAPI_ExpertChoose", &gs::ExpertChoose);
+  m.def("expert_choose", &gs::ExpertChoose);
+  m.def("_CAPI_ExpertChooseGrad", &gs::ExpertChooseGrad);
+  m.def("expert_choose_grad", &gs::ExpertChooseGrad);
+  m.def("_CAPI_ExpertMatmul", &gs::ExpertMatmul);
+  m.def("expert_matmul", &gs::ExpertMatmul);
+  m.def("_CAPI_ExpertMatmulGrad", &gs::ExpertMatmulGrad);
+  m.def("expert_matmul_grad", &gs::ExpertMatmulGrad);
+  m.def("_CAPI_Dropout", &gs::Dropout);
+  m.def("dropout", &gs::Dropout);
   // not in the reference: reproducible sampling (its seeds are compile-time constants)
   m.def("_CAPI_SetSeed", &SetSeed);
   m.def("_CAPI_SetThreadSeed", &SetThreadSeed);

@@ -2156,5 +2156,148 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& 
   return {dy, dw};
 }
 
+// ------------------------------------------- experts: choice, products, dropout ----
+std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(const torch::Tensor& logits, int64_t choices, bool normalize) {
+  const Rows l(logits, "logits");
+  TORCH_CHECK(l.t.size(1) <= 4096, "at most 4096 experts are taken, got ", l.t.size(1));
+  TORCH_CHECK(choices >= 0 && choices <= 64 && choices <= l.t.size(1), "choices must lie in [0, min(64, experts)], got ",
+              choices, " of ", l.t.size(1), " experts");
+  const int64_t tokens = l.t.size(0);
+  TORCH_CHECK(choices == 0 || tokens < ((int64_t(1) << 31) - 1) / choices, "at most 2^31 - 1 choices are taken, got ",
+              tokens, " times ", choices);
+  c10::hip::HIPGuard on(logits.device().index());
+  auto experts = torch::empty({tokens, choices}, torch::dtype(torch::kInt32).device(logits.device()));
+  auto weights = torch::empty({tokens, choices}, torch::dtype(torch::kFloat32).device(logits.device()));
+  Check(gs_expert_choose(l.t.data_ptr(), l.stride, l.type, tokens, l.t.size(1), choices, normalize ? 1 : 0,
+                         experts.data_ptr<int32_t>(), weights.data_ptr<float>(), Stream(logits)),
+        "gs_expert_choose");
+  return {experts, weights};
+}
+
+torch::Tensor ExpertChooseGrad(const torch::Tensor& dweights, const torch::Tensor& logits, const torch::Tensor& experts,
+                               const torch::Tensor& weights, bool normalize) {
+  const Rows l(logits, "logits");
+  const int64_t tokens = l.t.size(0), choices = experts.dim() == 2 ? experts.size(1) : -1;
+  NeedDevice(experts, "experts");
+  TORCH_CHECK(experts.scalar_type() == torch::kInt32 && experts.dim() == 2 && experts.size(0) == tokens,
+              "experts must be int32 [", tokens, ", choices], got ", experts.scalar_type(), " ", experts.sizes());
+  TORCH_CHECK(choices <= 64 && choices <= l.t.size(1) && l.t.size(1) <= 4096, "at most 64 choices of 4096 experts are taken");
+  for (const auto* t : {&weights, &dweights}) {
+    TORCH_CHECK(t->is_cuda(), "Not implemented warning: weights and their gradient must be GPU tensors");
+    TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->sizes() == experts.sizes(),
+                "weights and their gradient must be float32 of the shape of experts, ", experts.sizes());
+  }
+  TORCH_CHECK(experts.device() == logits.device() && weights.device() == logits.device() &&
+                  dweights.device() == logits.device(),
+              "logits, experts, weights and their gradient are on different devices");
+  c10::hip::HIPGuard on(logits.device().index());
+  const auto w = weights.contiguous().resolve_neg(), d = dweights.contiguous().resolve_neg();
+  auto out = torch::empty({tokens, l.t.size(1)}, Like(logits));
+  Check(gs_expert_choose_grad(l.t.data_ptr(), l.stride, l.type, experts.data_ptr<int32_t>(), w.data_ptr<float>(),
+                              d.data_ptr<float>(), tokens, l.t.size(1), choices, normalize ? 1 : 0, out.data_ptr(),
+                              Stream(logits)),
+        "gs_expert_choose_grad");
+  return out;
+}
+
+namespace {
+// [experts, inner, outer]: the values of a matrix's rows, or those of its columns, side by side
+struct Matrices {
+  torch::Tensor t;  // keeps a copy alive
+  int64_t expert_stride, stride;
+  int type;
+  bool transposed;
+  explicit Matrices(const torch::Tensor& weight) : t(weight) {
+    TORCH_CHECK(t.defined(), "weight is undefined");
+    TORCH_CHECK(t.is_cuda(), "Not implemented warning: weight must be a GPU tensor");
+    TORCH_CHECK(t.layout() == torch::kStrided, "weight must be a dense tensor");
+    TORCH_CHECK(t.dim() == 3, "weight must be [experts, inner, outer], got ", t.sizes());
+    type = ValueType(t, "weight");
+    TORCH_CHECK(t.size(1) < (int64_t(1) << 24) && t.size(2) < (int64_t(1) << 24),
+                "matrices of at most 2^24 - 1 rows and columns are taken, got ", t.sizes());
+    if (t.is_neg()) t = t.resolve_neg();
+    if (!(t.size(2) <= 1 || t.stride(2) == 1 || t.size(1) <= 1 || t.stride(1) == 1)) t = t.contiguous();
+    transposed = ColumnsContiguous(t);
+    expert_stride = t.stride(0);
+    stride = transposed ? t.stride(2) : t.stride(1);
+  }
+};
+
+const int64_t* Offsets(const torch::Tensor& offsets, const torch::Device& device, int64_t experts) {
+  LiveRows(offsets, device);
+  TORCH_CHECK(offsets.numel() == experts + 1, "offsets must be [experts + 1] = [", experts + 1, "], got ", offsets.sizes());
+  return offsets.data_ptr<int64_t>();
+}
+}  // namespace
+
+bool ColumnsContiguous(const torch::Tensor& weight) {
+  const bool rows = weight.size(2) <= 1 || weight.stride(2) == 1, columns = weight.size(1) <= 1 || weight.stride(1) == 1;
+  return columns && !rows;
+}
+
+torch::Tensor ExpertMatmul(const torch::Tensor& rows, const torch::Tensor& offsets, const torch::Tensor& weight) {
+  const Rows r(rows, "rows");
+  const Matrices w(weight);
+  TORCH_CHECK(weight.device() == rows.device(), "rows and weight are on different devices");
+  TORCH_CHECK(w.type == r.type, "rows and weight differ in type");
+  TORCH_CHECK(w.t.size(1) == r.t.size(1), "rows of ", r.t.size(1), " values for matrices ", weight.sizes());
+  TORCH_CHECK(r.t.size(0) < (int64_t(1) << 31), "at most 2^31 - 1 rows are taken, got ", r.t.size(0));
+  const int64_t* at = Offsets(offsets, rows.device(), w.t.size(0));
+  c10::hip::HIPGuard on(rows.device().index());
+  auto out = torch::empty({r.t.size(0), w.t.size(2)}, Like(rows));
+  Check(gs_expert_matmul(r.t.data_ptr(), r.stride, r.t.size(0), r.t.size(1), r.type, w.t.data_ptr(), w.expert_stride,
+                         w.stride, w.transposed ? 1 : 0, w.t.size(0), w.t.size(2), at, out.data_ptr(), Stream(rows)),
+        "gs_expert_matmul");
+  return out;
+}
+
+torch::Tensor ExpertMatmulGrad(const torch::Tensor& grad, const torch::Tensor& rows, const torch::Tensor& offsets,
+                               bool transposed) {
+  const Rows g(grad, "gradient"), r(rows, "rows");
+  TORCH_CHECK(grad.device() == rows.device(), "rows and gradient are on different devices");
+  TORCH_CHECK(g.type == r.type, "rows and gradient differ in type");
+  TORCH_CHECK(g.t.size(0) == r.t.size(0), "a gradient of ", g.t.size(0), " rows for ", r.t.size(0));
+  TORCH_CHECK(r.t.size(0) < (int64_t(1) << 31), "at most 2^31 - 1 rows are taken, got ", r.t.size(0));
+  LiveRows(offsets, rows.device());
+  const int64_t experts = offsets.numel() - 1, inner = r.t.size(1), outer = g.t.size(1);
+  c10::hip::HIPGuard on(rows.device().index());
+  const Rows &a = transposed ? g : r, &b = transposed ? r : g;
+  auto out = torch::empty({experts, a.t.size(1), b.t.size(1)}, Like(rows));
+  Check(gs_expert_matmul_grad(a.t.data_ptr(), a.stride, a.t.size(1), b.t.data_ptr(), b.stride, b.t.size(1), r.type,
+                              r.t.size(0), offsets.data_ptr<int64_t>(), experts, out.data_ptr(), Stream(rows)),
+        "gs_expert_matmul_grad");
+  TORCH_INTERNAL_ASSERT(out.numel() == experts * inner * outer);
+  return transposed ? out.transpose(1, 2) : out;
+}
+
+torch::Tensor Dropout(const torch::Tensor& x, double p, int64_t seed, const torch::Tensor& seed_at,
+                      const torch::Tensor& residual) {
+  TORCH_CHECK(x.defined(), "x is undefined");
+  TORCH_CHECK(x.is_cuda(), "Not implemented warning: x must be a GPU tensor");
+  TORCH_CHECK(x.layout() == torch::kStrided, "x must be a dense tensor");
+  const int type = ValueType(x, "x");
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, "p must be a probability, got ", p);
+  if (seed_at.defined()) {
+    NeedI64(seed_at, "seed");
+    TORCH_CHECK(seed_at.numel() == 1 && seed_at.device() == x.device(), "seed must be one int64 on ", x.device(), ", got ",
+                seed_at.sizes(), " on ", seed_at.device());
+  }
+  torch::Tensor r;
+  if (residual.defined()) {
+    TORCH_CHECK(residual.device() == x.device() && residual.scalar_type() == x.scalar_type() &&
+                    residual.sizes() == x.sizes() && residual.layout() == torch::kStrided,
+                "residual must be like x, ", x.scalar_type(), " ", x.sizes(), " on ", x.device(), ", got ",
+                residual.scalar_type(), " ", residual.sizes(), " on ", residual.device());
+  }
+  c10::hip::HIPGuard on(x.device().index());
+  const auto flat = x.contiguous().resolve_neg();
+  if (residual.defined()) r = residual.contiguous().resolve_neg();
+  auto out = torch::empty(x.sizes(), Like(x));
+  Check(gs_dropout(flat.data_ptr(), r.defined() ? r.data_ptr() : nullptr, flat.numel(), type, p, static_cast<uint64_t>(seed),
+                   seed_at.defined() ? seed_at.data_ptr<int64_t>() : nullptr, out.data_ptr(), Stream(x)),
+        "gs_dropout");
+  return out;
+}
+
 }  // namespace hip
 }  // namespace gs

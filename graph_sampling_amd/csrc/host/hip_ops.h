@@ -386,6 +386,21 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(const torch::Tensor& 
                                                            const torch::Tensor& offsets,
                                                            const torch::optional<torch::Tensor>& weights,
                                                            bool of_rows, bool of_weights);
+// {experts [tokens, choices] int32, weights fp32} of logits [tokens, experts]
+std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(const torch::Tensor& logits, int64_t choices, bool normalize);
+// [tokens, experts], like logits (which are looked at without normalize only; their shape and type always)
+torch::Tensor ExpertChooseGrad(const torch::Tensor& dweights, const torch::Tensor& logits, const torch::Tensor& experts,
+                               const torch::Tensor& weights, bool normalize);
+// [rows, outer] of rows [rows, inner] and weight [experts, inner, outer]
+torch::Tensor ExpertMatmul(const torch::Tensor& rows, const torch::Tensor& offsets, const torch::Tensor& weight);
+// [experts, inner, outer], laid out [experts, outer, inner] if transposed
+torch::Tensor ExpertMatmulGrad(const torch::Tensor& grad, const torch::Tensor& rows, const torch::Tensor& offsets,
+                               bool transposed);
+// whether the values of a column of each matrix lie side by side, those of a row apart
+bool ColumnsContiguous(const torch::Tensor& weight);
+// seed_at: one int64 on the device that holds the seed, or undefined
+torch::Tensor Dropout(const torch::Tensor& x, double p, int64_t seed, const torch::Tensor& seed_at,
+                      const torch::Tensor& residual);
 // whether the current stream of t's device is being recorded into a graph
 bool Capturing(const torch::Tensor& t);
 // whether the stream with this id is the current one of t's device, or is being recorded as well

@@ -123,6 +123,76 @@ struct CombineFunction : public torch::autograd::Function<CombineFunction> {
   }
 };
 
+struct ChooseFunction : public torch::autograd::Function<ChooseFunction> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, int64_t choices, bool normalize) {
+    const auto [experts, weights] = hip::ExpertChoose(logits, choices, normalize);
+    ctx->save_for_backward({logits, experts, weights});
+    ctx->saved_data["normalize"] = normalize;
+    ctx->mark_non_differentiable({experts});
+    ctx->set_materialize_grads(false);
+    return {experts, weights};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    if (!grads[1].defined()) return {{}, {}, {}};
+    NoSecond(true, "experts' weights");  // (they depend on the logits, which are followed)
+    at::NoGradGuard off;
+    return {hip::ExpertChooseGrad(grads[1], saved[0], saved[1], saved[2], ctx->saved_data["normalize"].toBool()), {}, {}};
+  }
+};
+
+struct MatmulFunction : public torch::autograd::Function<MatmulFunction> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& rows, const torch::Tensor& offsets,
+                               const torch::Tensor& weight) {
+    const bool of_rows = rows.requires_grad(), of_weight = weight.requires_grad();
+    // (each is kept for the other's gradient)
+    ctx->save_for_backward({of_weight ? rows : torch::Tensor(), offsets, of_rows ? weight : torch::Tensor()});
+    ctx->saved_data["rows"] = of_rows;
+    ctx->saved_data["weight"] = of_weight;
+    ctx->saved_data["transposed"] = hip::ColumnsContiguous(weight);
+    return hip::ExpertMatmul(rows, offsets, weight);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    if (!grads[0].defined()) return {{}, {}, {}};
+    const torch::Tensor &rows = saved[0], &weight = saved[2];
+    const bool of_rows = ctx->saved_data["rows"].toBool(), of_weight = ctx->saved_data["weight"].toBool();
+    NoSecond(grads[0].requires_grad() || (of_rows && weight.requires_grad()) || (of_weight && rows.requires_grad()),
+             "experts' products");
+    at::NoGradGuard off;
+    torch::Tensor d_rows, d_weight;
+    if (of_rows) d_rows = hip::ExpertMatmul(grads[0], saved[1], weight.transpose(1, 2));
+    if (of_weight) d_weight = hip::ExpertMatmulGrad(grads[0], rows, saved[1], ctx->saved_data["transposed"].toBool());
+    return {d_rows, {}, d_weight};
+  }
+};
+
+struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::optional<torch::Tensor>& added,
+                               double p, int64_t seed, const torch::optional<torch::Tensor>& seed_tensor) {
+    const auto residual = added.value_or(torch::Tensor()), seed_at = seed_tensor.value_or(torch::Tensor());
+    ctx->save_for_backward({seed_at});  // (a seed that changes between the passes is refused by its version)
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["x"] = x.requires_grad();
+    ctx->saved_data["residual"] = residual.defined() && residual.requires_grad();
+    return hip::Dropout(x, p, seed, seed_at, residual);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto seed_at = ctx->get_saved_variables()[0];
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
+    torch::Tensor dx, d_residual;
+    if (ctx->saved_data["residual"].toBool()) d_residual = grads[0];
+    if (ctx->saved_data["x"].toBool()) {
+      NoSecond(grads[0].requires_grad(), "a dropout");
+      at::NoGradGuard off;
+      dx = hip::Dropout(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_at,
+                        torch::Tensor());
+    }
+    return {dx, d_residual, {}, {}, {}};
+  }
+};
+
 // order is the caller's: the kernels go by place, but the three belong together
 void CheckOrder(const torch::Tensor& order, const torch::Tensor& place) {
   TORCH_CHECK(order.defined() && place.defined(), "order or place is undefined");
@@ -183,6 +253,47 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(torch::Tensor grad, t
   auto [dy, dw] = hip::ExpertCombineGrad(grad, y, place, offsets, weights, true, w.defined());
   if (!dw.defined()) dw = torch::empty({0}, grad.options());
   return {dy, dw};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(torch::Tensor logits, int64_t choices, bool normalize) {
+  if (!Followed(logits)) return hip::ExpertChoose(logits, choices, normalize);
+  const auto out = ChooseFunction::apply(logits, choices, normalize);
+  return {out[0], out[1]};
+}
+
+torch::Tensor ExpertChooseGrad(torch::Tensor grad, torch::Tensor logits, torch::Tensor experts, torch::Tensor weights,
+                               bool normalize) {
+  TORCH_CHECK(!Followed(grad) && !Followed(logits) && !Followed(weights),
+              "the gradient of experts' weights cannot be differentiated once more");
+  return hip::ExpertChooseGrad(grad, logits, experts, weights, normalize);
+}
+
+torch::Tensor ExpertMatmul(torch::Tensor rows, torch::Tensor order, torch::Tensor place, torch::Tensor offsets,
+                           torch::Tensor weight) {
+  CheckOrder(order, place);
+  const bool followed = Followed(rows), weighed = Followed(weight);
+  TORCH_CHECK(rows.dim() != 2 || rows.size(0) == place.numel(), "rows of ", rows.size(0), " items, places of ", place.numel());
+  return followed || weighed ? MatmulFunction::apply(rows, offsets, weight) : hip::ExpertMatmul(rows, offsets, weight);
+}
+
+torch::Tensor ExpertMatmulGrad(torch::Tensor grad, torch::Tensor rows, torch::Tensor offsets) {
+  TORCH_CHECK(!Followed(grad) && !Followed(rows), "the gradient of experts' products cannot be differentiated once more");
+  return hip::ExpertMatmulGrad(grad, rows, offsets, false);
+}
+
+torch::Tensor Dropout(torch::Tensor x, double p, torch::optional<int64_t> seed, torch::optional<torch::Tensor> seed_at,
+                      torch::optional<torch::Tensor> residual) {
+  const torch::Tensor at = seed_at.has_value() ? seed_at.value() : torch::Tensor();
+  const torch::Tensor r = residual.has_value() ? residual.value() : torch::Tensor();
+  TORCH_CHECK(!seed.has_value() || !at.defined(), "one seed, a number or a tensor, not both");
+  const bool followed = Followed(x), added = Followed(r);
+  // (a number would be recorded, and every replay draw the same)
+  TORCH_CHECK(seed.has_value() || at.defined() || !x.is_cuda() || !hip::Capturing(x),
+              "a graph is being recorded: dropout needs a seed, a tensor that changes between replays");
+  const int64_t number = seed.has_value() ? seed.value() : at.defined() ? 0 : static_cast<int64_t>(hip::NextSeed());
+  if (!at.defined()) seed_at = torch::nullopt;
+  if (!r.defined()) residual = torch::nullopt;
+  return followed || added ? DropoutFunction::apply(x, residual, p, number, seed_at) : hip::Dropout(x, p, number, at, r);
 }
 
 }  // namespace gs

@@ -37,4 +37,22 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertCombineGrad(torch::Tensor grad, t
                                                            torch::Tensor place, torch::Tensor offsets,
                                                            torch::optional<torch::Tensor> weights);
 
+// ---- what experts do in between: their choice, products with their matrices, dropout
+
+// {experts [tokens, choices] int32, weights fp32}: the experts with the largest of logits [tokens, experts] and their
+// shares, of the chosen ones' sum (normalize) or of all; see gs_expert_choose in gs_hip.h
+std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(torch::Tensor logits, int64_t choices, bool normalize);
+torch::Tensor ExpertChooseGrad(torch::Tensor grad, torch::Tensor logits, torch::Tensor experts, torch::Tensor weights,
+                               bool normalize);
+// [items, outer]: the rows of expert e (from offsets[e] to offsets[e + 1]) times weight[e], zeros behind the last;
+// weight: [experts, inner, outer], either of the last two contiguous
+torch::Tensor ExpertMatmul(torch::Tensor rows, torch::Tensor order, torch::Tensor place, torch::Tensor offsets,
+                           torch::Tensor weight);
+// the gradient of the matrices, [experts, inner, outer]
+torch::Tensor ExpertMatmulGrad(torch::Tensor grad, torch::Tensor rows, torch::Tensor offsets);
+// residual + x / (1 - p) where the draw for a position (row-major) is at least p, residual elsewhere.  The seed is `seed`,
+// or the value of seed_at at the time the kernels run, or else the next of those that the samplers count up.
+torch::Tensor Dropout(torch::Tensor x, double p, torch::optional<int64_t> seed, torch::optional<torch::Tensor> seed_at,
+                      torch::optional<torch::Tensor> residual);
+
 }  // namespace gs

@@ -1,7 +1,8 @@
 """Generalised SDDMM front end: gsddmm and the generated u_add_v ... e_dot_v helpers
 (surface of the reference's python/gs/ops/sddmm.py:35-131 and sparse.py:14-129); and, not in the
 reference, rows of features moved by ids, with gradients: `embedding`, and rows sorted by expert or
-node type and back, `expert_dispatch` and `expert_combine`."""
+node type and back, `expert_dispatch` and `expert_combine`; the choice of experts, `expert_choose`, the
+products with their matrices in between, `expert_matmul`, and `dropout`."""
 import sys
 from collections import namedtuple
 from itertools import product
@@ -12,7 +13,7 @@ from . import load_library
 from .format import _COO
 
 __all__ = ['gsddmm', 'embedding', 'ExpertOrder', 'expert_sort', 'expert_gather', 'expert_dispatch',
-           'expert_combine']
+           'expert_combine', 'expert_choose', 'expert_matmul', 'dropout']
 
 _TARGET = {'u': 0, 'e': 1, 'v': 2, 'src': 0, 'edge': 1, 'dst': 2}
 
@@ -143,3 +144,45 @@ def expert_combine(y, order, weights=None):
     """
     load_library()
     return torch.ops.gs_ops._CAPI_ExpertCombine(y, order.order, order.place, order.offsets, weights)
+
+
+def expert_choose(logits, choices, normalize=True):
+    """The `choices` experts (at most 64) with the largest of a router's `logits` ([tokens, experts]; up to 4096
+    experts; float32, float16 or bfloat16), and how much each is to count: (experts [tokens, choices] int32, weights
+    float32).  Experts come largest first, the lower one of equals; weights are shares of the softmax over the chosen
+    experts, or, without `normalize`, over all.  A logit of -inf stands for an expert the token may not have: it is
+    never chosen, and where no other is left the choice is -1 with weight 0.  Differentiable in `logits`, through the
+    weights.
+
+        experts, weights = gs.ops.expert_choose(x @ router, 2)
+        rows, order = gs.ops.expert_dispatch(x, experts, num_experts)
+    """
+    load_library()
+    return torch.ops.gs_ops._CAPI_ExpertChoose(logits, choices, normalize)
+
+
+def expert_matmul(rows, order, weight):
+    """The rows of expert e (offsets[e] to offsets[e + 1] of `rows`, [items, inner]) times weight[e] ([inner,
+    outer]): [items, outer], zeros behind the last expert's rows.  `weight` is [experts, inner, outer] of the rows'
+    type; a transposed view of [experts, outer, inner] is read as it lies.  Products are summed in float32 and rounded
+    once; no expert's number of rows is brought to the host.  Differentiable in `rows` and `weight`.
+
+        rows, order = gs.ops.expert_dispatch(x, experts, num_experts)
+        h = torch.relu(gs.ops.expert_matmul(rows, order, w_in))
+        out = gs.ops.expert_combine(gs.ops.expert_matmul(h, order, w_out), order, weights)
+    """
+    load_library()
+    return torch.ops.gs_ops._CAPI_ExpertMatmul(rows, order.order, order.place, order.offsets, weight)
+
+
+def dropout(x, p=0.5, seed=None, residual=None):
+    """x / (1 - p) with probability 1 - p, zero otherwise, plus `residual` (like `x`) if given, in float32, rounded
+    once.  What is dropped follows from `seed` and the position in `x` (row by row, as if contiguous) alone: a number, a
+    one-element int64 tensor on x's device that is read when the kernel runs -- change it between the replays of a
+    recorded graph, not between a forward pass and its backward pass --, or, by default, the next of the seeds that the
+    samplers count up (`_CAPI_SetSeed`).  No mask is stored; the backward pass draws it again.  Differentiable in `x`
+    and `residual`.  There is no switch for evaluation: leave the call out."""
+    load_library()
+    at = seed if isinstance(seed, torch.Tensor) else None
+    number = None if at is not None or seed is None else (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63  # (as 64 bits)
+    return torch.ops.gs_ops._CAPI_Dropout(x, p, number, at, residual)

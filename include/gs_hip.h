@@ -1087,6 +1087,49 @@ int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y,
                            const int32_t* place, int64_t tokens, int64_t choices, const int64_t* live,
                            const void* weights, int weight_type, void* dy, void* dweights, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* What experts do between their rows' going out and coming back: the choice of experts, */
+/* products with each expert's matrix, dropout.  No counterpart in the reference.  */
+/* ------------------------------------------------------------------------- */
+/* The choice of K = choices experts (up to 64, and up to as many as there are: 4096 at most) from a router's logits,
+ * row t from logits + t * stride values: chosen[t, 0..K) = the experts with the largest logits, largest first, the
+ * lower one of equals; weights[t, k] = exp(logit - the largest) over the sum of the same for the chosen experts
+ * (normalize) or for all.  A logit of -infinity is never chosen: where no other is left, -1 with weight 0.  NaN counts as
+ * the largest, and makes the token's weights NaN.  (No counterpart in the reference.) */
+int gs_expert_choose(const void* logits, int64_t stride, int type, int64_t tokens, int64_t experts, int64_t choices,
+                     int normalize, int32_t* chosen, float* weights, void* stream);
+
+/* Its gradient, dlogits: tokens x experts, from what it returned (chosen, weights) and the gradient of the weights.
+ * logits is read only without normalize.  A token's choices are different experts; one outside [0, experts) counts for
+ * nothing.  (No counterpart in the reference.) */
+int gs_expert_choose_grad(const void* logits, int64_t stride, int type, const int32_t* chosen, const float* weights,
+                          const float* dweights, int64_t tokens, int64_t experts, int64_t choices, int normalize,
+                          void* dlogits, void* stream);
+
+/* out[p, :] = rows[p, :] x the matrix of expert e for offsets[e] <= p < offsets[e + 1], zeros in the rows from
+ * offsets[num_experts] to n (below 2^31).  rows: n rows of `inner` values, row_stride apart; out: n x outer.  The
+ * matrix of expert e begins at weight + e * expert_stride: `inner` rows of `outer` values, weight_stride apart, or, if
+ * transposed, `outer` rows of `inner` values.  Products are exact, sums fp32 in the order of `inner`, rounded once.
+ * offsets ascend from 0; others leave out rows or write them twice, but nothing outside out.  Also the gradient of rows,
+ * with inner and outer, and transposed, the other way round.  (No counterpart in the reference.) */
+int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n, int64_t inner, int type, const void* weight,
+                     int64_t expert_stride, int64_t weight_stride, int transposed, int64_t num_experts, int64_t outer,
+                     const int64_t* offsets, void* out, void* stream);
+
+/* The gradient of the matrices: dweight[e] (inner x outer) = the sum over the rows p of expert e of
+ * rows[p, :]^T x grad[p, :], zeros for an expert without rows.  rows: n x inner, grad: n x outer, of any strides between
+ * rows.  Sums are fp32, in an order that the offsets alone decide.  (No counterpart in the reference.) */
+int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, const void* grad, int64_t grad_stride,
+                          int64_t outer, int type, int64_t n, const int64_t* offsets, int64_t num_experts, void* dweight,
+                          void* stream);
+
+/* out[i] = residual[i] (NULL: 0) + (draw(seed, tag 6, row 0, i) >= floor(p * 2^32) ? x[i] / (1 - p) : 0), i < n, in fp32,
+ * rounded once; p = 1 drops everything.  seed_at (device, may be NULL) holds the seed instead, so that a recorded call
+ * draws anew at each replay.  x is not read for its sign or value where it is dropped (NaN leaves no trace).  The gradient
+ * of x is the same call on the gradient, without residual.  (No counterpart in the reference.) */
+int gs_dropout(const void* x, const void* residual, int64_t n, int type, double p, uint64_t seed, const int64_t* seed_at,
+               void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
