@@ -42,7 +42,7 @@ def lib():
                      "gs_metapath_walk_workspace_bytes",
                      "gs_induced_slice_workspace_bytes", "gs_induced_slice_notify_workspace_bytes",
                      "gs_embedding_grad_workspace_bytes", "gs_embedding_sparse_grad_workspace_bytes",
-                     "gs_expert_sort_workspace_bytes"):
+                     "gs_expert_sort_workspace_bytes", "gs_expert_matmul_grad_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_size_t
         _lib.gs_sorted_union_max.restype = ctypes.c_int64
@@ -1527,8 +1527,10 @@ def expert_matmul_grad(grad, rows, offsets):
         raise GsError("rows, grad and offsets do not belong together")
     num = offsets.numel() - 1
     out = torch.empty(num, rows.size(1), grad.size(1), dtype=rows.dtype, device=rows.device)
+    ws = _scratch(lib().gs_expert_matmul_grad_workspace_bytes(_i64(rows.size(0)), inner, outer, _i64(num)), rows.device)
     _check(lib().gs_expert_matmul_grad(ptr, stride, inner, gptr, gstride, outer, kind, _i64(rows.size(0)), _ptr(offsets),
-                                       _i64(num), _ptr(out), _stream(rows.device)), "gs_expert_matmul_grad")
+                                       _i64(num), _ptr(out), _ptr(ws), ctypes.c_size_t(ws.numel()), _stream(rows.device)),
+           "gs_expert_matmul_grad")
     return out
 
 

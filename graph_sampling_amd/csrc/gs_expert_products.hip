@@ -9,7 +9,6 @@
 namespace gs {
 namespace {
 
-using products::Acc;
 using products::Group;
 using products::Operand;
 
@@ -17,13 +16,14 @@ using products::Operand;
 struct RowTile {
   int64_t expert, begin;  // of the tile's rows
   int64_t rows;           // up to the expert's last; none: no tile
-  int64_t tiles;          // of all experts
+  int64_t col;            // which tile of columns
 };
 
-// Every thread counts the tiles of its share of the experts; the one in whose share tile `at` lies finds it.
+// Every thread counts the tiles of rows of its share of the experts; the one in whose share the workgroup's lies finds it.
+// Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.
 template <int THREADS>
 __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
-                                             int64_t at) {
+                                             int64_t col_tiles) {
   __shared__ int64_t s_wave[THREADS / kWave];
   __shared__ RowTile s_found;
   const int64_t each = (experts + 1 + THREADS - 1) / THREADS, first = each * threadIdx.x;
@@ -46,6 +46,8 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
     if (w < static_cast<int>(threadIdx.x) / kWave) upto += s_wave[w];
     total += s_wave[w];
   }
+  const int64_t tiles = total * col_tiles, per_die = (tiles + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds;
+  const int64_t which = blockIdx.x % kXcds * per_die + slot, at = slot < per_die ? which / col_tiles : total;
   int64_t from = upto - mine;
   if (at >= from && at < upto) {
     for (int64_t e = first; e < last; ++e) {
@@ -62,7 +64,7 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
   }
   __syncthreads();
   RowTile t = s_found;
-  t.tiles = total;
+  t.col = which % col_tiles;
   return t;
 }
 
@@ -77,15 +79,15 @@ struct ProductArgs {
   int64_t col_tiles;
 };
 
-template <typename T, bool ACROSS, int BM, int BN, int WM, int WN>
+template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
 __global__ void __launch_bounds__(WM * WN * kWave)
 product_kernel(ProductArgs<T> p) {
-  using Tile = products::Tile<T, false, ACROSS, BM, BN, WM, WN>;
-  __shared__ __attribute__((aligned(16))) char s_steps[Tile::kBytes];
-  const int64_t at = blockIdx.x;
-  const RowTile t = find_tile<Tile::kThreads>(p.offsets, p.experts, p.n, BM, at / p.col_tiles);
+  using Tile = products::Tile<T, false, ACROSS, BM, BN, WM, WN, RING, DIRECT>;
+  __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
+  RowTile t = find_tile<Tile::kThreads>(p.offsets, p.experts, p.n, BM, p.col_tiles);
   if (t.rows <= 0) return;
-  const int64_t col = at % p.col_tiles * BN, rows = t.rows < BM ? t.rows : BM;
+  t = {products::uniform(t.expert), products::uniform(t.begin), products::uniform(t.rows), products::uniform(t.col)};
+  const int64_t col = t.col * BN, rows = t.rows < BM ? t.rows : BM;
   Tile tile;
   const bool live = t.expert < p.experts;
   const T* w = p.weight + (live ? t.expert * p.expert_stride : 0) + (ACROSS ? col : col * p.weight_stride);
@@ -93,10 +95,7 @@ product_kernel(ProductArgs<T> p) {
   const Operand<T> b = ACROSS ? Operand<T>{w, p.weight_stride, p.inner, p.outer - col}
                               : Operand<T>{w, p.weight_stride, p.outer - col, p.inner};
   tile.run(a, b, live ? p.inner : 0, s_steps);
-  T* const out = p.out + t.begin * p.outer + col;
-  tile.each([&](int m, int n, Acc v) {
-    if (m < rows) products::store_four(out + m * p.outer + n, v, p.outer - col - n);
-  });
+  tile.write(p.out + t.begin * p.outer + col, p.outer, rows, p.outer - col);
 }
 
 // Tiles of rows that there can be: a part of one for every expert that has rows, and for the rows behind.
@@ -104,14 +103,25 @@ int64_t most_row_tiles(int64_t n, int64_t experts, int64_t tile_rows) {
   return n / tile_rows + (experts + 1 < n ? experts + 1 : n);
 }
 
-template <typename T, bool ACROSS, int BM, int BN, int WM, int WN>
+template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
 int launch_product(ProductArgs<T> p, hipStream_t st) {
   constexpr int threads = WM * WN * kWave;
   p.col_tiles = (p.outer + BN - 1) / BN;
-  const int64_t blocks = most_row_tiles(p.n, p.experts, BM) * p.col_tiles;
+  const int64_t blocks = (most_row_tiles(p.n, p.experts, BM) * p.col_tiles + kXcds - 1) / kXcds * kXcds;
   GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, threads));
-  hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
+  hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN, RING, DIRECT>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
   return check_launch("expert_matmul");
+}
+
+template <typename T, bool ACROSS>
+int choose_product(const ProductArgs<T>& p, hipStream_t st) {
+  const bool direct = products::direct_rows(p.rows, p.row_stride, p.inner, 256) &&
+                      products::direct_rows(p.weight, p.weight_stride, ACROSS ? p.outer : p.inner, 256) &&
+                      p.expert_stride % Chunk<T>::kVec == 0;
+  if (!direct) return launch_product<T, ACROSS, 128, 128, 2, 2, 3, false>(p, st);
+  if constexpr (sizeof(T) == 2)
+    return launch_product<T, ACROSS, 256, 256, 2, 4, 4, true>(p, st);
+  return launch_product<T, ACROSS, 128, 128, 2, 2, 3, true>(p, st);
 }
 
 }  // namespace
@@ -141,6 +151,6 @@ extern "C" int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n,
     const ProductArgs<T> p{static_cast<const T*>(rows), row_stride, n, inner, static_cast<const T*>(weight), expert_stride,
                            weight_stride, num_experts, outer, offsets, static_cast<T*>(out), 0};
     const auto st = static_cast<hipStream_t>(stream);
-    return transposed ? launch_product<T, false, 128, 128, 2, 2>(p, st) : launch_product<T, true, 128, 128, 2, 2>(p, st);
+    return transposed ? choose_product<T, false>(p, st) : choose_product<T, true>(p, st);
   });
 }

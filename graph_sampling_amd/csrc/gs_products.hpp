@@ -2,8 +2,8 @@
 // the gradients of their matrices share.
 //
 // A workgroup makes a tile of C[m, n] = sum over k of A[m, k] * B[k, n].  It goes along k in steps of
-// 128 bytes (64 values of 16 bits, 32 fp32 values), which lie in LDS, two steps at a time: one is worked on
-// while the next is fetched.  Either operand comes in one of two orders: along k, where the values of one row (or
+// 64 bytes (32 values of 16 bits, 16 fp32 values), four of which have room in LDS: one is worked on, one has arrived,
+// two are on their way.  Either operand comes in one of two orders: along k, where the values of one row (or
 // column) of C lie side by side, or across k, where the rows of one k do.  Sums are fp32 in the
 // matrix cores' accumulators, in the order of k, rounded once at the end.
 #pragma once
@@ -13,14 +13,15 @@
 namespace gs {
 namespace products {
 
-constexpr int kStepBytes = 128;
+constexpr int kStepBytes = 64;
 template <typename T>
 constexpr int kStep = kStepBytes / static_cast<int>(sizeof(T));  // values of k a step
 
+// A fragment is what a wave holds of 16 rows (or columns) of C and a step: lane l has row l % 16, 16 bytes of k from
+// l / 16 * 16 bytes on.  The product of two: lane l gets C's row l % 16 of a, columns l / 16 * 4 .. + 3 of b.  (Products of
+// 32 x 32 and half the depth read and write their sums twice as often: power bounds large products, not instructions.)
 typedef float Acc __attribute__((ext_vector_type(4)));
 
-// What a lane holds for 16 rows (or columns) of C and 64 bytes of k: row lane % 16, k from lane / 16 * 16 bytes on.  The
-// product of two of those: lane l gets C's row (l % 16) of a, columns (l / 16) * 4 .. + 3 of b.
 __device__ __forceinline__ Acc multiply(Values<__bf16> b, Values<__bf16> a, Acc c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
 }
@@ -37,39 +38,56 @@ __device__ __forceinline__ Acc multiply(Values<float> b, Values<float> a, Acc c)
 // How an operand's WIDTH rows (or columns) of a step lie in LDS, in slots of 16 bytes.
 template <typename T, bool ACROSS, int WIDTH>
 struct Layout {
-  static constexpr int kVec = Chunk<T>::kVec;
+  static constexpr int kVec = Chunk<T>::kVec, kSize = static_cast<int>(sizeof(T));
   static constexpr int kSlots = WIDTH * (kStepBytes / 16);
   static constexpr int kBytes = kSlots * 16;
   static constexpr int kRowSlots = ACROSS ? WIDTH / kVec : kStepBytes / 16;  // slots of a row of the step
+  static constexpr int kUnitSlots = kSize == 4 ? 4 : 2;  // of a unit of 16 values
 
-  // Along k, row r holds 8 slots; a fragment's 16 rows are 128 bytes apart, so slot s keeps chunk s ^ (r % 8): the rows
-  // of a fragment then lie in different banks.  Across k, row k holds WIDTH values; fragments take 32 bytes (16 bits) or 64
-  // (fp32) of each of several rows, and such units trade places for the same reason.
-  static __device__ __forceinline__ int chunk_in(int row, int slot) {
-    if (!ACROSS) return slot ^ (row & 7);
-    if (sizeof(T) == 4) return (((slot >> 2) ^ ((row >> 2) & (WIDTH >= 64 ? 3 : 0))) << 2) | (slot & 3);
-    return (((slot >> 1) ^ turn(row)) << 1) | (slot & 1);
-  }
+  // What is read together lies in different banks (64 of 4 bytes).  Along k, row r holds 4 slots, and slot s keeps chunk
+  // s ^ (r / 2 % 4): lanes 0 - 3, 12 - 15 and 20 - 27 are served together, then the others.  Across k, row k holds WIDTH
+  // values in units of 16 that trade places: 32 lanes read a unit of rows k .. k + 3 and k + 8 .. k + 11 (16 bits), 64 lanes
+  // one of rows k, k + 4, k + 8 and k + 12 (fp32).
   static __device__ __forceinline__ int turn(int row) {
+    if (!ACROSS) return (row >> 1) & 3;
+    if (kSize == 4) return WIDTH >= 64 ? (row >> 2) & 3 : (row >> 2) & (WIDTH / 16 - 1);
     if (WIDTH >= 128) return (row & 3) | (((row >> 3) & 1) << 2);
-    if (WIDTH == 64) return ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
-    return 0;
+    return WIDTH == 64 ? ((row >> 1) & 1) | (((row >> 3) & 1) << 1) : 0;
   }
+  static __device__ __forceinline__ int chunk_in(int row, int slot) {
+    if (!ACROSS) return slot ^ turn(row);
+    return ((slot / kUnitSlots) ^ turn(row)) * kUnitSlots + slot % kUnitSlots;
+  }
+};
 
-  // the fragment of rows at .. at + 15 (a multiple of 16) and the step's half `half`
-  static __device__ __forceinline__ Values<T> fragment(const char* lds, int at, int half) {
+// Reads a wave's fragments out of LDS.
+template <typename T, bool ACROSS, int WIDTH>
+struct Reader {
+  using L = Layout<T, ACROSS, WIDTH>;
+  template <typename V>
+  using Lds = const __attribute__((address_space(3))) V;
+  static constexpr int kRow = WIDTH * L::kSize;  // bytes, across k
+  uint32_t base;  // the lane's part of the addresses
+
+  // lds: where the operand's part of the ring begins; first: the wave's first row, a multiple of its number of rows, which
+  // is a power of two
+  __device__ __forceinline__ Reader(uint32_t lds, int first) {
     const int lane = threadIdx.x % kWave, row16 = lane % 16, quarter = lane / 16;
+    if (!ACROSS) {
+      base = lds + (first + row16) * kStepBytes + (quarter ^ L::turn(row16)) * 16;
+    } else {
+      const int k = L::kSize == 4 ? quarter * 4 : quarter * 8 + row16 / 4;
+      base = lds + k * kRow + ((first / 16) ^ L::turn(k)) * (16 * L::kSize) + (L::kSize == 4 ? row16 * 4 : lane % 4 * 8);
+    }
+  }
+  // the wave's j-th fragment of a step that lies `step` bytes into the ring
+  __device__ __forceinline__ Values<T> fragment(int j, uint32_t step) const {
     if constexpr (!ACROSS) {
-      const int row = at + row16;
-      return *reinterpret_cast<const Values<T>*>(lds + row * kStepBytes + chunk_in(row, half * 4 + quarter) * 16);
-    } else if constexpr (sizeof(T) == 4) {
+      return *reinterpret_cast<Lds<Values<T>>*>(base + step + j * 16 * kStepBytes);
+    } else if constexpr (L::kSize == 4) {
       Values<T> v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = half * 16 + quarter * 4 + i;
-        const int unit = (at / 16) ^ ((k >> 2) & (WIDTH >= 64 ? 3 : 0));
-        v[i] = *reinterpret_cast<const T*>(lds + (k * WIDTH + unit * 16 + row16) * 4);
-      }
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<Lds<T>*>((base ^ (j * 64)) + step + i * kRow);
       return v;
     } else {
       // (a transposing read: 16 lanes take 4 rows of 16 values and get a column of 4 each)
@@ -80,12 +98,8 @@ struct Layout {
         Values<T> v;
       } u;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k = half * 32 + quarter * 8 + i * 4 + row16 / 4;
-        const int unit = (at / 16) ^ turn(k);
-        const char* p = lds + k * (WIDTH * 2) + unit * 32 + (lane % 4) * 8;
-        u.part[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(p));
-      }
+      for (int i = 0; i < 2; ++i)
+        u.part[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsFour*>((base ^ (j * 32)) + step + i * 4 * kRow));
       return u.v;
     }
   }
@@ -105,6 +119,19 @@ __device__ __forceinline__ Values<T> load_part(const T* p, int64_t there) {
   return v;
 }
 
+// Writes the first `there` of some values.
+template <typename T, typename V>
+__device__ __forceinline__ void store_part(T* p, V v, int64_t there) {
+  constexpr int kMany = static_cast<int>(sizeof(V) / sizeof(T));
+  if (there >= kMany) {
+    __builtin_memcpy(p, &v, sizeof(V));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMany - 1; ++i)
+      if (i < there) p[i] = v[i];
+  }
+}
+
 // An operand of a tile: `rows` rows (along k: of C; across k: of k), `stride` values apart, of `width` values.
 template <typename T>
 struct Operand {
@@ -114,12 +141,15 @@ struct Operand {
 
 // Fetches an operand step by step through registers.
 template <typename T, bool ACROSS, int WIDTH, int THREADS>
-struct Fetch {
+struct Staged {
   using L = Layout<T, ACROSS, WIDTH>;
   static constexpr int kEach = (L::kSlots + THREADS - 1) / THREADS;
+  Operand<T> x;
+  int64_t k0 = 0;
   Values<T> held[kEach];
 
-  __device__ __forceinline__ void load(const Operand<T>& x, int64_t k0) {
+  __device__ __forceinline__ explicit Staged(const Operand<T>& operand) : x(operand) {}
+  __device__ __forceinline__ void load() {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int q = i * THREADS + threadIdx.x;
@@ -128,6 +158,7 @@ struct Fetch {
       const bool in = q < L::kSlots && row < x.rows;
       held[i] = load_part(x.base + row * x.stride + col, in ? x.width - col : 0);
     }
+    k0 += kStep<T>;
   }
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
@@ -138,96 +169,279 @@ struct Fetch {
   }
 };
 
-// A tile of BM x BN by WM x WN waves.
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+// Fetches an operand step by step straight into LDS, 16 bytes a lane.  Chunks that do not exist are fetched from beyond
+// the buffer's end, and come as zeros.  The operand's rows are 16-byte aligned, its width is a multiple of 16 bytes, and
+// a step of a tile lies within 2^31 bytes.
+template <typename T, bool ACROSS, int WIDTH, int THREADS>
+struct Direct {
+  using L = Layout<T, ACROSS, WIDTH>;
+  typedef int Buffer __attribute__((ext_vector_type(4)));
+  static constexpr int kEach = L::kSlots / THREADS, kRowsApart = THREADS / L::kRowSlots;
+  static_assert(L::kSlots % THREADS == 0 && THREADS % L::kRowSlots == 0, "every lane has as many chunks");
+  static constexpr int kNowhere = static_cast<int>(0x80000000u);
+  uint64_t base;
+  int64_t step;  // bytes between steps
+  int at[kEach];
+
+  __device__ __forceinline__ explicit Direct(const Operand<T>& x) {
+    constexpr int kSize = static_cast<int>(sizeof(T));
+    base = reinterpret_cast<uint64_t>(x.base);
+    step = ACROSS ? kStep<T> * x.stride * kSize : kStepBytes;
+    const int64_t across = ACROSS ? x.width : x.rows;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      at[i] = static_cast<int>(row(i) * x.stride + chunk(i)) * kSize;
+      if ((ACROSS ? chunk(i) : row(i)) >= across) at[i] = kNowhere;
+    }
+  }
+  static __device__ __forceinline__ int row(int i) { return static_cast<int>(threadIdx.x) / L::kRowSlots + i * kRowsApart; }
+  static __device__ __forceinline__ int chunk(int i) { return L::chunk_in(row(i), threadIdx.x % L::kRowSlots) * L::kVec; }
+  // Written as instructions because the compiler, which cannot tell the ring's steps apart, would wait for all of them before
+  // each read of LDS; who reads waits by arrived().  (m0 holds nothing else: the compiler sets it in front of each use of
+  // its own.)
+  static __device__ __forceinline__ void put(uint64_t base, int bytes, int from, uint32_t lds, int offset) {
+    const Buffer buffer = {static_cast<int>(base), static_cast<int>(base >> 32), bytes, 0x00020000};
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+                 :
+                 : "s"(lds), "n"(offset), "v"(from), "s"(buffer)
+                 : "memory", "scc");
+  }
+  // Puts a part of the next step on its way to lds (an offset); bytes: all there are, or none, for zeros.
+  __device__ __forceinline__ void part(int i, uint32_t lds, int bytes) const {
+    put(base, bytes, at[i], lds, i * THREADS * 16);
+  }
+  __device__ __forceinline__ void advance() { base += step; }
+  // The first step: the last part of the depth, `rest` of a step, so that all others are whole.
+  __device__ __forceinline__ void first(int64_t whole_steps, int64_t rest, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      put(base + whole_steps * step, kAll, (ACROSS ? row(i) : chunk(i)) < rest ? at[i] : kNowhere, lds, i * THREADS * 16);
+  }
+  static constexpr int kAll = 0x7fffffff;
+};
+
+// Whether rows of `width` values, `stride` apart, can go straight into LDS, `rows` of them a step.
+template <typename T>
+bool direct_rows(const T* base, int64_t stride, int64_t width, int64_t rows) {
+  constexpr int64_t kVec = Chunk<T>::kVec;
+  return aligned_to(base, 16) && stride % kVec == 0 && width % kVec == 0 &&
+         stride < (int64_t(1) << 31) / (rows * static_cast<int64_t>(sizeof(T)));
+}
+
+// All but the last LEFT of a wave's fetches have arrived, and all waves of the workgroup have come here.
+template <int LEFT>
+__device__ __forceinline__ void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(LEFT) : "memory");
+}
+
+// A tile of BM x BN by WM x WN waves, RING steps in LDS (three or four).
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
 struct Tile {
   using LA = Layout<T, A_ACROSS, BM>;
   using LB = Layout<T, B_ACROSS, BN>;
+  using RA = Reader<T, A_ACROSS, BM>;
+  using RB = Reader<T, B_ACROSS, BN>;
   static constexpr int kThreads = WM * WN * kWave;
-  static constexpr int kMI = BM / WM / 16, kNI = BN / WN / 16;
-  static constexpr int kBytes = 2 * (LA::kBytes + LB::kBytes);  // of LDS
+  static constexpr int kMI = BM / WM / 16, kNI = BN / WN / 16, kFirst = kMI / 2;
+  static constexpr int kStage = LA::kBytes + LB::kBytes, kBytes = RING * kStage;  // of LDS
+  using FA = std::conditional_t<DIRECT, Direct<T, A_ACROSS, BM, kThreads>, Staged<T, A_ACROSS, BM, kThreads>>;
+  using FB = std::conditional_t<DIRECT, Direct<T, B_ACROSS, BN, kThreads>, Staged<T, B_ACROSS, BN, kThreads>>;
   Acc acc[kMI][kNI];
 
   static __device__ __forceinline__ int row0() { return static_cast<int>(threadIdx.x) / kWave / WN * (BM / WM); }
   static __device__ __forceinline__ int col0() { return static_cast<int>(threadIdx.x) / kWave % WN * (BN / WN); }
-
-  __device__ __forceinline__ void work(const char* a_lds, const char* b_lds) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      Values<T> a[kMI], b[kNI];
-#pragma unroll
-      for (int i = 0; i < kMI; ++i) a[i] = LA::fragment(a_lds, row0() + i * 16, half);
-#pragma unroll
-      for (int j = 0; j < kNI; ++j) b[j] = LB::fragment(b_lds, col0() + j * 16, half);
-#pragma unroll
-      for (int i = 0; i < kMI; ++i)
-#pragma unroll
-        for (int j = 0; j < kNI; ++j) acc[i][j] = multiply(b[j], a[i], acc[i][j]);
-    }
+  static __device__ __forceinline__ uint32_t lds_offset(char* lds) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
   }
 
-  // lds: kBytes
+  // Step s is multiplied in two halves of the wave's rows.  In front of the second one, step s + 1 has arrived everywhere,
+  // and nobody reads step s - 1 any more, whose place step s + RING - 1 takes: its fetches, and the reads of the fragments
+  // that step s + 1 begins with, stand between the products of the second half, in an order that is kept as it is written.
+  struct Fragments {
+    Values<T> a[kMI], b[2][kNI];
+  };
+  static constexpr int kFirstProducts = kFirst * kNI, kSecondProducts = (kMI - kFirst) * kNI;
+  static constexpr int kLater = kMI - kFirst, kAhead = kFirst + kNI, kFetches = FA::kEach + FB::kEach;
+  // The items of `many` that stand in front of product q of `products`, spread evenly; what is read ahead, in the first
+  // three quarters, so that it has come when the next step begins; what is fetched, a little behind what is read, since a
+  // wave finds time for three instructions behind a product, no more.
+  static constexpr int due(int q, int many, int products) { return (q * many + products - 1) / products; }
+  static constexpr int due_ahead(int q) {
+    const int r = (q * kAhead * 4 + 3 * kSecondProducts - 1) / (3 * kSecondProducts);
+    return r < kAhead ? r : kAhead;
+  }
+  static constexpr int due_fetch(int q) {
+    if (q >= kSecondProducts) return kFetches;
+    const int r = (4 * q * kFetches - kSecondProducts + 4 * kSecondProducts - 1) / (4 * kSecondProducts);
+    return r < 0 ? 0 : r;
+  }
+
+  struct Steps {
+    RA ra;
+    RB rb;
+    FA fa;
+    FB fb;
+    char* lds;
+    int64_t ahead;  // steps that are not on their way yet
+
+    __device__ __forceinline__ void fetch(int i, uint32_t to, int bytes) {
+      if (i < FA::kEach) fa.part(i, to, bytes);
+      else fb.part(i - FA::kEach, to + LA::kBytes, bytes);
+    }
+    __device__ __forceinline__ void advance() {
+      fa.advance();
+      fb.advance();
+      --ahead;
+    }
+  };
+
+  // a step in ring place `now`, its fragments of b in f.b[TURN]
+  template <int TURN>
+  __device__ __forceinline__ void step(Fragments& f, Steps& s, uint32_t now) {
+    const uint32_t next = now + kStage == kBytes ? 0 : now + kStage;
+#pragma unroll
+    for (int q = 0; q < kFirstProducts; ++q) {
+#pragma unroll
+      for (int r = due(q, kLater, kFirstProducts); r < due(q + 1, kLater, kFirstProducts); ++r)
+        f.a[kFirst + r] = s.ra.fragment(kFirst + r, now);
+      acc[q / kNI][q % kNI] = multiply(f.b[TURN][q % kNI], f.a[q / kNI], acc[q / kNI][q % kNI]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint32_t to = 0;
+    int bytes = 0;
+    if constexpr (DIRECT) {
+      arrived<(RING - 3) * kFetches>();
+      to = lds_offset(s.lds) + (now == 0 ? kBytes - kStage : now - kStage) +
+           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
+      bytes = s.ahead > 0 ? FA::kAll : 0;
+    } else {
+      __syncthreads();
+      char* const slot = s.lds + (now + 2 * kStage) % kBytes;
+      s.fa.store(slot);
+      s.fb.store(slot + LA::kBytes);
+      s.fa.load();
+      s.fb.load();
+    }
+    if (kFirst == 0) f.a[0] = s.ra.fragment(0, now);
+#pragma unroll
+    for (int q = 0; q < kSecondProducts; ++q) {
+      const int i = kFirst + q / kNI, j = q % kNI;
+#pragma unroll
+      for (int r = due_ahead(q); r < due_ahead(q + 1); ++r) {
+        if (r < kFirst) f.a[r] = s.ra.fragment(r, next);
+        else f.b[TURN ^ 1][r - kFirst] = s.rb.fragment(r - kFirst, next);
+      }
+      if constexpr (DIRECT) {
+#pragma unroll
+        for (int r = due_fetch(q); r < due_fetch(q + 1); ++r) s.fetch(r, to, bytes);
+      }
+      acc[i][j] = multiply(f.b[TURN][j], f.a[i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (DIRECT) s.advance();
+  }
+
+  // lds: kBytes, aligned to 1024 (parts of addresses are exchanged by exclusive or)
   __device__ __forceinline__ void run(const Operand<T>& a, const Operand<T>& b, int64_t depth, char* lds) {
 #pragma unroll
     for (int i = 0; i < kMI; ++i)
 #pragma unroll
       for (int j = 0; j < kNI; ++j) acc[i][j] = Acc{};
-    if (depth <= 0) return;
-    Fetch<T, A_ACROSS, BM, kThreads> fa;
-    Fetch<T, B_ACROSS, BN, kThreads> fb;
-    char* const a_lds[2] = {lds, lds + LA::kBytes};
-    char* const b_lds[2] = {lds + 2 * LA::kBytes, lds + 2 * LA::kBytes + LB::kBytes};
-    fa.load(a, 0);
-    fb.load(b, 0);
-    fa.store(a_lds[0]);
-    fb.store(b_lds[0]);
-    __syncthreads();
-    int now = 0;
-    for (int64_t k = kStep<T>; ; k += kStep<T>) {
-      const bool more = k < depth;
-      if (more) {
-        fa.load(a, k);
-        fb.load(b, k);
+    int64_t steps = (depth + kStep<T> - 1) / kStep<T>;
+    if (steps <= 0) return;
+    Steps s{RA(lds_offset(lds), row0()), RB(lds_offset(lds) + LA::kBytes, col0()), FA(a), FB(b), lds, steps};
+    if constexpr (DIRECT) {
+      const uint32_t to = lds_offset(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
+      const int64_t whole = depth / kStep<T>, rest = depth % kStep<T>;
+      if (rest > 0) {
+        s.fa.first(whole, rest, to);
+        s.fb.first(whole, rest, to + LA::kBytes);
+        --s.ahead;
       }
-      work(a_lds[now], b_lds[now]);
-      if (!more) break;
-      now ^= 1;  // (whose last readers are behind the barrier of the step before)
-      fa.store(a_lds[now]);
-      fb.store(b_lds[now]);
+#pragma unroll
+      for (int i = 0; i < RING - 1; ++i) {
+        if (i == 0 && rest > 0) continue;
+#pragma unroll
+        for (int r = 0; r < kFetches; ++r) s.fetch(r, to + i * kStage, s.ahead > 0 ? FA::kAll : 0);
+        s.advance();
+      }
+      arrived<(RING - 2) * kFetches>();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s.fa.load();
+        s.fb.load();
+        s.fa.store(lds + i * kStage);
+        s.fb.store(lds + i * kStage + LA::kBytes);
+      }
+      s.fa.load();
+      s.fb.load();
       __syncthreads();
     }
+    Fragments f;
+#pragma unroll
+    for (int j = 0; j < kNI; ++j) f.b[0][j] = s.rb.fragment(j, 0);
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) f.a[i] = s.ra.fragment(i, 0);
+    // (two steps a turn, so that what is read ahead stays in its registers; one behind the last is zeros)
+    uint32_t now = 0;
+    auto place = [&] {
+      const uint32_t here = now;
+      now = now + kStage == kBytes ? 0 : now + kStage;
+      return here;
+    };
+    for (; steps > 0; steps -= 2) {
+      step<0>(f, s, place());
+      step<1>(f, s, place());
+    }
+    if constexpr (DIRECT) arrived<0>();  // (nothing is on its way into LDS that the next workgroup has by then)
   }
 
-  // f(m, n, four values of row m from column n on)
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    const int lane = threadIdx.x % kWave;
+  // Rounds the sums, once, to nearest, ties to even, and writes rows 0 .. rows - 1 and columns 0 .. cols - 1 of the tile to out.
+  template <typename O>
+  __device__ __forceinline__ void write(O* out, int64_t stride, int64_t rows, int64_t cols) const {
+    typedef O Four __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x % kWave, quarter = lane / 16;
 #pragma unroll
-    for (int i = 0; i < kMI; ++i)
+    for (int i = 0; i < kMI; ++i) {
+      const int m = row0() + i * 16 + lane % 16;
+      O* const row = out + m * stride + col0();
+      const int64_t there = m < rows ? cols - col0() : 0;
+      if constexpr (sizeof(O) == 2 && kNI % 2 == 0) {
+        // two fragments' neighbouring quarters trade places, so that a lane has eight columns side by side
 #pragma unroll
-      for (int j = 0; j < kNI; ++j) f(row0() + i * 16 + lane % 16, col0() + j * 16 + lane / 16 * 4, acc[i][j]);
+        for (int j = 0; j < kNI; j += 2) {
+          typedef uint32_t Two __attribute__((ext_vector_type(2)));
+          const Two a = __builtin_bit_cast(Two, __builtin_convertvector(acc[i][j], Four));
+          const Two b = __builtin_bit_cast(Two, __builtin_convertvector(acc[i][j + 1], Four));
+          const Two x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+          const Two y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+          union {
+            uint32_t word[4];
+            Values<O> v;
+          } u = {{x[0], y[0], x[1], y[1]}};
+          const int n = (j + quarter % 2) * 16 + quarter / 2 * 8;
+          store_part(row + n, u.v, there - n);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kNI; ++j)
+          store_part(row + j * 16 + quarter * 4, __builtin_convertvector(acc[i][j], Four), there - j * 16 - quarter * 4);
+      }
+    }
   }
 };
-
-// `there` of four values, rounded once, to nearest, ties to even
-template <typename T>
-__device__ __forceinline__ void store_four(T* p, Acc v, int64_t there) {
-  typedef T Four __attribute__((ext_vector_type(4)));
-  const Four r = __builtin_convertvector(v, Four);
-  if (there >= 4) {
-    __builtin_memcpy(p, &r, sizeof(r));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < there) p[i] = r[i];
-  }
-}
 
 // Where an expert's rows begin and end, inside [0, n] whatever the offsets hold.  Expert `experts` has the rows behind the last.
 struct Group {
   int64_t begin, end;
   __device__ __forceinline__ int64_t rows() const { return end > begin ? end - begin : 0; }
 };
+__device__ __forceinline__ int64_t uniform(int64_t v) {  // (the same in all lanes)
+  const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+}
 __device__ __forceinline__ int64_t inside(int64_t v, int64_t n) { return v < 0 ? 0 : (v < n ? v : n); }
 __device__ __forceinline__ Group group_of(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int64_t e) {
   return {inside(offsets[e], n), e < experts ? inside(offsets[e + 1], n) : n};

@@ -2263,10 +2263,11 @@ torch::Tensor ExpertMatmulGrad(const torch::Tensor& grad, const torch::Tensor& r
   c10::hip::HIPGuard on(rows.device().index());
   const Rows &a = transposed ? g : r, &b = transposed ? r : g;
   auto out = torch::empty({experts, a.t.size(1), b.t.size(1)}, Like(rows));
+  auto ws = Scratch(gs_expert_matmul_grad_workspace_bytes(r.t.size(0), inner, outer, experts), rows);
   Check(gs_expert_matmul_grad(a.t.data_ptr(), a.stride, a.t.size(1), b.t.data_ptr(), b.stride, b.t.size(1), r.type,
-                              r.t.size(0), offsets.data_ptr<int64_t>(), experts, out.data_ptr(), Stream(rows)),
+                              r.t.size(0), offsets.data_ptr<int64_t>(), experts, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                              Stream(rows)),
         "gs_expert_matmul_grad");
-  TORCH_INTERNAL_ASSERT(out.numel() == experts * inner * outer);
   return transposed ? out.transpose(1, 2) : out;
 }
 

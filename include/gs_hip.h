@@ -1118,10 +1118,12 @@ int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n, int64_t in
 
 /* The gradient of the matrices: dweight[e] (inner x outer) = the sum over the rows p of expert e of
  * rows[p, :]^T x grad[p, :], zeros for an expert without rows.  rows: n x inner, grad: n x outer, of any strides between
- * rows.  Sums are fp32, in an order that the offsets alone decide.  (No counterpart in the reference.) */
+ * rows.  Sums are fp32, in an order that the offsets alone decide.  The workspace of sizes that no call takes is given as 256
+ * bytes; the call itself refuses them.  (No counterpart in the reference.) */
+size_t gs_expert_matmul_grad_workspace_bytes(int64_t n, int64_t inner, int64_t outer, int64_t num_experts);
 int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, const void* grad, int64_t grad_stride,
                           int64_t outer, int type, int64_t n, const int64_t* offsets, int64_t num_experts, void* dweight,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[i] = residual[i] (NULL: 0) + (draw(seed, tag 6, row 0, i) >= floor(p * 2^32) ? x[i] / (1 - p) : 0), i < n, in fp32,
  * rounded once; p = 1 drops everything.  seed_at (device, may be NULL) holds the seed instead, so that a recorded call

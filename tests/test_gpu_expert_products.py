@@ -548,9 +548,18 @@ def test_bad_arguments_are_refused_before_anything_is_launched():
                           (dict(rows=ctypes.c_void_p(at + 2)), b"aligned"), (dict(weight=ctypes.c_void_p(at + 1)), b"aligned")):
         fails(matmul(**change), match)
 
-    def grad(rows=buf, rstride=8, inner=8, g=buf, gstride=8, outer=8, kind=0, n=4, offsets=buf, num=3, out=buf):
+    def grad(rows=buf, rstride=8, inner=8, g=buf, gstride=8, outer=8, kind=0, n=4, offsets=buf, num=3, out=buf, ws=buf,
+             ws_bytes=256):
         return lib.gs_expert_matmul_grad(rows, i64(rstride), i64(inner), g, i64(gstride), i64(outer), kind, i64(n), offsets,
-                                         i64(num), out, None)
+                                         i64(num), out, ws, ctypes.c_size_t(ws_bytes), None)
+
+    sizes = lib.gs_expert_matmul_grad_workspace_bytes
+    assert sizes(i64(100), i64(64), i64(64), i64(4)) == 256
+    for bad in ((-1, 64, 64, 4), (1 << 31, 64, 64, 4), (1 << 30, 1 << 24, 64, 4), (1 << 30, 64, 1 << 40, 4), (1 << 30, 64, 64, 1 << 31),
+                (1 << 30, 64, 64, -1)):
+        assert sizes(*(i64(v) for v in bad)) == 256
+    assert sizes(i64(1 << 20), i64(64), i64(128), i64(3)) > 512 * 64 * 128 * 4
+    fails(grad(n=1 << 20, num=3), b"workspace")
 
     assert grad(inner=0) == grad(outer=0) == grad(num=0) == 0
     for change, match in ((dict(kind=7), b"value type"), (dict(n=-1), b"negative"), (dict(n=1 << 31), b"2^31"),
