@@ -4,87 +4,22 @@
 //   out[p, :] = 0                        for the rows behind the last expert's
 //
 // The gradient of the rows is the same product with the matrices transposed.  No counterpart in the reference.
-#include "gs_products.hpp"
+#include "gs_expert_products.hpp"
 
 namespace gs {
 namespace {
 
-using products::Group;
 using products::Operand;
+using products::ProductArgs;
+using products::RowTile;
+using products::Way;
 
-// Which tile of rows a workgroup makes: the tiles of all experts side by side, then those of the rows behind the last.
-struct RowTile {
-  int64_t expert, begin;  // of the tile's rows
-  int64_t rows;           // up to the expert's last; none: no tile
-  int64_t col;            // which tile of columns
-};
-
-// Every thread counts the tiles of rows of its share of the experts; the one in whose share the workgroup's lies finds it.
-// Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.
-template <int THREADS>
-__device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
-                                             int64_t col_tiles) {
-  __shared__ int64_t s_wave[THREADS / kWave];
-  __shared__ RowTile s_found;
-  const int64_t each = (experts + 1 + THREADS - 1) / THREADS, first = each * threadIdx.x;
-  const int64_t last = first + each < experts + 1 ? first + each : experts + 1;
-  int64_t mine = 0;
-  for (int64_t e = first; e < last; ++e)
-    mine += (products::group_of(offsets, experts, n, e).rows() + tile_rows - 1) / tile_rows;
-  int64_t upto = mine;
-  const int lane = threadIdx.x % kWave;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int64_t other = __shfl_up(upto, d, kWave);
-    if (lane >= d) upto += other;
-  }
-  if (lane == kWave - 1) s_wave[threadIdx.x / kWave] = upto;
-  if (threadIdx.x == 0) s_found.rows = 0;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < THREADS / kWave; ++w) {
-    if (w < static_cast<int>(threadIdx.x) / kWave) upto += s_wave[w];
-    total += s_wave[w];
-  }
-  const int64_t tiles = total * col_tiles, per_die = (tiles + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds;
-  const int64_t which = blockIdx.x % kXcds * per_die + slot, at = slot < per_die ? which / col_tiles : total;
-  int64_t from = upto - mine;
-  if (at >= from && at < upto) {
-    for (int64_t e = first; e < last; ++e) {
-      const Group g = products::group_of(offsets, experts, n, e);
-      const int64_t here = (g.rows() + tile_rows - 1) / tile_rows;
-      if (at < from + here) {
-        s_found.expert = e;
-        s_found.begin = g.begin + (at - from) * tile_rows;
-        s_found.rows = g.end - s_found.begin;
-        break;
-      }
-      from += here;
-    }
-  }
-  __syncthreads();
-  RowTile t = s_found;
-  t.col = which % col_tiles;
-  return t;
-}
-
-template <typename T>
-struct ProductArgs {
-  const T* rows;
-  int64_t row_stride, n, inner;
-  const T* weight;
-  int64_t expert_stride, weight_stride, experts, outer;
-  const int64_t* offsets;
-  T* out;
-  int64_t col_tiles;
-};
-
-template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
+template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, Way WAY>
 __global__ void __launch_bounds__(WM * WN * kWave)
 product_kernel(ProductArgs<T> p) {
-  using Tile = products::Tile<T, false, ACROSS, BM, BN, WM, WN, RING, DIRECT>;
+  using Tile = products::Tile<T, false, ACROSS, BM, BN, WM, WN, RING, WAY>;
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
-  RowTile t = find_tile<Tile::kThreads>(p.offsets, p.experts, p.n, BM, p.col_tiles);
+  RowTile t = products::find_tile<Tile::kThreads>(p.offsets, p.experts, p.n, BM, p.col_tiles);
   if (t.rows <= 0) return;
   t = {products::uniform(t.expert), products::uniform(t.begin), products::uniform(t.rows), products::uniform(t.col)};
   const int64_t col = t.col * BN, rows = t.rows < BM ? t.rows : BM;
@@ -98,30 +33,40 @@ product_kernel(ProductArgs<T> p) {
   tile.write(p.out + t.begin * p.outer + col, p.outer, rows, p.outer - col);
 }
 
-// Tiles of rows that there can be: a part of one for every expert that has rows, and for the rows behind.
-int64_t most_row_tiles(int64_t n, int64_t experts, int64_t tile_rows) {
-  return n / tile_rows + (experts + 1 < n ? experts + 1 : n);
-}
-
-template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
+template <typename T, bool ACROSS, int BM, int BN, int WM, int WN, int RING, Way WAY>
 int launch_product(ProductArgs<T> p, hipStream_t st) {
   constexpr int threads = WM * WN * kWave;
   p.col_tiles = (p.outer + BN - 1) / BN;
-  const int64_t blocks = (most_row_tiles(p.n, p.experts, BM) * p.col_tiles + kXcds - 1) / kXcds * kXcds;
+  const int64_t blocks = (products::most_row_tiles(p.n, p.experts, BM) * p.col_tiles + kXcds - 1) / kXcds * kXcds;
   GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, threads));
-  hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN, RING, DIRECT>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
+  hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN, RING, WAY>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
   return check_launch("expert_matmul");
 }
 
+// Large tiles read less, small ones fill the card with less work and waste less of it.  bf16, kernel times of tiles of 256 x
+// 256, 128 x 128, 64 x 128 and 64 x 64, us: 160 experts of 1024 x 1024, 200 rows each 130, 147, 161, 206; 32 of those 32, 28,
+// 29, 44; 32 of 1024 x 1024, 40 rows 26, 24, 23, 21; 160 of 256 x 256, 500 rows 33, 28, 30, 34 (too little depth for the
+// largest).  fp32, which is bound by its products, is within 5 % of its best with the smallest.
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
-  const bool direct = products::direct_rows(p.rows, p.row_stride, p.inner, 256) &&
-                      products::direct_rows(p.weight, p.weight_stride, ACROSS ? p.outer : p.inner, 256) &&
-                      p.expert_stride % Chunk<T>::kVec == 0;
-  if (!direct) return launch_product<T, ACROSS, 128, 128, 2, 2, 3, false>(p, st);
-  if constexpr (sizeof(T) == 2)
-    return launch_product<T, ACROSS, 256, 256, 2, 4, 4, true>(p, st);
-  return launch_product<T, ACROSS, 128, 128, 2, 2, 3, true>(p, st);
+  if (products::few_rows(p)) return products::launch_few_rows(p, ACROSS, st);
+  const Way way = products::slower(products::way_of(p.rows, p.row_stride, 0, p.inner, 256),
+                                   products::way_of(p.weight, p.weight_stride, p.expert_stride, ACROSS ? p.outer : p.inner, 256));
+  if (way == Way::kValues) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kValues>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.outer > 64 && products::likely_tiles(p, 128, 128) >= 600) {
+      if (way == Way::kChunks) return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kChunks>(p, st);
+      if (p.inner < 512 || products::likely_tiles(p, 256, 256) < 224)
+        return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kDirect>(p, st);
+    }
+    if (way == Way::kDirect && p.outer > 128 && p.inner >= 512 && p.n >= 64 * p.experts &&
+        products::likely_tiles(p, 256, 256) >= 224)
+      return launch_product<T, ACROSS, 256, 256, 2, 4, 4, Way::kDirect>(p, st);
+    if (way == Way::kDirect && p.outer > 64 && products::likely_tiles(p, 64, 128) >= 400)
+      return launch_product<T, ACROSS, 64, 128, 2, 2, 3, Way::kDirect>(p, st);
+  }
+  if (way == Way::kChunks) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kChunks>(p, st);
+  return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kDirect>(p, st);
 }
 
 }  // namespace

@@ -1,0 +1,104 @@
+// Products of rows sorted by expert: what the kernels for many rows and those for few share.
+#pragma once
+
+#include "gs_products.hpp"
+
+namespace gs {
+namespace products {
+
+// Which tile of rows a workgroup makes: the tiles of all experts side by side, then those of the rows behind the last.
+struct RowTile {
+  int64_t expert, begin;  // of the tile's rows
+  int64_t rows;           // up to the expert's last; none: no tile
+  int64_t col;            // which tile of columns
+};
+
+// Every thread counts the tiles of rows of its share of the experts; the one in whose share the workgroup's lies finds it.
+// Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.
+template <int THREADS>
+__device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
+                                             int64_t col_tiles) {
+  __shared__ int64_t s_wave[THREADS / kWave];
+  __shared__ RowTile s_found;
+  const int64_t each = (experts + 1 + THREADS - 1) / THREADS, first = each * threadIdx.x;
+  const int64_t last = first + each < experts + 1 ? first + each : experts + 1;
+  int64_t mine = 0;
+  for (int64_t e = first; e < last; ++e)
+    mine += (group_of(offsets, experts, n, e).rows() + tile_rows - 1) / tile_rows;
+  int64_t upto = mine;
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int64_t other = __shfl_up(upto, d, kWave);
+    if (lane >= d) upto += other;
+  }
+  if (lane == kWave - 1) s_wave[threadIdx.x / kWave] = upto;
+  if (threadIdx.x == 0) s_found.rows = 0;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < THREADS / kWave; ++w) {
+    if (w < static_cast<int>(threadIdx.x) / kWave) upto += s_wave[w];
+    total += s_wave[w];
+  }
+  const int64_t tiles = total * col_tiles, per_die = (tiles + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds;
+  const int64_t which = blockIdx.x % kXcds * per_die + slot, at = slot < per_die ? which / col_tiles : total;
+  int64_t from = upto - mine;
+  if (at >= from && at < upto) {
+    for (int64_t e = first; e < last; ++e) {
+      const Group g = group_of(offsets, experts, n, e);
+      const int64_t here = (g.rows() + tile_rows - 1) / tile_rows;
+      if (at < from + here) {
+        s_found.expert = e;
+        s_found.begin = g.begin + (at - from) * tile_rows;
+        s_found.rows = g.end - s_found.begin;
+        break;
+      }
+      from += here;
+    }
+  }
+  __syncthreads();
+  RowTile t = s_found;
+  t.col = which % col_tiles;
+  return t;
+}
+
+template <typename T>
+struct ProductArgs {
+  const T* rows;
+  int64_t row_stride, n, inner;
+  const T* weight;
+  int64_t expert_stride, weight_stride, experts, outer;
+  const int64_t* offsets;
+  T* out;
+  int64_t col_tiles;
+};
+
+// Tiles of rows that there can be: a part of one for every expert that has rows, and for the rows behind.
+inline int64_t most_row_tiles(int64_t n, int64_t experts, int64_t tile_rows) {
+  return n / tile_rows + (experts + 1 < n ? experts + 1 : n);
+}
+// Tiles that there will be, more or less: half a tile of rows for every expert is not full.
+template <typename T>
+int64_t likely_tiles(const ProductArgs<T>& p, int64_t tile_rows, int64_t tile_cols) {
+  const int64_t some = p.n < p.experts ? p.n : p.experts, full = p.n / tile_rows + p.experts / 2;
+  return (full > some ? full : some) * ((p.outer + tile_cols - 1) / tile_cols);
+}
+
+// The products of experts with few rows each (gs_expert_few_rows.hip), and whether they are such.
+template <typename T>
+int launch_few_rows(const ProductArgs<T>& p, bool across, hipStream_t st);
+
+// Where 64 x 64 tiles do not fill the card twice, the depth of a tile has to be shared out, too, if it is long; fp32, whose
+// products take sixteen times as long, gains by it with few rows whatever their number.  Kernel times of both, us, few
+// rows first: bf16, 32 experts of 4096 x 512, 16 rows each 36 and 74, 200 rows 109 and 85; of 1024 x 1024, 4 rows 16 and
+// 18; 160 of 1024 x 1024, 1 row 49 and 40; fp32, 32 of 4096 x 512, 40 rows 108 and 180; of 512 x 4096, 16 rows 94 and 80.
+template <typename T>
+bool few_rows(const ProductArgs<T>& p) {
+  const int64_t tiles = likely_tiles(p, 64, 64);
+  if (p.outer < 8) return false;
+  if (sizeof(T) == 4 && p.n <= 16 * p.experts && (p.n <= 4 * p.experts || tiles < 1400)) return true;
+  return tiles < 512 && (p.inner >= 512 || p.n <= 16 * p.experts);
+}
+
+}  // namespace products
+}  // namespace gs

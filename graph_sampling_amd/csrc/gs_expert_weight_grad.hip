@@ -10,6 +10,7 @@ namespace {
 
 using products::Group;
 using products::Operand;
+using products::Way;
 
 template <typename T>
 struct WeightGradArgs {
@@ -50,10 +51,10 @@ __device__ __forceinline__ int64_t find_expert(const int64_t* __restrict__ offse
   return products::uniform(s_found);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int RING, bool DIRECT, bool PIECES>
+template <typename T, int BM, int BN, int WM, int WN, int RING, Way WAY, bool PIECES>
 __global__ void __launch_bounds__(WM * WN * kWave)
 weight_grad_kernel(WeightGradArgs<T> p) {
-  using Tile = products::Tile<T, true, true, BM, BN, WM, WN, RING, DIRECT>;
+  using Tile = products::Tile<T, true, true, BM, BN, WM, WN, RING, WAY>;
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
   // (workgroups of one die make tiles of the same expert, or piece, which share its rows)
   const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? p.pieces : p.experts);
@@ -78,43 +79,76 @@ weight_grad_kernel(WeightGradArgs<T> p) {
     tile.write(p.out + (expert * p.inner + row) * p.outer + col, p.outer, p.inner - row, p.outer - col);
 }
 
-// dweight[e] = the sums of its pieces, one after the other.
+// dweight[e] = the sums of its pieces: 16 lanes a run of 64 values, SLICES of them an expert's pieces, slice by slice, the
+// slices one after the other.
 constexpr int kThreads = 256;
-template <typename T>
+template <typename T, int SLICES>
 __global__ void __launch_bounds__(kThreads)
-join_pieces_kernel(WeightGradArgs<T> p) {
-  const int64_t size = p.inner * p.outer, total = p.experts * size;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t e = i / size, at = i - e * size;
+join_pieces_kernel(WeightGradArgs<T> p, int64_t runs) {
+  constexpr int kRuns = kThreads / 16 / SLICES;  // of a workgroup
+  typedef float Four __attribute__((ext_vector_type(4)));
+  typedef T Narrow __attribute__((ext_vector_type(4)));
+  __shared__ Four s_sums[SLICES][kRuns * 16];
+  const int in_run = threadIdx.x % (kRuns * 16), slice = threadIdx.x / (kRuns * 16);
+  const int64_t size = p.inner * p.outer, chunk = static_cast<int64_t>(blockIdx.x) * (kRuns * 16) + in_run;
+  const int64_t e = chunk / (runs * 16), at = (chunk - e * (runs * 16)) * 4, there = e < p.experts ? size - at : 0;
+  Four sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (there > 0) {
     const Pieces of = pieces_of(products::group_of(p.offsets, p.experts, p.n, e), e, p.piece);
-    float sum = 0.0f;
-    for (int64_t q = of.first; q <= of.last; ++q) sum += p.sums[q * size + at];
-    p.out[i] = static_cast<T>(sum);
+    const int64_t many = of.last < of.first ? 0 : of.last - of.first + 1, each = (many + SLICES - 1) / SLICES;
+    const int64_t first = of.first + slice * each, end = first + each <= of.last ? first + each : of.last + 1;
+    const float* from = p.sums + at;
+#pragma unroll 4
+    for (int64_t q = first; q < end; ++q) {
+      Four v;
+      if (there >= 4) {
+        __builtin_memcpy(&v, from + q * size, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < there ? from[q * size + i] : 0.0f;
+      }
+      sum += v;
+    }
   }
+  s_sums[slice][in_run] = sum;
+  __syncthreads();
+  if (slice != 0 || there <= 0) return;
+#pragma unroll
+  for (int k = 1; k < SLICES; ++k) sum += s_sums[k][in_run];
+  products::store_part(p.out + e * size + at, __builtin_convertvector(sum, Narrow), there);
 }
 
 // How the rows are cut: not at all (0) where there are tiles enough.
+constexpr int64_t tiles_of(int64_t inner, int64_t outer) { return (inner + 63) / 64 * ((outer + 63) / 64); }
 int64_t piece_rows(int64_t n, int64_t experts, int64_t tiles) {
-  constexpr int64_t kTiles = 1024, kRows = 512;
+  constexpr int64_t kTiles = 2048, kRows = 128;
   if (tiles * experts >= kTiles / 2 || n < 2 * kRows * experts) return 0;
   const int64_t pieces = kTiles / tiles, rows = (n + pieces - 1) / pieces;
   return rows < kRows ? kRows : (rows + 31) / 32 * 32;
 }
 int64_t pieces_there(int64_t n, int64_t experts, int64_t piece) { return (n + piece - 1) / piece + experts; }
 
-template <typename T, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
+template <typename T, int SLICES>
+int launch_join(const WeightGradArgs<T>& p, hipStream_t st) {
+  const int64_t runs = (p.inner * p.outer + 63) / 64, a_block = kThreads / 16 / SLICES;
+  const int64_t blocks = (p.experts * runs + a_block - 1) / a_block;
+  GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul_grad", blocks, kThreads));
+  hipLaunchKernelGGL((join_pieces_kernel<T, SLICES>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, p, runs);
+  return check_launch("expert_matmul_grad");
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int RING, Way WAY>
 int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_bytes, hipStream_t st) {
   constexpr int threads = WM * WN * kWave;
   p.row_tiles = (p.inner + BM - 1) / BM;
   p.col_tiles = (p.outer + BN - 1) / BN;
   const int64_t tiles = p.row_tiles * p.col_tiles;
-  p.piece = piece_rows(p.n, p.experts, (p.inner + 127) / 128 * ((p.outer + 127) / 128));
+  p.piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer));
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
   if (items > most_blocks(threads) / tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
   const dim3 grid(static_cast<unsigned>((items * tiles + kXcds - 1) / kXcds * kXcds));
   if (!p.piece) {
-    hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, DIRECT, false>), grid, dim3(threads), 0, st, p);
+    hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, false>), grid, dim3(threads), 0, st, p);
     return check_launch("expert_matmul_grad");
   }
   p.pieces = items;
@@ -125,23 +159,32 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
                    gs_expert_matmul_grad_workspace_bytes(p.n, p.inner, p.outer, p.experts));
     return GS_ERR_WORKSPACE;
   }
-  hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, DIRECT, true>), grid, dim3(threads), 0, st, p);
+  hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, true>), grid, dim3(threads), 0, st, p);
   GS_RETURN_IF_ERROR(check_launch("expert_matmul_grad"));
-  const int64_t blocks = (p.experts * p.inner * p.outer + kThreads - 1) / kThreads;
-  hipLaunchKernelGGL((join_pieces_kernel<T>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, st, p);
-  return check_launch("expert_matmul_grad");
+  return items > 16 * p.experts ? launch_join<T, 16>(p, st) : launch_join<T, 4>(p, st);
 }
 
+// As for the products of rows; here a matrix is a product of its own.  bf16, tiles of 256 x 256, 128 x 128 and 64 x 64, us: 32
+// experts of 1024 x 1024, 2000 rows each 164, 217, 371; 4 of those, 500 rows 26, 14, 15; 32 of 256 x 256, 500 rows 32, 15,
+// 12.  fp32 is within 12 % of its best with the smallest.
 template <typename T>
 int choose_weight_grad(const WeightGradArgs<T>& p, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  const bool direct = products::direct_rows(p.rows, p.row_stride, p.inner, 32) &&
-                      products::direct_rows(p.grad, p.grad_stride, p.outer, 32);
-  if (!direct) return launch_weight_grad<T, 128, 128, 2, 2, 3, false>(p, workspace, workspace_bytes, st);
+  const Way way = products::slower(products::way_of(p.rows, p.row_stride, 0, p.inner, 256),
+                                   products::way_of(p.grad, p.grad_stride, 0, p.outer, 256));
+  if (way == Way::kValues) return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kValues>(p, workspace, workspace_bytes, st);
   if constexpr (sizeof(T) == 2) {
-    if (p.inner > 128 && p.outer > 128)
-      return launch_weight_grad<T, 256, 256, 2, 4, 4, true>(p, workspace, workspace_bytes, st);
+    const int64_t tiles128 = (p.inner + 127) / 128 * ((p.outer + 127) / 128) * p.experts;
+    const int64_t tiles256 = (p.inner + 255) / 256 * ((p.outer + 255) / 256) * p.experts;
+    const bool wide = p.inner > 64 && p.outer > 64, wider = p.inner > 128 && p.outer > 128;
+    if (way == Way::kDirect && wider && (tiles256 >= 200 || (tiles256 >= 64 && p.n >= 4096 * p.experts)))
+      return launch_weight_grad<T, 256, 256, 2, 4, 4, Way::kDirect>(p, workspace, workspace_bytes, st);
+    if (wide && tiles128 >= 250) {
+      return way == Way::kDirect ? launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st)
+                                 : launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kChunks>(p, workspace, workspace_bytes, st);
+    }
   }
-  return launch_weight_grad<T, 128, 128, 2, 2, 3, true>(p, workspace, workspace_bytes, st);
+  return way == Way::kDirect ? launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st)
+                             : launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kChunks>(p, workspace, workspace_bytes, st);
 }
 
 }  // namespace
@@ -156,7 +199,7 @@ size_t gs_expert_matmul_grad_workspace_bytes(int64_t n, int64_t inner, int64_t o
   if (n <= 0 || n >= (int64_t(1) << 31) || inner <= 0 || inner >= kMost || outer <= 0 || outer >= kMost || num_experts <= 0 ||
       num_experts >= (int64_t(1) << 31))
     return 256;
-  const int64_t piece = piece_rows(n, num_experts, (inner + 127) / 128 * ((outer + 127) / 128));
+  const int64_t piece = piece_rows(n, num_experts, tiles_of(inner, outer));
   return piece ? padded(static_cast<size_t>(pieces_there(n, num_experts, piece) * inner * outer) * sizeof(float)) : 256;
 }
 

@@ -139,33 +139,103 @@ struct Operand {
   int64_t stride, rows, width;
 };
 
-// Fetches an operand step by step through registers.
-template <typename T, bool ACROSS, int WIDTH, int THREADS>
+// The values of a chunk from the s-th on, zeros behind them.
+template <typename T>
+__device__ __forceinline__ Values<T> shifted(Values<T> v, int s) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
+  Words w = __builtin_bit_cast(Words, v);
+  const int words = sizeof(T) == 4 ? s : s / 2;
+  if (words & 2) w = Words{w[2], w[3], 0, 0};
+  if (words & 1) w = Words{w[1], w[2], w[3], 0};
+  if (sizeof(T) == 2 && (s & 1)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] >> 16) | (i < 3 ? w[i < 3 ? i + 1 : 3] << 16 : 0);
+  }
+  return __builtin_bit_cast(Values<T>, w);
+}
+
+// How an operand comes: straight into LDS, through registers in chunks of any alignment, or, where there is no whole chunk
+// or a step's chunks lie more than 2^31 bytes apart, value by value.
+enum class Way { kDirect, kChunks, kValues };
+
+// Fetches an operand step by step through registers, kHeld steps ahead of their stores to LDS.  In chunks, one of which a
+// part exists is read from as far in front of it as it lacks, and shifted.  Rows and columns that C does not have are given
+// others' values, which nobody looks at; what lies behind the depth is zeros.
+constexpr int kHeld = 4;
+template <typename T, bool ACROSS, int WIDTH, int THREADS, bool CHUNKS>
 struct Staged {
   using L = Layout<T, ACROSS, WIDTH>;
   static constexpr int kEach = (L::kSlots + THREADS - 1) / THREADS;
   Operand<T> x;
-  int64_t k0 = 0;
-  Values<T> held[kEach];
+  const T* next;
+  int64_t step, k0 = 0;  // values between steps; k of the next step
+  bool ragged;           // a part of a chunk exists
+  int at[kEach], lack[kEach];
+  Values<T> held[kHeld][kEach];
 
-  __device__ __forceinline__ explicit Staged(const Operand<T>& operand) : x(operand) {}
-  __device__ __forceinline__ void load() {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int q = i * THREADS + threadIdx.x;
-      const int r = q / L::kRowSlots, c = L::chunk_in(r, q % L::kRowSlots) * L::kVec;
-      const int64_t row = ACROSS ? k0 + r : r, col = ACROSS ? c : k0 + c;
-      const bool in = q < L::kSlots && row < x.rows;
-      held[i] = load_part(x.base + row * x.stride + col, in ? x.width - col : 0);
-    }
-    k0 += kStep<T>;
+  static __device__ __forceinline__ int row(int i) { return (i * THREADS + static_cast<int>(threadIdx.x)) / L::kRowSlots; }
+  static __device__ __forceinline__ int chunk(int i) {
+    return L::chunk_in(row(i), (i * THREADS + static_cast<int>(threadIdx.x)) % L::kRowSlots) * L::kVec;
   }
-  __device__ __forceinline__ void store(char* lds) const {
+  static __device__ __forceinline__ bool mine(int i) {
+    return L::kSlots % THREADS == 0 || i * THREADS + static_cast<int>(threadIdx.x) < L::kSlots;
+  }
+  __device__ __forceinline__ explicit Staged(const Operand<T>& operand) : x(operand), next(operand.base) {
+    step = ACROSS ? kStep<T> * x.stride : kStep<T>;
+    ragged = CHUNKS && ACROSS && x.width < WIDTH && x.width % L::kVec != 0;
+#pragma unroll
+    for (int i = 0; i < kEach && CHUNKS; ++i) {
+      const int64_t across = ACROSS ? x.width - chunk(i) : x.rows - row(i);
+      const bool in = across > 0 && mine(i);
+      lack[i] = ACROSS && in && across < L::kVec ? L::kVec - static_cast<int>(across) : 0;
+      // (a chunk that does not exist: the first one of the row, or of the first row; the tile's first one may lack, too)
+      const int first = ACROSS && x.width < L::kVec ? static_cast<int>(x.width) - L::kVec : 0;
+      at[i] = static_cast<int>((in || (ACROSS && mine(i)) ? row(i) : 0) * x.stride) + (in ? chunk(i) - lack[i] : ACROSS ? first : 0);
+    }
+  }
+  // The first step: the last part of the depth, `rest` of a step, so that all others are whole.
+  __device__ __forceinline__ void load_rest(int64_t whole_steps, int64_t rest) {
+    const T* const from = x.base + whole_steps * step;
+    k0 = whole_steps * kStep<T>;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int q = i * THREADS + threadIdx.x;
-      if (L::kSlots % THREADS == 0 || q < L::kSlots) *reinterpret_cast<Values<T>*>(lds + q * 16) = held[i];
+      if (!CHUNKS) {
+        held[0][i] = part(i, rest);
+      } else {
+        held[0][i] = Values<T>{};
+        const int64_t left = rest - (ACROSS ? row(i) : chunk(i));
+        const int less = !ACROSS && left < L::kVec ? L::kVec - static_cast<int>(left) : 0;
+        if (left > 0 && mine(i)) held[0][i] = shifted<T>(load_chunk(from + row_start(i) + (ACROSS ? 0 : chunk(i) - less), L::kVec), less);
+      }
     }
+    k0 = 0;
+  }
+  __device__ __forceinline__ int row_start(int i) const { return ACROSS ? at[i] : at[i] - (row(i) < x.rows ? chunk(i) : 0); }
+  __device__ __forceinline__ Values<T> part(int i, int64_t left) const {
+    const int64_t r = ACROSS ? k0 + row(i) : row(i), c = ACROSS ? chunk(i) : k0 + chunk(i);
+    const bool in = mine(i) && (ACROSS ? row(i) < left : r < x.rows);
+    return load_part(x.base + r * x.stride + c, in ? (ACROSS ? x.width - c : left - chunk(i)) : 0);
+  }
+  // The next step; more: it is not the last one (which is read again, and not used, behind the end).  whole: there is one.
+  template <int SLOT>
+  __device__ __forceinline__ void load(bool whole, bool more) {
+    if (!whole) return;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) held[SLOT][i] = CHUNKS ? load_chunk(next + at[i], L::kVec) : part(i, kStep<T>);
+    if (more) {
+      k0 += kStep<T>;
+      next += step;
+    }
+  }
+  template <int SLOT>
+  __device__ __forceinline__ void store(char* lds) {
+    if (ragged) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) held[SLOT][i] = shifted<T>(held[SLOT][i], lack[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (mine(i)) *reinterpret_cast<Values<T>*>(lds + (i * THREADS + threadIdx.x) * 16) = held[SLOT][i];
   }
 };
 
@@ -220,13 +290,15 @@ struct Direct {
   static constexpr int kAll = 0x7fffffff;
 };
 
-// Whether rows of `width` values, `stride` apart, can go straight into LDS, `rows` of them a step.
+// How rows of `width` values, `stride` apart, come, up to `rows` of them a step; `apart`: other matrices' distance.
 template <typename T>
-bool direct_rows(const T* base, int64_t stride, int64_t width, int64_t rows) {
+Way way_of(const T* base, int64_t stride, int64_t apart, int64_t width, int64_t rows) {
   constexpr int64_t kVec = Chunk<T>::kVec;
-  return aligned_to(base, 16) && stride % kVec == 0 && width % kVec == 0 &&
-         stride < (int64_t(1) << 31) / (rows * static_cast<int64_t>(sizeof(T)));
+  if (width < kVec || stride >= (int64_t(1) << 31) / (rows * static_cast<int64_t>(sizeof(T)))) return Way::kValues;
+  const bool aligned = aligned_to(base, 16) && stride % kVec == 0 && apart % kVec == 0 && width % kVec == 0;
+  return aligned ? Way::kDirect : Way::kChunks;
 }
+inline Way slower(Way a, Way b) { return a > b ? a : b; }
 
 // All but the last LEFT of a wave's fetches have arrived, and all waves of the workgroup have come here.
 template <int LEFT>
@@ -235,7 +307,7 @@ __device__ __forceinline__ void arrived() {
 }
 
 // A tile of BM x BN by WM x WN waves, RING steps in LDS (three or four).
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING, bool DIRECT>
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING, Way WAY>
 struct Tile {
   using LA = Layout<T, A_ACROSS, BM>;
   using LB = Layout<T, B_ACROSS, BN>;
@@ -244,8 +316,9 @@ struct Tile {
   static constexpr int kThreads = WM * WN * kWave;
   static constexpr int kMI = BM / WM / 16, kNI = BN / WN / 16, kFirst = kMI / 2;
   static constexpr int kStage = LA::kBytes + LB::kBytes, kBytes = RING * kStage;  // of LDS
-  using FA = std::conditional_t<DIRECT, Direct<T, A_ACROSS, BM, kThreads>, Staged<T, A_ACROSS, BM, kThreads>>;
-  using FB = std::conditional_t<DIRECT, Direct<T, B_ACROSS, BN, kThreads>, Staged<T, B_ACROSS, BN, kThreads>>;
+  static constexpr bool kDirect = WAY == Way::kDirect, kChunks = WAY == Way::kChunks;
+  using FA = std::conditional_t<kDirect, Direct<T, A_ACROSS, BM, kThreads>, Staged<T, A_ACROSS, BM, kThreads, kChunks>>;
+  using FB = std::conditional_t<kDirect, Direct<T, B_ACROSS, BN, kThreads>, Staged<T, B_ACROSS, BN, kThreads, kChunks>>;
   Acc acc[kMI][kNI];
 
   static __device__ __forceinline__ int row0() { return static_cast<int>(threadIdx.x) / kWave / WN * (BM / WM); }
@@ -283,10 +356,22 @@ struct Tile {
     FB fb;
     char* lds;
     int64_t ahead;  // steps that are not on their way yet
+    bool whole;     // there are whole ones
 
     __device__ __forceinline__ void fetch(int i, uint32_t to, int bytes) {
       if (i < FA::kEach) fa.part(i, to, bytes);
       else fb.part(i - FA::kEach, to + LA::kBytes, bytes);
+    }
+    template <int SLOT>
+    __device__ __forceinline__ void load() {  // (through registers)
+      fa.template load<SLOT>(whole, ahead > 1);
+      fb.template load<SLOT>(whole, ahead > 1);
+      --ahead;
+    }
+    template <int SLOT>
+    __device__ __forceinline__ void store(char* to) {
+      fa.template store<SLOT>(to);
+      fb.template store<SLOT>(to + LA::kBytes);
     }
     __device__ __forceinline__ void advance() {
       fa.advance();
@@ -295,7 +380,7 @@ struct Tile {
     }
   };
 
-  // a step in ring place `now`, its fragments of b in f.b[TURN]
+  // a step in ring place `now`, its fragments of b in f.b[TURN % 2]
   template <int TURN>
   __device__ __forceinline__ void step(Fragments& f, Steps& s, uint32_t now) {
     const uint32_t next = now + kStage == kBytes ? 0 : now + kStage;
@@ -304,23 +389,20 @@ struct Tile {
 #pragma unroll
       for (int r = due(q, kLater, kFirstProducts); r < due(q + 1, kLater, kFirstProducts); ++r)
         f.a[kFirst + r] = s.ra.fragment(kFirst + r, now);
-      acc[q / kNI][q % kNI] = multiply(f.b[TURN][q % kNI], f.a[q / kNI], acc[q / kNI][q % kNI]);
+      acc[q / kNI][q % kNI] = multiply(f.b[TURN % 2][q % kNI], f.a[q / kNI], acc[q / kNI][q % kNI]);
       __builtin_amdgcn_sched_barrier(0);
     }
     uint32_t to = 0;
     int bytes = 0;
-    if constexpr (DIRECT) {
+    if constexpr (kDirect) {
       arrived<(RING - 3) * kFetches>();
       to = lds_offset(s.lds) + (now == 0 ? kBytes - kStage : now - kStage) +
            __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
       bytes = s.ahead > 0 ? FA::kAll : 0;
     } else {
       __syncthreads();
-      char* const slot = s.lds + (now + 2 * kStage) % kBytes;
-      s.fa.store(slot);
-      s.fb.store(slot + LA::kBytes);
-      s.fa.load();
-      s.fb.load();
+      s.template store<(TURN + 2) % kHeld>(s.lds + (now + 2 * kStage) % kBytes);
+      s.template load<(TURN + 2) % kHeld>();
     }
     if (kFirst == 0) f.a[0] = s.ra.fragment(0, now);
 #pragma unroll
@@ -329,16 +411,16 @@ struct Tile {
 #pragma unroll
       for (int r = due_ahead(q); r < due_ahead(q + 1); ++r) {
         if (r < kFirst) f.a[r] = s.ra.fragment(r, next);
-        else f.b[TURN ^ 1][r - kFirst] = s.rb.fragment(r - kFirst, next);
+        else f.b[(TURN + 1) % 2][r - kFirst] = s.rb.fragment(r - kFirst, next);
       }
-      if constexpr (DIRECT) {
+      if constexpr (kDirect) {
 #pragma unroll
         for (int r = due_fetch(q); r < due_fetch(q + 1); ++r) s.fetch(r, to, bytes);
       }
-      acc[i][j] = multiply(f.b[TURN][j], f.a[i], acc[i][j]);
+      acc[i][j] = multiply(f.b[TURN % 2][j], f.a[i], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (DIRECT) s.advance();
+    if constexpr (kDirect) s.advance();
   }
 
   // lds: kBytes, aligned to 1024 (parts of addresses are exchanged by exclusive or)
@@ -349,8 +431,8 @@ struct Tile {
       for (int j = 0; j < kNI; ++j) acc[i][j] = Acc{};
     int64_t steps = (depth + kStep<T> - 1) / kStep<T>;
     if (steps <= 0) return;
-    Steps s{RA(lds_offset(lds), row0()), RB(lds_offset(lds) + LA::kBytes, col0()), FA(a), FB(b), lds, steps};
-    if constexpr (DIRECT) {
+    Steps s{RA(lds_offset(lds), row0()), RB(lds_offset(lds) + LA::kBytes, col0()), FA(a), FB(b), lds, steps, depth >= kStep<T>};
+    if constexpr (kDirect) {
       const uint32_t to = lds_offset(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
       const int64_t whole = depth / kStep<T>, rest = depth % kStep<T>;
       if (rest > 0) {
@@ -367,15 +449,21 @@ struct Tile {
       }
       arrived<(RING - 2) * kFetches>();
     } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s.fa.load();
-        s.fb.load();
-        s.fa.store(lds + i * kStage);
-        s.fb.store(lds + i * kStage + LA::kBytes);
+      const int64_t whole = depth / kStep<T>, rest = depth % kStep<T>;
+      if (rest > 0) {
+        s.fa.load_rest(whole, rest);
+        s.fb.load_rest(whole, rest);
+        --s.ahead;
+      } else {
+        s.template load<0>();
       }
-      s.fa.load();
-      s.fb.load();
+      s.template load<1>();
+      s.template load<2>();
+      s.template load<3>();
+      s.template store<0>(lds);
+      s.template load<0>();
+      s.template store<1>(lds + kStage);
+      s.template load<1>();
       __syncthreads();
     }
     Fragments f;
@@ -383,18 +471,32 @@ struct Tile {
     for (int j = 0; j < kNI; ++j) f.b[0][j] = s.rb.fragment(j, 0);
 #pragma unroll
     for (int i = 0; i < kFirst; ++i) f.a[i] = s.ra.fragment(i, 0);
-    // (two steps a turn, so that what is read ahead stays in its registers; one behind the last is zeros)
+    // (two steps a turn, or four, so that what is read ahead stays in its registers; straight into LDS, one behind the last
+    // is zeros)
     uint32_t now = 0;
     auto place = [&] {
       const uint32_t here = now;
       now = now + kStage == kBytes ? 0 : now + kStage;
       return here;
     };
-    for (; steps > 0; steps -= 2) {
-      step<0>(f, s, place());
-      step<1>(f, s, place());
+    if constexpr (kDirect) {
+      for (; steps > 0; steps -= 2) {
+        step<0>(f, s, place());
+        step<1>(f, s, place());
+      }
+    } else {
+      while (true) {
+        step<0>(f, s, place());
+        if (--steps == 0) break;
+        step<1>(f, s, place());
+        if (--steps == 0) break;
+        step<2>(f, s, place());
+        if (--steps == 0) break;
+        step<3>(f, s, place());
+        if (--steps == 0) break;
+      }
     }
-    if constexpr (DIRECT) arrived<0>();  // (nothing is on its way into LDS that the next workgroup has by then)
+    if constexpr (kDirect) arrived<0>();  // (nothing is on its way into LDS that the next workgroup has by then)
   }
 
   // Rounds the sums, once, to nearest, ties to even, and writes rows 0 .. rows - 1 and columns 0 .. cols - 1 of the tile to out.
