@@ -80,7 +80,7 @@ inline int64_t most_row_tiles(int64_t n, int64_t experts, int64_t tile_rows) {
 // Tiles that there will be, more or less: half a tile of rows for every expert is not full.
 template <typename T>
 int64_t likely_tiles(const ProductArgs<T>& p, int64_t tile_rows, int64_t tile_cols) {
-  const int64_t some = p.n < p.experts ? p.n : p.experts, full = p.n / tile_rows + p.experts / 2;
+  const int64_t some = p.n < p.experts ? p.n : p.experts, full = p.n / tile_rows + some / 2;
   return (full > some ? full : some) * ((p.outer + tile_cols - 1) / tile_cols);
 }
 
