@@ -56,7 +56,7 @@ few_rows_kernel(ProductArgs<T> p) {
   __shared__ __attribute__((aligned(16))) float s_sums[kWaves][kRows][kPad];
   RowTile t = find_tile<kThreads>(p.offsets, p.experts, p.n, kRows, p.col_tiles);
   if (t.rows <= 0) return;
-  t = {uniform(t.expert), uniform(t.begin), uniform(t.rows), uniform(t.col)};
+  t = {uniform(t.expert), uniform(t.begin), uniform(t.rows), uniform(t.col), -1};
   const int lane = threadIdx.x % kWave, row16 = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t rows = t.rows < kRows ? t.rows : kRows;

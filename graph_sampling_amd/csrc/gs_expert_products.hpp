@@ -11,11 +11,15 @@ struct RowTile {
   int64_t expert, begin;  // of the tile's rows
   int64_t rows;           // up to the expert's last; none: no tile
   int64_t col;            // which tile of columns
+  int64_t quarter;        // of the tile, or -1: the whole of it
 };
 
+constexpr int64_t kCus = 256;  // workgroups of large tiles that run at once
+
 // Every thread counts the tiles of rows of its share of the experts; the one in whose share the workgroup's lies finds it.
-// Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.
-template <int THREADS>
+// Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.  QUARTERS: tiles that
+// would fill less than half of the card, after all others have filled it, are made in quarters.
+template <int THREADS, bool QUARTERS = false>
 __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
                                              int64_t col_tiles) {
   __shared__ int64_t s_wave[THREADS / kWave];
@@ -40,8 +44,13 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
     if (w < static_cast<int>(threadIdx.x) / kWave) upto += s_wave[w];
     total += s_wave[w];
   }
-  const int64_t tiles = total * col_tiles, per_die = (tiles + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds;
-  const int64_t which = blockIdx.x % kXcds * per_die + slot, at = slot < per_die ? which / col_tiles : total;
+  const int64_t tiles = total * col_tiles, rest = QUARTERS && tiles % kCus <= kCus / 2 ? tiles % kCus : 0;
+  const int64_t whole = tiles - rest, whole_blocks = (whole + kXcds - 1) / kXcds * kXcds;
+  const bool part = QUARTERS && blockIdx.x >= whole_blocks;
+  const int64_t block = part ? blockIdx.x - whole_blocks : blockIdx.x, many = part ? rest * 4 : whole;
+  const int64_t per_die = (many + kXcds - 1) / kXcds, slot = block / kXcds, nth = block % kXcds * per_die + slot;
+  const int64_t which = part ? whole + nth / 4 : nth;
+  const int64_t at = slot < per_die && nth < many ? which / col_tiles : total;
   int64_t from = upto - mine;
   if (at >= from && at < upto) {
     for (int64_t e = first; e < last; ++e) {
@@ -59,6 +68,7 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
   __syncthreads();
   RowTile t = s_found;
   t.col = which % col_tiles;
+  t.quarter = part ? nth % 4 : -1;
   return t;
 }
 
