@@ -56,10 +56,19 @@ __global__ void __launch_bounds__(WM * WN * kWave)
 weight_grad_kernel(WeightGradArgs<T> p) {
   using Tile = products::Tile<T, true, true, BM, BN, WM, WN, RING, WAY>;
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
-  // (workgroups of one die make tiles of the same expert, or piece, which share its rows)
+  // Workgroups of one die make tiles that share rows: neighbours of one expert, or piece.  Every die has its share of each
+  // expert with many tiles, because one may have many more rows than the next.
   const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? p.pieces : p.experts);
-  const int64_t per_die = (all + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds, which = blockIdx.x % kXcds * per_die + slot;
-  if (slot >= per_die || which >= all) return;
+  const int64_t die = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  int64_t which;
+  if (in_expert >= 2 * kXcds) {
+    const int64_t share = (in_expert + kXcds - 1) / kXcds, nth = die * share + slot % share;
+    which = nth < in_expert ? slot / share * in_expert + nth : all;
+  } else {
+    const int64_t per_die = (all + kXcds - 1) / kXcds;
+    which = slot < per_die ? die * per_die + slot : all;
+  }
+  if (which >= all) return;
   const int64_t at = which % in_expert, row = at / p.col_tiles * BM, col = at % p.col_tiles * BN;
   int64_t expert = which / in_expert;
   if (PIECES) expert = find_expert<Tile::kThreads>(p.offsets, p.experts, p.n, p.piece, which / in_expert);
@@ -145,8 +154,9 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   const int64_t tiles = p.row_tiles * p.col_tiles;
   p.piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer));
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
-  if (items > most_blocks(threads) / tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
-  const dim3 grid(static_cast<unsigned>((items * tiles + kXcds - 1) / kXcds * kXcds));
+  const int64_t padded_tiles = tiles >= 2 * kXcds ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;  // (a share a die)
+  if (items > most_blocks(threads) / padded_tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
+  const dim3 grid(static_cast<unsigned>((items * padded_tiles + kXcds - 1) / kXcds * kXcds));
   if (!p.piece) {
     hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, false>), grid, dim3(threads), 0, st, p);
     return check_launch("expert_matmul_grad");
