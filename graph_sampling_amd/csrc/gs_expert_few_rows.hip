@@ -14,39 +14,6 @@ namespace {
 
 constexpr int kWaves = 8, kThreads = kWaves * kWave;
 
-// A step of `wide` columns: what a lane holds of it.
-//   across the depth: column group l % 16, kVec rows of k from (l / 16) * kVec on, COLS values of each
-//   along the depth: columns l % 16 of kFrags groups of 16, kVec values of k from (l / 16) * kVec on
-template <typename T, bool ACROSS, int COLS>
-struct Slab {
-  static constexpr int kVec = Chunk<T>::kVec;
-  static constexpr int kLoads = ACROSS ? kVec : COLS;  // (COLS fragments)
-  static constexpr int kWide = 16 * COLS;              // columns
-  typedef T Piece __attribute__((ext_vector_type(ACROSS ? COLS : kVec)));
-  Piece held[kLoads];
-
-  // The fragment of columns (l % 16) * COLS + c, or c * 16 + l % 16.
-  __device__ __forceinline__ Values<T> fragment(int c) const {
-    if constexpr (!ACROSS) {
-      return held[c];
-    } else if constexpr (sizeof(T) == 4) {
-      return Values<T>{held[0][c], held[1][c], held[2][c], held[3][c]};
-    } else {
-      typedef uint32_t Words __attribute__((ext_vector_type(COLS / 2)));
-      union {
-        uint32_t word[4];
-        Values<T> v;
-      } u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t low = __builtin_bit_cast(Words, held[2 * i])[c / 2], high = __builtin_bit_cast(Words, held[2 * i + 1])[c / 2];
-        u.word[i] = __builtin_amdgcn_perm(high, low, c % 2 ? 0x07060302u : 0x05040100u);
-      }
-      return u.v;
-    }
-  }
-};
-
 template <typename T, bool ACROSS, int MI, int COLS>
 __global__ void __launch_bounds__(kThreads)
 few_rows_kernel(ProductArgs<T> p) {

@@ -70,6 +70,7 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
 // largest).  fp32, which is bound by its products, is within 5 % of its best with the smallest.
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
+  if (products::narrow(p)) return products::launch_narrow(p, ACROSS, st);
   if (products::few_rows(p)) return products::launch_few_rows(p, ACROSS, st);
   const Way way = products::slower(products::way_of(p.rows, p.row_stride, 0, p.inner, 256),
                                    products::way_of(p.weight, p.weight_stride, p.expert_stride, ACROSS ? p.outer : p.inner, 256));
@@ -105,8 +106,8 @@ extern "C" int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n,
   GS_REQUIRE(inner < (int64_t(1) << 24) && outer < (int64_t(1) << 24),
              "gs_expert_matmul: rows of %lld and %lld values, at most 2^24 - 1 are taken", static_cast<long long>(inner),
              static_cast<long long>(outer));
-  GS_REQUIRE(num_experts < (int64_t(1) << 31), "gs_expert_matmul: %lld experts, at most 2^31 - 1 are taken",
-             static_cast<long long>(num_experts));
+  GS_REQUIRE(num_experts <= products::kMostExperts, "gs_expert_matmul: %lld experts, at most %lld are taken",
+             static_cast<long long>(num_experts), static_cast<long long>(products::kMostExperts));
   GS_REQUIRE(row_stride >= 0 && expert_stride >= 0 && weight_stride >= 0, "gs_expert_matmul: negative stride");
   if (n == 0 || outer == 0) return GS_OK;
   GS_REQUIRE(offsets && out && (inner == 0 || (rows && (num_experts == 0 || weight))), "gs_expert_matmul: null array");

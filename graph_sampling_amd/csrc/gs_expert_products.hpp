@@ -94,9 +94,58 @@ int64_t likely_tiles(const ProductArgs<T>& p, int64_t tile_rows, int64_t tile_co
   return (full > some ? full : some) * ((p.outer + tile_cols - 1) / tile_cols);
 }
 
+// A step of 16 * COLS columns of a matrix: what a lane holds of it.
+//   across the depth: column group l % 16, kVec rows of k from (l / 16) * kVec on, COLS values of each
+//   along the depth: columns l % 16 of kFrags groups of 16, kVec values of k from (l / 16) * kVec on
+template <typename T, bool ACROSS, int COLS>
+struct Slab {
+  static constexpr int kVec = Chunk<T>::kVec;
+  static constexpr int kLoads = ACROSS ? kVec : COLS;  // (COLS fragments)
+  static constexpr int kWide = 16 * COLS;              // columns
+  typedef T Piece __attribute__((ext_vector_type(ACROSS ? COLS : kVec)));
+  Piece held[kLoads];
+
+  // The fragment of columns (l % 16) * COLS + c, or c * 16 + l % 16.
+  __device__ __forceinline__ Values<T> fragment(int c) const {
+    if constexpr (!ACROSS) {
+      return held[c];
+    } else if constexpr (sizeof(T) == 4) {
+      return Values<T>{held[0][c], held[1][c], held[2][c], held[3][c]};
+    } else {
+      typedef uint32_t Words __attribute__((ext_vector_type(COLS / 2)));
+      union {
+        uint32_t word[4];
+        Values<T> v;
+      } u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t low = __builtin_bit_cast(Words, held[2 * i])[c / 2], high = __builtin_bit_cast(Words, held[2 * i + 1])[c / 2];
+        u.word[i] = __builtin_amdgcn_perm(high, low, c % 2 ? 0x07060302u : 0x05040100u);
+      }
+      return u.v;
+    }
+  }
+};
+
 // The products of experts with few rows each (gs_expert_few_rows.hip), and whether they are such.
 template <typename T>
 int launch_few_rows(const ProductArgs<T>& p, bool across, hipStream_t st);
+
+// The products with small matrices (gs_expert_narrow.hip), and whether they are such: a wave's registers hold one, and each
+// workgroup of one round has rows enough to make up for fetching it.  Kernel times of this and of tiles, us: bf16, 5 experts
+// of 100 x 128, 150 000 rows 18 and 27, 700 000 rows 64 and 123; 64 x 128, 150 000 rows 17 and 17, transposed, 300 000 rows 25
+// and 28; 256 x 64, 150 000 rows 25 and 22, 300 000 rows 39 and 39; 64 experts of 128 x 64, 150 000 rows 17 and 16, 300 000 rows
+// 23 and 28; fp32, 5 experts of 64 x 128, 150 000 rows 37 and 37, 700 000 rows 126 and 174; 60 x 40, 300 000 rows 36 and 35; 64
+// experts of 128 x 64, 700 000 rows 149 and 136.
+template <typename T>
+int launch_narrow(const ProductArgs<T>& p, bool across, hipStream_t st);
+template <typename T>
+bool narrow(const ProductArgs<T>& p) {
+  constexpr bool kHalf = sizeof(T) == 2;
+  const int64_t steps = (p.inner + kStep<T> - 1) / kStep<T>;
+  const bool held = p.inner >= 8 && p.outer >= 8 && p.outer <= 128 && steps <= (p.outer <= 64 ? 8 : 4);
+  return held && p.n >= (kHalf ? 1 << 18 : 1 << 19) && p.experts <= (kHalf ? 64 : 16);
+}
 
 // Where 64 x 64 tiles do not fill the card twice, the depth of a tile has to be shared out, too, if it is long; fp32, whose
 // products take sixteen times as long, gains by it with few rows whatever their number.  Kernel times of both, us, few

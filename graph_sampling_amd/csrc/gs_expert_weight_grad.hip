@@ -207,16 +207,15 @@ extern "C" {
 size_t gs_expert_matmul_grad_workspace_bytes(int64_t n, int64_t inner, int64_t outer, int64_t num_experts) {
   constexpr int64_t kMost = int64_t(1) << 24;
   if (n <= 0 || n >= (int64_t(1) << 31) || inner <= 0 || inner >= kMost || outer <= 0 || outer >= kMost || num_experts <= 0 ||
-      num_experts >= (int64_t(1) << 31))
+      num_experts > products::kMostExperts)
     return 256;
   const int64_t piece = piece_rows(n, num_experts, tiles_of(inner, outer));
   return piece ? padded(static_cast<size_t>(pieces_there(n, num_experts, piece) * inner * outer) * sizeof(float)) : 256;
 }
 
-int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, const void* grad,
-                                     int64_t grad_stride, int64_t outer, int type, int64_t n, const int64_t* offsets,
-                                     int64_t num_experts, void* dweight, void* workspace, size_t workspace_bytes,
-                          void* stream) {
+int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, const void* grad, int64_t grad_stride,
+                          int64_t outer, int type, int64_t n, const int64_t* offsets, int64_t num_experts, void* dweight,
+                          void* workspace, size_t workspace_bytes, void* stream) {
   GS_REQUIRE(type == GS_F32 || type == GS_F16 || type == GS_BF16,
              "gs_expert_matmul_grad: value type %d is none of GS_F32, GS_F16, GS_BF16", type);
   GS_REQUIRE(n >= 0 && inner >= 0 && outer >= 0 && num_experts >= 0, "gs_expert_matmul_grad: negative size");
@@ -225,8 +224,8 @@ int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, c
   GS_REQUIRE(inner < (int64_t(1) << 24) && outer < (int64_t(1) << 24),
              "gs_expert_matmul_grad: rows of %lld and %lld values, at most 2^24 - 1 are taken",
              static_cast<long long>(inner), static_cast<long long>(outer));
-  GS_REQUIRE(num_experts < (int64_t(1) << 31), "gs_expert_matmul_grad: %lld experts, at most 2^31 - 1 are taken",
-             static_cast<long long>(num_experts));
+  GS_REQUIRE(num_experts <= products::kMostExperts, "gs_expert_matmul_grad: %lld experts, at most %lld are taken",
+             static_cast<long long>(num_experts), static_cast<long long>(products::kMostExperts));
   GS_REQUIRE(row_stride >= 0 && grad_stride >= 0, "gs_expert_matmul_grad: negative stride");
   if (num_experts == 0 || inner == 0 || outer == 0) return GS_OK;
   GS_REQUIRE(offsets && dweight && (n == 0 || (rows && grad)), "gs_expert_matmul_grad: null array");

@@ -132,6 +132,35 @@ __device__ __forceinline__ void store_part(T* p, V v, int64_t there) {
   }
 }
 
+// Rounds a lane's sums, columns j * 16 + (l / 16) * 4 .. of a row, once, to nearest, ties to even, and writes the first
+// `there` columns of the row.
+template <int FRAGMENTS, typename O>
+__device__ __forceinline__ void write_row(const Acc* acc, O* row, int64_t there) {
+  typedef O Four __attribute__((ext_vector_type(4)));
+  const int quarter = threadIdx.x % kWave / 16;
+  if constexpr (sizeof(O) == 2 && FRAGMENTS % 2 == 0) {
+    // two fragments' neighbouring quarters trade places, so that a lane has eight columns side by side
+#pragma unroll
+    for (int j = 0; j < FRAGMENTS; j += 2) {
+      typedef uint32_t Two __attribute__((ext_vector_type(2)));
+      const Two a = __builtin_bit_cast(Two, __builtin_convertvector(acc[j], Four));
+      const Two b = __builtin_bit_cast(Two, __builtin_convertvector(acc[j + 1], Four));
+      const Two x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+      const Two y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+      union {
+        uint32_t word[4];
+        Values<O> v;
+      } u = {{x[0], y[0], x[1], y[1]}};
+      const int n = (j + quarter % 2) * 16 + quarter / 2 * 8;
+      store_part(row + n, u.v, there - n);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < FRAGMENTS; ++j)
+      store_part(row + j * 16 + quarter * 4, __builtin_convertvector(acc[j], Four), there - j * 16 - quarter * 4);
+  }
+}
+
 // An operand of a tile: `rows` rows (along k: of C; across k: of k), `stride` values apart, of `width` values.
 template <typename T>
 struct Operand {
@@ -502,37 +531,16 @@ struct Tile {
   // Rounds the sums, once, to nearest, ties to even, and writes rows 0 .. rows - 1 and columns 0 .. cols - 1 of the tile to out.
   template <typename O>
   __device__ __forceinline__ void write(O* out, int64_t stride, int64_t rows, int64_t cols) const {
-    typedef O Four __attribute__((ext_vector_type(4)));
-    const int lane = threadIdx.x % kWave, quarter = lane / 16;
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
-      const int m = row0() + i * 16 + lane % 16;
-      O* const row = out + m * stride + col0();
-      const int64_t there = m < rows ? cols - col0() : 0;
-      if constexpr (sizeof(O) == 2 && kNI % 2 == 0) {
-        // two fragments' neighbouring quarters trade places, so that a lane has eight columns side by side
-#pragma unroll
-        for (int j = 0; j < kNI; j += 2) {
-          typedef uint32_t Two __attribute__((ext_vector_type(2)));
-          const Two a = __builtin_bit_cast(Two, __builtin_convertvector(acc[i][j], Four));
-          const Two b = __builtin_bit_cast(Two, __builtin_convertvector(acc[i][j + 1], Four));
-          const Two x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-          const Two y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-          union {
-            uint32_t word[4];
-            Values<O> v;
-          } u = {{x[0], y[0], x[1], y[1]}};
-          const int n = (j + quarter % 2) * 16 + quarter / 2 * 8;
-          store_part(row + n, u.v, there - n);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kNI; ++j)
-          store_part(row + j * 16 + quarter * 4, __builtin_convertvector(acc[i][j], Four), there - j * 16 - quarter * 4);
-      }
+      const int m = row0() + i * 16 + static_cast<int>(threadIdx.x) % 16;
+      write_row<kNI>(acc[i], out + m * stride + col0(), m < rows ? cols - col0() : 0);
     }
   }
 };
+
+// Every workgroup looks through all experts' offsets for its own rows, up to half a megabyte.
+constexpr int64_t kMostExperts = 1 << 16;
 
 // Where an expert's rows begin and end, inside [0, n] whatever the offsets hold.  Expert `experts` has the rows behind the last.
 struct Group {

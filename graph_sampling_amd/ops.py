@@ -164,8 +164,8 @@ def expert_choose(logits, choices, normalize=True):
 def expert_matmul(rows, order, weight):
     """The rows of expert e (offsets[e] to offsets[e + 1] of `rows`, [items, inner]) times weight[e] ([inner,
     outer]): [items, outer], zeros behind the last expert's rows.  `weight` is [experts, inner, outer] of the rows'
-    type; a transposed view of [experts, outer, inner] is read as it lies.  Products are summed in float32 and rounded
-    once; no expert's number of rows is brought to the host.  Differentiable in `rows` and `weight`.
+    type, up to 65536 experts; a transposed view of [experts, outer, inner] is read as it lies.  Products are summed in
+    float32 and rounded once; no expert's number of rows is brought to the host.  Differentiable in `rows` and `weight`.
 
         rows, order = gs.ops.expert_dispatch(x, experts, num_experts)
         h = torch.relu(gs.ops.expert_matmul(rows, order, w_in))

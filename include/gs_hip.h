@@ -1107,7 +1107,7 @@ int gs_expert_choose_grad(const void* logits, int64_t stride, int type, const in
                           void* dlogits, void* stream);
 
 /* out[p, :] = rows[p, :] x the matrix of expert e for offsets[e] <= p < offsets[e + 1], zeros in the rows from
- * offsets[num_experts] to n (below 2^31).  rows: n rows of `inner` values, row_stride apart; out: n x outer.  The
+ * offsets[num_experts] to n (below 2^31); up to 65536 experts.  rows: n rows of `inner` values, row_stride apart; out: n x outer.  The
  * matrix of expert e begins at weight + e * expert_stride: `inner` rows of `outer` values, weight_stride apart, or, if
  * transposed, `outer` rows of `inner` values.  Products are exact, sums fp32 in the order of `inner`, rounded once.
  * offsets ascend from 0; others leave out rows or write them twice, but nothing outside out.  Also the gradient of rows,
@@ -1127,8 +1127,8 @@ int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, c
 
 /* out[i] = residual[i] (NULL: 0) + (draw(seed, tag 6, row 0, i) >= floor(p * 2^32) ? x[i] / (1 - p) : 0), i < n, in fp32,
  * rounded once; p = 1 drops everything.  seed_at (device, may be NULL) holds the seed instead, so that a recorded call
- * draws anew at each replay.  x is not read for its sign or value where it is dropped (NaN leaves no trace).  The gradient
- * of x is the same call on the gradient, without residual.  (No counterpart in the reference.) */
+ * draws anew at each replay.  What is dropped leaves no trace (NaN neither).  The gradient of x is the same call on the
+ * gradient, without residual.  (No counterpart in the reference.) */
 int gs_dropout(const void* x, const void* residual, int64_t n, int type, double p, uint64_t seed, const int64_t* seed_at,
                void* out, void* stream);
 

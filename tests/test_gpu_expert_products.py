@@ -525,6 +525,64 @@ def test_a_layer_of_experts_end_to_end(dev):
             assert (a.double() - b).abs().max() <= (T * K + 300) * 2.0 ** -23 * b.abs().max()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_with_small_matrices(dev, dtype):
+    """Types of nodes: from 2^18 rows on (fp32 2^19), matrices of a few dozen to a few hundred values a side; whole numbers."""
+    n = (1 << (19 if dtype == torch.float32 else 18)) + 77
+    for experts, inner, outer, kind, transposed in (
+            (5, 100, 128, "skewed", False), (5, 128, 100, "skewed", True), (64, 8, 8, "skewed", False), (16, 8, 8, "skewed", True), (3, 33, 65, "even", True),
+            (1, 256, 64, "first", False), (2, 31, 9, "last", False), (4, 64, 127, "skewed", True), (0, 16, 24, "none", False),
+            (7, 129, 40, "skewed", True), (2, 9, 15, "none", False), (65, 40, 24, "even", False), (3, 16, 7, "skewed", False)):
+        loads = loads_of(kind, n, experts, experts + inner)
+        order = order_of(loads, n, dev)
+        rows = whole(n, inner, dtype=dtype, dev=dev, seed=inner)
+        weight = weights_of(whole, experts, inner, outer, transposed, dtype=dtype, dev=dev, seed=outer)
+        want = formula(rows, loads, weight)[0].to(dtype)
+        assert torch.equal(gs.ops.expert_matmul(rows, order, weight), want)
+        wide = whole(n, inner + 3, dtype=dtype, dev=dev, seed=1)  # rows that lie apart, at odd places
+        assert torch.equal(gs.ops.expert_matmul(wide[:, 2:inner + 2], order, weight),
+                           gs.ops.expert_matmul(wide[:, 2:inner + 2].contiguous(), order, weight))
+        if experts > 1 and loads.min() > 0:  # what is others' does not matter
+            at = np.append(0, np.cumsum(loads))
+            rows[at[1]:at[2]], weight[1] = float("nan"), float("inf")
+            rows[at[-1]:] = float("nan")
+            got = gs.ops.expert_matmul(rows, order, weight)
+            assert torch.equal(got[:at[1]], want[:at[1]]) and torch.equal(got[at[2]:], want[at[2]:])
+            assert not got[at[1]:at[2]].isfinite().any()
+
+
+@gpu
+def test_values_below_the_normal_ones(dev):
+    """The smallest numbers of a type count like others."""
+    for dtype, small, large in ((torch.float16, 2.0 ** -24, 2.0 ** 12), (torch.bfloat16, 2.0 ** -133, 2.0 ** 100),
+                                (torch.float32, 2.0 ** -149, 2.0 ** 100)):
+        for n, inner, outer in ((20, 64, 72), (700, 200, 136), ((1 << 19) + 5, 32, 24)):
+            x = (whole(n, inner, dtype=torch.float64, dev=dev, seed=1) * small).to(dtype)
+            w = (whole(2, inner, outer, dtype=torch.float64, dev=dev, seed=2) * large).to(dtype)
+            loads = np.array([n // 2, n - n // 2])
+            want = formula(x, loads, w)[0]
+            assert (want != 0).any()
+            assert torch.equal(gs.ops.expert_matmul(x, order_of(loads, n, dev), w), want.to(dtype))
+
+
+@gpu
+def test_as_many_experts_as_there_may_be(dev):
+    n, experts = 70_000, 65_536
+    loads = loads_of("even", n, experts, 1)
+    order = order_of(loads, n, dev)
+    rows, weight = (whole(*s, dtype=torch.bfloat16, dev=dev, seed=s[-1]) for s in ((n, 16), (experts, 16, 24)))
+    grad = whole(n, 24, dtype=torch.bfloat16, dev=dev, seed=3)
+    of = torch.repeat_interleave(torch.arange(experts, device=dev), torch.from_numpy(loads).to(dev))
+    want = (rows.float()[:, :, None] * weight.float()[of]).sum(1)
+    assert torch.equal(gs.ops.expert_matmul(rows, order, weight).float(), want.bfloat16().float())
+    dw = torch.zeros(experts, 16, 24, device=dev).index_add_(0, of, rows.float()[:, :, None] * grad.float()[:, None])
+    assert torch.equal(capi.expert_matmul_grad(grad, rows, order.offsets).float(), dw.bfloat16().float())
+    too_many = gs.ops.ExpertOrder(order.order, order.place, torch.zeros(experts + 2, dtype=torch.int64, device=dev))
+    with pytest.raises(RuntimeError, match="experts"):
+        gs.ops.expert_matmul(rows, too_many, weight[:1].expand(experts + 1, 16, 24))
+
+
 # ------------------------------------------------------------------ no GPU ----
 def test_bad_arguments_are_refused_before_anything_is_launched():
     import ctypes
@@ -574,3 +632,15 @@ def test_cpu_tensors_are_refused():
     order = gs.ops.ExpertOrder(p, p, torch.zeros(3, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="GPU tensor"):
         gs.ops.expert_matmul(torch.zeros(3, 4), order, torch.zeros(2, 4, 5))
+
+
+def test_more_experts_than_are_taken():
+    import ctypes
+    lib, i64 = capi.lib(), ctypes.c_int64
+    buf = (ctypes.c_int64 * 64)()
+    rc = lib.gs_expert_matmul(buf, i64(8), i64(4), i64(8), 0, buf, i64(64), i64(8), 0, i64(65537), i64(8), buf, buf, None)
+    assert rc < 0 and b"65537 experts" in lib.gs_status_string(rc)
+    rc = lib.gs_expert_matmul_grad(buf, i64(8), i64(8), buf, i64(8), i64(8), 0, i64(4), buf, i64(65537), buf, buf,
+                                   ctypes.c_size_t(256), None)
+    assert rc < 0 and b"65537 experts" in lib.gs_status_string(rc)
+    assert lib.gs_expert_matmul_grad_workspace_bytes(i64(1 << 30), i64(8), i64(8), i64(65537)) == 256
