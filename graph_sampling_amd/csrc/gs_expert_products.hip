@@ -64,30 +64,32 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
   return check_launch("expert_matmul");
 }
 
-// Large tiles read less, small ones fill the card with less work and waste less of it.  bf16, kernel times of tiles of 256 x
-// 256, 128 x 128, 64 x 128 and 64 x 64, us: 160 experts of 1024 x 1024, 200 rows each 130, 147, 161, 206; 32 of those 32, 28,
-// 29, 44; 32 of 1024 x 1024, 40 rows 26, 24, 23, 21; 160 of 256 x 256, 500 rows 33, 28, 30, 34 (too little depth for the
-// largest).  fp32, which is bound by its products, is within 5 % of its best with the smallest.
+// Large tiles read less, small ones fill the card with less work and waste less of it; chunks that are not aligned come more
+// slowly, and make large tiles worth while sooner.  bf16, kernel times of tiles of 256 x 256, 128 x 128, 64 x 128 and 64 x 64, us
+// (aligned: 1152 x 896, 336 x 1008 and 152 x 256; not: 1150 x 890 and 333 x 1001):
+//   32 experts of 1152 x 896, 1000 rows each 63, 74, 88, 115; 200 rows 31, 26, 29, 44; 40 rows (tiles of 64 x 64 fill the card
+//   but twice) 32, 28, 26, 25; of 336 x 1008, 500 rows 29, 28, 33, 44; 5000 rows 204, 236, 287, 348
+//   32 of 1150 x 890, 1000 rows 85, 105, 121, 178; 200 rows 33, 31, 35, 51; of 333 x 1001, 1000 rows 53, 60, 70, 84
+//   160 of 152 x 256, 100 rows 14, 10, 10, 9
+// fp32, which is bound by its products, is within 5 % of its best with the smallest.
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
   if (products::narrow(p)) return products::launch_narrow(p, ACROSS, st);
   if (products::few_rows(p)) return products::launch_few_rows(p, ACROSS, st);
-  const Way way = products::slower(products::way_of(p.rows, p.row_stride, 0, p.inner, 256),
-                                   products::way_of(p.weight, p.weight_stride, p.expert_stride, ACROSS ? p.outer : p.inner, 256));
+  const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256),
+                                   products::way_of<T>(p.weight_stride, ACROSS ? p.outer : p.inner, 256));
   if (way == Way::kValues) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kValues>(p, st);
   if constexpr (sizeof(T) == 2) {
-    if (p.outer > 64 && products::likely_tiles(p, 128, 128) >= 600) {
-      if (way == Way::kChunks) return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kChunks>(p, st);
-      if (p.inner < 512 || products::likely_tiles(p, 256, 256) < 224)
-        return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kDirect>(p, st);
-    }
-    if (way == Way::kDirect && p.outer > 128 && p.inner >= 512 && p.n >= 64 * p.experts &&
-        products::likely_tiles(p, 256, 256) >= 224)
+    const bool aligned = products::aligned_rows(p.rows, p.row_stride, 0) &&
+                         products::aligned_rows(p.weight, p.weight_stride, p.expert_stride);
+    const int64_t enough = !aligned ? 160 : p.inner >= 512 ? 224 : 400;
+    if (p.outer > 128 && p.inner >= 256 && p.n >= 128 * p.experts && products::likely_tiles(p, 256, 256) >= enough)
       return launch_product<T, ACROSS, 256, 256, 2, 4, 4, Way::kDirect>(p, st);
-    if (way == Way::kDirect && p.outer > 64 && products::likely_tiles(p, 64, 128) >= 400)
+    if (p.outer > 64 && p.n >= 64 * p.experts && products::likely_tiles(p, 128, 128) >= 400)
+      return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kDirect>(p, st);
+    if (p.outer > 64 && products::likely_tiles(p, 64, 128) >= 300)
       return launch_product<T, ACROSS, 64, 128, 2, 2, 3, Way::kDirect>(p, st);
   }
-  if (way == Way::kChunks) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kChunks>(p, st);
   return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kDirect>(p, st);
 }
 

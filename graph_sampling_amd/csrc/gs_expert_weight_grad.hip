@@ -51,17 +51,25 @@ __device__ __forceinline__ int64_t find_expert(const int64_t* __restrict__ offse
   return products::uniform(s_found);
 }
 
+// Whether every die has its share of each expert's tiles.  Experts by the die have their rows read by one of them, and leave
+// dies idle whose experts have few; of few experts, or many tiles, that is worse.  bf16, shares and whole experts, us: 8 experts of
+// 4096 x 2048, 2000 rows each 254 and 290; 32 of 250 x 1150, 500 rows 29 and 22; of 2048 x 1024, 200 rows 52 and 58; 160 of
+// 336 x 1008, 200 rows 70 and 48.
+__host__ __device__ __forceinline__ bool shares(int64_t in_expert, int64_t experts) {
+  return in_expert >= (experts < 24 ? 2 * kXcds : 100);
+}
+
 template <typename T, int BM, int BN, int WM, int WN, int RING, Way WAY, bool PIECES>
 __global__ void __launch_bounds__(WM * WN * kWave)
 weight_grad_kernel(WeightGradArgs<T> p) {
   using Tile = products::Tile<T, true, true, BM, BN, WM, WN, RING, WAY>;
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
-  // Workgroups of one die make tiles that share rows: neighbours of one expert, or piece.  Every die has its share of each
-  // expert with many tiles, because one may have many more rows than the next.
+  // Workgroups of one die make tiles that share rows: neighbours of one expert, or piece.  Which die has an expert, or a part
+  // of each, is `shares`.
   const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? p.pieces : p.experts);
   const int64_t die = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
   int64_t which;
-  if (in_expert >= 2 * kXcds) {
+  if (shares(in_expert, p.experts)) {
     const int64_t share = (in_expert + kXcds - 1) / kXcds, nth = die * share + slot % share;
     which = nth < in_expert ? slot / share * in_expert + nth : all;
   } else {
@@ -154,7 +162,7 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   const int64_t tiles = p.row_tiles * p.col_tiles;
   p.piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer));
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
-  const int64_t padded_tiles = tiles >= 2 * kXcds ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;  // (a share a die)
+  const int64_t padded_tiles = shares(tiles, p.experts) ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;
   if (items > most_blocks(threads) / padded_tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
   const dim3 grid(static_cast<unsigned>((items * padded_tiles + kXcds - 1) / kXcds * kXcds));
   if (!p.piece) {
@@ -174,27 +182,26 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   return items > 16 * p.experts ? launch_join<T, 16>(p, st) : launch_join<T, 4>(p, st);
 }
 
-// As for the products of rows; here a matrix is a product of its own.  bf16, tiles of 256 x 256, 128 x 128 and 64 x 64, us: 32
-// experts of 1024 x 1024, 2000 rows each 164, 217, 371; 4 of those, 500 rows 26, 14, 15; 32 of 256 x 256, 500 rows 32, 15,
-// 12.  fp32 is within 12 % of its best with the smallest.
+// As for the products of rows; here a matrix, or what a piece adds to it, is a product of its own, and one of few rows is not
+// worth a large tile's start and end.  bf16, tiles of 256 x 256, 128 x 128 and 64 x 64, us: 32 experts of 1024 x 1024, 2000 rows
+// each 164, 217, 371; of 1152 x 896, 500 rows 68, 60, 71; of 256 x 256, 500 rows (pieces of 128) 30, 30, 32; of 336 x 1008, 1000 rows
+// 53, 61, 84; 4 of those, 5000 rows (28 pieces) 41, 54, 63, 200 rows 13, 7, 6; 4 of 333 x 1001 (not aligned), 40 000 rows 209, 307,
+// 545.  fp32 is within 12 % of its best with the smallest.
 template <typename T>
 int choose_weight_grad(const WeightGradArgs<T>& p, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  const Way way = products::slower(products::way_of(p.rows, p.row_stride, 0, p.inner, 256),
-                                   products::way_of(p.grad, p.grad_stride, 0, p.outer, 256));
+  const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256), products::way_of<T>(p.grad_stride, p.outer, 256));
   if (way == Way::kValues) return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kValues>(p, workspace, workspace_bytes, st);
   if constexpr (sizeof(T) == 2) {
-    const int64_t tiles128 = (p.inner + 127) / 128 * ((p.outer + 127) / 128) * p.experts;
-    const int64_t tiles256 = (p.inner + 255) / 256 * ((p.outer + 255) / 256) * p.experts;
-    const bool wide = p.inner > 64 && p.outer > 64, wider = p.inner > 128 && p.outer > 128;
-    if (way == Way::kDirect && wider && (tiles256 >= 200 || (tiles256 >= 64 && p.n >= 4096 * p.experts)))
+    const int64_t piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer)), each = p.n / p.experts;
+    const int64_t items = piece ? pieces_there(p.n, p.experts, piece) : p.experts, rows = piece && piece < each ? piece : each;
+    const int64_t tiles128 = (p.inner + 127) / 128 * ((p.outer + 127) / 128) * items;
+    const int64_t tiles256 = (p.inner + 255) / 256 * ((p.outer + 255) / 256) * items;
+    if (p.inner > 128 && p.outer > 128 && rows >= 300 && tiles256 >= (piece ? 128 : rows >= 4000 ? 150 : 200))
       return launch_weight_grad<T, 256, 256, 2, 4, 4, Way::kDirect>(p, workspace, workspace_bytes, st);
-    if (wide && tiles128 >= 250) {
-      return way == Way::kDirect ? launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st)
-                                 : launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kChunks>(p, workspace, workspace_bytes, st);
-    }
+    if (p.inner > 64 && p.outer > 64 && tiles128 >= 200)
+      return launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
   }
-  return way == Way::kDirect ? launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st)
-                             : launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kChunks>(p, workspace, workspace_bytes, st);
+  return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
 }
 
 }  // namespace

@@ -553,6 +553,30 @@ def test_many_rows_with_small_matrices(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large_tiles_of_any_alignment(dev, dtype):
+    """Widths that end a few values into a tile or a chunk, rows at odd places; whole numbers."""
+    for n, experts, inner, outer, kind in ((12_100, 2, 259, 1027, "skewed"), (12_100, 2, 1027, 259, "first"),
+                                           (9_001, 3, 1001, 1285, "even"), (6_000, 2, 2049, 1031, "skewed"),
+                                           (30_000, 2, 513, 262, "even"), (3_000, 2, 1999, 1543, "last")):
+        loads = loads_of(kind, n, experts, inner)
+        order = order_of(loads, n, dev)
+        for transposed in (False, True):
+            rows = whole(n, inner + 2, dtype=dtype, dev=dev, seed=1)[:, 1:inner + 1]
+            grad = whole(n, outer + 1, dtype=dtype, dev=dev, seed=2)[:, 1:]
+            weight = weights_of(whole, experts, inner, outer, transposed, dtype=dtype, dev=dev, seed=3)
+            if dtype == torch.float16:  # (within its range)
+                rows, grad = rows.clamp(-1, 1), grad.clamp(-1, 1)
+                rows, grad = (torch.cat([t, t[:, :1]], 1)[:, :t.shape[1]] for t in (rows, grad))
+            x, w = rows.detach().requires_grad_(True), weight.detach().requires_grad_(True)
+            out = gs.ops.expert_matmul(x, order, w)
+            got = torch.autograd.grad(out, (x, w), grad)
+            want = formula(rows, loads, weight, grad)
+            assert torch.equal(out, want[0].to(dtype))
+            assert torch.equal(got[0], want[2].to(dtype)) and torch.equal(got[1], want[4].to(dtype))
+
+
+@gpu
 def test_values_below_the_normal_ones(dev):
     """The smallest numbers of a type count like others."""
     for dtype, small, large in ((torch.float16, 2.0 ** -24, 2.0 ** 12), (torch.bfloat16, 2.0 ** -133, 2.0 ** 100),
