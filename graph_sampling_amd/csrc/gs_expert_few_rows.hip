@@ -147,7 +147,7 @@ few_rows_kernel(ProductArgs<T> p) {
 template <typename T, bool ACROSS, int MI, int COLS>
 int launch(ProductArgs<T> p, hipStream_t st) {
   p.col_tiles = (p.outer + 16 * COLS - 1) / (16 * COLS);
-  const int64_t blocks = (most_row_tiles(p.n, p.experts, 16 * MI) * p.col_tiles + kXcds - 1) / kXcds * kXcds;
+  const int64_t blocks = blocks_of(most_row_tiles(p.n, p.experts, 16 * MI), p.col_tiles);
   GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, kThreads));
   hipLaunchKernelGGL((few_rows_kernel<T, ACROSS, MI, COLS>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, p);
   return check_launch("expert_matmul");

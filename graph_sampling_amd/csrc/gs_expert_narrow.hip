@@ -18,25 +18,37 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int resident(int steps, int fragments) { return steps * fragments >= 32 ? 1 : 2; }
 constexpr int kAhead = 4;  // strips on their way
 
+// Every workgroup writes its share of `many` zeros.
+template <typename T>
+__device__ __forceinline__ void zero(T* out, int64_t many) {
+  constexpr int kVec = Chunk<T>::kVec;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kVec; at < many; at += threads * kVec)
+    store_part(out + at, Values<T>{}, many - at);
+}
+
 // STEPS: of the depth, at least as many as there are; SLABS slabs of COLS * 16 columns
 template <typename T, bool ACROSS, int STEPS, int COLS, int SLABS>
 __global__ void __launch_bounds__(kThreads, resident(STEPS, COLS* SLABS))
-narrow_kernel(ProductArgs<T> p, int tile_rows) {
+narrow_kernel(ProductArgs<T> p, int shares) {
   constexpr int kVec = Chunk<T>::kVec, kWide = 16 * COLS, kFrags = COLS * SLABS;
-  RowTile t = find_tile<kThreads>(p.offsets, p.experts, p.n, tile_rows, p.col_tiles);
+  const int64_t live = inside(p.offsets[p.experts], p.n);
+  zero(p.out + live * p.outer, (p.n - live) * p.outer);
+  const int64_t each = (live + shares - 1) / shares;
+  const int tile_rows = each > 0 ? static_cast<int>((each + 16 * kWaves - 1) / (16 * kWaves) * (16 * kWaves)) : 16 * kWaves;
+  RowTile t = find_tile<kThreads>(p.offsets, p.experts, live, tile_rows, p.col_tiles);
   if (t.rows <= 0) return;
   t = {uniform(t.expert), uniform(t.begin), uniform(t.rows), uniform(t.col), -1};
   const int lane = threadIdx.x % kWave, row16 = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rows = static_cast<int>(t.rows < tile_rows ? t.rows : tile_rows);
-  const bool live = t.expert < p.experts;
-  const int inner = live ? static_cast<int>(p.inner) : 0, steps = (inner + kStep<T> - 1) / kStep<T>;
+  const int inner = static_cast<int>(p.inner), steps = (inner + kStep<T> - 1) / kStep<T>;
   const int64_t col = t.col * (kWide * SLABS);
 
   // the matrix
   Values<T> b[STEPS][kFrags];
   int first[SLABS];  // the lane's columns of a slab, across the depth
-  const T* const w = p.weight + (live ? t.expert * p.expert_stride : 0);
+  const T* const w = p.weight + t.expert * p.expert_stride;
 #pragma unroll
   for (int s = 0; s < SLABS; ++s) {
     const int64_t most = p.outer - COLS - col - s * kWide;  // (a slab's last lanes end where the matrix does; behind it, none)
@@ -146,11 +158,10 @@ template <typename T, bool ACROSS, int STEPS, int COLS, int SLABS>
 int launch(ProductArgs<T> p, hipStream_t st) {
   p.col_tiles = (p.outer + 16 * COLS * SLABS - 1) / (16 * COLS * SLABS);
   const int64_t shares = kCus * resident(STEPS, COLS * SLABS) / p.col_tiles - p.experts - 1;
-  const int64_t each = (p.n + shares - 1) / shares, tile_rows = (each + 16 * kWaves - 1) / (16 * kWaves) * (16 * kWaves);
-  const int64_t blocks = (most_row_tiles(p.n, p.experts, tile_rows) * p.col_tiles + kXcds - 1) / kXcds * kXcds;
+  const int64_t blocks = blocks_of(shares + p.experts, p.col_tiles);  // (a part of a share for every expert)
   GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, kThreads));
   hipLaunchKernelGGL((narrow_kernel<T, ACROSS, STEPS, COLS, SLABS>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, p,
-                     static_cast<int>(tile_rows));
+                     static_cast<int>(shares));
   return check_launch("expert_matmul");
 }
 

@@ -58,7 +58,7 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
   constexpr int threads = WM * WN * kWave;
   p.col_tiles = (p.outer + BN - 1) / BN;
   const int64_t more = BM == 256 && BN == 256 ? products::kCus / 2 * 3 : 0;  // (where some are made in quarters)
-  const int64_t blocks = (products::most_row_tiles(p.n, p.experts, BM) * p.col_tiles + more + kXcds - 1) / kXcds * kXcds;
+  const int64_t blocks = products::blocks_of(products::most_row_tiles(p.n, p.experts, BM), p.col_tiles, more);
   GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, threads));
   hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN, RING, WAY>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
   return check_launch("expert_matmul");

@@ -18,14 +18,15 @@ constexpr int64_t kCus = 256;  // workgroups of large tiles that run at once
 
 // Every thread counts the tiles of rows of its share of the experts; the one in whose share the workgroup's lies finds it.
 // Workgroups of one die take tiles that lie side by side, so that its cache holds what they share.  QUARTERS: tiles that
-// would fill less than half of the card, after all others have filled it, are made in quarters.
+// would fill less than half of the card, after all others have filled it, are made in quarters.  The rows behind the last come
+// after all of these, so that every die has its share of the work.
 template <int THREADS, bool QUARTERS = false>
 __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
                                              int64_t col_tiles) {
   __shared__ int64_t s_wave[THREADS / kWave];
   __shared__ RowTile s_found;
-  const int64_t each = (experts + 1 + THREADS - 1) / THREADS, first = each * threadIdx.x;
-  const int64_t last = first + each < experts + 1 ? first + each : experts + 1;
+  const int64_t each = (experts + THREADS - 1) / THREADS, first = each * threadIdx.x;
+  const int64_t last = first + each < experts ? first + each : experts;
   int64_t mine = 0;
   for (int64_t e = first; e < last; ++e)
     mine += (group_of(offsets, experts, n, e).rows() + tile_rows - 1) / tile_rows;
@@ -44,25 +45,37 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
     if (w < static_cast<int>(threadIdx.x) / kWave) upto += s_wave[w];
     total += s_wave[w];
   }
-  const int64_t tiles = total * col_tiles, rest = QUARTERS && tiles % kCus <= kCus / 2 ? tiles % kCus : 0;
-  const int64_t whole = tiles - rest, whole_blocks = (whole + kXcds - 1) / kXcds * kXcds;
-  const bool part = QUARTERS && blockIdx.x >= whole_blocks;
-  const int64_t block = part ? blockIdx.x - whole_blocks : blockIdx.x, many = part ? rest * 4 : whole;
+  // blocks of whole tiles, of quarters, of the rows behind
+  const Group behind = group_of(offsets, experts, n, experts);
+  const int64_t tiles = total * col_tiles, rest = QUARTERS && tiles % kCus <= kCus / 2 ? tiles % kCus : 0, whole = tiles - rest;
+  const int64_t whole_blocks = (whole + kXcds - 1) / kXcds * kXcds, part_blocks = (rest * 4 + kXcds - 1) / kXcds * kXcds;
+  int64_t block = blockIdx.x, many = whole;
+  bool part = false, dead = false;
+  if (block >= whole_blocks) {
+    block -= whole_blocks;
+    part = block < part_blocks;
+    dead = !part;
+    if (dead) block -= part_blocks;
+    many = part ? rest * 4 : (behind.rows() + tile_rows - 1) / tile_rows * col_tiles;
+  }
   const int64_t per_die = (many + kXcds - 1) / kXcds, slot = block / kXcds, nth = block % kXcds * per_die + slot;
-  const int64_t which = part ? whole + nth / 4 : nth;
-  const int64_t at = slot < per_die && nth < many ? which / col_tiles : total;
-  int64_t from = upto - mine;
-  if (at >= from && at < upto) {
-    for (int64_t e = first; e < last; ++e) {
-      const Group g = group_of(offsets, experts, n, e);
-      const int64_t here = (g.rows() + tile_rows - 1) / tile_rows;
-      if (at < from + here) {
-        s_found.expert = e;
-        s_found.begin = g.begin + (at - from) * tile_rows;
-        s_found.rows = g.end - s_found.begin;
-        break;
+  const int64_t which = part ? whole + nth / 4 : nth, at = which / col_tiles;
+  if (slot < per_die && nth < many) {
+    int64_t from = upto - mine;
+    if (dead) {
+      if (threadIdx.x == 0) s_found = {experts, behind.begin + at * tile_rows, behind.rows() - at * tile_rows, 0, 0};
+    } else if (at >= from && at < upto) {
+      for (int64_t e = first; e < last; ++e) {
+        const Group g = group_of(offsets, experts, n, e);
+        const int64_t here = (g.rows() + tile_rows - 1) / tile_rows;
+        if (at < from + here) {
+          s_found.expert = e;
+          s_found.begin = g.begin + (at - from) * tile_rows;
+          s_found.rows = g.end - s_found.begin;
+          break;
+        }
+        from += here;
       }
-      from += here;
     }
   }
   __syncthreads();
@@ -86,6 +99,10 @@ struct ProductArgs {
 // Tiles of rows that there can be: a part of one for every expert that has rows, and for the rows behind.
 inline int64_t most_row_tiles(int64_t n, int64_t experts, int64_t tile_rows) {
   return n / tile_rows + (experts + 1 < n ? experts + 1 : n);
+}
+// Workgroups for them; more: where some are made in quarters.
+inline int64_t blocks_of(int64_t row_tiles, int64_t col_tiles, int64_t more = 0) {
+  return (row_tiles * col_tiles + more + kXcds - 1) / kXcds * kXcds + 2 * kXcds;
 }
 // Tiles that there will be, more or less: half a tile of rows for every expert is not full.
 template <typename T>

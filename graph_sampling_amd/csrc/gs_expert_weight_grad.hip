@@ -66,7 +66,10 @@ weight_grad_kernel(WeightGradArgs<T> p) {
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
   // Workgroups of one die make tiles that share rows: neighbours of one expert, or piece.  Which die has an expert, or a part
   // of each, is `shares`.
-  const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? p.pieces : p.experts);
+  // (behind the last expert's rows there are no pieces)
+  const int64_t live = PIECES ? products::inside(p.offsets[p.experts], p.n) : 0;
+  const int64_t pieces = live > 0 ? (live - 1) / p.piece + p.experts : 0;
+  const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? pieces : p.experts);
   const int64_t die = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
   int64_t which;
   if (shares(in_expert, p.experts)) {
