@@ -14,6 +14,8 @@ namespace gs {
 namespace {
 
 constexpr int kThreads = 256;
+template <int V>
+using N = std::integral_constant<int, V>;
 
 // Order-preserving, both zeros the same, NaN the largest; 0: not to be chosen.
 __device__ __forceinline__ uint32_t rank_of(float f) {
@@ -39,6 +41,10 @@ __device__ __forceinline__ float value_of_key(uint32_t key) {
   return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(rank & 0x8000u ? rank & 0x7FFFu : ~rank)));
 }
 
+// A sum's term, exp(d) for d <= 0: off by |d| * 2^-23 of itself, which is never more than 2^-24 of the largest term, and by two
+// steps.
+__device__ __forceinline__ float term(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
+
 // Lanes of a row of 16 exchange within the instruction, larger groups by shuffles on top.
 template <int CTRL>
 __device__ __forceinline__ uint32_t from_lane(uint32_t v) {
@@ -47,10 +53,10 @@ __device__ __forceinline__ uint32_t from_lane(uint32_t v) {
 constexpr int kSwapNeighbours = 0xb1, kSwapPairs = 0x4e, kMirrorEight = 0x141, kMirrorRow = 0x140;
 template <int G, typename F>
 __device__ __forceinline__ uint32_t group_reduce(uint32_t v, F&& f) {
-  v = f(v, from_lane<kSwapNeighbours>(v));
-  v = f(v, from_lane<kSwapPairs>(v));
-  v = f(v, from_lane<kMirrorEight>(v));
-  v = f(v, from_lane<kMirrorRow>(v));
+  if (G >= 2) v = f(v, from_lane<kSwapNeighbours>(v));
+  if (G >= 4) v = f(v, from_lane<kSwapPairs>(v));
+  if (G >= 8) v = f(v, from_lane<kMirrorEight>(v));
+  if (G >= 16) v = f(v, from_lane<kMirrorRow>(v));
 #pragma unroll
   for (int m = 16; m < G; m *= 2) v = f(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, kWave)));
   return v;
@@ -70,8 +76,10 @@ __device__ __forceinline__ float group_sum(float v) {
 //   16-bit logits: what is left is what lies below the last choice's key; less that key, with the borrow lost, it comes
 //   before all others, so that a look at an expert is a subtraction and a maximum, and nothing is taken out.
 //   fp32: the rank that was chosen is taken out in its lane, the first of equals, which has the lowest experts.
-// Both are bound by those instructions: 100 003 x 160 fp16, 6 choices, 7 us of bytes, 23 us (39 as fp32 is done); 16384 x 256 fp32, 8
-// choices, 3.6 us of bytes, 14 us (22 with exchanges through LDS).
+// Both are bound by those instructions, and by what is exchanged: as few lanes as there are choices have the fewest experts
+// each that will do.  100 003 x 160 fp16, 6 choices, 7 us of bytes, 23 us; 16384 x 256 fp32, 8 choices, 3.6 us of bytes, 13.5 us;
+// 500 000 x 27 bf16, 4 choices, 10 us of bytes, 18 us with 4 lanes of 8, 41 with 16 of 4; 500 000 x 264, 140 us with 16 of 20, 403
+// with 64 of 16.
 template <typename T, int G, int EACH>
 __global__ void __launch_bounds__(kThreads)
 choose_kernel(const T* __restrict__ logits, int64_t stride, int64_t tokens, int experts, int choices, bool normalize,
@@ -161,8 +169,8 @@ choose_kernel(const T* __restrict__ logits, int64_t stride, int64_t tokens, int 
     sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      if constexpr (kKeys) sum += rank[j] ? expf(value_of_key<T>(rank[j]) - most) : 0.0f;
-      else sum += v[j] == -__builtin_inff() ? 0.0f : expf(v[j] - most);
+      if constexpr (kKeys) sum += rank[j] ? term(value_of_key<T>(rank[j]) - most) : 0.0f;
+      else sum += v[j] == -__builtin_inff() ? 0.0f : term(v[j] - most);
     }
   }
   sum = group_sum<G>(sum);
@@ -172,17 +180,21 @@ choose_kernel(const T* __restrict__ logits, int64_t stride, int64_t tokens, int 
   }
 }
 
-// G lanes a token: its row is put together in LDS, and written in chunks.
+// G lanes a token: what the chosen experts get is put to its place in LDS, and read, and written, in chunks with the rest.
+// Memory bounds large ones: 500 000 x 264 bf16, 264 MB written, 64 us, and as much read without normalize, 128; groups of lanes
+// about as many as a third of the chunks lose least at a row's end (500 000 x 27: 14 us with 4, 87 with 64).
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads)
 choose_grad_kernel(const T* __restrict__ logits, int64_t stride, const int32_t* __restrict__ chosen,
                    const float* __restrict__ weights, const float* __restrict__ dweights, int64_t tokens, int experts,
                    int choices, bool normalize, T* __restrict__ dlogits) {
-  extern __shared__ float s_rows[];
+  extern __shared__ __attribute__((aligned(16))) float s_rows[];
+  constexpr int kVec = Chunk<T>::kVec;
   const int lane = threadIdx.x % G, group0 = threadIdx.x % kWave / G * G;
+  const int chunks = (experts + kVec - 1) / kVec;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
   if (t >= tokens) return;
-  float* const s_row = s_rows + threadIdx.x / G * experts;
+  float* const s_row = s_rows + threadIdx.x / G * (chunks * kVec);
   float w = 0.0f, dw = 0.0f;
   int32_t which = -1;
   if (lane < choices) {
@@ -193,21 +205,23 @@ choose_grad_kernel(const T* __restrict__ logits, int64_t stride, const int32_t* 
   const bool there = which >= 0 && which < experts;
   const float d = group_sum<G>(there ? w * dw : 0.0f);
   const int32_t first = __shfl(which, group0, kWave);
-  const bool any = first >= 0 && first < experts;
-  if (normalize || !any) {
-    for (int e = lane; e < experts; e += G) s_row[e] = 0.0f;
-  } else {
-    const T* const row = logits + t * stride;
-    const float top = static_cast<float>(row[first]), per = __shfl(w, group0, kWave) * d;
-    for (int e = lane; e < experts; e += G) {
-      const float v = static_cast<float>(row[e]);
-      s_row[e] = v == -__builtin_inff() ? 0.0f : -(expf(v - top) * per);
-    }
-  }
+  for (int c = lane; c < chunks; c += G) *reinterpret_cast<Wide<T>*>(s_row + c * kVec) = Wide<T>{};
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (a group is inside a wave, whose LDS accesses stay in order)
   if (there) s_row[which] += w * (normalize ? dw - d : dw);
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  for (int e = lane; e < experts; e += G) dlogits[t * experts + e] = static_cast<T>(s_row[e]);
+  const T* const row = logits + t * stride;
+  const bool rest = !normalize && first >= 0 && first < experts;  // all others have shares, too
+  const float top = rest ? static_cast<float>(row[first]) : 0.0f, per = __shfl(w, group0, kWave) * d;
+  for (int c = lane; c < chunks; c += G) {
+    const int e = c * kVec;
+    Wide<T> sum = *reinterpret_cast<const Wide<T>*>(s_row + e);
+    if (rest) {
+      const Wide<T> v = widen<T>(load_chunk(row + e, experts - e));
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum[i] -= v[i] == -__builtin_inff() ? 0.0f : expf(v[i] - top) * per;
+    }
+    store_chunk(dlogits + t * experts + e, narrow<T>(sum), experts - e);
+  }
 }
 
 int check_choice(const char* what, int64_t tokens, int64_t experts, int64_t choices, int type, int64_t stride) {
@@ -246,18 +260,19 @@ int gs_expert_choose(const void* logits, int64_t stride, int type, int64_t token
                          static_cast<int>(experts), static_cast<int>(choices), normalize != 0, chosen, weights);
       return check_launch("expert_choose");
     };
-    using Few = std::integral_constant<int, 16>;
-    using All = std::integral_constant<int, kWave>;
-    if (choices <= 16 && experts <= 256) {
-      if (experts <= 16) return go(Few(), std::integral_constant<int, 1>());
-      if (experts <= 64) return go(Few(), std::integral_constant<int, 4>());
-      if (experts <= 128) return go(Few(), std::integral_constant<int, 8>());
-      if (experts <= 192) return go(Few(), std::integral_constant<int, 12>());
-      return go(Few(), std::integral_constant<int, 16>());
-    }
-    if (experts <= 256) return go(All(), std::integral_constant<int, 4>());
-    if (experts <= 1024) return go(All(), std::integral_constant<int, 16>());
-    return go(All(), std::integral_constant<int, 64>());
+    auto four = [&](auto g, auto a, auto b, auto c, auto d) {  // the fewest experts a lane that will do
+      constexpr int G = decltype(g)::value;
+      if (experts <= G * decltype(a)::value) return go(g, a);
+      if (experts <= G * decltype(b)::value) return go(g, b);
+      return experts <= G * decltype(c)::value ? go(g, c) : go(g, d);
+    };
+    if (choices <= 4 && experts <= 32) return four(N<4>(), N<2>(), N<4>(), N<6>(), N<8>());
+    if (choices <= 8 && experts <= 64) return four(N<8>(), N<4>(), N<6>(), N<8>(), N<8>());
+    if (choices <= 16 && experts <= 192) return four(N<16>(), N<4>(), N<6>(), N<8>(), N<12>());
+    if (choices <= 16 && experts <= 384) return four(N<16>(), N<16>(), N<20>(), N<24>(), N<24>());
+    if (choices <= 32 && experts <= 512) return four(N<32>(), N<4>(), N<8>(), N<12>(), N<16>());
+    if (experts <= 1024) return four(N<kWave>(), N<4>(), N<8>(), N<12>(), N<16>());
+    return four(N<kWave>(), N<24>(), N<32>(), N<48>(), N<64>());
   });
 }
 
@@ -272,18 +287,22 @@ int gs_expert_choose_grad(const void* logits, int64_t stride, int type, const in
              "gs_expert_choose_grad: logits not aligned to their type");
   return with_value_type(type, "gs_expert_choose_grad", [&](auto zero) {
     using T = decltype(zero);
+    const int64_t chunks = (experts + Chunk<T>::kVec - 1) / Chunk<T>::kVec;
     auto go = [&](auto lanes) {
       constexpr int G = decltype(lanes)::value, kTokens = kThreads / G;
       const int64_t blocks = (tokens + kTokens - 1) / kTokens;
       GS_RETURN_IF_ERROR(check_grid("gs_expert_choose_grad", blocks, kThreads));
       hipLaunchKernelGGL((choose_grad_kernel<T, G>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
-                         kTokens * static_cast<size_t>(experts) * sizeof(float), static_cast<hipStream_t>(stream),
+                         static_cast<size_t>(kTokens * chunks * Chunk<T>::kVec) * sizeof(float), static_cast<hipStream_t>(stream),
                          static_cast<const T*>(logits), stride, chosen, weights, dweights, tokens,
                          static_cast<int>(experts), static_cast<int>(choices), normalize != 0, static_cast<T*>(dlogits));
       return check_launch("expert_choose_grad");
     };
-    return choices <= 16 && experts <= 256 ? go(std::integral_constant<int, 16>())
-                                           : go(std::integral_constant<int, kWave>());
+    if (choices <= 4 && chunks <= 8) return go(N<4>());
+    if (choices <= 8 && chunks <= 24) return go(N<8>());
+    if (choices <= 16 && chunks <= 64) return go(N<16>());
+    if (choices <= 32 && chunks <= 128) return go(N<32>());
+    return go(N<kWave>());
   });
 }
 

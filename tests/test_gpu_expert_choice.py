@@ -264,6 +264,26 @@ def test_refusals(dev):
         torch.func.grad(lambda t: gs.ops.expert_choose(t, 2)[1].sum())(l.detach())
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_experts_and_choices_around_every_limit(dev, dtype):
+    for num in (4, 8, 9, 15, 16, 17, 24, 25, 31, 32, 33, 48, 49, 64, 65, 96, 97, 128, 129, 192, 193, 255, 256, 257, 320, 321, 384,
+                385, 511, 512, 513, 768, 769, 1024, 1025, 1536, 1537, 2048, 2049, 4095, 4096):
+        for choices in {min(k, num) for k in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64)}:
+            tokens = 5 + num % 7
+            logits = logits_of("masked" if choices % 2 else "ties", tokens, num, dtype, dev, num + choices)
+            for normalize in (True, False):
+                x = logits.detach().requires_grad_(True)
+                experts, weights = gs.ops.expert_choose(x, choices, normalize)
+                grad = torch.randn(tokens, choices, generator=torch.Generator().manual_seed(1)).to(dev)
+                dx, = torch.autograd.grad(weights, x, grad)
+                want = formula(logits, choices, normalize, grad)
+                assert np.array_equal(experts.cpu().numpy(), want[0])
+                assert np.allclose(weights.detach().cpu().numpy(), want[1], rtol=(200 + num + 12) * STEP, atol=TINY)
+                tol = want[3] * (200 + num + 20) * STEP + np.abs(want[2]) * half_step(dtype) + smallest(dtype)
+                assert (np.abs(dx.double().cpu().numpy() - want[2]) <= tol).all()
+
+
 # ------------------------------------------------------------------ no GPU ----
 def test_bad_arguments_are_refused_before_anything_is_launched():
     import ctypes
