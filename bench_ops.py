@@ -4,8 +4,8 @@
 bench.py measures the GraphSAGE minibatch; this script times the other rows of the scope
 table at the sizes of their configurations -- induced-subgraph slicing, format conversions,
 weighted sampling with and without replacement, list sampling, the super-batch helpers,
-walks, SDDMM, rows moved by ids, segment and COO sums, row slicing -- through the same C ABI
-(graph_sampling_amd/capi.py), with `algorithmic` = the bytes the operator must move at the
+walks, SDDMM, rows moved by ids, experts' choice and products, dropout, segment and COO sums,
+row slicing -- through the same C ABI (graph_sampling_amd/capi.py), with `algorithmic` = the bytes the operator must move at the
 least (stated per line) over the median of the timed calls, and four whole samplers (LADIES
 and GraphSAGE written against Matrix, as written and through jit.compile) by wall clock.
 Timing of the operators: torch.cuda.Event pairs on the current stream, which is the stream the
@@ -234,6 +234,19 @@ def main():
     run("expert_combine_grad", "gs_expert_combine_grad: with weights, both gradients; 3 x 256 B + 12 B per row",
         lambda: capi.expert_combine_grad(feat[:600_000], t_rows, t_place, t_offsets, t_weights),
         lambda o: (600_000 * (768 + 12), 600_000, "rows"))
+    # what experts do in between: products with a matrix of each type or expert, their choice, dropout
+    own = torch.Generator(device=dev).manual_seed(12)
+    t_weight, t_grad = torch.rand(5, 64, 128, generator=own, device=dev), torch.rand(600_000, 128, generator=own, device=dev)
+    run("expert_matmul", "gs_expert_matmul: the same rows times a 64 x 128 matrix of their type, fp32; 256 + 512 B per row",
+        lambda: capi.expert_matmul(t_rows, t_offsets, t_weight), lambda o: (600_000 * 768, 600_000, "rows"))
+    run("expert_matmul_grad", "gs_expert_matmul_grad: the gradient of the 5 matrices; 256 + 512 B per row",
+        lambda: capi.expert_matmul_grad(t_grad, t_rows, t_offsets), lambda o: (600_000 * 768, 600_000, "rows"))
+    t_logits = torch.randn(600_000, 64, generator=own, device=dev)
+    run("expert_choose", "gs_expert_choose: 2 of 64 experts for 600 k tokens, fp32; 256 + 16 B per token",
+        lambda: capi.expert_choose(t_logits, 2), lambda o: (600_000 * 272, 600_000, "tokens"))
+    run("dropout", "gs_dropout: half of 600 k rows of 64 fp32, with a residual; 3 x 256 B per row",
+        lambda: capi.dropout(feat[:600_000], 0.5, 7, t_rows), lambda o: (600_000 * 768, 600_000, "rows"))
+    del t_weight, t_grad, t_logits
     # Divide(divisor, axis=0) on the CSC: out[e] = w[e] / divisor[column of e], scalar per edge
     out_w = torch.empty(E, 1, device=dev)
     run("sddmm_div_csc", "gs_sddmm_csc e_div_v over the whole graph (edge weight / per-column scalar): "
