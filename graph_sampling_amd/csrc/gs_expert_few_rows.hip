@@ -156,22 +156,36 @@ int launch(ProductArgs<T> p, hipStream_t st) {
 
 }  // namespace
 
-// Twice the rows where experts have more than 16; for 16-bit values twice the columns, and wider loads, where there are
-// workgroups enough: 32 experts of 1024 x 1024 bf16, a row each, 15 us and 11, of 4096 x 512 22 and 26.
+// Twice the rows where experts have more than 16, and twice the columns with 16-bit values, whose loads are wider then, where there
+// are workgroups enough; half the columns where they would fill the card but once, since a workgroup's own loads bound it then,
+// and its products in fp32, most of whose rows are missing where experts have one or two.  Kernel times, us: 32 experts of 1024 x 1024,
+// bf16, a row each, 128 columns 11, 64 15; of 4096 x 512 26 and 22; 8 of 4096 x 1024, 2 rows, 64 columns 16 to 20, 32 15; 4 of
+// 3496 x 72, 40 rows (32 at once) 16 to 18, 64 columns of 16 rows 13 to 16, 32 9 to 11; fp32 39 to 50, 25 to 33, 17 to 20; 160 of 1001 x 333,
+// a row each, fp32 35 to 44 and 31 to 35.
 template <typename T>
 int launch_few_rows(const ProductArgs<T>& p, bool across, hipStream_t st) {
   auto go = [&](auto mi, auto cols) {
     constexpr int MI = decltype(mi)::value, COLS = decltype(cols)::value;
     return across ? launch<T, true, MI, COLS>(p, st) : launch<T, false, MI, COLS>(p, st);
   };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  if (likely_tiles(p, 16, 32) <= kCus || (sizeof(T) == 4 && p.n <= 2 * p.experts)) return go(One(), Two());
+  if (likely_tiles(p, 16, 64) <= kCus) return go(One(), Four());
   auto with_rows = [&](auto mi) {
-    if constexpr (sizeof(T) == 2) {
-      if (likely_tiles(p, 16 * decltype(mi)::value, 64) >= 320) return go(mi, std::integral_constant<int, 8>());
+    constexpr int MI = decltype(mi)::value;
+    if constexpr (sizeof(T) == 2) {  // (twice of both along the depth is more than the registers hold)
+      const bool many = likely_tiles(p, 16 * MI, 64) >= 320;
+      if (many && across) return launch<T, true, MI, 8>(p, st);
+      if constexpr (MI == 1) {
+        if (many) return launch<T, false, MI, 8>(p, st);
+      }
     }
-    return go(mi, std::integral_constant<int, 4>());
+    return go(mi, Four());
   };
-  if (p.n > 16 * p.experts) return with_rows(std::integral_constant<int, 2>());
-  return with_rows(std::integral_constant<int, 1>());
+  if (p.n > 16 * p.experts) return with_rows(Two());
+  return with_rows(One());
 }
 template int launch_few_rows<float>(const ProductArgs<float>&, bool, hipStream_t);
 template int launch_few_rows<_Float16>(const ProductArgs<_Float16>&, bool, hipStream_t);

@@ -77,7 +77,7 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
   if (products::narrow(p)) return products::launch_narrow(p, ACROSS, st);
-  if (products::few_rows(p)) return products::launch_few_rows(p, ACROSS, st);
+  if (products::few_rows(p, ACROSS)) return products::launch_few_rows(p, ACROSS, st);
   const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256),
                                    products::way_of<T>(p.weight_stride, ACROSS ? p.outer : p.inner, 256));
   if (way == Way::kValues) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kValues>(p, st);

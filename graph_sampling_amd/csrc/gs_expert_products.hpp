@@ -164,16 +164,23 @@ bool narrow(const ProductArgs<T>& p) {
   return held && p.n >= (kHalf ? 1 << 18 : 1 << 19) && p.experts <= (kHalf ? 64 : 16);
 }
 
-// Where 64 x 64 tiles do not fill the card twice, the depth of a tile has to be shared out, too, if it is long; fp32, whose
-// products take sixteen times as long, gains by it with few rows whatever their number.  Kernel times of both, us, few
-// rows first: bf16, 32 experts of 4096 x 512, 16 rows each 36 and 74, 200 rows 109 and 85; of 1024 x 1024, 4 rows 16 and
-// 18; 160 of 1024 x 1024, 1 row 49 and 40; fp32, 32 of 4096 x 512, 40 rows 108 and 180; of 512 x 4096, 16 rows 94 and 80.
+// Where 64 x 64 tiles do not fill the card twice, the depth of a tile has to be shared out, too, if it is long: the more tiles
+// there are, the longer it has to be, and longer still where the matrix's values lie along the depth, which is read in pieces of 64
+// bytes, at odd places above all.  fp32, whose products take sixteen times as long, gains by it with few rows whatever their number.
+// Kernel times of both, us, few rows first: bf16, 32 experts of 4096 x 512, 16 rows each 36 and 74; of 1024 x 1024, 4 rows 16 and
+// 18; 16 of 1001 x 333, 40 rows 11 and 13, 100 rows 15 and 13, transposed 17 and 13, 29 and 13; 4 of 2048 x 1024, 200 rows 17 and
+// 29, transposed 35 and 22, 40 rows 14 and 15; 17 of 2733 x 1051, transposed, 2 rows 34 and 41; 64 of 1001 x 333, 3 rows 23 and 18;
+// fp32, 32 of 4096 x 512, 40 rows 108 and 180; 16 of 2048 x 1024, transposed, 40 rows 68 and 57; of 1001 x 333, 40 rows 18 and 26.
 template <typename T>
-bool few_rows(const ProductArgs<T>& p) {
+bool few_rows(const ProductArgs<T>& p, bool across) {
+  constexpr bool kHalf = sizeof(T) == 2;
   const int64_t tiles = likely_tiles(p, 64, 64);
   if (p.outer < 8) return false;
-  if (sizeof(T) == 4 && p.n <= 16 * p.experts && (p.n <= 4 * p.experts || tiles < 1400)) return true;
-  return tiles < 512 && (p.inner >= 512 || p.n <= 16 * p.experts);
+  if (!kHalf && p.n <= 16 * p.experts && (p.n <= 4 * p.experts || tiles < 1400)) return true;
+  const bool odd = kHalf && !across && !(aligned_to(p.weight, 4) && p.weight_stride % 2 == 0 && p.expert_stride % 2 == 0);
+  if (tiles >= 512) return false;
+  if (p.n <= (odd ? 2 : 16) * p.experts) return true;
+  return p.inner >= 512 && tiles * (!kHalf ? (across ? 3 : 10) : odd ? 40 : across ? 6 : 20) <= p.inner;
 }
 
 }  // namespace products

@@ -577,6 +577,23 @@ def test_large_tiles_of_any_alignment(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows_and_long_depths(dev, dtype):
+    """The depth shared out: from one tile of columns to many, depths that end anywhere, whole numbers."""
+    for n, experts, inner, outer, kind in ((7, 4, 3497, 70, "skewed"), (160, 4, 3500, 72, "even"), (40, 4, 2053, 1030, "skewed"),
+                                           (16, 16, 1001, 333, "even"), (300, 3, 4096, 33, "skewed"), (500, 4, 2048, 1024, "even"),
+                                           (33, 2, 777, 31, "last"), (64, 64, 520, 1290, "skewed"), (90, 1, 1600, 9, "first"),
+                                           (200, 4, 6400, 2500, "even")):
+        loads = loads_of(kind, n, experts, inner)
+        order = order_of(loads, n, dev)
+        for transposed in (False, True):
+            rows = whole(n, inner, dtype=dtype, dev=dev, seed=1)
+            weight = weights_of(whole, experts, inner, outer, transposed, dtype=dtype, dev=dev, seed=2)
+            got = gs.ops.expert_matmul(rows, order, weight)
+            assert torch.equal(got, formula(rows, loads, weight)[0].to(dtype))
+
+
+@gpu
 def test_values_below_the_normal_ones(dev):
     """The smallest numbers of a type count like others."""
     for dtype, small, large in ((torch.float16, 2.0 ** -24, 2.0 ** 12), (torch.bfloat16, 2.0 ** -133, 2.0 ** 100),
