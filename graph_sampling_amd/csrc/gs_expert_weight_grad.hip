@@ -5,6 +5,8 @@
 // Products whose depth is an expert's number of rows.  8 experts of 4096 x 2048, 2000 rows each, bf16: 264 us, 1.02 PFLOP/s, bound
 // as large products of rows are; 5 types of 64 x 128, 120 000 rows each, fp32: 123 us in 2000 pieces and 8 to join them, 3.8 TB/s
 // with the matrix cores half busy.  No counterpart in the reference.
+#include <cmath>
+
 #include "gs_products.hpp"
 
 namespace gs {
@@ -140,12 +142,21 @@ join_pieces_kernel(WeightGradArgs<T> p, int64_t runs) {
   products::store_part(p.out + e * size + at, __builtin_convertvector(sum, Narrow), there);
 }
 
-// How the rows are cut: not at all (0) where there are tiles enough.
+// How the rows are cut: not at all (0) where there are tiles enough, or where pieces would not be much shorter.  A piece of R rows
+// keeps a workgroup busy for R / 100 us or so, and its sums are written and read, 8 bytes each at 4 TB/s: the two together are
+// least at R^2 = n * inner * outer / 5000.  No more pieces than give 2048 small tiles: by then the card is full.  With three experts or
+// less an uncut one takes its rows' time, with more the largest one's, which has twice the others' or so.  bf16, us: 2 experts of 512 x 512,
+// 1000 rows each, uncut 11, pieces of 256 17, of 128 20; 2000 rows 33, 17 (of 512), 30 (of 128); 32 of 256 x 256, 300 rows 8 uncut,
+// 27 in pieces of 128, 2000 rows 62 and 36 (of 512); 5 of 64 x 128, 120 000 rows, pieces of 608 56, of 1184 43.
 constexpr int64_t tiles_of(int64_t inner, int64_t outer) { return (inner + 63) / 64 * ((outer + 63) / 64); }
-int64_t piece_rows(int64_t n, int64_t experts, int64_t tiles) {
+int64_t piece_rows(int64_t n, int64_t experts, int64_t inner, int64_t outer) {
   constexpr int64_t kTiles = 2048, kRows = 128;
+  const int64_t tiles = tiles_of(inner, outer);
   if (tiles * experts >= kTiles / 2 || n < 2 * kRows * experts) return 0;
-  const int64_t pieces = kTiles / tiles, rows = (n + pieces - 1) / pieces;
+  const int64_t full = (n * tiles + kTiles - 1) / kTiles;
+  const int64_t least = static_cast<int64_t>(std::sqrt(static_cast<double>(n) * static_cast<double>(inner * outer) / 5000.0));
+  const int64_t rows = least > full ? least : full;
+  if (10 * n < (experts < 4 ? 32 : 19) * rows * experts) return 0;
   return rows < kRows ? kRows : (rows + 31) / 32 * 32;
 }
 int64_t pieces_there(int64_t n, int64_t experts, int64_t piece) { return (n + piece - 1) / piece + experts; }
@@ -165,7 +176,7 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   p.row_tiles = (p.inner + BM - 1) / BM;
   p.col_tiles = (p.outer + BN - 1) / BN;
   const int64_t tiles = p.row_tiles * p.col_tiles;
-  p.piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer));
+  p.piece = piece_rows(p.n, p.experts, p.inner, p.outer);
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
   const int64_t padded_tiles = shares(tiles, p.experts) ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;
   if (items > most_blocks(threads) / padded_tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
@@ -197,7 +208,7 @@ int choose_weight_grad(const WeightGradArgs<T>& p, void* workspace, size_t works
   const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256), products::way_of<T>(p.grad_stride, p.outer, 256));
   if (way == Way::kValues) return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kValues>(p, workspace, workspace_bytes, st);
   if constexpr (sizeof(T) == 2) {
-    const int64_t piece = piece_rows(p.n, p.experts, tiles_of(p.inner, p.outer)), each = p.n / p.experts;
+    const int64_t piece = piece_rows(p.n, p.experts, p.inner, p.outer), each = p.n / p.experts;
     const int64_t items = piece ? pieces_there(p.n, p.experts, piece) : p.experts, rows = piece && piece < each ? piece : each;
     const int64_t tiles128 = (p.inner + 127) / 128 * ((p.outer + 127) / 128) * items;
     const int64_t tiles256 = (p.inner + 255) / 256 * ((p.outer + 255) / 256) * items;
@@ -221,7 +232,7 @@ size_t gs_expert_matmul_grad_workspace_bytes(int64_t n, int64_t inner, int64_t o
   if (n <= 0 || n >= (int64_t(1) << 31) || inner <= 0 || inner >= kMost || outer <= 0 || outer >= kMost || num_experts <= 0 ||
       num_experts > products::kMostExperts)
     return 256;
-  const int64_t piece = piece_rows(n, num_experts, tiles_of(inner, outer));
+  const int64_t piece = piece_rows(n, num_experts, inner, outer);
   return piece ? padded(static_cast<size_t>(pieces_there(n, num_experts, piece) * inner * outer) * sizeof(float)) : 256;
 }
 
