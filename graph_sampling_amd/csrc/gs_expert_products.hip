@@ -73,6 +73,10 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
 //   but twice) 32, 28, 26, 25; of 336 x 1008, 500 rows 29, 28, 33, 44; 5000 rows 204, 236, 287, 348
 //   32 of 1150 x 890, 1000 rows 85, 105, 121, 178; 200 rows 33, 31, 35, 51; of 333 x 1001, 1000 rows 53, 60, 70, 84
 //   160 of 152 x 256, 100 rows 14, 10, 10, 9
+// Where one round of workgroups is all there is, nobody works while one waits, and more steps on their way (a ring of four for 128 x
+// 128, five for 64 x 128, six for 64 x 64) hide the rest; otherwise three, which leave room for more workgroups, are better:
+//   16 of 1150 x 890, 200 rows, 128 x 128, 18 with four, 27 with three; 64 x 128, 21 with five, 23 with three
+//   3 of 1152 x 896, 1000 rows, 64 x 64, 16 with six, 19 with three; 16 of 64 x 128, 5000 rows, 16 and 10
 // fp32, which is bound by its products, is within 5 % of its best with the smallest.
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
@@ -81,18 +85,26 @@ int choose_product(const ProductArgs<T>& p, hipStream_t st) {
   const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256),
                                    products::way_of<T>(p.weight_stride, ACROSS ? p.outer : p.inner, 256));
   if (way == Way::kValues) return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kValues>(p, st);
+  const bool deep = p.inner >= 8 * products::kStep<T>;
   if constexpr (sizeof(T) == 2) {
     const bool aligned = products::aligned_rows(p.rows, p.row_stride, 0) &&
                          products::aligned_rows(p.weight, p.weight_stride, p.expert_stride);
-    const int64_t enough = !aligned ? 160 : p.inner >= 512 ? 224 : 400;
+    const int64_t enough = !aligned ? 160 : p.inner >= 512 ? 224 : 600, tiles128 = products::likely_tiles(p, 128, 128);
     if (p.outer > 128 && p.inner >= 256 && p.n >= 128 * p.experts && products::likely_tiles(p, 256, 256) >= enough)
       return launch_product<T, ACROSS, 256, 256, 2, 4, 4, Way::kDirect>(p, st);
-    if (p.outer > 64 && p.n >= 64 * p.experts && products::likely_tiles(p, 128, 128) >= 400)
+    if (p.outer > 64 && deep && tiles128 >= 160 && tiles128 <= products::kCus)
+      return launch_product<T, ACROSS, 128, 128, 2, 2, 4, Way::kDirect>(p, st);
+    if (p.outer > 64 && p.n >= 64 * p.experts && tiles128 >= 350)
       return launch_product<T, ACROSS, 128, 128, 2, 2, 3, Way::kDirect>(p, st);
-    if (p.outer > 64 && products::likely_tiles(p, 64, 128) >= 300)
-      return launch_product<T, ACROSS, 64, 128, 2, 2, 3, Way::kDirect>(p, st);
+    const int64_t tiles = products::likely_tiles(p, 64, 128);
+    if (p.outer > 64 && tiles >= 150) {
+      return deep && tiles < 2 * products::kCus ? launch_product<T, ACROSS, 64, 128, 2, 2, 5, Way::kDirect>(p, st)
+                                                : launch_product<T, ACROSS, 64, 128, 2, 2, 3, Way::kDirect>(p, st);
+    }
   }
-  return launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kDirect>(p, st);
+  return deep && products::likely_tiles(p, 64, 64) <= 4 * products::kCus
+             ? launch_product<T, ACROSS, 64, 64, 2, 2, 6, Way::kDirect>(p, st)
+             : launch_product<T, ACROSS, 64, 64, 2, 2, 3, Way::kDirect>(p, st);
 }
 
 }  // namespace

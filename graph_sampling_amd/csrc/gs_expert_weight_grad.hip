@@ -199,25 +199,32 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
 }
 
 // As for the products of rows; here a matrix, or what a piece adds to it, is a product of its own, and one of few rows is not
-// worth a large tile's start and end.  bf16, tiles of 256 x 256, 128 x 128 and 64 x 64, us: 32 experts of 1024 x 1024, 2000 rows
-// each 164, 217, 371; of 1152 x 896, 500 rows 68, 60, 71; of 256 x 256, 500 rows (pieces of 128) 30, 30, 32; of 336 x 1008, 1000 rows
-// 53, 61, 84; 4 of those, 5000 rows (28 pieces) 41, 54, 63, 200 rows 13, 7, 6; 4 of 333 x 1001 (not aligned), 40 000 rows 209, 307,
-// 545.  fp32 is within 12 % of its best with the smallest.
+// worth a large tile's start and end, nor a deep ring's.  bf16, tiles of 256 x 256, 128 x 128 (ring of four, and of three), 64 x 128
+// (five) and 64 x 64 (six), us: 32 experts of 1024 x 1024, 2000 rows each 164, -, 217, -, 371; 60 of 1152 x 896, 300 rows 72, 64, 61,
+// 84, 93; 16 of 1150 x 890, 1000 rows 63, 50, 50, 64, 84; 60 of 336 x 1008, 500 rows 50, 42, 45, 55, 71; 3 of 1152 x 896, 1000 rows
+// 31, 15, 23, 13, 14, 2000 rows 57, 26, 44, 20, 22; 4 of 333 x 1001 (not aligned), 40 000 rows 209, -, 307, -, 545.  fp32 is within 12 %
+// of its best with the smallest; 64 of 256 x 256, 2000 rows 184 with a ring of six, 271 with three.
 template <typename T>
 int choose_weight_grad(const WeightGradArgs<T>& p, void* workspace, size_t workspace_bytes, hipStream_t st) {
   const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256), products::way_of<T>(p.grad_stride, p.outer, 256));
   if (way == Way::kValues) return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kValues>(p, workspace, workspace_bytes, st);
+  const int64_t piece = piece_rows(p.n, p.experts, p.inner, p.outer), each = p.n / p.experts;
+  const int64_t items = piece ? pieces_there(p.n, p.experts, piece) : p.experts, rows = piece && piece < each ? piece : each;
+  const auto tiles = [&](int64_t rows_of, int64_t cols_of) {
+    return (p.inner + rows_of - 1) / rows_of * ((p.outer + cols_of - 1) / cols_of) * items;
+  };
   if constexpr (sizeof(T) == 2) {
-    const int64_t piece = piece_rows(p.n, p.experts, p.inner, p.outer), each = p.n / p.experts;
-    const int64_t items = piece ? pieces_there(p.n, p.experts, piece) : p.experts, rows = piece && piece < each ? piece : each;
-    const int64_t tiles128 = (p.inner + 127) / 128 * ((p.outer + 127) / 128) * items;
-    const int64_t tiles256 = (p.inner + 255) / 256 * ((p.outer + 255) / 256) * items;
-    if (p.inner > 128 && p.outer > 128 && rows >= 300 && tiles256 >= (piece ? 128 : rows >= 4000 ? 150 : 200))
+    if (p.inner > 128 && p.outer > 128 && rows >= 300 && tiles(256, 256) >= (piece ? 128 : 600))
       return launch_weight_grad<T, 256, 256, 2, 4, 4, Way::kDirect>(p, workspace, workspace_bytes, st);
-    if (p.inner > 64 && p.outer > 64 && tiles128 >= 200)
-      return launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
+    if (p.inner > 64 && p.outer > 64 && tiles(128, 128) >= 250)
+      return rows >= 128 ? launch_weight_grad<T, 128, 128, 2, 2, 4, Way::kDirect>(p, workspace, workspace_bytes, st)
+                         : launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
+    if (p.outer > 64 && rows >= 128 && tiles(64, 128) >= 140 && tiles(64, 128) <= 512)
+      return launch_weight_grad<T, 64, 128, 2, 2, 5, Way::kDirect>(p, workspace, workspace_bytes, st);
   }
-  return launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
+  return rows >= (sizeof(T) == 2 ? 200 : 128) && tiles(64, 64) <= 1024
+             ? launch_weight_grad<T, 64, 64, 2, 2, 6, Way::kDirect>(p, workspace, workspace_bytes, st)
+             : launch_weight_grad<T, 64, 64, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
 }
 
 }  // namespace
