@@ -3,7 +3,7 @@
 //   dweight[e] = sum over the rows p of expert e of rows[p, :]^T * grad[p, :],   zeros for an expert without rows
 //
 // Products whose depth is an expert's number of rows.  8 experts of 4096 x 2048, 2000 rows each, bf16: 264 us, 1.02 PFLOP/s, bound
-// as large products of rows are; 5 types of 64 x 128, 120 000 rows each, fp32: 123 us in 2000 pieces and 8 to join them, 3.8 TB/s
+// as large products of rows are; 5 types of 64 x 128, 120 000 rows each, fp32: 120 us in 610 pieces and 7 to join them, 3.8 TB/s
 // with the matrix cores half busy.  No counterpart in the reference.
 #include <cmath>
 

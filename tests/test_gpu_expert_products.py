@@ -594,6 +594,26 @@ def test_few_rows_and_long_depths(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sizes_between_few_and_many(dev, dtype):
+    """Every tile and number of steps on the way, with rows behind the last and experts without any; whole numbers."""
+    for n, experts, inner, outer, kind in ((6000, 3, 300, 512, "skewed"), (3000, 3, 1152, 896, "even"), (20_000, 2, 512, 512, "skewed"),
+                                           (1500, 40, 320, 384, "skewed"), (4000, 4, 1003, 341, "skewed"), (700, 2, 96, 64, "even"),
+                                           (9000, 30, 256, 264, "even"), (16_000, 10, 130, 400, "skewed"), (2500, 1, 2000, 200, "first")):
+        loads = loads_of(kind, n, experts, inner)
+        order = order_of(loads, n, dev)
+        for transposed in (False, True):
+            rows, grad = (whole(n, d, dtype=dtype, dev=dev, seed=d).clamp(-1, 1) for d in (inner, outer))
+            weight = weights_of(whole, experts, inner, outer, transposed, dtype=dtype, dev=dev, seed=3)
+            x, w = rows.requires_grad_(True), weight.detach().requires_grad_(True)
+            out = gs.ops.expert_matmul(x, order, w)
+            got = torch.autograd.grad(out, (x, w), grad)
+            want = formula(rows, loads, weight, grad)
+            assert torch.equal(out, want[0].to(dtype))
+            assert torch.equal(got[0], want[2].to(dtype)) and torch.equal(got[1], want[4].to(dtype))
+
+
+@gpu
 def test_values_below_the_normal_ones(dev):
     """The smallest numbers of a type count like others."""
     for dtype, small, large in ((torch.float16, 2.0 ** -24, 2.0 ** 12), (torch.bfloat16, 2.0 ** -133, 2.0 ** 100),
