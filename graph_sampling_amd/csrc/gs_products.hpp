@@ -2,10 +2,10 @@
 // the gradients of their matrices share.
 //
 // A workgroup makes a tile of C[m, n] = sum over k of A[m, k] * B[k, n].  It goes along k in steps of
-// 64 bytes (32 values of 16 bits, 16 fp32 values), four of which have room in LDS: one is worked on, one has arrived,
-// two are on their way.  Either operand comes in one of two orders: along k, where the values of one row (or
+// 64 bytes (32 values of 16 bits, 16 fp32 values), three to six of which have room in LDS: one is worked on, the next has
+// arrived, or is about to, the others are on their way.  Either operand comes in one of two orders: along k, where the values of one row (or
 // column) of C lie side by side, or across k, where the rows of one k do.  Sums are fp32 in the
-// matrix cores' accumulators, in the order of k, rounded once at the end.
+// matrix cores' accumulators, in the order of k (what is left of the last step first), rounded once at the end.
 #pragma once
 
 #include "gs_rows.hpp"
@@ -357,7 +357,7 @@ __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(LEFT) : "memory");
 }
 
-// A tile of BM x BN by WM x WN waves, RING steps in LDS (three or four).
+// A tile of BM x BN by WM x WN waves, RING steps in LDS, three at least.
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING, Way WAY>
 struct Tile {
   using LA = Layout<T, A_ACROSS, BM>;

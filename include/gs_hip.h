@@ -1107,18 +1107,19 @@ int gs_expert_choose_grad(const void* logits, int64_t stride, int type, const in
                           void* dlogits, void* stream);
 
 /* out[p, :] = rows[p, :] x the matrix of expert e for offsets[e] <= p < offsets[e + 1], zeros in the rows from
- * offsets[num_experts] to n (below 2^31); up to 65536 experts.  rows: n rows of `inner` values, row_stride apart; out: n x outer.  The
- * matrix of expert e begins at weight + e * expert_stride: `inner` rows of `outer` values, weight_stride apart, or, if
- * transposed, `outer` rows of `inner` values.  Products are exact, sums fp32 in the order of `inner`, rounded once.
- * offsets ascend from 0; others leave out rows or write them twice, but nothing outside out.  Also the gradient of rows,
- * with inner and outer, and transposed, the other way round.  (No counterpart in the reference.) */
+ * offsets[num_experts] to n (below 2^31); up to 65536 experts.  rows: n rows of `inner` values, row_stride apart; out:
+ * n x outer.  The matrix of expert e begins at weight + e * expert_stride: `inner` rows of `outer` values, weight_stride
+ * apart, or, if transposed, `outer` rows of `inner` values.  Sums are fp32, in an order that sizes, strides and alignment
+ * alone decide, rounded once.  offsets ascend from 0; others leave out rows or write them twice, but nothing outside
+ * out.  Also the gradient of rows, with inner and outer, and transposed, the other way round.  (No counterpart in the
+ * reference.) */
 int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n, int64_t inner, int type, const void* weight,
                      int64_t expert_stride, int64_t weight_stride, int transposed, int64_t num_experts, int64_t outer,
                      const int64_t* offsets, void* out, void* stream);
 
 /* The gradient of the matrices: dweight[e] (inner x outer) = the sum over the rows p of expert e of
  * rows[p, :]^T x grad[p, :], zeros for an expert without rows.  rows: n x inner, grad: n x outer, of any strides between
- * rows.  Sums are fp32, in an order that the offsets alone decide.  The workspace of sizes that no call takes is given as 256
+ * rows.  Sums are fp32, in an order that sizes and offsets alone decide.  The workspace of sizes that no call takes is given as 256
  * bytes; the call itself refuses them.  (No counterpart in the reference.) */
 size_t gs_expert_matmul_grad_workspace_bytes(int64_t n, int64_t inner, int64_t outer, int64_t num_experts);
 int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, const void* grad, int64_t grad_stride,

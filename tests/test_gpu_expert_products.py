@@ -614,6 +614,26 @@ def test_sizes_between_few_and_many(dev, dtype):
 
 
 @gpu
+def test_many_rows_and_offsets_that_no_sort_left(dev):
+    n = (1 << 18) + 9
+    x, w = whole(n, 40, dtype=torch.bfloat16, dev=dev, seed=1), whole(3, 40, 56, dtype=torch.bfloat16, dev=dev, seed=2)
+    grad = whole(n, 56, dtype=torch.bfloat16, dev=dev, seed=3)
+    p = torch.arange(n, device=dev, dtype=torch.int32)
+    for at in ([0, 2 ** 40, 2 ** 40, 2 ** 62], [-5, 10, 20, n + 400], [0, n, 100, 3], [n, 200, 100, 0], [-2 ** 62, -7, -1, -1],
+               [0, n, 0, n], [-2 ** 63, 2 ** 63 - 1, -2 ** 63, 2 ** 63 - 1]):
+        order = gs.ops.ExpertOrder(p, p, torch.tensor(at, device=dev))
+        buffers = [torch.full((1 << 20,), 7.0, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+        assert gs.ops.expert_matmul(x, order, w).shape == (n, 56)
+        assert capi.expert_matmul_grad(grad, x, order.offsets).shape == (3, 40, 56)
+        assert all(bool((b == 7).all()) for b in buffers)
+    order = gs.ops.ExpertOrder(p, p, torch.tensor([0, 100, 100, 200_000], device=dev))
+    got = gs.ops.expert_matmul(x, order, w)
+    assert torch.equal(got[:100].float(), (x[:100].float() @ w[0].float()).bfloat16().float())
+    assert torch.equal(got[100:200_000].float(), (x[100:200_000].float() @ w[2].float()).bfloat16().float())
+    assert not got[200_000:].any()
+
+
+@gpu
 def test_values_below_the_normal_ones(dev):
     """The smallest numbers of a type count like others."""
     for dtype, small, large in ((torch.float16, 2.0 ** -24, 2.0 ** 12), (torch.bfloat16, 2.0 ** -133, 2.0 ** 100),
