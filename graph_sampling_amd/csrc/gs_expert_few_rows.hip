@@ -1,8 +1,8 @@
 // Products of rows sorted by expert with each expert's matrix (gs_expert_products.hip) where experts have few rows, on
 // gfx950: tokens that are being generated.
 //
-// Every matrix that is met is read once, which bounds them: 16 rows x 2048 x 1024 of 13 experts, bf16, 12.6 us, 4.3 TB/s,
-// start and end included.  A workgroup takes up to 16 * MI rows of an expert and 16 *
+// Every matrix that is met is read once, which bounds them: 30 experts of 4096 x 256, 8 rows each, bf16, 16 us, 3.9
+// TB/s, start and end included.  A workgroup takes up to 16 * MI rows of an expert and 16 *
 // kWide columns (or half as many); its waves share out the depth, step by step, each with several steps of the matrix
 // on their way to registers, and their sums meet in LDS.  No value goes through LDS on its way in: a lane's chunks
 // are what the matrix cores take (along the depth), or become that by exchanging halves of registers (across it).

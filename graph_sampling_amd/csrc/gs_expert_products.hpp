@@ -164,23 +164,24 @@ bool narrow(const ProductArgs<T>& p) {
   return held && p.n >= (kHalf ? 1 << 18 : 1 << 19) && p.experts <= (kHalf ? 64 : 16);
 }
 
-// Where 64 x 64 tiles do not fill the card twice, the depth of a tile has to be shared out, too, if it is long: the more tiles
-// there are, the longer it has to be, and longer still where the matrix's values lie along the depth, which is read in pieces of 64
-// bytes, at odd places above all.  fp32, whose products take sixteen times as long, gains by it with few rows whatever their number.
-// Kernel times of both, us, few rows first: bf16, 32 experts of 4096 x 512, 16 rows each 36 and 74; of 1024 x 1024, 4 rows 16 and
-// 18; 16 of 1001 x 333, 40 rows 11 and 13, 100 rows 15 and 13, transposed 17 and 13, 29 and 13; 4 of 2048 x 1024, 200 rows 17 and
-// 29, transposed 35 and 22, 40 rows 14 and 15; 17 of 2733 x 1051, transposed, 2 rows 34 and 41; 64 of 1001 x 333, 3 rows 23 and 18;
-// fp32, 32 of 4096 x 512, 40 rows 108 and 180; 16 of 2048 x 1024, transposed, 40 rows 68 and 57; of 1001 x 333, 40 rows 18 and 26.
+// Where 64 x 64 tiles do not fill the card, the depth of a tile has to be shared out, too, if it is long: the more tiles
+// there are, the longer it has to be, and much longer where the matrix's values lie along the depth, which is read in pieces of
+// 64 bytes, at odd places above all.  With eight rows an expert or less a tile's products are mostly of no row: then fp32, whose
+// products take sixteen times as long, gains whatever their number, 16-bit values if the depth is very long.  Kernel times of both, us,
+// few rows first: bf16, 3 experts of 520 x 512, 60 rows each 6 and 6; 9 of 2048 x 1024, 2 rows 9 and 12; 30 of 4096 x 256, 8 rows 16
+// and 19; of 2048 x 1024, 16 rows 32 and 21; of 2053 x 1030, transposed, 8 rows 89 and 39; 100 of 3504 x 1760, 2 rows 185 and 229;
+// of 1001 x 333, 8 rows 22 and 18; fp32, 100 of 2048 x 1024, 8 rows 172 and 264, 16 rows 212 and 269, transposed 258 and 246; 3 of
+// 250 x 700, 60 rows 6 and 10; 9 of 2048 x 1024, 60 rows 55 and 47.
 template <typename T>
 bool few_rows(const ProductArgs<T>& p, bool across) {
   constexpr bool kHalf = sizeof(T) == 2;
   const int64_t tiles = likely_tiles(p, 64, 64);
   if (p.outer < 8) return false;
-  if (!kHalf && p.n <= 16 * p.experts && (p.n <= 4 * p.experts || tiles < 1400)) return true;
   const bool odd = kHalf && !across && !(aligned_to(p.weight, 4) && p.weight_stride % 2 == 0 && p.expert_stride % 2 == 0);
-  if (tiles >= 512) return false;
-  if (p.n <= (odd ? 2 : 16) * p.experts) return true;
-  return p.inner >= 512 && tiles * (!kHalf ? (across ? 3 : 10) : odd ? 40 : across ? 6 : 20) <= p.inner;
+  if (odd) return tiles * 80 <= p.inner;
+  if (p.n <= 8 * p.experts && p.inner >= (kHalf ? 3000 : 128)) return true;
+  if (p.n <= 16 * p.experts && (tiles < 160 || (!kHalf && across && p.inner >= 512))) return true;
+  return p.inner >= 128 && tiles < 200 && tiles * (kHalf ? (across ? 24 : 100) : across ? 2 : 5) <= p.inner;
 }
 
 }  // namespace products
