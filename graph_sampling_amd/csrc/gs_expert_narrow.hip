@@ -1,5 +1,5 @@
-// Products of rows sorted by expert with each expert's matrix (gs_expert_products.hip) where matrices are small and rows
-// many, on gfx950: the types of the nodes of a frontier.
+// Products of rows sorted by expert with each expert's matrix (gs_expert_products.hip) where matrices are small, or low, and
+// rows many, on gfx950: the types of the nodes of a frontier.
 //
 // Rows bound them, in and out.  A wave holds an expert's matrix (up to 128 columns of it) in registers, as what
 // the matrix cores take, and streams rows past it, 16 at a time, several of those on their way; nothing goes through LDS.  One

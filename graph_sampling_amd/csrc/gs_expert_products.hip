@@ -80,7 +80,7 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
 // fp32, which is bound by its products, is within 5 % of its best with the smallest.
 template <typename T, bool ACROSS>
 int choose_product(const ProductArgs<T>& p, hipStream_t st) {
-  if (products::narrow(p)) return products::launch_narrow(p, ACROSS, st);
+  if (products::narrow(p, ACROSS)) return products::launch_narrow(p, ACROSS, st);
   if (products::few_rows(p, ACROSS)) return products::launch_few_rows(p, ACROSS, st);
   const Way way = products::slower(products::way_of<T>(p.row_stride, p.inner, 256),
                                    products::way_of<T>(p.weight_stride, ACROSS ? p.outer : p.inner, 256));

@@ -154,14 +154,19 @@ int launch_few_rows(const ProductArgs<T>& p, bool across, hipStream_t st);
 // and 28; 256 x 64, 150 000 rows 25 and 22, 300 000 rows 39 and 39; 64 experts of 128 x 64, 150 000 rows 17 and 16, 300 000 rows
 // 23 and 28; fp32, 5 experts of 64 x 128, 150 000 rows 37 and 37, 700 000 rows 126 and 174; 60 x 40, 300 000 rows 36 and 35; 64
 // experts of 128 x 64, 700 000 rows 149 and 136.
+// More than 128 columns take a wave for each 128, which all fetch the rows: 3 experts of 64 x 1024, 42 838 rows, bf16, 21 and 28,
+// transposed 26 and 28, fp32 72 and 84; 8 of 42 x 477, 81 744 rows, bf16, 19 and 34; 5 of 144 x 352, 390 000 rows, bf16, 176 and 143;
+// 3 of 64 x 512, 20 000 rows, bf16, 10 and 10, transposed 14 and 10, fp32 25 and 23.
 template <typename T>
 int launch_narrow(const ProductArgs<T>& p, bool across, hipStream_t st);
 template <typename T>
-bool narrow(const ProductArgs<T>& p) {
+bool narrow(const ProductArgs<T>& p, bool across) {
   constexpr bool kHalf = sizeof(T) == 2;
   const int64_t steps = (p.inner + kStep<T> - 1) / kStep<T>;
-  const bool held = p.inner >= 8 && p.outer >= 8 && p.outer <= 128 && steps <= (p.outer <= 64 ? 8 : 4);
-  return held && p.n >= (kHalf ? 1 << 18 : 1 << 19) && p.experts <= (kHalf ? 64 : 16);
+  if (p.inner < 8 || p.outer < 8 || p.experts > (kHalf ? 64 : 16)) return false;
+  if (p.outer <= 128) return steps <= (p.outer <= 64 ? 8 : 4) && p.n >= (kHalf ? 1 << 18 : 1 << 19);
+  const int64_t shares = kCus / ((p.outer + 127) / 128) - p.experts - 1;
+  return across && steps <= 4 && shares >= 4 && shares >= 2 * p.experts && p.n >= (kHalf ? 1 << 23 : 1 << 24) / p.outer;
 }
 
 // Where 64 x 64 tiles do not fill the card, the depth of a tile has to be shared out, too, if it is long: the more tiles

@@ -533,7 +533,8 @@ def test_many_rows_with_small_matrices(dev, dtype):
     for experts, inner, outer, kind, transposed in (
             (5, 100, 128, "skewed", False), (5, 128, 100, "skewed", True), (64, 8, 8, "skewed", False), (16, 8, 8, "skewed", True), (3, 33, 65, "even", True),
             (1, 256, 64, "first", False), (2, 31, 9, "last", False), (4, 64, 127, "skewed", True), (0, 16, 24, "none", False),
-            (7, 129, 40, "skewed", True), (2, 9, 15, "none", False), (65, 40, 24, "even", False), (3, 16, 7, "skewed", False)):
+            (7, 129, 40, "skewed", True), (3, 40, 333, "skewed", False), (2, 33, 517, "last", False), (9, 64, 200, "skewed", True),
+            (2, 9, 15, "none", False), (65, 40, 24, "even", False), (3, 16, 7, "skewed", False)):
         loads = loads_of(kind, n, experts, experts + inner)
         order = order_of(loads, n, dev)
         rows = whole(n, inner, dtype=dtype, dev=dev, seed=inner)
