@@ -176,6 +176,27 @@ def test_gradient_against_differences(dev):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_the_sum_of_all_shares_leans_to_no_side(dev, dtype):
+    """Of 2^15 tokens, 4095 experts 7.5 to 9 below the first: half of a sum is exponentials of such differences.  An
+    exponential that is right to a step, above as often as below, leaves a mean error far below one: 70 roundings of 2^-24, evenly
+    spread, are 2.9e-7 a token, six standard deviations of 2^15 tokens' mean 9.6e-9.  An eighth of a step, 2^-26, is allowed; the
+    product with log2(e) rounded to fp32, 1.3e-8 of the difference too small, would lean by four times that.
+
+    fp16 has 256 values in that range, so that tokens share their roundings: in the lane that has the first expert's 1, sums are
+    multiples of 2^-23, and what an addition loses follows from the term alone.  256 losses spread over 2^-24 either way have a
+    mean of 2^-24 / sqrt(3) / 16 = 2.2e-9, 31.5 of them follow the 1, of a sum of 2.17: 3.1e-8, six times that is allowed as well."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    logits = -7.5 - 1.5 * torch.rand(1 << 15, 4096, generator=g, device=dev)
+    first = torch.randint(4096, (1 << 15, 1), generator=g, device=dev)
+    logits = logits.scatter_(1, first, 0.0).to(dtype)
+    experts, weights = gs.ops.expert_choose(logits, 1, False)
+    assert torch.equal(experts.long(), first)
+    want = 1.0 / torch.exp(logits.double()).sum(1, keepdim=True)
+    assert abs(float((weights.double() / want - 1.0).mean())) < 2.0 ** -26 + (6 * 3.1e-8 if dtype == torch.float16 else 0.0)
+
+
+@gpu
 def test_recorded_and_replayed(dev):
     for tokens, num, k in ((4, 64, 4), (900, 160, 6), (30, 600, 20)):
         l = logits_of("normal", tokens, num, torch.bfloat16, dev, 1).requires_grad_(True)
