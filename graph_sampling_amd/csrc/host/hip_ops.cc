@@ -1893,15 +1893,16 @@ torch::Tensor IndexSearch(const torch::Tensor& data, const torch::Tensor& keys) 
 
 // ------------------------------------------------------- rows moved by ids ----
 namespace {
-int ValueType(const torch::Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
+int ValueType(torch::ScalarType type, const char* name) {
+  switch (type) {
     case torch::kFloat32: return GS_F32;
     case torch::kFloat16: return GS_F16;
     case torch::kBFloat16: return GS_BF16;
     default:
-      TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+      TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", type);
   }
 }
+int ValueType(const torch::Tensor& t, const char* name) { return ValueType(t.scalar_type(), name); }
 
 // A 2-D tensor whose rows the kernels can walk: values of a row side by side, rows any distance apart.
 struct Rows {
@@ -2174,30 +2175,53 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(const torch::Tensor& logit
   return {experts, weights};
 }
 
+namespace {
+// What a choice returned and the gradient of its weights, beside logits [tokens, num_experts] on `device`.
+struct Chosen {
+  torch::Tensor weights, dweights;  // keep copies alive
+  const int32_t* experts;
+  int64_t tokens, choices;
+  Chosen(const torch::Tensor& d, const torch::Tensor& e, const torch::Tensor& w, int64_t num_tokens, int64_t num_experts,
+         const torch::Device& device) {
+    NeedDevice(e, "experts");
+    TORCH_CHECK(e.scalar_type() == torch::kInt32 && e.dim() == 2 && e.size(0) == num_tokens, "experts must be int32 [",
+                num_tokens, ", choices], got ", e.scalar_type(), " ", e.sizes());
+    tokens = num_tokens, choices = e.size(1);
+    TORCH_CHECK(choices <= 64 && choices <= num_experts && num_experts <= 4096, "at most 64 choices of 4096 experts are taken");
+    for (const auto* t : {&w, &d}) {
+      TORCH_CHECK(t->is_cuda(), "Not implemented warning: weights and their gradient must be GPU tensors");
+      TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->sizes() == e.sizes(),
+                  "weights and their gradient must be float32 of the shape of experts, ", e.sizes());
+    }
+    TORCH_CHECK(e.device() == device && w.device() == device && d.device() == device,
+                "logits, experts, weights and their gradient are on different devices");
+    experts = e.data_ptr<int32_t>(), weights = w.contiguous().resolve_neg(), dweights = d.contiguous().resolve_neg();
+  }
+};
+
+torch::Tensor ChooseGrad(const Chosen& c, const void* logits, int64_t stride, int type, int64_t num_experts, bool normalize,
+                         const torch::TensorOptions& like) {
+  auto out = torch::empty({c.tokens, num_experts}, like);
+  Check(gs_expert_choose_grad(logits, stride, type, c.experts, c.weights.data_ptr<float>(), c.dweights.data_ptr<float>(),
+                              c.tokens, num_experts, c.choices, normalize ? 1 : 0, out.data_ptr(), Stream(out)),
+        "gs_expert_choose_grad");
+  return out;
+}
+}  // namespace
+
 torch::Tensor ExpertChooseGrad(const torch::Tensor& dweights, const torch::Tensor& logits, const torch::Tensor& experts,
                                const torch::Tensor& weights, bool normalize) {
   const Rows l(logits, "logits");
-  const int64_t tokens = l.t.size(0), choices = experts.dim() == 2 ? experts.size(1) : -1;
-  NeedDevice(experts, "experts");
-  TORCH_CHECK(experts.scalar_type() == torch::kInt32 && experts.dim() == 2 && experts.size(0) == tokens,
-              "experts must be int32 [", tokens, ", choices], got ", experts.scalar_type(), " ", experts.sizes());
-  TORCH_CHECK(choices <= 64 && choices <= l.t.size(1) && l.t.size(1) <= 4096, "at most 64 choices of 4096 experts are taken");
-  for (const auto* t : {&weights, &dweights}) {
-    TORCH_CHECK(t->is_cuda(), "Not implemented warning: weights and their gradient must be GPU tensors");
-    TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->sizes() == experts.sizes(),
-                "weights and their gradient must be float32 of the shape of experts, ", experts.sizes());
-  }
-  TORCH_CHECK(experts.device() == logits.device() && weights.device() == logits.device() &&
-                  dweights.device() == logits.device(),
-              "logits, experts, weights and their gradient are on different devices");
   c10::hip::HIPGuard on(logits.device().index());
-  const auto w = weights.contiguous().resolve_neg(), d = dweights.contiguous().resolve_neg();
-  auto out = torch::empty({tokens, l.t.size(1)}, Like(logits));
-  Check(gs_expert_choose_grad(l.t.data_ptr(), l.stride, l.type, experts.data_ptr<int32_t>(), w.data_ptr<float>(),
-                              d.data_ptr<float>(), tokens, l.t.size(1), choices, normalize ? 1 : 0, out.data_ptr(),
-                              Stream(logits)),
-        "gs_expert_choose_grad");
-  return out;
+  const Chosen c(dweights, experts, weights, l.t.size(0), l.t.size(1), logits.device());
+  return ChooseGrad(c, l.t.data_ptr(), l.stride, l.type, l.t.size(1), normalize, Like(logits));
+}
+
+torch::Tensor ExpertChooseGradOfChosen(const torch::Tensor& dweights, const torch::Tensor& experts, const torch::Tensor& weights,
+                                       int64_t num_experts, torch::ScalarType type) {
+  c10::hip::HIPGuard on(experts.device().index());
+  const Chosen c(dweights, experts, weights, experts.size(0), num_experts, experts.device());
+  return ChooseGrad(c, nullptr, 0, ValueType(type, "logits"), num_experts, true, torch::dtype(type).device(experts.device()));
 }
 
 namespace {

@@ -391,6 +391,9 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(const torch::Tensor& logit
 // [tokens, experts], like logits (which are looked at without normalize only; their shape and type always)
 torch::Tensor ExpertChooseGrad(const torch::Tensor& dweights, const torch::Tensor& logits, const torch::Tensor& experts,
                                const torch::Tensor& weights, bool normalize);
+// the same with normalize, which looks at no logits: [tokens, num_experts] of their type
+torch::Tensor ExpertChooseGradOfChosen(const torch::Tensor& dweights, const torch::Tensor& experts, const torch::Tensor& weights,
+                                       int64_t num_experts, torch::ScalarType type);
 // [rows, outer] of rows [rows, inner] and weight [experts, inner, outer]
 torch::Tensor ExpertMatmul(const torch::Tensor& rows, const torch::Tensor& offsets, const torch::Tensor& weight);
 // [experts, inner, outer], laid out [experts, outer, inner] if transposed

@@ -126,8 +126,11 @@ struct CombineFunction : public torch::autograd::Function<CombineFunction> {
 struct ChooseFunction : public torch::autograd::Function<ChooseFunction> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, int64_t choices, bool normalize) {
     const auto [experts, weights] = hip::ExpertChoose(logits, choices, normalize);
-    ctx->save_for_backward({logits, experts, weights});
+    // (with normalize the logits are not looked at again: nothing of them is kept)
+    ctx->save_for_backward({normalize ? torch::Tensor() : logits, experts, weights});
     ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["num"] = logits.size(1);
+    ctx->saved_data["type"] = static_cast<int64_t>(logits.scalar_type());
     ctx->mark_non_differentiable({experts});
     ctx->set_materialize_grads(false);
     return {experts, weights};
@@ -137,7 +140,12 @@ struct ChooseFunction : public torch::autograd::Function<ChooseFunction> {
     if (!grads[1].defined()) return {{}, {}, {}};
     NoSecond(true, "experts' weights");  // (they depend on the logits, which are followed)
     at::NoGradGuard off;
-    return {hip::ExpertChooseGrad(grads[1], saved[0], saved[1], saved[2], ctx->saved_data["normalize"].toBool()), {}, {}};
+    if (ctx->saved_data["normalize"].toBool())
+      return {hip::ExpertChooseGradOfChosen(grads[1], saved[1], saved[2], ctx->saved_data["num"].toInt(),
+                                            static_cast<torch::ScalarType>(ctx->saved_data["type"].toInt())),
+              {},
+              {}};
+    return {hip::ExpertChooseGrad(grads[1], saved[0], saved[1], saved[2], false), {}, {}};
   }
 };
 

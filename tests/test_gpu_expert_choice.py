@@ -197,6 +197,32 @@ def test_the_sum_of_all_shares_leans_to_no_side(dev, dtype):
 
 
 @gpu
+def test_normalized_shares_keep_no_logits(dev):
+    """Their gradient looks at none: the logits may change, and their memory goes back, before the backward pass."""
+    for dtype in TYPES:
+        x = logits_of("normal", 4096, 1000, dtype, dev, 2).requires_grad_(True)
+        grad = torch.randn(4096, 5, device=dev)
+        want, = torch.autograd.grad(gs.ops.expert_choose(x * 1.0, 5)[1], x, grad)
+        logits = x * 1.0
+        weights = gs.ops.expert_choose(logits, 5)[1]
+        with torch.no_grad():
+            logits.fill_(float("nan"))
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(dev)
+        del logits
+        assert before - torch.cuda.memory_allocated(dev) >= 4096 * 1000 * torch.finfo(dtype).bits // 8
+        got, = torch.autograd.grad(weights, x, grad)
+        assert torch.equal(got, want)
+        # over all experts, they are kept, and a change is noticed
+        logits = x * 1.0
+        weights = gs.ops.expert_choose(logits, 5, False)[1]
+        with torch.no_grad():
+            logits.fill_(0.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(weights, x, grad)
+
+
+@gpu
 def test_recorded_and_replayed(dev):
     for tokens, num, k in ((4, 64, 4), (900, 160, 6), (30, 600, 20)):
         l = logits_of("normal", tokens, num, torch.bfloat16, dev, 1).requires_grad_(True)
