@@ -251,12 +251,16 @@ int gs_expert_choose(const void* logits, int64_t stride, int type, int64_t token
     using T = decltype(zero);
     auto go = [&](auto lanes, auto each) {
       constexpr int G = decltype(lanes)::value, kTokens = kThreads / G;
-      const int64_t blocks = (tokens + kTokens - 1) / kTokens;
-      GS_RETURN_IF_ERROR(check_grid("gs_expert_choose", blocks, kThreads));
-      hipLaunchKernelGGL((choose_kernel<T, G, decltype(each)::value>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
-                         0, static_cast<hipStream_t>(stream), static_cast<const T*>(logits), stride, tokens,
-                         static_cast<int>(experts), static_cast<int>(choices), normalize != 0, chosen, weights);
-      return check_launch("expert_choose");
+      constexpr int64_t kMost = most_blocks(kThreads) * kTokens;  // tokens a launch
+      for (int64_t t = 0; t < tokens; t += kMost) {
+        const int64_t here = tokens - t < kMost ? tokens - t : kMost;
+        hipLaunchKernelGGL((choose_kernel<T, G, decltype(each)::value>), dim3(static_cast<unsigned>((here + kTokens - 1) / kTokens)),
+                           dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(logits) + t * stride, stride,
+                           here, static_cast<int>(experts), static_cast<int>(choices), normalize != 0, chosen + t * choices,
+                           weights + t * choices);
+        GS_RETURN_IF_ERROR(check_launch("expert_choose"));
+      }
+      return static_cast<int>(GS_OK);
     };
     auto four = [&](auto g, auto a, auto b, auto c, auto d) {  // the fewest experts a lane that will do
       constexpr int G = decltype(g)::value;
@@ -288,13 +292,18 @@ int gs_expert_choose_grad(const void* logits, int64_t stride, int type, const in
     const int64_t chunks = (experts + Chunk<T>::kVec - 1) / Chunk<T>::kVec;
     auto go = [&](auto lanes) {
       constexpr int G = decltype(lanes)::value, kTokens = kThreads / G;
-      const int64_t blocks = (tokens + kTokens - 1) / kTokens;
-      GS_RETURN_IF_ERROR(check_grid("gs_expert_choose_grad", blocks, kThreads));
-      hipLaunchKernelGGL((choose_grad_kernel<T, G>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
-                         static_cast<size_t>(kTokens * chunks * Chunk<T>::kVec) * sizeof(float), static_cast<hipStream_t>(stream),
-                         static_cast<const T*>(logits), stride, chosen, weights, dweights, tokens,
-                         static_cast<int>(experts), static_cast<int>(choices), normalize != 0, static_cast<T*>(dlogits));
-      return check_launch("expert_choose_grad");
+      constexpr int64_t kMost = most_blocks(kThreads) * kTokens;
+      for (int64_t t = 0; t < tokens; t += kMost) {
+        const int64_t here = tokens - t < kMost ? tokens - t : kMost, item = t * choices;
+        hipLaunchKernelGGL((choose_grad_kernel<T, G>), dim3(static_cast<unsigned>((here + kTokens - 1) / kTokens)), dim3(kThreads),
+                           static_cast<size_t>(kTokens * chunks * Chunk<T>::kVec) * sizeof(float), static_cast<hipStream_t>(stream),
+                           logits ? static_cast<const T*>(logits) + t * stride : nullptr, stride, chosen ? chosen + item : nullptr,
+                           weights ? weights + item : nullptr, dweights ? dweights + item : nullptr, here,
+                           static_cast<int>(experts), static_cast<int>(choices), normalize != 0,
+                           static_cast<T*>(dlogits) + t * experts);
+        GS_RETURN_IF_ERROR(check_launch("expert_choose_grad"));
+      }
+      return static_cast<int>(GS_OK);
     };
     if (choices <= 4 && chunks <= 8) return go(N<4>());
     if (choices <= 8 && chunks <= 24) return go(N<8>());

@@ -2164,7 +2164,7 @@ std::tuple<torch::Tensor, torch::Tensor> ExpertChoose(const torch::Tensor& logit
   TORCH_CHECK(choices >= 0 && choices <= 64 && choices <= l.t.size(1), "choices must lie in [0, min(64, experts)], got ",
               choices, " of ", l.t.size(1), " experts");
   const int64_t tokens = l.t.size(0);
-  TORCH_CHECK(choices == 0 || tokens < ((int64_t(1) << 31) - 1) / choices, "at most 2^31 - 1 choices are taken, got ",
+  TORCH_CHECK(choices == 0 || tokens <= ((int64_t(1) << 31) - 1) / choices, "at most 2^31 - 1 choices are taken, got ",
               tokens, " times ", choices);
   c10::hip::HIPGuard on(logits.device().index());
   auto experts = torch::empty({tokens, choices}, torch::dtype(torch::kInt32).device(logits.device()));

@@ -267,6 +267,36 @@ def test_offsets_beyond_32_bits(dev):
 
 
 @gpu
+def test_as_many_choices_as_there_may_be(dev):
+    """2^31 - 1 tokens, of one choice each: more than one launch has workgroups for."""
+    if torch.cuda.mem_get_info(dev)[0] < 120 << 30:
+        pytest.skip("needs about 60 GB of free device memory")
+    n = 2 ** 31 - 1
+    l = torch.zeros(n, 2, dtype=torch.bfloat16, device=dev)
+    mine = torch.tensor([0, 7, 2 ** 30 - 65, 2 ** 30 - 64, 2 ** 30, 2 ** 30 + 1, n - 2, n - 1], device=dev)
+    l[mine, 1] = 1.0
+    for normalize in (True, False):
+        experts, weights = gs.ops.expert_choose(l, 1, normalize)
+        assert experts.shape == (n, 1) and int(experts.sum()) == 8 and bool((experts[mine] == 1).all())
+        # (half a step of a sum of two, and the quotient's)
+        assert abs(float(weights.min()) - (1.0 if normalize else 0.5)) < 2.0 ** -22
+        assert abs(float(weights.max()) - (1.0 if normalize else 1 / (1 + np.exp(-1)))) < 2.0 ** -22
+        d = capi.expert_choose_grad(weights, l, experts, weights, normalize)
+        if normalize:  # (a share of one is always 1)
+            assert not d.any()
+        else:
+            share = 1 / (1 + np.exp(-1))
+            for row, want in ((1, 0.125), (2 ** 30 - 66, 0.125), (2 ** 30 + 2, 0.125), (n - 3, 0.125)):
+                assert d[row].tolist() == [want, -want]
+            want = share * share * (1 - share)
+            off = (d[mine].double() - torch.tensor([-want, want], device=dev, dtype=torch.float64)).abs().max()
+            assert float(off) <= want * (half_step(torch.bfloat16) + 2.0 ** -20)
+        del experts, weights, d
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        gs.ops.expert_choose(l[:2 ** 30], 2)
+
+
+@gpu
 def test_recording_is_refused_where_it_would_end_the_process(dev):
     l = logits_of("normal", 4, 8, torch.float32, dev, 1).requires_grad_(True)
     eager = gs.ops.expert_choose(l, 2)[1]
