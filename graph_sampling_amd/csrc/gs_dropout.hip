@@ -14,11 +14,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kTagDropout = 6u;
 
-// A chunk of values a lane.
-template <typename T>
+// A chunk of values a lane.  LATER: a launch behind the first, whose values begin at block0 of the draws (the first one does without
+// the sum: 16384 x 2048 bf16 21.1 us with it, 20.6 without).
+template <typename T, bool LATER>
 __global__ void __launch_bounds__(kThreads)
 dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, int64_t n, uint32_t least, bool none, float scale,
-               uint64_t seed, const int64_t* __restrict__ seed_at, T* __restrict__ out) {
+               uint64_t seed, const int64_t* __restrict__ seed_at, T* __restrict__ out, uint64_t block0) {
   constexpr int kVec = Chunk<T>::kVec;
   if (seed_at) seed = static_cast<uint64_t>(*seed_at);
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kVec;
@@ -29,7 +30,7 @@ dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, int64_t 
   if (residual) r = widen<T>(load_chunk(residual + first, there));
 #pragma unroll
   for (int i = 0; i < kVec; i += 4) {
-    const U4 draws = draw_block(seed, kTagDropout, 0, static_cast<uint64_t>(first + i) >> 2);
+    const U4 draws = draw_block(seed, kTagDropout, 0, (LATER ? block0 : 0) + (static_cast<uint64_t>(first + i) >> 2));
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (draws.v[j] >= least && !none) r[i + j] = __fmaf_rn(v[i + j], scale, r[i + j]);
@@ -58,12 +59,16 @@ extern "C" int gs_dropout(const void* x, const void* residual, int64_t n, int ty
   const float scale = none ? 0.0f : static_cast<float>(1.0 / (1.0 - p));
   return with_value_type(type, "gs_dropout", [&](auto zero) {
     using T = decltype(zero);
-    constexpr int64_t kBlock = kThreads * Chunk<T>::kVec;
-    const int64_t blocks = (n + kBlock - 1) / kBlock;
-    GS_RETURN_IF_ERROR(check_grid("gs_dropout", blocks, kThreads));
-    hipLaunchKernelGGL((dropout_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(x), static_cast<const T*>(residual), n, least,
-                       none, scale, seed, seed_at, static_cast<T*>(out));
-    return check_launch("dropout");
+    constexpr int64_t kBlock = kThreads * Chunk<T>::kVec, kMost = most_blocks(kThreads) * kBlock;  // values a launch
+    for (int64_t base = 0; base < n; base += kMost) {
+      const int64_t here = n - base < kMost ? n - base : kMost;
+      const dim3 grid(static_cast<unsigned>((here + kBlock - 1) / kBlock));
+      hipLaunchKernelGGL((base == 0 ? dropout_kernel<T, false> : dropout_kernel<T, true>), grid, dim3(kThreads), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const T*>(x) + base,
+                         residual ? static_cast<const T*>(residual) + base : nullptr, here, least, none, scale, seed, seed_at,
+                         static_cast<T*>(out) + base, static_cast<uint64_t>(base) / 4);
+      GS_RETURN_IF_ERROR(check_launch("dropout"));
+    }
+    return static_cast<int>(GS_OK);
   });
 }

@@ -222,6 +222,18 @@ def test_positions_beyond_32_bits(dev):
 
 
 @gpu
+def test_more_values_than_one_launch_has_workgroups_for(dev):
+    if torch.cuda.mem_get_info(dev)[0] < 200 << 30:
+        pytest.skip("needs about 140 GB of free device memory")
+    n = 2 ** 34 + 1027
+    out = gs.ops.dropout(torch.ones(n, device=dev), 0.5, 22)
+    for first in (0, 2 ** 34 - 2048, 2 ** 34 - 1024, 2 ** 34):
+        kept = words(22, range(first // 4, first // 4 + 256)).astype(np.uint64) >= np.uint64(2 ** 31)
+        assert np.array_equal(out[first:first + 1024].cpu().numpy(), np.where(kept, 2.0, 0.0))
+    assert np.array_equal(out[-3:].cpu().numpy(), np.where(words(22, [2 ** 32 + 256])[:3] >= 2 ** 31, 2.0, 0.0))
+
+
+@gpu
 def test_refusals(dev):
     x = values((6, 5), torch.float32, dev, 1)
     for args, match in (((x.double(), 0.5, 1), "float32, float16 or bfloat16"), ((x, 1.5, 1), "probability"), ((x, -0.1, 1), "probability"),
