@@ -22,7 +22,7 @@ few_rows_kernel(ProductArgs<T> p) {
   constexpr int kVec = S::kVec, kRows = 16 * MI, kDepth = 4;  // steps on their way
   constexpr int kPad = S::kWide + 4;
   __shared__ __attribute__((aligned(16))) float s_sums[kWaves][kRows][kPad];
-  RowTile t = find_tile<kThreads>(p.offsets, p.experts, p.n, kRows, p.col_tiles);
+  RowTile t = find_tile<kThreads>(p.offsets, p.experts, p.n, kRows, p.col_tiles, p.first_block);
   if (t.rows <= 0) return;
   t = {uniform(t.expert), uniform(t.begin), uniform(t.rows), uniform(t.col), -1};
   const int lane = threadIdx.x % kWave, row16 = lane % 16, quarter = lane / 16;
@@ -149,9 +149,7 @@ template <typename T, bool ACROSS, int MI, int COLS>
 int launch(ProductArgs<T> p, hipStream_t st) {
   p.col_tiles = (p.outer + 16 * COLS - 1) / (16 * COLS);
   const int64_t blocks = blocks_of(most_row_tiles(p.n, p.experts, 16 * MI), p.col_tiles);
-  GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, kThreads));
-  hipLaunchKernelGGL((few_rows_kernel<T, ACROSS, MI, COLS>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, p);
-  return check_launch("expert_matmul");
+  return launch_blocks(few_rows_kernel<T, ACROSS, MI, COLS>, p, blocks, kThreads, "expert_matmul", st);
 }
 
 }  // namespace

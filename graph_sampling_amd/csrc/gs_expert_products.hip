@@ -39,7 +39,7 @@ product_kernel(ProductArgs<T> p) {
   using Tile = products::Tile<T, false, ACROSS, BM, BN, WM, WN, RING, WAY>;
   constexpr bool kQuarters = BM == 256 && BN == 256;
   __shared__ __attribute__((aligned(1024))) char s_steps[Tile::kBytes];
-  RowTile t = products::find_tile<Tile::kThreads, kQuarters>(p.offsets, p.experts, p.n, BM, p.col_tiles);
+  RowTile t = products::find_tile<Tile::kThreads, kQuarters>(p.offsets, p.experts, p.n, BM, p.col_tiles, p.first_block);
   if (t.rows <= 0) return;
   t = {products::uniform(t.expert), products::uniform(t.begin), products::uniform(t.rows), products::uniform(t.col),
        products::uniform(t.quarter)};
@@ -61,9 +61,7 @@ int launch_product(ProductArgs<T> p, hipStream_t st) {
   p.col_tiles = (p.outer + BN - 1) / BN;
   const int64_t more = BM == 256 && BN == 256 ? products::kCus / 2 * 3 : 0;  // (where some are made in quarters)
   const int64_t blocks = products::blocks_of(products::most_row_tiles(p.n, p.experts, BM), p.col_tiles, more);
-  GS_RETURN_IF_ERROR(check_grid("gs_expert_matmul", blocks, threads));
-  hipLaunchKernelGGL((product_kernel<T, ACROSS, BM, BN, WM, WN, RING, WAY>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, st, p);
-  return check_launch("expert_matmul");
+  return products::launch_blocks(product_kernel<T, ACROSS, BM, BN, WM, WN, RING, WAY>, p, blocks, threads, "expert_matmul", st);
 }
 
 // Large tiles read less, small ones fill the card with less work and waste less of it; chunks that are not aligned come more
@@ -132,7 +130,7 @@ extern "C" int gs_expert_matmul(const void* rows, int64_t row_stride, int64_t n,
   return with_value_type(type, "gs_expert_matmul", [&](auto zero) {
     using T = decltype(zero);
     const ProductArgs<T> p{static_cast<const T*>(rows), row_stride, n, inner, static_cast<const T*>(weight), expert_stride,
-                           weight_stride, num_experts, outer, offsets, static_cast<T*>(out), 0};
+                           weight_stride, num_experts, outer, offsets, static_cast<T*>(out), 0, 0};
     const auto st = static_cast<hipStream_t>(stream);
     return transposed ? choose_product<T, false>(p, st) : choose_product<T, true>(p, st);
   });

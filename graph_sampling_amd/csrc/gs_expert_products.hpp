@@ -22,7 +22,7 @@ constexpr int64_t kCus = 256;  // workgroups of large tiles that run at once
 // after all of these, so that every die has its share of the work.
 template <int THREADS, bool QUARTERS = false>
 __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets, int64_t experts, int64_t n, int tile_rows,
-                                             int64_t col_tiles) {
+                                             int64_t col_tiles, int64_t first_block = 0) {
   __shared__ int64_t s_wave[THREADS / kWave];
   __shared__ RowTile s_found;
   const int64_t each = (experts + THREADS - 1) / THREADS, first = each * threadIdx.x;
@@ -49,7 +49,7 @@ __device__ __forceinline__ RowTile find_tile(const int64_t* __restrict__ offsets
   const Group behind = group_of(offsets, experts, n, experts);
   const int64_t tiles = total * col_tiles, rest = QUARTERS && tiles % kCus <= kCus / 2 ? tiles % kCus : 0, whole = tiles - rest;
   const int64_t whole_blocks = (whole + kXcds - 1) / kXcds * kXcds, part_blocks = (rest * 4 + kXcds - 1) / kXcds * kXcds;
-  int64_t block = blockIdx.x, many = whole;
+  int64_t block = first_block + blockIdx.x, many = whole;
   bool part = false, dead = false;
   if (block >= whole_blocks) {
     block -= whole_blocks;
@@ -94,6 +94,7 @@ struct ProductArgs {
   const int64_t* offsets;
   T* out;
   int64_t col_tiles;
+  int64_t first_block;  // of the launch
 };
 
 // Tiles of rows that there can be: a part of one for every expert that has rows, and for the rows behind.

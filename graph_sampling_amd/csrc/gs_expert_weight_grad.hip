@@ -29,6 +29,7 @@ struct WeightGradArgs {
   // where the rows are cut into pieces of `piece` for the sake of more workgroups: the sums of each, and how many there are
   float* sums;
   int64_t piece, pieces;
+  int64_t first_block;  // of the launch
 };
 
 // Pieces are cut at multiples of `piece`, and where an expert ends.  Of expert e, piece c (from piece * c on) is the
@@ -74,7 +75,7 @@ weight_grad_kernel(WeightGradArgs<T> p) {
   const int64_t live = PIECES ? products::inside(p.offsets[p.experts], p.n) : 0;
   const int64_t pieces = live > 0 ? (live - 1) / p.piece + p.experts : 0;
   const int64_t in_expert = p.row_tiles * p.col_tiles, all = in_expert * (PIECES ? pieces : p.experts);
-  const int64_t die = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  const int64_t die = blockIdx.x % kXcds, slot = (p.first_block + blockIdx.x) / kXcds;
   int64_t which;
   if (shares(in_expert, p.experts)) {
     const int64_t share = (in_expert + kXcds - 1) / kXcds, nth = die * share + slot % share;
@@ -179,12 +180,9 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   p.piece = piece_rows(p.n, p.experts, p.inner, p.outer);
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
   const int64_t padded_tiles = shares(tiles, p.experts) ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;
-  if (items > most_blocks(threads) / padded_tiles - kXcds) return check_grid("gs_expert_matmul_grad", most_blocks(threads) + 1, threads);
-  const dim3 grid(static_cast<unsigned>((items * padded_tiles + kXcds - 1) / kXcds * kXcds));
-  if (!p.piece) {
-    hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, false>), grid, dim3(threads), 0, st, p);
-    return check_launch("expert_matmul_grad");
-  }
+  const int64_t blocks = (items * padded_tiles + kXcds - 1) / kXcds * kXcds;
+  if (!p.piece)
+    return products::launch_blocks(weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, false>, p, blocks, threads, "expert_matmul_grad", st);
   p.pieces = items;
   Carver ws(workspace, workspace_bytes);
   p.sums = ws.take<float>(static_cast<size_t>(items * p.inner * p.outer));
@@ -193,8 +191,8 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
                    gs_expert_matmul_grad_workspace_bytes(p.n, p.inner, p.outer, p.experts));
     return GS_ERR_WORKSPACE;
   }
-  hipLaunchKernelGGL((weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, true>), grid, dim3(threads), 0, st, p);
-  GS_RETURN_IF_ERROR(check_launch("expert_matmul_grad"));
+  GS_RETURN_IF_ERROR(
+      products::launch_blocks(weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, true>, p, blocks, threads, "expert_matmul_grad", st));
   return items > 16 * p.experts ? launch_join<T, 16>(p, st) : launch_join<T, 4>(p, st);
 }
 
@@ -265,7 +263,7 @@ int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, c
   return with_value_type(type, "gs_expert_matmul_grad", [&](auto zero) {
     using T = decltype(zero);
     const WeightGradArgs<T> p{static_cast<const T*>(rows), row_stride, static_cast<const T*>(grad), grad_stride, n, inner, outer,
-                              offsets, num_experts, static_cast<T*>(dweight), 0, 0, nullptr, 0, 0};
+                              offsets, num_experts, static_cast<T*>(dweight), 0, 0, nullptr, 0, 0, 0};
     return choose_weight_grad<T>(p, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   });
 }

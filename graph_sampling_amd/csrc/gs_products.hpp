@@ -591,5 +591,17 @@ __device__ __forceinline__ Group group_of(const int64_t* __restrict__ offsets, i
   return {inside(offsets[e], n), e < experts ? inside(offsets[e + 1], n) : n};
 }
 
+// Launches a kernel of one argument for so many workgroups, in turns where one launch does not take them.
+template <typename Args>
+int launch_blocks(void (*kernel)(Args), Args args, int64_t blocks, int threads, const char* what, hipStream_t st) {
+  const int64_t most = most_blocks(threads) / kXcds * kXcds;  // (every turn begins at the first die)
+  for (args.first_block = 0; args.first_block < blocks; args.first_block += most) {
+    const int64_t here = blocks - args.first_block < most ? blocks - args.first_block : most;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(here)), dim3(threads), 0, st, args);
+    GS_RETURN_IF_ERROR(check_launch(what));
+  }
+  return GS_OK;
+}
+
 }  // namespace products
 }  // namespace gs

@@ -665,6 +665,38 @@ def test_as_many_experts_as_there_may_be(dev):
         gs.ops.expert_matmul(rows, too_many, weight[:1].expand(experts + 1, 16, 24))
 
 
+@gpu
+def test_more_tiles_than_one_launch_has_workgroups_for(dev):
+    """Of as many experts as there may be, wide matrices: more than 2^24 workgroups of 256 threads, or 2^23 of 512.  Whole numbers."""
+    if torch.cuda.mem_get_info(dev)[0] < 100 << 30:
+        pytest.skip("needs about 40 GB of free device memory")
+    n, experts = 70_000, 65_536
+    loads = loads_of("even", n - 40, experts, 2)
+    order = order_of(loads, n, dev)
+    of = torch.repeat_interleave(torch.arange(experts, device=dev), torch.from_numpy(loads).to(dev))
+    live = of.numel()
+    some = torch.cat([torch.arange(200, device=dev), torch.randint(live, (600,), device=dev), torch.arange(live - 200, live, device=dev)])
+    for inner, outer in ((8, 16384), (128, 4096)):  # tiles of 64 x 64; few rows
+        rows = whole(n, inner, dtype=torch.float32, dev=dev, seed=inner)
+        # (matrices that overlap: each begins a value behind the one before)
+        weight = whole(inner * outer + experts, dtype=torch.float32, dev=dev, seed=outer).as_strided((experts, inner, outer), (1, outer, 1))
+        out = gs.ops.expert_matmul(rows, order, weight)
+        for part in some.split(100):
+            want = torch.bmm(rows[part][:, None].double(), weight[of[part]].double())[:, 0]
+            assert torch.equal(out[part].double(), want)
+        assert torch.equal(out[:live].double().sum(1), (rows[:live].double() * weight.sum(2).double()[of]).sum(1))
+        assert not out[live:].any()
+        del out, weight
+    inner, outer = 4, 16448
+    rows, grad = (whole(n, d, dtype=torch.float32, dev=dev, seed=d) for d in (inner, outer))
+    dw = capi.expert_matmul_grad(grad, rows, order.offsets)
+    want = torch.zeros(experts, inner, device=dev).index_add_(0, of, rows[:live] * grad[:live].sum(1, keepdim=True))
+    assert torch.equal(dw.sum(2), want)
+    for e in [0, 1, 2, 12_345, 65_534, 65_535]:
+        mine = of == e
+        assert torch.equal(dw[e], rows[:live][mine].t() @ grad[:live][mine])
+
+
 # ------------------------------------------------------------------ no GPU ----
 def test_bad_arguments_are_refused_before_anything_is_launched():
     import ctypes
