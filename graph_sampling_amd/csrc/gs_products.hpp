@@ -302,14 +302,12 @@ struct Direct {
   static __device__ __forceinline__ int row(int i) { return static_cast<int>(threadIdx.x) / L::kRowSlots + i * kRowsApart; }
   static __device__ __forceinline__ int chunk(int i) { return L::chunk_in(row(i), threadIdx.x % L::kRowSlots) * L::kVec; }
   // Written as instructions because the compiler, which cannot tell the ring's steps apart, would wait for all of them before
-  // each read of LDS; who reads waits by arrived().  (m0 holds nothing else: the compiler sets it in front of each use of
-  // its own.)
+  // each read of LDS; who reads waits by arrived().  (m0, where the place in LDS goes, is set by the compiler, which so knows what it
+  // holds; the instruction behind has to wait for a cycle.)
   static __device__ __forceinline__ void put(uint64_t base, int bytes, int from, uint32_t lds, int offset) {
     const Buffer buffer = {static_cast<int>(base), static_cast<int>(base >> 32), bytes, 0x00020000};
-    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
-                 :
-                 : "s"(lds), "n"(offset), "v"(from), "s"(buffer)
-                 : "memory", "scc");
+    register uint32_t place asm("m0") = lds + offset;
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(place), "v"(from), "s"(buffer) : "memory");
   }
   // Puts a part of the next step on its way to lds (an offset); bytes: all there are, or none, for zeros.
   __device__ __forceinline__ void part(int i, uint32_t lds, int bytes) const {

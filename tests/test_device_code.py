@@ -52,3 +52,20 @@ def test_stores_have_arrived_before_the_workgroup_counts_itself(source, kernel, 
         stored, barrier = _last(before, publish), _last(before, r"^s_barrier")
         assert 0 <= stored < barrier
         assert any(re.match(r"s_waitcnt vmcnt\(0\)", line) for line in before[stored:barrier])
+
+
+@pytest.mark.skipif(not os.path.exists(build.HIPCC), reason="no hipcc")
+@pytest.mark.parametrize("source", ["gs_expert_products.hip", "gs_expert_weight_grad.hip"])
+def test_the_compiler_knows_what_m0_holds(source, tmp_path):
+    """Loads that go straight into LDS are written as instructions and take their place from m0, a register that the
+    compiler may keep a value of its own in: it has to set it itself, as an operand, not one of the instructions written."""
+    text = _assembly(source, tmp_path)
+    written = re.findall(r";;#ASMSTART(.*?);;#ASMEND", text, re.S)
+    loads = [w for w in written if re.search(r"buffer_load_dwordx4 .* lds", w)]
+    assert len(loads) > 100
+    for w in loads:
+        assert not re.search(r"\bm0\b", w)
+        # one cycle between m0's change and its use
+        assert re.search(r"s_nop 0\s+buffer_load_dwordx4", w)
+    before = [line.split(";")[0].strip() for line in text.split("\n")]
+    assert sum(bool(re.match(r"s_(mov|add)\w+ m0,", line)) for line in before) >= 10
