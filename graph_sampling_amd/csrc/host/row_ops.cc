@@ -152,13 +152,14 @@ struct ChooseFunction : public torch::autograd::Function<ChooseFunction> {
 struct MatmulFunction : public torch::autograd::Function<MatmulFunction> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& rows, const torch::Tensor& offsets,
                                const torch::Tensor& weight) {
+    const auto out = hip::ExpertMatmul(rows, offsets, weight);  // (refuses what else would be asked for its sizes here)
     const bool of_rows = rows.requires_grad(), of_weight = weight.requires_grad();
     // (each is kept for the other's gradient)
     ctx->save_for_backward({of_weight ? rows : torch::Tensor(), offsets, of_rows ? weight : torch::Tensor()});
     ctx->saved_data["rows"] = of_rows;
     ctx->saved_data["weight"] = of_weight;
     ctx->saved_data["transposed"] = hip::ColumnsContiguous(weight);
-    return hip::ExpertMatmul(rows, offsets, weight);
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();

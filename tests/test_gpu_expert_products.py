@@ -748,6 +748,24 @@ def test_cpu_tensors_are_refused():
         gs.ops.expert_matmul(torch.zeros(3, 4), order, torch.zeros(2, 4, 5))
 
 
+def test_matrices_that_are_none_are_refused_alike_with_and_without_gradients():
+    p = torch.zeros(3, dtype=torch.int32)
+    order = gs.ops.ExpertOrder(p, p, torch.zeros(3, dtype=torch.int64))
+    for shape in ((4, 5), (4,), (), (2, 4, 5)):
+        for followed in (False, True):
+            with pytest.raises(RuntimeError, match="GPU tensor"):
+                gs.ops.expert_matmul(torch.zeros(3, 4), order, torch.zeros(shape, requires_grad=followed))
+
+
+@gpu
+def test_matrices_of_two_dimensions_are_refused_with_gradients(dev):
+    x = normal(10, 4, dtype=torch.float32, dev=dev, seed=1)
+    order = order_of(np.array([3, 3, 4]), 10, dev)
+    for shape in ((4, 5), (4,)):
+        with pytest.raises(RuntimeError, match="inner, outer"):
+            gs.ops.expert_matmul(x, order, torch.zeros(shape, device=dev, requires_grad=True))
+
+
 def test_more_experts_than_are_taken():
     import ctypes
     lib, i64 = capi.lib(), ctypes.c_int64
