@@ -26,9 +26,9 @@ struct WeightGradArgs {
   int64_t experts;
   T* out;
   int64_t row_tiles, col_tiles;
-  // where the rows are cut into pieces of `piece` for the sake of more workgroups: the sums of each, and how many there are
+  // where the rows are cut into pieces of `piece` for the sake of more workgroups: the sums of each
   float* sums;
-  int64_t piece, pieces;
+  int64_t piece;
   int64_t first_block;  // of the launch
 };
 
@@ -171,7 +171,8 @@ int launch_join(const WeightGradArgs<T>& p, hipStream_t st) {
   return check_launch("expert_matmul_grad");
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int RING, Way WAY>
+// CUT: whether the rows can be in pieces (which have 128 rows at least, as the experts have then: a tile for fewer makes whole ones).
+template <typename T, int BM, int BN, int WM, int WN, int RING, Way WAY, bool CUT = true>
 int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_bytes, hipStream_t st) {
   constexpr int threads = WM * WN * kWave;
   p.row_tiles = (p.inner + BM - 1) / BM;
@@ -181,19 +182,20 @@ int launch_weight_grad(WeightGradArgs<T> p, void* workspace, size_t workspace_by
   const int64_t items = p.piece ? pieces_there(p.n, p.experts, p.piece) : p.experts;
   const int64_t padded_tiles = shares(tiles, p.experts) ? (tiles + kXcds - 1) / kXcds * kXcds : tiles;
   const int64_t blocks = (items * padded_tiles + kXcds - 1) / kXcds * kXcds;
-  if (!p.piece)
+  if (!CUT || !p.piece)
     return products::launch_blocks(weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, false>, p, blocks, threads, "expert_matmul_grad", st);
-  p.pieces = items;
-  Carver ws(workspace, workspace_bytes);
-  p.sums = ws.take<float>(static_cast<size_t>(items * p.inner * p.outer));
-  if (!ws.ok) {
-    set_error_text("gs_expert_matmul_grad: workspace needs %zu bytes, 256-byte aligned",
-                   gs_expert_matmul_grad_workspace_bytes(p.n, p.inner, p.outer, p.experts));
-    return GS_ERR_WORKSPACE;
+  if constexpr (CUT) {
+    Carver ws(workspace, workspace_bytes);
+    p.sums = ws.take<float>(static_cast<size_t>(items * p.inner * p.outer));
+    if (!ws.ok) {
+      set_error_text("gs_expert_matmul_grad: workspace needs %zu bytes, 256-byte aligned",
+                     gs_expert_matmul_grad_workspace_bytes(p.n, p.inner, p.outer, p.experts));
+      return GS_ERR_WORKSPACE;
+    }
+    GS_RETURN_IF_ERROR(
+        products::launch_blocks(weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, true>, p, blocks, threads, "expert_matmul_grad", st));
+    return items > 16 * p.experts ? launch_join<T, 16>(p, st) : launch_join<T, 4>(p, st);
   }
-  GS_RETURN_IF_ERROR(
-      products::launch_blocks(weight_grad_kernel<T, BM, BN, WM, WN, RING, WAY, true>, p, blocks, threads, "expert_matmul_grad", st));
-  return items > 16 * p.experts ? launch_join<T, 16>(p, st) : launch_join<T, 4>(p, st);
 }
 
 // As for the products of rows; here a matrix, or what a piece adds to it, is a product of its own, and one of few rows is not
@@ -216,7 +218,7 @@ int choose_weight_grad(const WeightGradArgs<T>& p, void* workspace, size_t works
       return launch_weight_grad<T, 256, 256, 2, 4, 4, Way::kDirect>(p, workspace, workspace_bytes, st);
     if (p.inner > 64 && p.outer > 64 && tiles(128, 128) >= 250)
       return rows >= 128 ? launch_weight_grad<T, 128, 128, 2, 2, 4, Way::kDirect>(p, workspace, workspace_bytes, st)
-                         : launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect>(p, workspace, workspace_bytes, st);
+                         : launch_weight_grad<T, 128, 128, 2, 2, 3, Way::kDirect, false>(p, workspace, workspace_bytes, st);
     if (p.outer > 64 && rows >= 128 && tiles(64, 128) >= 140 && tiles(64, 128) <= 512)
       return launch_weight_grad<T, 64, 128, 2, 2, 5, Way::kDirect>(p, workspace, workspace_bytes, st);
   }
@@ -263,7 +265,7 @@ int gs_expert_matmul_grad(const void* rows, int64_t row_stride, int64_t inner, c
   return with_value_type(type, "gs_expert_matmul_grad", [&](auto zero) {
     using T = decltype(zero);
     const WeightGradArgs<T> p{static_cast<const T*>(rows), row_stride, static_cast<const T*>(grad), grad_stride, n, inner, outer,
-                              offsets, num_experts, static_cast<T*>(dweight), 0, 0, nullptr, 0, 0, 0};
+                              offsets, num_experts, static_cast<T*>(dweight), 0, 0, nullptr, 0, 0};
     return choose_weight_grad<T>(p, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   });
 }

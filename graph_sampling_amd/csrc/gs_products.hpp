@@ -48,11 +48,11 @@ struct Layout {
   // s ^ (r / 2 % 4): lanes 0 - 3, 12 - 15 and 20 - 27 are served together, then the others.  Across k, row k holds WIDTH
   // values in units of 16 that trade places: 32 lanes read a unit of rows k .. k + 3 and k + 8 .. k + 11 (16 bits), 64 lanes
   // one of rows k, k + 4, k + 8 and k + 12 (fp32).
+  static_assert(WIDTH >= 64, "four units of a row trade places");
   static __device__ __forceinline__ int turn(int row) {
     if (!ACROSS) return (row >> 1) & 3;
-    if (kSize == 4) return WIDTH >= 64 ? (row >> 2) & 3 : (row >> 2) & (WIDTH / 16 - 1);
-    if (WIDTH >= 128) return (row & 3) | (((row >> 3) & 1) << 2);
-    return WIDTH == 64 ? ((row >> 1) & 1) | (((row >> 3) & 1) << 1) : 0;
+    if (kSize == 4) return (row >> 2) & 3;
+    return WIDTH >= 128 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
   }
   static __device__ __forceinline__ int chunk_in(int row, int slot) {
     if (!ACROSS) return slot ^ turn(row);
@@ -229,7 +229,8 @@ constexpr int kHeld = 4;
 template <typename T, bool ACROSS, int WIDTH, int THREADS>
 struct Staged {
   using L = Layout<T, ACROSS, WIDTH>;
-  static constexpr int kEach = (L::kSlots + THREADS - 1) / THREADS;
+  static constexpr int kEach = L::kSlots / THREADS;
+  static_assert(L::kSlots % THREADS == 0, "every lane has as many chunks");
   Operand<T> x;
   int64_t k0 = 0;  // of the next step
   Values<T> held[kHeld][kEach];
@@ -237,9 +238,6 @@ struct Staged {
   static __device__ __forceinline__ int row(int i) { return (i * THREADS + static_cast<int>(threadIdx.x)) / L::kRowSlots; }
   static __device__ __forceinline__ int chunk(int i) {
     return L::chunk_in(row(i), (i * THREADS + static_cast<int>(threadIdx.x)) % L::kRowSlots) * L::kVec;
-  }
-  static __device__ __forceinline__ bool mine(int i) {
-    return L::kSlots % THREADS == 0 || i * THREADS + static_cast<int>(threadIdx.x) < L::kSlots;
   }
   __device__ __forceinline__ explicit Staged(const Operand<T>& operand) : x(operand) {}
   // The first step: the last part of the depth, `rest` of a step, so that all others are whole.
@@ -251,7 +249,7 @@ struct Staged {
   }
   __device__ __forceinline__ Values<T> part(int i, int64_t left) const {
     const int64_t r = ACROSS ? k0 + row(i) : row(i), c = ACROSS ? chunk(i) : k0 + chunk(i);
-    const bool in = mine(i) && (ACROSS ? row(i) < left : r < x.rows);
+    const bool in = ACROSS ? row(i) < left : r < x.rows;
     return load_part(x.base + r * x.stride + c, in ? (ACROSS ? x.width - c : left - chunk(i)) : 0);
   }
   // The next step; more: it is not the last one (which is read again, and not used, behind the end).  whole: there is one.
@@ -265,8 +263,7 @@ struct Staged {
   template <int SLOT>
   __device__ __forceinline__ void store(char* lds) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (mine(i)) *reinterpret_cast<Values<T>*>(lds + (i * THREADS + threadIdx.x) * 16) = held[SLOT][i];
+    for (int i = 0; i < kEach; ++i) *reinterpret_cast<Values<T>*>(lds + (i * THREADS + threadIdx.x) * 16) = held[SLOT][i];
   }
 };
 
@@ -364,6 +361,7 @@ struct Tile {
   using RB = Reader<T, B_ACROSS, BN>;
   static constexpr int kThreads = WM * WN * kWave;
   static constexpr int kMI = BM / WM / 16, kNI = BN / WN / 16, kFirst = kMI / 2;
+  static_assert(kFirst >= 1, "either half of a step has rows");
   static constexpr int kStage = LA::kBytes + LB::kBytes, kBytes = RING * kStage;  // of LDS
   static constexpr bool kDirect = WAY == Way::kDirect;
   using FA = std::conditional_t<kDirect, Direct<T, A_ACROSS, BM, kThreads>, Staged<T, A_ACROSS, BM, kThreads>>;
@@ -453,7 +451,6 @@ struct Tile {
       s.template store<(TURN + 2) % kHeld>(s.lds + (now + 2 * kStage) % kBytes);
       s.template load<(TURN + 2) % kHeld>();
     }
-    if (kFirst == 0) f.a[0] = s.ra.fragment(0, now);
 #pragma unroll
     for (int q = 0; q < kSecondProducts; ++q) {
       const int i = kFirst + q / kNI, j = q % kNI;
