@@ -1,4 +1,5 @@
-"""Every kernel of gs.ops.expert_matmul and its gradients, in whole numbers: equal to the formulas in 64 bits.
+"""Every kernel of gs.ops.expert_matmul and its gradients, in whole numbers: equal to the formulas in 64 bits, with nothing
+around their results touched.
 
 Which kernel a call takes is a rule on its sizes, types and alignment.  CASES reach every one that the library holds, of
 widths that are odd, and that are not, where it can have both; without a GPU it is checked that they still do, by the library's own
@@ -76,6 +77,63 @@ def test_every_kernel(dev, n, experts, inner, outer, transposed, dtype):
         d = capi.expert_matmul_grad(grad, rows, order.offsets)
         assert torch.equal(d[:e], got[2][:e]) and torch.equal(d[e + 1:], got[2][e + 1:])
         assert loads[e] == 0 or not d[e].isfinite().any()
+
+
+def guarded(shape, dtype, dev):
+    """A tensor in the middle of a larger one full of a value, and whether what lies around it still has that value."""
+    size = int(np.prod(shape)) * torch.finfo(dtype).bits // 8
+    room = 1 << 16
+    whole_of = torch.full((room + (size + 255) // 256 * 256 + room,), 0x5a, dtype=torch.uint8, device=dev)
+    mine = whole_of[room:room + size].view(dtype).view(shape)
+
+    def untouched():
+        return bool((whole_of[:room] == 0x5a).all()) and bool((whole_of[room + size:] == 0x5a).all())
+
+    return mine, untouched
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,experts,inner,outer", [
+    (90, 3, 1001, 333), (24, 3, 3497, 72), (700, 3, 2070, 351),                # few rows
+    ((1 << 19) + 9, 3, 40, 56), ((1 << 19) + 9, 3, 33, 67), (9000, 3, 27, 1971),  # small matrices, many rows
+    (300, 3, 24, 40), (300, 3, 5, 3), (5011, 3, 146, 165), (14_813, 3, 784, 912), (12_100, 3, 259, 1027),  # tiles
+    (100_001, 3, 33, 9), (3018, 3, 176, 1840),                                 # pieces of rows
+])
+def test_nothing_around_the_results_is_touched_whatever_the_offsets_hold(dev, n, experts, inner, outer, dtype):
+    """The C entry points, results and workspace in the middle of memory that is looked at afterwards.  Offsets that ascend once they
+    are brought between 0 and n have their rows' results; others leave rows out, or write them twice."""
+    lib, i64 = capi.lib(), ctypes.c_int64
+    kind = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    rows, grad = (whole(n, d, dtype=dtype, dev=dev, seed=d) for d in (inner, outer))
+    for at in ([0, n // 3, n // 2, n], [0, 2 ** 40, 2 ** 40, 2 ** 62], [-5, 10, 20, n + 400], [0, n, n // 3, 3], [n, n // 2, n // 3, 0],
+               [-2 ** 62, -7, -1, -1], [0, n, 0, n], [-2 ** 63, 2 ** 63 - 1, -2 ** 63, 2 ** 63 - 1], [7, n // 3, n // 3, n - 9]):
+        offsets = torch.tensor(at, device=dev)
+        held = np.clip(np.array(at, dtype=object), 0, n).astype(np.int64)
+        ascend = bool((np.diff(held) >= 0).all())
+        loads = np.append(held[0], np.diff(held))  # (rows before the first offset are nobody's, and not written)
+        for transposed in (False, True):
+            weight = weights_of(whole, experts, inner, outer, transposed, dtype=dtype, dev=dev, seed=3)
+            out, untouched = guarded((n, outer), dtype, dev)
+            stride = inner if transposed else outer
+            rc = lib.gs_expert_matmul(capi._ptr(rows), i64(inner), i64(n), i64(inner), kind, capi._ptr(weight), i64(inner * outer),
+                                      i64(stride), int(transposed), i64(experts), i64(outer), capi._ptr(offsets), capi._ptr(out),
+                                      capi._stream(dev))
+            assert rc == 0 and untouched()
+            if ascend:
+                nobody = torch.zeros(1, inner, outer, dtype=dtype, device=dev)
+                want = formula(rows, loads, torch.cat([nobody, weight]))[0].to(dtype)
+                assert torch.equal(out[held[0]:], want[held[0]:])
+        dw, untouched = guarded((experts, inner, outer), dtype, dev)
+        size = lib.gs_expert_matmul_grad_workspace_bytes(i64(n), i64(inner), i64(outer), i64(experts))
+        ws, ws_untouched = guarded((size // 4,), torch.float32, dev)
+        rc = lib.gs_expert_matmul_grad(capi._ptr(rows), i64(inner), i64(inner), capi._ptr(grad), i64(outer), i64(outer), kind, i64(n),
+                                       capi._ptr(offsets), i64(experts), capi._ptr(dw), capi._ptr(ws), ctypes.c_size_t(size),
+                                       capi._stream(dev))
+        assert rc == 0 and untouched() and ws_untouched()
+        if ascend:
+            want = formula(rows, loads, torch.zeros(experts + 1, inner, outer, dtype=dtype, device=dev), grad)[4][1:]
+            assert torch.equal(dw, want.to(dtype))
 
 
 # ------------------------------------------------------------------ no GPU ----
