@@ -1,9 +1,9 @@
-// Products of rows sorted by expert with each expert's matrix (gs_expert_products.hip) where experts have few rows, on
-// gfx950: tokens that are being generated.
+// Products of rows sorted by expert with each expert's matrix (gs_expert_products.hip) where experts have few rows, whose tiles would
+// not fill the card, or deep matrices, on gfx950: tokens that are being generated.
 //
 // Every matrix that is met is read once, which bounds them: 30 experts of 4096 x 256, 8 rows each, bf16, 16 us, 3.9
 // TB/s, start and end included.  A workgroup takes up to 16 * MI rows of an expert and 16 *
-// kWide columns (or half as many); its waves share out the depth, step by step, each with several steps of the matrix
+// COLS columns; its waves share out the depth, step by step, each with several steps of the matrix
 // on their way to registers, and their sums meet in LDS.  No value goes through LDS on its way in: a lane's chunks
 // are what the matrix cores take (along the depth), or become that by exchanging halves of registers (across it).
 // No counterpart in the reference.
