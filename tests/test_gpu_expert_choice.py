@@ -253,6 +253,36 @@ def test_recorded_and_replayed(dev):
 
 
 @gpu
+def test_normalized_shares_recorded_and_replayed(dev):
+    """Their backward pass, which has no logits, in a graph: other logits at each replay."""
+    l = logits_of("normal", 700, 96, torch.float16, dev, 1).requires_grad_(True)
+    grad = torch.randn(700, 4, device=dev)
+
+    def step():
+        experts, weights = gs.ops.expert_choose(l * 1.0, 4)
+        return experts, weights.detach(), torch.autograd.grad(weights, l, grad)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for rep in range(4):
+        with torch.no_grad():
+            l.copy_(logits_of("masked" if rep % 2 else "ties", 700, 96, torch.float16, dev, 20 + rep))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@gpu
 def test_offsets_beyond_32_bits(dev):
     if torch.cuda.mem_get_info(dev)[0] < 60 << 30:
         pytest.skip("needs about 20 GB of free device memory")

@@ -136,6 +136,35 @@ def test_nothing_around_the_results_is_touched_whatever_the_offsets_hold(dev, n,
             assert torch.equal(dw, want.to(dtype))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_around_choices_and_what_dropout_leaves_is_touched(dev, dtype):
+    """Numbers of tokens, experts and values that end inside a workgroup, a group of lanes and a chunk."""
+    lib, i64 = capi.lib(), ctypes.c_int64
+    kind = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    for tokens, num, choices in ((1, 1, 1), (65, 3, 2), (33, 17, 3), (50, 65, 8), (9, 193, 16), (7, 385, 17), (5, 1001, 64), (3, 4095, 5)):
+        logits = whole(tokens, num, dtype=dtype, dev=dev, seed=num)
+        for normalize in (0, 1):
+            weights, w_ok = guarded((tokens, choices), torch.float32, dev)
+            experts, e_ok = guarded((tokens, choices), torch.float32, dev)  # (as wide as int32)
+            d, d_ok = guarded((tokens, num), dtype, dev)
+            assert lib.gs_expert_choose(capi._ptr(logits), i64(num), kind, i64(tokens), i64(num), i64(choices), normalize,
+                                        capi._ptr(experts), capi._ptr(weights), capi._stream(dev)) == 0
+            assert lib.gs_expert_choose_grad(capi._ptr(logits), i64(num), kind, capi._ptr(experts), capi._ptr(weights),
+                                             capi._ptr(weights), i64(tokens), i64(num), i64(choices), normalize, capi._ptr(d),
+                                             capi._stream(dev)) == 0
+            assert w_ok() and e_ok() and d_ok()
+            want = capi.expert_choose(logits, choices, bool(normalize))
+            assert torch.equal(experts.view(torch.int32), want[0]) and torch.equal(weights, want[1])
+            assert torch.equal(d, capi.expert_choose_grad(weights.clone(), logits, want[0], want[1], bool(normalize)))
+    for n in (1, 7, 8, 1023, 2048, 2049, 100_003):
+        x = whole(n, dtype=dtype, dev=dev, seed=n)
+        out, untouched = guarded((n,), dtype, dev)
+        assert lib.gs_dropout(capi._ptr(x), None, i64(n), kind, ctypes.c_double(0.5), ctypes.c_uint64(3), None, capi._ptr(out),
+                              capi._stream(dev)) == 0
+        assert untouched() and torch.equal(out, capi.dropout(x, 0.5, 3))
+
+
 # ------------------------------------------------------------------ no GPU ----
 _WRITTEN_DOWN = """
 import ctypes, json, sys
