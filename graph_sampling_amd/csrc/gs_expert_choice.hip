@@ -163,8 +163,8 @@ choose_kernel(const T* __restrict__ logits, int64_t stride, int64_t tokens, int 
   const float share = which >= 0 ? expf(value - most) : 0.0f;
   float sum = share;
   if (!normalize) {
-    // (By expf, as in the gradient.  exp2 of a product with log2(e), rounded once, is 1.3e-8 of the difference too small, to the same side for
-    // all; without normalize 16384 x 256 fp32 takes 12.1 us by expf and 11.0 so, 100 003 x 160 fp16 27 and 24.)
+    // (By expf, as in the gradient.  exp2 of a product with log2(e), rounded once, is 1.3e-8 of the difference too small, to
+    // the same side for all; without normalize 16384 x 256 fp32 takes 12.1 us by expf and 11.0 so, 100 003 x 160 fp16 27 and 24.)
     sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {

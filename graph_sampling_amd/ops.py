@@ -148,8 +148,8 @@ def expert_combine(y, order, weights=None):
 
 def expert_choose(logits, choices, normalize=True):
     """The `choices` experts (at most 64) with the largest of a router's `logits` ([tokens, experts]; up to 4096
-    experts, tokens x choices below 2**31; float32, float16 or bfloat16), and how much each is to count: (experts [tokens, choices] int32, weights
-    float32).  Experts come largest first, the lower one of equals; weights are shares of the softmax over the chosen
+    experts, tokens x choices below 2**31; float32, float16 or bfloat16), and how much each is to count: (experts
+    [tokens, choices] int32, weights float32).  Experts come largest first, the lower one of equals; weights are shares of the softmax over the chosen
     experts, or, without `normalize`, over all.  A logit of -inf stands for an expert the token may not have: it is
     never chosen, and where no other is left the choice is -1 with weight 0.  Differentiable in `logits`, through the
     weights.

@@ -1091,8 +1091,8 @@ int gs_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y,
 /* What experts do between their rows' going out and coming back: the choice of experts, */
 /* products with each expert's matrix, dropout.  No counterpart in the reference.  */
 /* ------------------------------------------------------------------------- */
-/* The choice of K = choices experts (up to 64, and up to as many as there are: 4096 at most; tokens x K below 2^31) from a router's logits,
- * row t from logits + t * stride values: chosen[t, 0..K) = the experts with the largest logits, largest first, the
+/* The choice of K = choices experts (up to 64, and up to as many as there are: 4096 at most; tokens x K below 2^31) from a
+ * router's logits, row t from logits + t * stride values: chosen[t, 0..K) = the experts with the largest logits, largest first, the
  * lower one of equals; weights[t, k] = exp(logit - the largest) over the sum of the same for the chosen experts
  * (normalize) or for all.  A logit of -infinity is never chosen: where no other is left, -1 with weight 0.  NaN counts as
  * the largest, and makes the token's weights NaN.  (No counterpart in the reference.) */

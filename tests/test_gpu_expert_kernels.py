@@ -189,7 +189,8 @@ def grad(n, num, inner, outer, kind):
 
 def choose(num, choices, kind):
     return (launched(lib.gs_expert_choose(at[0], i64(num), kind, i64(50), i64(num), i64(choices), 1, at[1], at[2], None)) +
-            launched(lib.gs_expert_choose_grad(at[0], i64(num), kind, at[1], at[2], at[3], i64(50), i64(num), i64(choices), 1, at[4], None)))
+            launched(lib.gs_expert_choose_grad(at[0], i64(num), kind, at[1], at[2], at[3], i64(50), i64(num), i64(choices), 1, at[4],
+                                               None)))
 
 out = [{"matmul": matmul, "grad": grad, "choose": choose}[call[0]](*call[1:]) for call in json.loads(sys.stdin.read())]
 print(json.dumps({"calls": out, "kernels": stand_in.kernels().decode().split()}))
